@@ -7,6 +7,7 @@ directory).  Public surface:
 * ``HipVectorStore``  -- drop-in for the reference's ``BaseVDB`` / ``PGVector`` (``store.py``)
 * ``HvsComm`` / ``ShardedSearch`` / ``sharded_kmeans_step`` -- one process per GPU over RCCL (``sharded.py``)
 * ``HvsGraph``        -- knowledge graph in HBM + personalised PageRank (``graph.py``)
+* ``QueryAdapters``, ``preference_loss``, ``clip_grad_norm`` -- per-tenant query adapters learned from feedback (``adapters.py``)
 * ``HipGraphStore`` / ``FusionQueryService`` -- graph tables and the fusion step after retrieval (``graph_store.py``)
 """
 
@@ -34,6 +35,10 @@ def __getattr__(name):
         from . import cluster_filter
 
         return getattr(cluster_filter, name)
+    if name in ("QueryAdapters", "FeedbackGradients", "preference_loss", "clip_grad_norm"):
+        from . import adapters
+
+        return getattr(adapters, name)
     if name in ("ShardedSearch", "HvsComm", "host_exchange", "sharded_kmeans_step", "shard_range"):
         from . import sharded
 

@@ -43,6 +43,33 @@ class HvsFilterStruct(ctypes.Structure):
                 ("uris", c_void_p), ("n_uris", c_int32)]
 
 
+HVS_MAX_ADAPTER_DIM = 16384
+HVS_MAX_ADAPTER_RANK = 128
+HVS_MAX_ADAPTERS = 16382
+
+
+class HvsAdaptersStruct(ctypes.Structure):
+    """``hvs_adapters``: the weights of the query adapters."""
+
+    _fields_ = [("projection", c_void_p), ("a", c_void_p), ("b", c_void_p), ("scale", c_void_p), ("dtype", c_int32), ("d_in", c_int32),
+                ("d_out", c_int32), ("rank", c_int32), ("n_adapters", c_int32)]
+
+
+class HvsPreferenceStruct(ctypes.Structure):
+    """``hvs_preference``: one batch of preference pairs."""
+
+    _fields_ = [("queries", c_void_p), ("ld_queries", c_int64), ("reference", c_void_p), ("ld_reference", c_int64), ("offsets", c_void_p),
+                ("chosen", c_void_p), ("rejected", c_void_p), ("weights", c_void_p), ("loss", c_void_p), ("margin", c_void_p), ("grad", c_void_p),
+                ("ld_grad", c_int64), ("n_queries", c_int64), ("n_pairs", c_int64), ("query_dtype", c_int32), ("beta", c_float),
+                ("label_smoothing", c_float)]
+
+
+class HvsTensorStruct(ctypes.Structure):
+    """``hvs_tensor``: one tensor of a global norm."""
+
+    _fields_ = [("data", c_void_p), ("out", c_void_p), ("numel", c_int64), ("dtype", c_int32)]
+
+
 # name -> (restype, argtypes): every symbol include/hvs.h declares
 SIGNATURES = {
     "hvs_last_error": (c_char_p, []),
@@ -110,6 +137,15 @@ SIGNATURES = {
     "hvs_graph_top_chunks": (c_int, [c_void_p, c_int, c_void_p, c_void_p, POINTER(c_int)]),
     "hvs_cosine_matrix": (c_int, [c_int, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_void_p, c_int]),
     "hvs_kmeans_assign": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int]),
+    "hvs_adapters_workspace": (c_int, [c_void_p, c_int64, c_int64, c_int, POINTER(c_uint64)]),
+    "hvs_adapters_apply": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_uint64]),
+    "hvs_adapters_backward": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int64,
+                                      c_void_p, c_void_p, c_void_p, c_uint64]),
+    "hvs_preference_workspace": (c_int, [c_void_p, c_int, POINTER(c_uint64)]),
+    "hvs_preference_loss": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int64, c_int64, c_void_p, c_uint64]),
+    "hvs_index_preference_loss": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_uint64]),
+    "hvs_clip_workspace": (c_int, [c_void_p, c_int, POINTER(c_uint64)]),
+    "hvs_clip_grad_norm": (c_int, [c_int, c_void_p, c_void_p, c_int, c_double, c_int, c_void_p, c_void_p, c_uint64]),
     "hvs_profile_enable": (c_int, [c_void_p, c_int]),
     "hvs_profile_get": (c_int, [c_void_p, c_int, POINTER(c_double), POINTER(c_int64)]),
     "hvs_profile_reset": (c_int, [c_void_p]),

@@ -1,0 +1,1012 @@
+// Low-rank adapters of many tenants beside one shared projection (C ABI: include/hvs.h).
+//
+//     y_i = W x_i + s_c B_c (A_c x_i),  c = code of row i            (forward)
+//     v_i = s_c B_c^T g_i,  dx_i = W^T g_i + A_c^T v_i,  dA_c = sum v_i x_i^T,  dB_c = s_c sum g_i u_i^T   (backward)
+//
+// Two routes.  Few rows (FEW_ROWS): every 16-column slice of W is read once by its own block, bound by the latency of
+// reading W; rows stay in arrival order.  Many rows: rows are ordered by code (a stable counting sort), so that a tile of
+// rows meets few adapters; the low-rank term is put into the accumulators of the tile product first and W x is added by
+// the same matrix-pipe loop as the searches use, so y is rounded and written once.
+//
+// u = A_c x is held in fp32.  For 16-bit weights the product with B runs on the 16-bit pipe: u is divided by a power of
+// two that brings its largest element to [0.5, 1) (no overflow in fp16 whatever the inputs), split into two 16-bit parts
+// hi + lo (relative error 2^-16 for bf16, 2^-22 for fp16: far below the output's own rounding), and the accumulators are
+// multiplied by that power and by s_c before W x is added.
+#include "hvs_learn.h"
+
+#define FEW_ROWS 64
+#define GROUP_CHUNK 1024  // rows per block of the grouping kernels
+#define MAX_CHUNK_ROWS 65536
+
+// ---------------------------------------------------------------------------------------------------------------
+// grouping: rows ordered by adapter, equal codes in row order
+// ---------------------------------------------------------------------------------------------------------------
+// bin 0: no adapter, bin c + 1: adapter c, bin S + 1: codes past the last adapter
+__device__ __forceinline__ int group_bin(int32_t code, int S) { return code < 0 ? 0 : (code >= S ? S + 1 : code + 1); }
+
+__global__ __launch_bounds__(GROUP_CHUNK) void group_count_kernel(const int32_t *__restrict__ codes, int n, int S, uint32_t *__restrict__ counts) {
+    extern __shared__ uint32_t hist[];  // [S + 2]
+    const int nb = S + 2;
+    for (int b = threadIdx.x; b < nb; b += GROUP_CHUNK) hist[b] = 0;
+    __syncthreads();
+    const int i = blockIdx.x * GROUP_CHUNK + threadIdx.x;
+    if (i < n) atomicAdd(&hist[group_bin(codes[i], S)], 1u);  // whole numbers: the order does not matter
+    __syncthreads();
+    for (int b = threadIdx.x; b < nb; b += GROUP_CHUNK) counts[(size_t)blockIdx.x * nb + b] = hist[b];
+}
+
+// Every block adds up the counts of all chunks itself (bins in rounds of 1024: a block scan with a carry) and places its
+// own rows: the 16 waves take turns, and inside a wave lanes of one bin find each other with one ballot per bit of the bin.
+__global__ __launch_bounds__(GROUP_CHUNK) void group_place_kernel(const int32_t *__restrict__ codes, int n, int S, int bits, int chunks,
+                                                                  const uint32_t *__restrict__ counts, uint32_t *__restrict__ order,
+                                                                  int32_t *__restrict__ scodes, uint32_t *__restrict__ seg_begin) {
+    extern __shared__ uint32_t next[];  // [S + 2] next free place of every bin
+    __shared__ uint32_t wave_sum[GROUP_CHUNK / 64];
+    const int nb = S + 2, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int i = blockIdx.x * GROUP_CHUNK + tid;
+    const int32_t code = i < n ? codes[i] : 0;
+    const uint32_t bin = i < n ? group_bin(code, S) : 0;
+    if (chunks == 1) {  // no counting launch: count here
+        for (int b = tid; b < nb; b += GROUP_CHUNK) next[b] = 0;
+        __syncthreads();
+        if (i < n) atomicAdd(&next[bin], 1u);
+        __syncthreads();
+    }
+    uint32_t carry = 0;
+    for (int b0 = 0; b0 < nb; b0 += GROUP_CHUNK) {
+        const int b = b0 + tid;
+        uint32_t total = 0, before = 0;
+        if (b < nb) {
+            if (chunks == 1) total = next[b];
+            else
+                for (int k = 0; k < chunks; k++) {
+                    const uint32_t v = counts[(size_t)k * nb + b];
+                    total += v;
+                    before += k < (int)blockIdx.x ? v : 0u;
+                }
+        }
+        uint32_t inc = total;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint32_t v = __shfl_up(inc, o);
+            if (lane >= o) inc += v;
+        }
+        if (lane == 63) wave_sum[wave] = inc;
+        __syncthreads();
+        uint32_t base = carry, all = 0;
+#pragma unroll
+        for (int w = 0; w < GROUP_CHUNK / 64; w++) {
+            if (w < wave) base += wave_sum[w];
+            all += wave_sum[w];
+        }
+        const uint32_t start = base + inc - total;
+        if (b < nb) {
+            next[b] = start + before;
+            if (blockIdx.x == 0 && b >= 1) seg_begin[b - 1] = start;  // seg_begin[S] = end of the last adapter's rows
+        }
+        carry += all;
+        __syncthreads();
+    }
+    uint64_t peers = __ballot(i < n);
+    for (int bit = 0; bit < bits; bit++) {
+        const bool one = (bin >> bit) & 1u;
+        const uint64_t m = __ballot(one);
+        peers &= one ? m : ~m;
+    }
+    const uint64_t below = (1ull << lane) - 1ull;
+    for (int w = 0; w < GROUP_CHUNK / 64; w++) {
+        if (w == wave && i < n) {
+            const uint32_t place = next[bin] + (uint32_t)__popcll(peers & below);
+            order[place] = (uint32_t)i;
+            scodes[place] = code;
+        }
+        __syncthreads();
+        if (w == wave && i < n && (peers >> lane) == 1ull) next[bin] += (uint32_t)__popcll(peers);  // the highest of its peers
+        __syncthreads();
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// u = A_c x
+// ---------------------------------------------------------------------------------------------------------------
+struct ShrinkParams {
+    const void *x;
+    int64_t ld_x;
+    const void *a;  // [S][r] rows of K elements, pitch lda
+    int64_t lda;
+    const int32_t *codes;   // in the order of `order` when that is given, else by row
+    const uint32_t *order;  // row numbers ordered by code, or NULL
+    int n, K, r, rp, S;     // rp: r rounded up to 16
+    float *hidden;          // [n][r] by row, or NULL
+    void *u_hi, *u_lo;      // [n][rp] in the order of `order` (fp32: u_hi alone), or NULL
+    float *factor;          // [n] likewise: what the tile product multiplies the low-rank sums by
+    const float *scale;
+};
+
+#define SHRINK_WAVES 8
+// One block per 16 rows (and per share blockIdx.y of the adapters among them): D[rank][row] on 16x16 matrix tiles, the
+// block's waves split K and add up through LDS.  Every adapter that occurs is read once per tile of rows that uses it;
+// loads go straight to registers (a lane's 16 bytes are a fragment).
+template <int DT, int RT, bool ALIGNED>
+__global__ __launch_bounds__(64 * SHRINK_WAVES) void shrink_kernel(ShrinkParams p) {
+    typedef typename Elem<DT>::type E;
+    constexpr int EPC = Elem<DT>::EPC, STEP = 4 * EPC;
+    __shared__ float part[SHRINK_WAVES][RT * 16][17];
+    __shared__ float row_max[16];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int m = lane & 15, g = lane >> 4;
+    const int at = blockIdx.x * 16 + m;
+    const bool valid = at < p.n;
+    const int32_t code = valid ? p.codes[at] : -1;
+    const int row = valid ? (p.order ? (int)p.order[at] : at) : 0;
+    const E *x = reinterpret_cast<const E *>(p.x) + (int64_t)row * p.ld_x;
+    uint32_t todo = (uint32_t)__ballot(valid) & 0xFFFFu;
+    for (int ordinal = 0; todo; ordinal++) {
+        const int lead = __builtin_ctz(todo);
+        const int32_t c = __builtin_amdgcn_readlane(code, lead);
+        const uint32_t members = (uint32_t)__ballot(valid && code == c) & 0xFFFFu;
+        todo &= ~members;
+        if (ordinal % (int)gridDim.y != (int)blockIdx.y) continue;
+        f32x4 acc[RT];
+#pragma unroll
+        for (int t = 0; t < RT; t++) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        const bool known = c >= 0 && c < p.S;
+        if (known) {
+            const E *a = reinterpret_cast<const E *>(p.a) + (int64_t)c * p.r * p.lda;
+            constexpr int UNROLL = RT <= 2 ? 4 : 2;
+            for (int k0 = wave * STEP; k0 < p.K; k0 += SHRINK_WAVES * STEP * UNROLL) {
+                f32x4 fx[UNROLL], fa[UNROLL][RT];
+#pragma unroll
+                for (int s = 0; s < UNROLL; s++) {
+                    const int k = k0 + s * SHRINK_WAVES * STEP + g * EPC;
+                    fx[s] = load_chunk<DT, ALIGNED>(x, k, valid ? p.K : 0);
+#pragma unroll
+                    for (int t = 0; t < RT; t++) {
+                        const int j = t * 16 + m;
+                        fa[s][t] = load_chunk<DT, ALIGNED>(a + (int64_t)(j < p.r ? j : 0) * p.lda, k, j < p.r ? p.K : 0);
+                    }
+                }
+#pragma unroll
+                for (int s = 0; s < UNROLL; s++)
+#pragma unroll
+                    for (int t = 0; t < RT; t++) acc[t] = mfma_chunk<DT>(fa[s][t], fx[s], acc[t]);
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < RT; t++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) part[wave][t * 16 + 4 * g + e][m] = acc[t][e];
+        __syncthreads();
+        // thread (j, m') owns rank j of row m': the waves' sums in wave order
+        for (int q = tid; q < RT * 256; q += 64 * SHRINK_WAVES) {
+            float s = 0.0f;
+#pragma unroll
+            for (int w = 0; w < SHRINK_WAVES; w++) s += part[w][q >> 4][q & 15];
+            part[0][q >> 4][q & 15] = c < p.S ? s : __builtin_nanf("");  // (its own cell: nobody else reads it before the barrier)
+        }
+        __syncthreads();
+        if (tid < 16) {
+            float mx = 0.0f;
+            for (int j = 0; j < p.r; j++) mx = fmaxf(mx, fabsf(part[0][j][tid]));
+            row_max[tid] = mx;
+        }
+        __syncthreads();
+        if (p.hidden)
+            for (int q = tid; q < 16 * p.r; q += 64 * SHRINK_WAVES) {
+                const int mm = q / p.r, j = q - mm * p.r;
+                if (members >> mm & 1) {
+                    const int64_t out_row = p.order ? (int64_t)p.order[blockIdx.x * 16 + mm] : (int64_t)blockIdx.x * 16 + mm;
+                    p.hidden[out_row * p.r + j] = part[0][j][mm];
+                }
+            }
+        if (p.u_hi) {
+            for (int q = tid; q < 16 * p.rp; q += 64 * SHRINK_WAVES) {
+                const int mm = q / p.rp, j = q - mm * p.rp;
+                if (!(members >> mm & 1)) continue;
+                const int64_t o = ((int64_t)blockIdx.x * 16 + mm) * p.rp + j;
+                float u = j < p.r && known ? part[0][j < RT * 16 ? j : 0][mm] : 0.0f;
+                if (DT == HVS_F32) reinterpret_cast<float *>(p.u_hi)[o] = u;
+                else {
+                    const float mx = row_max[mm];
+                    if (mx > 0.0f && mx < __builtin_inff()) u = ldexpf(u, -ilogbf(mx) - 1);
+                    const E hi = learn_from_float<E>(u);
+                    reinterpret_cast<E *>(p.u_hi)[o] = hi;
+                    reinterpret_cast<E *>(p.u_lo)[o] = learn_from_float<E>(u - learn_to_float(hi));
+                }
+            }
+            if (tid < 16 && (members >> tid & 1)) {
+                float f = c >= p.S ? __builtin_nanf("") : 1.0f;
+                if (known) {
+                    const float mx = row_max[tid];
+                    f = p.scale[c];
+                    if (DT != HVS_F32 && mx > 0.0f && mx < __builtin_inff()) f = ldexpf(f, ilogbf(mx) + 1);
+                }
+                p.factor[blockIdx.x * 16 + tid] = f;
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// few rows: y = W x + s B u
+// ---------------------------------------------------------------------------------------------------------------
+struct ProjectParams {
+    const void *x;
+    int64_t ld_x;
+    const void *w;  // [N] rows of K elements, pitch ldw
+    int64_t ldw;
+    const void *b;  // [S][N] rows of r elements, pitch ldb
+    int64_t ldb;
+    const float *scale;
+    const int32_t *codes;   // few rows: by row; many rows: in the order of `order`
+    const uint32_t *order;
+    const float *hidden;    // few rows: [n][r]
+    const void *u_hi, *u_lo;
+    const float *factor;
+    void *out;
+    int64_t ld_out;
+    int n, K, N, r, rp, S;
+    int b_aligned;   // rows of b start on 16 bytes and r is a whole number of chunks
+    int out_vec;     // four consecutive outputs may be stored at once
+};
+
+#define FEW_WAVES 8
+// One block per 16 columns of y: the block's waves split K, W and x fragments go straight from memory to registers, the
+// partial sums meet in LDS, the low-rank term is added per output.
+template <int DT, int NT, bool ALIGNED>
+__global__ __launch_bounds__(64 * FEW_WAVES) void project_few_kernel(ProjectParams p) {
+    typedef typename Elem<DT>::type E;
+    constexpr int EPC = Elem<DT>::EPC, STEP = 4 * EPC, UNROLL = 4;
+    __shared__ float part[FEW_WAVES][NT * 16][17];  // [wave][row][column]
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int m = lane & 15, g = lane >> 4;
+    const int col0 = blockIdx.x * 16;
+    const bool col_ok = col0 + m < p.N;
+    const E *w = reinterpret_cast<const E *>(p.w) + (int64_t)(col_ok ? col0 + m : 0) * p.ldw;
+    f32x4 acc[NT];
+#pragma unroll
+    for (int t = 0; t < NT; t++) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int k0 = wave * STEP; k0 < p.K; k0 += FEW_WAVES * STEP * UNROLL) {
+        f32x4 fw[UNROLL], fx[UNROLL][NT];
+#pragma unroll
+        for (int s = 0; s < UNROLL; s++) {
+            const int k = k0 + s * FEW_WAVES * STEP + g * EPC;
+            fw[s] = load_chunk<DT, ALIGNED>(w, k, col_ok ? p.K : 0);
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                const int row = t * 16 + m;
+                fx[s][t] = load_chunk<DT, ALIGNED>(reinterpret_cast<const E *>(p.x) + (int64_t)(row < p.n ? row : 0) * p.ld_x, k, row < p.n ? p.K : 0);
+            }
+        }
+#pragma unroll
+        for (int s = 0; s < UNROLL; s++)
+#pragma unroll
+            for (int t = 0; t < NT; t++) acc[t] = mfma_chunk<DT>(fw[s], fx[s][t], acc[t]);
+    }
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) part[wave][t * 16 + m][4 * g + e] = acc[t][e];
+    __syncthreads();
+    for (int q = tid; q < p.n * 16; q += 64 * FEW_WAVES) {
+        const int row = q >> 4, col = col0 + (q & 15);
+        if (col >= p.N) continue;
+        const int32_t c = p.codes[row];
+        float low = 0.0f;
+        if (c >= 0 && c < p.S) {
+            const E *b = reinterpret_cast<const E *>(p.b) + ((int64_t)c * p.N + col) * p.ldb;
+            const float *u = p.hidden + (int64_t)row * p.r;
+            for (int j = 0; j < p.r; j++) low = fmaf(learn_to_float(b[j]), u[j], low);
+            low *= p.scale[c];
+        }
+        float s = 0.0f;
+#pragma unroll
+        for (int w8 = 0; w8 < FEW_WAVES; w8++) s += part[w8][row][q & 15];
+        s = c >= p.S ? __builtin_nanf("") : s + low;
+        reinterpret_cast<E *>(p.out)[(int64_t)row * p.ld_out + col] = learn_from_float<E>(s);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// many rows: the tile product
+// ---------------------------------------------------------------------------------------------------------------
+// Offsets of a tile's 16-byte chunks for the LDS-DMA: tile row t is row rows[t] of the matrix (order == NULL: row0 + t).
+// Tile rows past the end re-read the last one.  `base` must be wave-uniform and every offset below 2^31.
+template <class T>
+__device__ __forceinline__ void adapter_src_init(TileSrcT<T::DMA_N> &t, const void *base, const uint32_t *order, int row0, int n_rows, int64_t pitch_bytes,
+                                                 int64_t num_bytes, int tid) {
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)base);
+    const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)((uintptr_t)base >> 32));
+    const int bytes = __builtin_amdgcn_readfirstlane((int)num_bytes);
+    t.rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)(((uintptr_t)hi << 32) | lo), 0, bytes, 0x00020000);
+#pragma unroll
+    for (int i = 0; i < T::DMA_N; i++) {
+        const int P = T::GT * i + tid;
+        const int slot = P >> 3, kc = (P & 7) ^ lds_swz(slot);
+        int row = row0 + slot;
+        row = row < n_rows ? row : n_rows - 1;
+        if (order) row = (int)order[row];
+        t.voff[i] = (int)(row * pitch_bytes) + kc * 16;
+    }
+}
+// The last k-step of rows that end inside its 128 bytes: chunks past the row's end are sent past the buffer's end, where
+// loads return 0 (they would otherwise read the next row).
+template <class T> __device__ __forceinline__ void adapter_src_tail(TileSrcT<T::DMA_N> &t, int chunks_left, int tid) {
+#pragma unroll
+    for (int i = 0; i < T::DMA_N; i++) {
+        const int P = T::GT * i + tid;
+        const int kc = (P & 7) ^ lds_swz(P >> 3);
+        if (kc >= chunks_left) t.voff[i] = 0x7FFFFFFF - 15;
+    }
+}
+
+template <int DT, class T>
+__global__ __launch_bounds__(T::GT, T::GT <= 256 ? 2 : 1) void project_tile_kernel(ProjectParams p) {
+#if defined(__HIP_DEVICE_COMPILE__)  // device-only types (buffer descriptors) inside
+    typedef typename Elem<DT>::type E;
+    constexpr int EPC = Elem<DT>::EPC, MT = T::MT, NT = T::NT;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = wave / T::WN, wn = wave % T::WN;
+    const int l32 = lane & 31, h = lane >> 5;
+    // blocks of one XCD (dispatched round robin) take consecutive tiles, columns first: they share rows of x and all of W
+    const int CT = (p.N + T::BM - 1) / T::BM;
+    const int total = gridDim.x, xcd = blockIdx.x & 7, q8 = total >> 3, rem = total & 7;
+    const int tile = xcd * q8 + (xcd < rem ? xcd : rem) + (blockIdx.x >> 3);
+    const int rt = tile / CT, ct = tile - rt * CT;
+    const int row0 = rt * T::BN, col0 = ct * T::BM;
+
+    TileSrcT<T::DMA_N> srcA, srcB;
+    const int k_bytes = p.K * (int)sizeof(E);
+    const int nks = (k_bytes + KB - 1) / KB, tail = (k_bytes % KB) / 16;
+    {
+        const int rows_a = p.N - col0;
+        const char *wbase = reinterpret_cast<const char *>(p.w) + (int64_t)col0 * p.ldw * sizeof(E);
+        const int last = rows_a < T::BM ? rows_a : T::BM;
+        adapter_src_init<T>(srcA, wbase, nullptr, 0, last, p.ldw * sizeof(E), (int64_t)(last - 1) * p.ldw * sizeof(E) + k_bytes, tid);
+        adapter_src_init<T>(srcB, p.x, p.order, row0, p.n, p.ld_x * sizeof(E), (int64_t)(p.n - 1) * p.ld_x * sizeof(E) + k_bytes, tid);
+    }
+    auto before_step = [&](int ks) {  // the sources of step ks are about to be used
+        if (tail && ks == nks - 1) {
+            adapter_src_tail<T>(srcA, tail, tid);
+            adapter_src_tail<T>(srcB, tail, tid);
+        }
+    };
+    before_step(0);
+    dma_tiles<T>(srcA, srcB, smem, koff_plain(0), wave);
+
+    f32x16 acc[MT][NT];
+    zero_acc(acc);
+    // low-rank term of this wave's columns and rows, adapter by adapter
+    const int wcol = col0 + wm * (MT * 32), wrow = row0 + wn * (NT * 32);
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+        const int j = wrow + nt * 32 + l32;
+        const bool valid = j < p.n;
+        const int32_t code = valid ? p.codes[j] : -1;
+        const bool use = code >= 0 && code < p.S;
+        uint32_t todo = (uint32_t)__ballot(use);
+        while (todo) {
+            const int32_t c = __builtin_amdgcn_readlane(code, __builtin_ctz(todo));
+            const bool mine = use && code == c;
+            todo &= ~(uint32_t)__ballot(mine);
+            const E *b = reinterpret_cast<const E *>(p.b) + (int64_t)c * p.N * p.ldb;
+            // sums of their own, taken over only by the rows of this adapter: a weight that is not finite stays with its tenant
+            f32x16 low[MT];
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) low[mt][e] = 0.0f;
+            for (int k0 = 0; k0 < p.rp; k0 += 2 * EPC) {
+                const int k = k0 + h * EPC;
+                f32x4 ub = {0.0f, 0.0f, 0.0f, 0.0f}, ul = ub;
+                if (mine) {
+                    ub = *reinterpret_cast<const f32x4 *>(reinterpret_cast<const E *>(p.u_hi) + (int64_t)j * p.rp + k);
+                    if (DT != HVS_F32) ul = *reinterpret_cast<const f32x4 *>(reinterpret_cast<const E *>(p.u_lo) + (int64_t)j * p.rp + k);
+                }
+#pragma unroll
+                for (int mt = 0; mt < MT; mt++) {
+                    const int col = wcol + mt * 32 + l32;
+                    const int r_here = col < p.N ? p.r : 0;
+                    const E *brow = b + (int64_t)(col < p.N ? col : 0) * p.ldb;
+                    const f32x4 fb = p.b_aligned ? load_chunk<DT, true>(brow, k, r_here) : load_chunk<DT, false>(brow, k, r_here);
+                    if (DT == HVS_F32) {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) low[mt] = __builtin_amdgcn_mfma_f32_32x32x2f32(fb[e], ub[e], low[mt], 0, 0, 0);
+                    } else {
+                        low[mt] = mfma16<DT>(fb, ub, low[mt]);
+                        low[mt] = mfma16<DT>(fb, ul, low[mt]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) acc[mt][nt][e] = mine ? low[mt][e] : acc[mt][nt][e];
+        }
+        const float f = valid ? p.factor[j] : 1.0f;
+#pragma unroll
+        for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) acc[mt][nt][e] *= f;
+    }
+    __syncthreads();
+
+    int cur = 0;
+    for (int ks = 0; ks < nks; ks++) {
+        // the step after the last one fetches that one again; the stage it fills is never read
+        const int next = ks + 1 < nks ? ks + 1 : ks;
+        if (ks + 1 < nks) before_step(next);
+        compute_step<DT, T>(acc, smem + cur * T::STAGE_BYTES, wm, wn, lane, srcA, srcB, smem + (cur ^ 1) * T::STAGE_BYTES, koff_plain(next), wave);
+        __syncthreads();
+        cur ^= 1;
+    }
+
+    // accumulator element e of lane (l32, h): column 8 (e / 4) + 4 h + e % 4 of its 32, row l32
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+        const int j = wrow + nt * 32 + l32;
+        if (j >= p.n) continue;
+        E *out = reinterpret_cast<E *>(p.out) + (int64_t)p.order[j] * p.ld_out;
+#pragma unroll
+        for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+            for (int e4 = 0; e4 < 4; e4++) {
+                const int col = wcol + mt * 32 + 8 * e4 + 4 * h;
+                E v[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[e] = learn_from_float<E>(acc[mt][nt][4 * e4 + e]);
+                if (p.out_vec && col + 3 < p.N) {
+                    typedef E vec __attribute__((ext_vector_type(4)));
+                    *reinterpret_cast<vec *>(out + col) = vec{v[0], v[1], v[2], v[3]};
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        if (col + e < p.N) out[col + e] = v[e];
+                }
+            }
+    }
+#endif
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// layout: rows brought to 16-byte pitch, transposed weights for the backward pass
+// ---------------------------------------------------------------------------------------------------------------
+template <typename E>
+__global__ __launch_bounds__(256) void pack_rows_kernel(const E *__restrict__ src, int64_t ld, int n, int K, int Kp, E *__restrict__ dst) {
+    const int64_t total = (int64_t)n * Kp;
+    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int64_t r = i / Kp;
+        const int k = (int)(i - r * Kp);
+        dst[i] = k < K ? src[r * ld + k] : (E)0.0f;
+    }
+}
+
+// dst[z][c][r] = src[z][r][c] for matrices of R x C; dst rows have pitch ld (>= R), filled with zeros past R
+template <typename E>
+__global__ __launch_bounds__(256) void transpose_kernel(const E *__restrict__ src, int R, int C, int ld, E *__restrict__ dst) {
+    __shared__ E tile[64][65];
+    const int64_t z = blockIdx.z;
+    const E *s = src + z * (int64_t)R * C;
+    E *d = dst + z * (int64_t)C * ld;
+    const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;
+    for (int i = threadIdx.x; i < 4096; i += 256) {
+        const int r = r0 + (i >> 6), c = c0 + (i & 63);
+        tile[i >> 6][i & 63] = r < R && c < C ? s[(int64_t)r * C + c] : (E)0.0f;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 4096; i += 256) {
+        const int c = c0 + (i >> 6), r = r0 + (i & 63);
+        if (c < C && r < ld) d[(int64_t)c * ld + r] = tile[i & 63][i >> 6];
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// gradients of the stacks: G_c[j][col] = s_c sum over the rows of adapter c of q[row][j] X[row][col]
+// ---------------------------------------------------------------------------------------------------------------
+struct OuterParams {
+    const float *q;  // [n][r] by row
+    const void *x;   // [n][d], pitch ld_x
+    int64_t ld_x;
+    const int32_t *scodes;
+    const uint32_t *order;
+    const uint32_t *seg_begin;  // [S + 1]
+    const float *scale;
+    float *out;      // [S][r][d], or [S][d][r] when transposed
+    float *partial;  // [2 tiles][r][d]
+    int n, d, r, S, rows_per, transposed, accumulate;
+};
+
+// Rows are cut into tiles of rows_per (in code order).  A block walks the adapters of its tile, for 16 chunks of columns;
+// fp32 matrix products (16x16x4: lane = (rank or column chunk, row), so q needs no rounding and X no transposition).  An
+// adapter whose rows all lie in the tile is written out; one that goes on in a neighbouring tile leaves its sum in
+// `partial` (slot 0: it began in an earlier tile, slot 1: it begins here), and outer_join_kernel adds those in tile order.
+template <int DT, int RT, bool ALIGNED> __global__ __launch_bounds__(256) void outer_kernel(OuterParams p) {
+    typedef typename Elem<DT>::type E;
+    constexpr int EPC = Elem<DT>::EPC, CC = 16 * EPC;
+    __shared__ float red[RT * 16][CC + 1];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int m = lane & 15, g = lane >> 4;
+    const int lo = blockIdx.x * p.rows_per, hi = lo + p.rows_per < p.n ? lo + p.rows_per : p.n;
+    const int c0 = blockIdx.y * CC, j0 = blockIdx.z * (RT * 16);
+    int i = lo;
+    while (i < hi) {
+        const int32_t c = p.scodes[i];
+        if (c < 0 || c >= p.S) {  // rows without an adapter come first, codes past the last one come last
+            i = c < 0 ? ((int)p.seg_begin[0] < hi ? (int)p.seg_begin[0] : hi) : hi;
+            continue;
+        }
+        const int seg_lo = (int)p.seg_begin[c], seg_hi = (int)p.seg_begin[c + 1];
+        const int end = seg_hi < hi ? seg_hi : hi;
+        f32x4 acc[RT][EPC];
+#pragma unroll
+        for (int t = 0; t < RT; t++)
+#pragma unroll
+            for (int e = 0; e < EPC; e++) acc[t][e] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        constexpr int UNROLL = RT <= 2 ? 4 : 2;
+        for (int b = i + 4 * wave; b < end; b += 16 * UNROLL) {
+            f32x4 fx[UNROLL];
+            float fq[UNROLL][RT];
+#pragma unroll
+            for (int s = 0; s < UNROLL; s++) {
+                const int at = b + 16 * s + g;
+                const bool ok = at < end;
+                const int64_t row = p.order[ok ? at : i];
+                fx[s] = load_chunk<DT, ALIGNED>(reinterpret_cast<const E *>(p.x) + row * p.ld_x, c0 + m * EPC, ok ? p.d : 0);
+#pragma unroll
+                for (int t = 0; t < RT; t++) {
+                    const int j = j0 + t * 16 + m;
+                    fq[s][t] = ok && j < p.r ? p.q[row * p.r + j] : 0.0f;
+                }
+            }
+#pragma unroll
+            for (int s = 0; s < UNROLL; s++) {
+                float v[EPC];
+                chunk_to_float<DT>(fx[s], v);
+#pragma unroll
+                for (int t = 0; t < RT; t++)
+#pragma unroll
+                    for (int e = 0; e < EPC; e++) acc[t][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(fq[s][t], v[e], acc[t][e], 0, 0, 0);
+            }
+        }
+        // the four waves' sums, in wave order
+        for (int w = 0; w < 4; w++) {
+            if (w == wave) {
+#pragma unroll
+                for (int t = 0; t < RT; t++)
+#pragma unroll
+                    for (int e = 0; e < EPC; e++)
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            float *cell = &red[t * 16 + 4 * g + k][m * EPC + e];
+                            *cell = w == 0 ? acc[t][e][k] : *cell + acc[t][e][k];
+                        }
+            }
+            __syncthreads();
+        }
+        const bool whole = seg_lo >= lo && seg_hi <= hi;
+        const float s = p.scale[c];
+        float *part = p.partial + (int64_t)(2 * blockIdx.x + (seg_lo < lo ? 0 : 1)) * p.r * p.d;
+        const int rn = p.r - j0 < RT * 16 ? p.r - j0 : RT * 16, cn = p.d - c0 < CC ? p.d - c0 : CC;
+        if (whole && p.transposed) {
+            float *out = p.out + (int64_t)c * p.r * p.d;
+            for (int k = tid; k < rn * cn; k += 256) {
+                const int col = k / rn, j = k - col * rn;
+                float *o = out + (int64_t)(c0 + col) * p.r + j0 + j;
+                *o = s * red[j][col] + (p.accumulate ? *o : 0.0f);
+            }
+        } else {
+            float *out = whole ? p.out + (int64_t)c * p.r * p.d : part;
+            for (int k = tid; k < rn * cn; k += 256) {
+                const int j = k / cn, col = k - j * cn;
+                float *o = out + (int64_t)(j0 + j) * p.d + c0 + col;
+                *o = whole ? s * red[j][col] + (p.accumulate ? *o : 0.0f) : red[j][col];
+            }
+        }
+        __syncthreads();
+        i = end;
+    }
+}
+
+// adapters without rows: zero; adapters over several tiles: their partial sums in tile order
+__global__ __launch_bounds__(256) void outer_join_kernel(OuterParams p) {
+    const int c = blockIdx.x;
+    const int lo = (int)p.seg_begin[c], hi = (int)p.seg_begin[c + 1];
+    const int64_t size = (int64_t)p.r * p.d;
+    float *out = p.out + (int64_t)c * size;
+    if (lo == hi) {
+        if (!p.accumulate)
+            for (int64_t k = blockIdx.y * 256ll + threadIdx.x; k < size; k += gridDim.y * 256ll) out[k] = 0.0f;
+        return;
+    }
+    const int t0 = lo / p.rows_per, t1 = (hi - 1) / p.rows_per;
+    if (t0 == t1) return;
+    const float s = p.scale[c];
+    for (int64_t k = blockIdx.y * 256ll + threadIdx.x; k < size; k += gridDim.y * 256ll) {
+        const int64_t at = p.transposed ? (k % p.r) * p.d + k / p.r : k;
+        float v = p.partial[(int64_t)(2 * t0 + 1) * size + at];
+        for (int t = t0 + 1; t <= t1; t++) v += p.partial[(int64_t)(2 * t) * size + at];
+        out[k] = s * v + (p.accumulate ? out[k] : 0.0f);
+    }
+}
+
+__global__ __launch_bounds__(256) void fill_zero_kernel(float *dst, int64_t n) {
+    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) dst[i] = 0.0f;
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------------------------------------------
+static int check_adapters(const char *who, const hvs_adapters *ad) {
+    HVS_REQUIRE(ad != nullptr, "%s: adapters is NULL", who);
+    HVS_REQUIRE(learn_dtype_ok(ad->dtype), "%s: unknown dtype %d", who, ad->dtype);
+    HVS_REQUIRE(ad->d_in >= 1 && ad->d_in <= HVS_MAX_ADAPTER_DIM && ad->d_out >= 1 && ad->d_out <= HVS_MAX_ADAPTER_DIM,
+                "%s: projection %d x %d, both sides must be in [1, %d]", who, ad->d_out, ad->d_in, HVS_MAX_ADAPTER_DIM);
+    HVS_REQUIRE(ad->rank >= 1 && ad->rank <= HVS_MAX_ADAPTER_RANK, "%s: rank %d not in [1, %d]", who, ad->rank, HVS_MAX_ADAPTER_RANK);
+    HVS_REQUIRE(ad->n_adapters >= 1 && ad->n_adapters <= HVS_MAX_ADAPTERS, "%s: %d adapters, must be in [1, %d]", who, ad->n_adapters, HVS_MAX_ADAPTERS);
+    return 0;
+}
+static int round_up(int v, int to) { return (v + to - 1) / to * to; }
+static int elems_per_chunk(int dtype) { return dtype == HVS_F32 ? 4 : 8; }
+
+// rows handled at once: the grouping's counters and the 31-bit offsets of the tile loads set the limit
+static int64_t chunk_rows(int64_t n, int64_t max_ld, int es) {
+    int64_t by_offset = ((int64_t)0x7FFFFFFF - 65536) / ((max_ld + 8) * es);  // + 8: the pitch of rows that are brought to whole chunks
+    int64_t c = by_offset < MAX_CHUNK_ROWS ? by_offset : MAX_CHUNK_ROWS;
+    if (c < 1) c = 1;
+    return n < c ? n : c;
+}
+
+// what one chunk of rows needs; every pass of a direction shares it
+struct AdapterWs {
+    uint32_t *order, *seg_begin, *counts;
+    int32_t *scodes;
+    float *factor, *hidden, *partial;
+    char *u_hi, *u_lo, *packed_w, *packed_x, *w_t, *a_t, *b_t;
+};
+
+// rows of a tile of the stack gradients: about OUTER_BLOCKS blocks, at least OUTER_MIN_ROWS rows each
+#define OUTER_BLOCKS 1024
+#define OUTER_MIN_ROWS 32
+static int outer_cols(int d, int dtype) { return (d + 16 * elems_per_chunk(dtype) - 1) / (16 * elems_per_chunk(dtype)); }
+static int outer_rows_per(int n, int d, int dtype) {
+    const int rows = (int)(((int64_t)n * outer_cols(d, dtype) + OUTER_BLOCKS - 1) / OUTER_BLOCKS);
+    return round_up(rows < OUTER_MIN_ROWS ? OUTER_MIN_ROWS : rows, 16);
+}
+// the most tiles n rows or fewer are cut into (fewer rows may be cut into more tiles than n, by rounding)
+static int64_t outer_max_tiles(int64_t n, int d, int dtype) {
+    const int64_t by_blocks = (OUTER_BLOCKS + outer_cols(d, dtype) - 1) / outer_cols(d, dtype), by_rows = (n + OUTER_MIN_ROWS - 1) / OUTER_MIN_ROWS;
+    return by_blocks < by_rows ? by_blocks : by_rows;
+}
+
+static uint64_t cut_workspace(const hvs_adapters *ad, int64_t nc, int backward, void *base, AdapterWs *ws) {
+    WorkspaceCut w(base);
+    const int es = hvs_elem_size(ad->dtype), epc = elems_per_chunk(ad->dtype), rp = round_up(ad->rank, 16);
+    const int64_t chunks = (nc + GROUP_CHUNK - 1) / GROUP_CHUNK;
+    const int wide = ad->d_in > ad->d_out ? ad->d_in : ad->d_out;
+    ws->hidden = w.take<float>(nc * ad->rank * 4);
+    ws->order = w.take<uint32_t>(nc * 4);
+    ws->scodes = w.take<int32_t>(nc * 4);
+    ws->seg_begin = w.take<uint32_t>(((uint64_t)ad->n_adapters + 1) * 4);
+    ws->counts = w.take<uint32_t>(chunks > 1 ? (uint64_t)chunks * (ad->n_adapters + 2) * 4 : 0);
+    ws->factor = w.take<float>(nc * 4);
+    ws->u_hi = w.take<char>(nc * rp * es);
+    ws->u_lo = w.take<char>(ad->dtype == HVS_F32 ? 0 : nc * rp * es);
+    ws->packed_w = w.take<char>(nc > FEW_ROWS ? (uint64_t)wide * round_up(wide, epc) * es : 0);
+    ws->packed_x = w.take<char>(nc > FEW_ROWS ? (uint64_t)nc * round_up(wide, epc) * es : 0);
+    if (backward) {
+        ws->w_t = w.take<char>((uint64_t)ad->d_in * round_up(ad->d_out, epc) * es);
+        ws->b_t = w.take<char>((uint64_t)ad->n_adapters * ad->rank * round_up(ad->d_out, epc) * es);
+        ws->a_t = w.take<char>((uint64_t)ad->n_adapters * ad->d_in * rp * es);
+        uint64_t part = 0;
+        for (int d : {ad->d_in, ad->d_out}) {
+            const uint64_t b = 2ull * outer_max_tiles(nc, d, ad->dtype) * ad->rank * d * 4;
+            part = b > part ? b : part;
+        }
+        ws->partial = w.take<float>(part);
+    }
+    return w.used;
+}
+
+extern "C" int hvs_adapters_workspace(const hvs_adapters *ad, int64_t n, int64_t max_ld, int backward, uint64_t *out_bytes) {
+    HVS_TRY(check_adapters("hvs_adapters_workspace", ad));
+    HVS_REQUIRE(n >= 0 && out_bytes, "hvs_adapters_workspace: negative row count or NULL argument");
+    const int64_t nc = chunk_rows(n, max_ld > 0 ? max_ld : 1, hvs_elem_size(ad->dtype));
+    AdapterWs ws;
+    *out_bytes = cut_workspace(ad, nc, backward, nullptr, &ws);
+    return 0;
+}
+
+static int launch_group(hipStream_t st, const int32_t *codes, int n, int S, const AdapterWs &ws) {
+    const int chunks = (n + GROUP_CHUNK - 1) / GROUP_CHUNK;
+    const size_t lds = (size_t)(S + 2) * 4;
+    int bits = 1;
+    while ((1 << bits) < S + 2) bits++;
+    if (lds > 48 * 1024) {
+        HVS_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(&group_count_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+        HVS_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(&group_place_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+    }
+    if (chunks > 1) group_count_kernel<<<chunks, GROUP_CHUNK, lds, st>>>(codes, n, S, ws.counts);
+    group_place_kernel<<<chunks, GROUP_CHUNK, lds, st>>>(codes, n, S, bits, chunks, ws.counts, ws.order, ws.scodes, ws.seg_begin);
+    HVS_HIP(hipGetLastError());
+    return 0;
+}
+
+template <int DT> static int launch_shrink(hipStream_t st, const ShrinkParams &p, int shares) {
+    const int es = hvs_elem_size(DT);
+    const bool al = learn_aligned(p.x, p.ld_x * es, (int64_t)p.K * es) && learn_aligned(p.a, p.lda * es, (int64_t)p.K * es);
+    const dim3 grid((p.n + 15) / 16, shares);
+#define SHRINK(RT_) \
+    (al ? shrink_kernel<DT, RT_, true><<<grid, 64 * SHRINK_WAVES, 0, st>>>(p) : shrink_kernel<DT, RT_, false><<<grid, 64 * SHRINK_WAVES, 0, st>>>(p))
+    if (p.r <= 16) SHRINK(1);
+    else if (p.r <= 32) SHRINK(2);
+    else if (p.r <= 64) SHRINK(4);
+    else SHRINK(8);
+#undef SHRINK
+    HVS_HIP(hipGetLastError());
+    return 0;
+}
+
+template <int DT> static int launch_few(hipStream_t st, const ProjectParams &p) {
+    const int es = hvs_elem_size(DT);
+    const bool al = learn_aligned(p.x, p.ld_x * es, (int64_t)p.K * es) && learn_aligned(p.w, p.ldw * es, (int64_t)p.K * es);
+    const int grid = (p.N + 15) / 16;
+#define FEW(NT_) \
+    (al ? project_few_kernel<DT, NT_, true><<<grid, 64 * FEW_WAVES, 0, st>>>(p) : project_few_kernel<DT, NT_, false><<<grid, 64 * FEW_WAVES, 0, st>>>(p))
+    if (p.n <= 16) FEW(1);
+    else if (p.n <= 32) FEW(2);
+    else FEW(4);
+#undef FEW
+    HVS_HIP(hipGetLastError());
+    return 0;
+}
+
+template <int DT, class T> static int launch_tile(hipStream_t st, const ProjectParams &p) {
+    const int tiles = ((p.N + T::BM - 1) / T::BM) * ((p.n + T::BN - 1) / T::BN);
+    const size_t lds = 2 * T::STAGE_BYTES;
+    HVS_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(&project_tile_kernel<DT, T>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+    project_tile_kernel<DT, T><<<tiles, T::GT, lds, st>>>(p);
+    HVS_HIP(hipGetLastError());
+    return 0;
+}
+
+template <int DT> static int launch_pack(hipStream_t st, const void *src, int64_t ld, int n, int K, int Kp, void *dst) {
+    typedef typename Elem<DT>::type E;
+    const int64_t blocks = ((int64_t)n * Kp + 255) / 256;
+    pack_rows_kernel<E><<<(int)(blocks < 4096 ? blocks : 4096), 256, 0, st>>>((const E *)src, ld, n, K, Kp, (E *)dst);
+    HVS_HIP(hipGetLastError());
+    return 0;
+}
+
+template <int DT> static int launch_transpose(hipStream_t st, const void *src, int64_t count, int R, int C, int ld, void *dst) {
+    typedef typename Elem<DT>::type E;
+    // the last row tile covers the pitch, so that the padding is written
+    for (int64_t z0 = 0; z0 < count; z0 += 65535) {
+        const int64_t zn = count - z0 < 65535 ? count - z0 : 65535;
+        const dim3 grid((C + 63) / 64, (ld + 63) / 64, (unsigned)zn);
+        transpose_kernel<E><<<grid, 256, 0, st>>>((const E *)src + z0 * R * C, R, C, ld, (E *)dst + z0 * C * ld);
+    }
+    HVS_HIP(hipGetLastError());
+    return 0;
+}
+
+// One direction for one chunk of rows: u = A x into hidden, y = W x + s B u into out.  A: [S][r] rows of K, pitch lda;
+// W: [N] rows of K, pitch ldw; B: [S][N] rows of r, pitch ldb.
+struct Direction {
+    const void *x, *a, *w, *b;
+    int64_t ld_x, lda, ldw, ldb;
+    int K, N;
+    bool b_padded;  // rows of b are zero from r to their pitch
+    void *out;  // NULL: u alone
+    int64_t ld_out;
+};
+
+template <int DT>
+static int run_direction(hipStream_t st, const hvs_adapters *ad, const Direction &d, const int32_t *codes, int n, float *hidden, AdapterWs &ws, bool grouped) {
+    const int es = hvs_elem_size(DT), epc = Elem<DT>::EPC;
+    const bool few = n <= FEW_ROWS;
+    Direction dd = d;
+    if (!few && d.out) {
+        // the tile loads take whole 16-byte chunks: rows that do not offer them are brought to that pitch first
+        const int Kp = round_up(d.K, epc);
+        if (!learn_aligned(d.x, d.ld_x * es, (int64_t)d.K * es)) {
+            HVS_TRY(launch_pack<DT>(st, d.x, d.ld_x, n, d.K, Kp, ws.packed_x));
+            dd.x = ws.packed_x;
+            dd.ld_x = Kp;
+        }
+        if (!learn_aligned(d.w, d.ldw * es, (int64_t)d.K * es)) {
+            HVS_TRY(launch_pack<DT>(st, d.w, d.ldw, d.N, d.K, Kp, ws.packed_w));
+            dd.w = ws.packed_w;
+            dd.ldw = Kp;
+        }
+    }
+    ShrinkParams s = {};
+    s.x = d.x, s.ld_x = d.ld_x, s.a = d.a, s.lda = d.lda;
+    s.n = n, s.K = d.K, s.r = ad->rank, s.rp = round_up(ad->rank, 16), s.S = ad->n_adapters, s.scale = ad->scale;
+    s.hidden = hidden;
+    ProjectParams p = {};
+    p.x = dd.x, p.ld_x = dd.ld_x, p.w = dd.w, p.ldw = dd.ldw, p.b = d.b, p.ldb = d.ldb, p.scale = ad->scale;
+    p.out = d.out, p.ld_out = d.ld_out, p.n = n, p.K = d.K, p.N = d.N, p.r = s.r, p.rp = s.rp, p.S = s.S;
+    if (few) {
+        if (!hidden) s.hidden = ws.hidden;
+        s.codes = codes;
+        HVS_TRY(launch_shrink<DT>(st, s, n < 16 ? n : 16));
+        if (!d.out) return 0;
+        p.codes = codes;
+        p.hidden = s.hidden;
+        return launch_few<DT>(st, p);
+    }
+    if (!grouped) HVS_TRY(launch_group(st, codes, n, s.S, ws));
+    s.codes = ws.scodes, s.order = ws.order;
+    if (d.out) s.u_hi = ws.u_hi, s.u_lo = ws.u_lo, s.factor = ws.factor;
+    HVS_TRY(launch_shrink<DT>(st, s, 2));
+    if (!d.out) return 0;
+    p.K = round_up(d.K, epc);  // whole chunks: K itself where rows were taken as they are, their padded width where they were packed
+    p.codes = ws.scodes, p.order = ws.order, p.u_hi = ws.u_hi, p.u_lo = ws.u_lo, p.factor = ws.factor;
+    p.b_aligned = learn_aligned(d.b, d.ldb * es, 0) && (d.b_padded || s.r % epc == 0);
+    p.out_vec = ((uintptr_t)d.out % (4 * es)) == 0 && (d.ld_out * es) % (4 * es) == 0;
+    if (DT == HVS_F32) return launch_tile<DT, Tile128>(st, p);
+    // the largest tile that still gives every CU one: a larger tile reads less per product, idle CUs cost more
+    auto tiles = [&](int t) { return (int64_t)((p.N + t - 1) / t) * ((n + t - 1) / t); };
+    if (tiles(256) >= 256) return launch_tile<DT, Tile256>(st, p);
+    if (tiles(128) >= 256) return launch_tile<DT, Tile128>(st, p);
+    return launch_tile<DT, Tile64>(st, p);
+}
+
+static int dispatch_direction(hipStream_t st, const hvs_adapters *ad, const Direction &d, const int32_t *codes, int n, float *hidden, AdapterWs &ws, bool grouped) {
+    if (ad->dtype == HVS_F32) return run_direction<HVS_F32>(st, ad, d, codes, n, hidden, ws, grouped);
+    if (ad->dtype == HVS_F16) return run_direction<HVS_F16>(st, ad, d, codes, n, hidden, ws, grouped);
+    return run_direction<HVS_BF16>(st, ad, d, codes, n, hidden, ws, grouped);
+}
+
+static int check_rows(const char *who, const char *what, const void *p, int64_t ld, int width, int es) {
+    HVS_REQUIRE(p != nullptr, "%s: %s is NULL", who, what);
+    HVS_REQUIRE(ld >= width, "%s: row pitch %lld of %s is below its %d columns", who, (long long)ld, what, width);
+    HVS_REQUIRE((uintptr_t)p % es == 0, "%s: %s is not aligned to its elements", who, what);
+    HVS_REQUIRE(ld <= ((int64_t)0x7FFFFFFF - 65536) / es - 8, "%s: row pitch %lld of %s is 2 GB or more", who, (long long)ld, what);
+    return 0;
+}
+static int check_workspace(const char *who, const hvs_adapters *ad, int64_t n, int64_t max_ld, int backward, const void *ws, uint64_t bytes) {
+    uint64_t need = 0;
+    HVS_TRY(hvs_adapters_workspace(ad, n, max_ld, backward, &need));
+    HVS_REQUIRE(ws != nullptr && ((uintptr_t)ws & 255) == 0 && bytes >= need, "%s: workspace of %llu bytes at %p, needs %llu aligned to 256", who,
+                (unsigned long long)bytes, ws, (unsigned long long)need);
+    return 0;
+}
+static int check_weights(const char *who, const hvs_adapters *ad) {
+    const int es = hvs_elem_size(ad->dtype);
+    HVS_REQUIRE(ad->projection && ad->a && ad->b && ad->scale, "%s: a weight is NULL", who);
+    HVS_REQUIRE((uintptr_t)ad->projection % es == 0 && (uintptr_t)ad->a % es == 0 && (uintptr_t)ad->b % es == 0 && (uintptr_t)ad->scale % 4 == 0,
+                "%s: a weight is not aligned to its elements", who);
+    return 0;
+}
+
+extern "C" int hvs_adapters_apply(int device_id, void *stream, const hvs_adapters *ad, const void *x, int64_t ld_x, const int32_t *codes, int64_t n,
+                                  void *out, int64_t ld_out, float *hidden, void *workspace, uint64_t workspace_bytes) {
+    const char *who = "hvs_adapters_apply";
+    HVS_TRY(check_adapters(who, ad));
+    HVS_REQUIRE(n >= 0, "%s: negative row count", who);
+    if (n == 0) return 0;
+    const int es = hvs_elem_size(ad->dtype);
+    HVS_TRY(check_weights(who, ad));
+    HVS_TRY(check_rows(who, "x", x, ld_x, ad->d_in, es));
+    HVS_TRY(check_rows(who, "out", out, ld_out, ad->d_out, es));
+    HVS_REQUIRE(codes != nullptr, "%s: codes is NULL", who);
+    HVS_REQUIRE(!learn_overlap(x, n, ld_x * es, (int64_t)ad->d_in * es, out, n, ld_out * es, (int64_t)ad->d_out * es), "%s: out overlaps x", who);
+    const int64_t max_ld = ld_x > ld_out ? ld_x : ld_out;
+    HVS_TRY(check_workspace(who, ad, n, max_ld, 0, workspace, workspace_bytes));
+    DeviceGuard guard(device_id);
+    HVS_HIP(guard.status);
+    const int64_t nc = chunk_rows(n, max_ld, es);
+    AdapterWs ws;
+    cut_workspace(ad, nc, 0, workspace, &ws);
+    for (int64_t r0 = 0; r0 < n; r0 += nc) {
+        const int rows = (int)(n - r0 < nc ? n - r0 : nc);
+        Direction d = {};
+        d.x = (const char *)x + r0 * ld_x * es, d.ld_x = ld_x;
+        d.a = ad->a, d.lda = ad->d_in, d.w = ad->projection, d.ldw = ad->d_in, d.b = ad->b, d.ldb = ad->rank;
+        d.K = ad->d_in, d.N = ad->d_out;
+        d.out = (char *)out + r0 * ld_out * es, d.ld_out = ld_out;
+        HVS_TRY(dispatch_direction((hipStream_t)stream, ad, d, codes + r0, rows, hidden ? hidden + r0 * ad->rank : nullptr, ws, false));
+    }
+    return 0;
+}
+
+template <int DT> static int launch_outer(hipStream_t st, OuterParams p) {
+    constexpr int EPC = Elem<DT>::EPC;
+    const int es = hvs_elem_size(DT);
+    const bool al = learn_aligned(p.x, p.ld_x * es, (int64_t)p.d * es);
+    const int tiles = (p.n + p.rows_per - 1) / p.rows_per, cols = (p.d + 16 * EPC - 1) / (16 * EPC);
+#define OUTER(RT_)                                                                                                           \
+    do {                                                                                                                     \
+        const dim3 grid(tiles, cols, (p.r + 16 * RT_ - 1) / (16 * RT_));                                                     \
+        if (al) outer_kernel<DT, RT_, true><<<grid, 256, 0, st>>>(p);                                                        \
+        else outer_kernel<DT, RT_, false><<<grid, 256, 0, st>>>(p);                                                          \
+    } while (0)
+    if (p.r <= 16) OUTER(1);
+    else if (p.r <= 32) OUTER(2);
+    else OUTER(4);
+#undef OUTER
+    const int64_t size = (int64_t)p.r * p.d;
+    const int by = (int)(size / 1024 < 1 ? 1 : (size / 1024 > 64 ? 64 : size / 1024));
+    outer_join_kernel<<<dim3(p.S, by), 256, 0, st>>>(p);
+    HVS_HIP(hipGetLastError());
+    return 0;
+}
+
+template <int DT>
+static int run_backward(hipStream_t st, const hvs_adapters *ad, const void *grad, int64_t ld_grad, const void *x, int64_t ld_x, const int32_t *codes,
+                        const float *hidden, int64_t n, void *grad_x, int64_t ld_gx, float *grad_a, float *grad_b, int64_t nc, AdapterWs &ws) {
+    const int es = hvs_elem_size(DT), epc = Elem<DT>::EPC, rp = round_up(ad->rank, 16);
+    const int dop = round_up(ad->d_out, epc);
+    // the weights of the transposed product; frozen W too is laid out by every call, so that nothing can be out of date
+    if (grad_x) {
+        HVS_TRY(launch_transpose<DT>(st, ad->projection, 1, ad->d_out, ad->d_in, dop, ws.w_t));
+        HVS_TRY(launch_transpose<DT>(st, ad->a, ad->n_adapters, ad->rank, ad->d_in, rp, ws.a_t));
+    }
+    HVS_TRY(launch_transpose<DT>(st, ad->b, ad->n_adapters, ad->d_out, ad->rank, dop, ws.b_t));
+    for (int64_t r0 = 0; r0 < n; r0 += nc) {
+        const int rows = (int)(n - r0 < nc ? n - r0 : nc);
+        HVS_TRY(launch_group(st, codes + r0, rows, ad->n_adapters, ws));
+        Direction d = {};
+        d.x = (const char *)grad + r0 * ld_grad * es, d.ld_x = ld_grad;
+        d.a = ws.b_t, d.lda = dop, d.w = ws.w_t, d.ldw = dop, d.b = ws.a_t, d.ldb = rp, d.b_padded = true;
+        d.K = ad->d_out, d.N = ad->d_in;
+        d.out = grad_x ? (char *)grad_x + r0 * ld_gx * es : nullptr, d.ld_out = ld_gx;
+        HVS_TRY(run_direction<DT>(st, ad, d, codes + r0, rows, ws.hidden, ws, true));
+        OuterParams o = {};
+        o.scodes = ws.scodes, o.order = ws.order, o.seg_begin = ws.seg_begin, o.scale = ad->scale, o.partial = ws.partial;
+        o.n = rows, o.r = ad->rank, o.S = ad->n_adapters, o.accumulate = r0 > 0;
+        o.q = ws.hidden, o.x = (const char *)x + r0 * ld_x * es, o.ld_x = ld_x, o.d = ad->d_in, o.out = grad_a, o.transposed = 0;
+        o.rows_per = outer_rows_per(rows, o.d, DT);
+        HVS_TRY(launch_outer<DT>(st, o));
+        o.q = hidden + r0 * ad->rank, o.x = d.x, o.ld_x = ld_grad, o.d = ad->d_out, o.out = grad_b, o.transposed = 1;
+        o.rows_per = outer_rows_per(rows, o.d, DT);
+        HVS_TRY(launch_outer<DT>(st, o));
+    }
+    return 0;
+}
+
+extern "C" int hvs_adapters_backward(int device_id, void *stream, const hvs_adapters *ad, const void *grad, int64_t ld_grad, const void *x, int64_t ld_x,
+                                     const int32_t *codes, const float *hidden, int64_t n, void *grad_x, int64_t ld_gx, float *grad_a, float *grad_b,
+                                     void *workspace, uint64_t workspace_bytes) {
+    const char *who = "hvs_adapters_backward";
+    HVS_TRY(check_adapters(who, ad));
+    HVS_REQUIRE(n >= 0, "%s: negative row count", who);
+    HVS_REQUIRE(grad_a && grad_b, "%s: grad_a or grad_b is NULL", who);
+    HVS_REQUIRE((uintptr_t)grad_a % 4 == 0 && (uintptr_t)grad_b % 4 == 0, "%s: grad_a or grad_b is not aligned to its elements", who);
+    hipStream_t st = (hipStream_t)stream;
+    const int64_t size_a = (int64_t)ad->n_adapters * ad->rank * ad->d_in, size_b = (int64_t)ad->n_adapters * ad->rank * ad->d_out;
+    if (n == 0) {
+        DeviceGuard guard(device_id);
+        HVS_HIP(guard.status);
+        fill_zero_kernel<<<1024, 256, 0, st>>>(grad_a, size_a);
+        fill_zero_kernel<<<1024, 256, 0, st>>>(grad_b, size_b);
+        HVS_HIP(hipGetLastError());
+        return 0;
+    }
+    const int es = hvs_elem_size(ad->dtype);
+    HVS_TRY(check_weights(who, ad));
+    HVS_TRY(check_rows(who, "grad", grad, ld_grad, ad->d_out, es));
+    HVS_TRY(check_rows(who, "x", x, ld_x, ad->d_in, es));
+    HVS_REQUIRE(codes && hidden, "%s: codes or hidden is NULL", who);
+    int64_t max_ld = ld_grad > ld_x ? ld_grad : ld_x;
+    if (grad_x) {
+        HVS_TRY(check_rows(who, "grad_x", grad_x, ld_gx, ad->d_in, es));
+        HVS_REQUIRE(!learn_overlap(grad, n, ld_grad * es, (int64_t)ad->d_out * es, grad_x, n, ld_gx * es, (int64_t)ad->d_in * es) &&
+                        !learn_overlap(x, n, ld_x * es, (int64_t)ad->d_in * es, grad_x, n, ld_gx * es, (int64_t)ad->d_in * es),
+                    "%s: grad_x overlaps an input", who);
+        max_ld = max_ld > ld_gx ? max_ld : ld_gx;
+    }
+    HVS_TRY(check_workspace(who, ad, n, max_ld, 1, workspace, workspace_bytes));
+    DeviceGuard guard(device_id);
+    HVS_HIP(guard.status);
+    const int64_t nc = chunk_rows(n, max_ld, es);
+    AdapterWs ws;
+    cut_workspace(ad, nc, 1, workspace, &ws);
+    if (ad->dtype == HVS_F32) return run_backward<HVS_F32>(st, ad, grad, ld_grad, x, ld_x, codes, hidden, n, grad_x, ld_gx, grad_a, grad_b, nc, ws);
+    if (ad->dtype == HVS_F16) return run_backward<HVS_F16>(st, ad, grad, ld_grad, x, ld_x, codes, hidden, n, grad_x, ld_gx, grad_a, grad_b, nc, ws);
+    return run_backward<HVS_BF16>(st, ad, grad, ld_grad, x, ld_x, codes, hidden, n, grad_x, ld_gx, grad_a, grad_b, nc, ws);
+}

@@ -1,0 +1,606 @@
+// The loss that query adapters are trained with, and the clipping of their gradients (C ABI: include/hvs.h).
+#include <algorithm>
+#include <new>
+#include <utility>
+#include <vector>
+
+#include "hvs_learn.h"
+
+// ---------------------------------------------------------------------------------------------------------------
+// preference loss
+// ---------------------------------------------------------------------------------------------------------------
+// With c^ = c / |c| etc. and s = cos(y, c) - cos(y, r):  d s / d y = (c^ - r^ - s y^) / |y|, so the gradient of a query is
+//     (sum_p g_p (c^_p - r^_p)  -  (sum_p g_p s_p) y^) / |y|,   g_p = w_p beta (e sigma(h_p) - (1 - e) sigma(-h_p)):
+// one vector and one number are kept over the pairs of a query, and every row is read once.
+struct PreferenceParams {
+    const void *y, *ref;
+    int64_t ld_y, ld_ref;
+    const int64_t *offsets, *chosen, *rejected;
+    const float *weights;
+    float *loss, *margin;
+    void *grad;
+    int64_t ld_grad;
+    int64_t n_pairs;
+    const void *rows;
+    int64_t ld_rows, n_rows;
+    int dim;
+    float beta, smoothing, default_weight;
+    float *part_vec;  // [n_queries][shares][dim] sums of queries that several blocks work on
+    float *part_num;  // [n_queries][shares]
+    int per_block;    // pairs a block takes before a second one joins in
+};
+
+// eight consecutive elements of a row as fp32, zeros past its end
+template <int DT, bool ALIGNED> __device__ __forceinline__ void load8(const void *base, int64_t row, int64_t ld, int k, int dim, float *out) {
+    typedef typename Elem<DT>::type E;
+    constexpr int EPC = Elem<DT>::EPC;
+    const E *p = reinterpret_cast<const E *>(base) + row * ld;
+#pragma unroll
+    for (int i = 0; i < 8; i += EPC) chunk_to_float<DT>(load_chunk<DT, ALIGNED>(p, k + i, dim), out + i);
+}
+
+__device__ __forceinline__ float softplus(float z) { return fmaxf(z, 0.0f) + log1pf(expf(-fabsf(z))); }
+__device__ __forceinline__ float inverse_norm(float sum_of_squares) { return sum_of_squares == 0.0f ? 0.0f : 1.0f / sqrtf(sum_of_squares); }
+
+// a x - b y with each product rounded by itself: equal pairs give exactly 0, which a fused multiply-add would not
+__device__ __forceinline__ float product_difference(float a, float x, float b, float y) {
+#pragma clang fp contract(off)
+    const float ax = a * x, by = b * y;
+    return ax - by;
+}
+
+// how the pairs [b0, b1) of a query are shared out; the same on every side that asks
+__device__ __forceinline__ void pair_share(const PreferenceParams &p, int64_t q, int shares, int64_t &b0, int64_t &b1, int64_t &per, int &used) {
+    b0 = p.offsets[q];
+    b1 = p.offsets[q + 1];
+    b0 = b0 < 0 ? 0 : (b0 > p.n_pairs ? p.n_pairs : b0);
+    b1 = b1 < b0 ? b0 : (b1 > p.n_pairs ? p.n_pairs : b1);
+    const int64_t len = b1 - b0;
+    per = (len + shares - 1) / shares;
+    per = per < p.per_block ? p.per_block : per;
+    used = len > 0 ? (int)((len + per - 1) / per) : 1;
+}
+
+// A team of TW waves holds a whole row in registers, CH x 8 elements a lane: the query, the reference query, the two rows
+// of the pair at hand and the gradient sum.  The block's teams take the pairs of its share in turn and add up in team order.
+template <int QDT, int RDT, int CH, int TW, int WAVES, bool ALIGNED>
+__global__ __launch_bounds__(64 * WAVES) void preference_kernel(PreferenceParams p) {
+    typedef typename Elem<QDT>::type Q;
+    constexpr int TEAMS = WAVES / TW, NE = CH * 8;
+    extern __shared__ float vec[];  // [dim]
+    __shared__ float sums[WAVES][8];
+    __shared__ float num[TEAMS];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int team = wave / TW, tl = (wave % TW) * 64 + lane;
+    const int64_t q = blockIdx.x;
+    const int z = blockIdx.y, shares = gridDim.y;
+    int64_t b0, b1, per;
+    int used;
+    pair_share(p, q, shares, b0, b1, per, used);
+    if (z >= used) return;
+    const int64_t lo = b0 + z * per, hi = lo + per < b1 ? lo + per : b1;
+
+    // sums over a team's elements, the same value in every lane
+    auto team_sum = [&](float *v, int count) {
+#pragma unroll 8
+        for (int i = 0; i < count; i++) v[i] = learn_wave_sum(v[i]);
+        if (TW > 1) {
+            __syncthreads();
+            if (lane == 0)
+                for (int i = 0; i < count; i++) sums[wave][i] = v[i];
+            __syncthreads();
+            for (int i = 0; i < count; i++) {
+                v[i] = 0.0f;
+#pragma unroll
+                for (int w = 0; w < TW; w++) v[i] += sums[team * TW + w][i];
+            }
+        }
+    };
+
+    float y[NE], f[NE], g[NE];
+    float norms[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int c = 0; c < CH; c++) {
+        const int k = (c * TW * 64 + tl) * 8;
+        load8<QDT, ALIGNED>(p.y, q, p.ld_y, k, p.dim, y + c * 8);
+        if (p.ref) load8<QDT, ALIGNED>(p.ref, q, p.ld_ref, k, p.dim, f + c * 8);
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            if (!p.ref) f[c * 8 + i] = 0.0f;
+            norms[0] = fmaf(y[c * 8 + i], y[c * 8 + i], norms[0]);
+            norms[1] = fmaf(f[c * 8 + i], f[c * 8 + i], norms[1]);
+            g[c * 8 + i] = 0.0f;
+        }
+    }
+    team_sum(norms, 2);
+    const float inv_y = inverse_norm(norms[0]), inv_f = inverse_norm(norms[1]);
+    float total = 0.0f;  // sum of g_p s_p
+
+    for (int64_t i = lo + team; i < hi; i += TEAMS) {
+        const int64_t a = p.chosen[i], b = p.rejected[i];
+        if (a < 0 || b < 0 || a >= p.n_rows || b >= p.n_rows) {
+            const bool left_out = a < 0 || b < 0;
+            const float v = left_out ? 0.0f : __builtin_nanf("");
+            if (tl == 0) p.loss[i] = p.margin[i] = v;
+            total += v;
+            continue;
+        }
+        float ra[NE], rb[NE];
+#pragma unroll
+        for (int c = 0; c < CH; c++) {
+            const int k = (c * TW * 64 + tl) * 8;
+            load8<RDT, ALIGNED>(p.rows, a, p.ld_rows, k, p.dim, ra + c * 8);
+            load8<RDT, ALIGNED>(p.rows, b, p.ld_rows, k, p.dim, rb + c * 8);
+        }
+        float s[6] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int e = 0; e < NE; e++) {
+            s[0] = fmaf(y[e], ra[e], s[0]);
+            s[1] = fmaf(y[e], rb[e], s[1]);
+            s[2] = fmaf(ra[e], ra[e], s[2]);
+            s[3] = fmaf(rb[e], rb[e], s[3]);
+            s[4] = fmaf(f[e], ra[e], s[4]);
+            s[5] = fmaf(f[e], rb[e], s[5]);
+        }
+        team_sum(s, 6);
+        const float ia = inverse_norm(s[2]), ib = inverse_norm(s[3]);
+        const float cos = inv_y * product_difference(s[0], ia, s[1], ib);
+        const float m = product_difference(1.0f, cos, inv_f, product_difference(s[4], ia, s[5], ib));
+        const float h = p.beta * m, e = p.smoothing;
+        const float up = 1.0f / (1.0f + expf(-h)), down = 1.0f / (1.0f + expf(h));  // sigma(h), sigma(-h): each without cancellation
+        if (tl == 0) {
+            p.loss[i] = (1.0f - e) * softplus(-h) + e * softplus(h);
+            p.margin[i] = m;
+        }
+        const float w = (p.weights ? p.weights[i] : p.default_weight) * p.beta * (e * up - (1.0f - e) * down);
+        total = fmaf(w, cos, total);
+        const float wa = w * ia, wb = w * ib;
+#pragma unroll
+        for (int k = 0; k < NE; k++) g[k] = fmaf(wa, ra[k], fmaf(-wb, rb[k], g[k]));
+    }
+
+    // the teams that had pairs, in team order
+    const int busy = TEAMS == 1 ? 1 : (hi - lo < TEAMS ? (hi - lo > 0 ? (int)(hi - lo) : 1) : TEAMS);
+    if (tl == 0) num[team] = total;
+    for (int t = 0; t < busy; t++) {
+        if (team == t) {
+#pragma unroll
+            for (int c = 0; c < CH; c++) {
+                const int k = (c * TW * 64 + tl) * 8;
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    if (k + i < p.dim) vec[k + i] = t == 0 ? g[c * 8 + i] : vec[k + i] + g[c * 8 + i];
+            }
+        }
+        __syncthreads();
+    }
+    float sum = 0.0f;
+    for (int t = 0; t < busy; t++) sum += num[t];
+    if (used == 1) {
+        const Q *yr = reinterpret_cast<const Q *>(p.y) + q * p.ld_y;
+        Q *out = reinterpret_cast<Q *>(p.grad) + q * p.ld_grad;
+        for (int k = tid; k < p.dim; k += 64 * WAVES) out[k] = learn_from_float<Q>(inv_y * (vec[k] - sum * inv_y * learn_to_float(yr[k])));
+    } else {
+        float *pv = p.part_vec + (q * shares + z) * p.dim;
+        for (int k = tid; k < p.dim; k += 64 * WAVES) pv[k] = vec[k];
+        if (tid == 0) p.part_num[q * shares + z] = sum;
+    }
+}
+
+// queries whose pairs several blocks shared: their sums in share order
+template <int QDT> __global__ __launch_bounds__(256) void preference_join_kernel(PreferenceParams p, int shares) {
+    typedef typename Elem<QDT>::type Q;
+    __shared__ float part[4];
+    const int64_t q = blockIdx.x;
+    int64_t b0, b1, per;
+    int used;
+    pair_share(p, q, shares, b0, b1, per, used);
+    if (used == 1) return;
+    const Q *y = reinterpret_cast<const Q *>(p.y) + q * p.ld_y;
+    Q *out = reinterpret_cast<Q *>(p.grad) + q * p.ld_grad;
+    float yy = 0.0f;
+    for (int k = threadIdx.x; k < p.dim; k += 256) {
+        const float v = learn_to_float(y[k]);
+        yy = fmaf(v, v, yy);
+    }
+    yy = learn_wave_sum(yy);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = yy;
+    __syncthreads();
+    const float inv_y = inverse_norm(part[0] + part[1] + part[2] + part[3]);
+    float sum = 0.0f;
+    for (int z = 0; z < used; z++) sum += p.part_num[q * shares + z];
+    for (int k = threadIdx.x; k < p.dim; k += 256) {
+        float v = 0.0f;
+        for (int z = 0; z < used; z++) v += p.part_vec[(q * shares + z) * p.dim + k];
+        out[k] = learn_from_float<Q>(inv_y * (v - sum * inv_y * learn_to_float(y[k])));
+    }
+}
+
+#define PREF_FEW 512      // queries up to which a block has 16 waves and several blocks may share a query's pairs
+#define PREF_BLOCKS 1024  // ... so that about this many blocks are launched
+#define PREF_WAVE_DIM 2048
+
+static int preference_shares(const hvs_preference *p) {
+    if (p->n_queries < 1 || p->n_queries >= PREF_FEW || p->n_pairs <= 16) return 1;
+    const int64_t by_blocks = PREF_BLOCKS / p->n_queries, by_pairs = (p->n_pairs + 15) / 16;
+    return (int)(by_blocks < by_pairs ? by_blocks : by_pairs);
+}
+
+static int check_preference(const char *who, const hvs_preference *p, int dim) {
+    HVS_REQUIRE(p != nullptr, "%s: NULL argument", who);
+    HVS_REQUIRE(learn_dtype_ok(p->query_dtype), "%s: unknown query dtype %d", who, p->query_dtype);
+    HVS_REQUIRE(dim >= 1 && dim <= 16384, "%s: dim %d not in [1, 16384]", who, dim);
+    HVS_REQUIRE(p->n_queries >= 0 && p->n_pairs >= 0, "%s: negative count", who);
+    HVS_REQUIRE(p->n_queries <= 0x7FFFFFFF, "%s: %lld queries, at most 2^31 - 1", who, (long long)p->n_queries);
+    HVS_REQUIRE(p->beta > 0.0f && std::isfinite(p->beta), "%s: beta %g must be positive and finite", who, (double)p->beta);
+    HVS_REQUIRE(p->label_smoothing >= 0.0f && p->label_smoothing <= 0.5f, "%s: label_smoothing %g not in [0, 0.5]", who, (double)p->label_smoothing);
+    return 0;
+}
+
+extern "C" int hvs_preference_workspace(const hvs_preference *p, int dim, uint64_t *out_bytes) {
+    HVS_TRY(check_preference("hvs_preference_workspace", p, dim));
+    HVS_REQUIRE(out_bytes != nullptr, "hvs_preference_workspace: NULL argument");
+    const int shares = preference_shares(p);
+    WorkspaceCut w(nullptr);
+    if (shares > 1) {
+        w.take<float>((uint64_t)p->n_queries * shares * dim * 4);
+        w.take<float>((uint64_t)p->n_queries * shares * 4);
+    }
+    *out_bytes = w.used;
+    return 0;
+}
+
+template <int QDT, int RDT, int CH, int TW, int WAVES>
+static int launch_preference(hipStream_t st, const PreferenceParams &p, int64_t nq, int shares, bool aligned) {
+    const dim3 grid((unsigned)nq, shares);
+    const size_t lds = (size_t)p.dim * 4;
+    if (aligned) {
+        if (lds > 48 * 1024)
+            HVS_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(&preference_kernel<QDT, RDT, CH, TW, WAVES, true>),
+                                        hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+        preference_kernel<QDT, RDT, CH, TW, WAVES, true><<<grid, 64 * WAVES, lds, st>>>(p);
+    } else {
+        if (lds > 48 * 1024)
+            HVS_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(&preference_kernel<QDT, RDT, CH, TW, WAVES, false>),
+                                        hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+        preference_kernel<QDT, RDT, CH, TW, WAVES, false><<<grid, 64 * WAVES, lds, st>>>(p);
+    }
+    HVS_HIP(hipGetLastError());
+    return 0;
+}
+
+template <int QDT, int RDT> static int run_preference(hipStream_t st, const PreferenceParams &p, int64_t nq, int shares) {
+    const int qs = hvs_elem_size(QDT), rs = hvs_elem_size(RDT);
+    const bool al = p.dim % 8 == 0 && learn_aligned(p.y, p.ld_y * qs, 0) && (!p.ref || learn_aligned(p.ref, p.ld_ref * qs, 0)) &&
+                    learn_aligned(p.rows, p.ld_rows * rs, 0);
+    if (p.dim > 8192) HVS_TRY((launch_preference<QDT, RDT, 2, 16, 16>(st, p, nq, shares, al)));
+    else if (p.dim > PREF_WAVE_DIM) HVS_TRY((launch_preference<QDT, RDT, 1, 16, 16>(st, p, nq, shares, al)));
+    else {
+        const int ch = (p.dim + 511) / 512;
+        // few queries: 16 waves a block, so that the pairs of one query are in flight together
+#define PREF(CH_) (nq < PREF_FEW ? launch_preference<QDT, RDT, CH_, 1, 16>(st, p, nq, shares, al) : launch_preference<QDT, RDT, CH_, 1, 4>(st, p, nq, shares, al))
+        if (ch == 1) HVS_TRY(PREF(1));
+        else if (ch == 2) HVS_TRY(PREF(2));
+        else if (ch == 3) HVS_TRY(PREF(3));
+        else HVS_TRY(PREF(4));
+#undef PREF
+    }
+    if (shares > 1) {
+        preference_join_kernel<QDT><<<(unsigned)nq, 256, 0, st>>>(p, shares);
+        HVS_HIP(hipGetLastError());
+    }
+    return 0;
+}
+
+static int preference_core(const char *who, hipStream_t st, const hvs_preference *p, const void *rows, int rows_dtype, int dim, int64_t ld_rows,
+                           int64_t n_rows, void *workspace, uint64_t workspace_bytes) {
+    const int qs = hvs_elem_size(p->query_dtype);
+    HVS_REQUIRE(p->queries && p->grad && p->offsets, "%s: queries, grad or offsets is NULL", who);
+    HVS_REQUIRE(p->n_pairs == 0 || (p->chosen && p->rejected && p->loss && p->margin), "%s: chosen, rejected, loss or margin is NULL", who);
+    HVS_REQUIRE(n_rows >= 0 && (n_rows == 0 || rows), "%s: rows is NULL or n_rows negative", who);
+    HVS_REQUIRE(p->ld_queries >= dim && p->ld_grad >= dim && ld_rows >= dim && (!p->reference || p->ld_reference >= dim), "%s: a row pitch is below dim %d", who, dim);
+    HVS_REQUIRE((uintptr_t)p->queries % qs == 0 && (uintptr_t)p->reference % qs == 0 && (uintptr_t)p->grad % qs == 0 &&
+                    (uintptr_t)rows % hvs_elem_size(rows_dtype) == 0,
+                "%s: a tensor is not aligned to its elements", who);
+    HVS_REQUIRE(!learn_overlap(p->queries, p->n_queries, p->ld_queries * qs, (int64_t)dim * qs, p->grad, p->n_queries, p->ld_grad * qs, (int64_t)dim * qs) &&
+                    !(p->reference && learn_overlap(p->reference, p->n_queries, p->ld_reference * qs, (int64_t)dim * qs, p->grad, p->n_queries, p->ld_grad * qs,
+                                                    (int64_t)dim * qs)),
+                "%s: grad overlaps an input", who);
+    uint64_t need = 0;
+    HVS_TRY(hvs_preference_workspace(p, dim, &need));
+    HVS_REQUIRE(need == 0 || (workspace && ((uintptr_t)workspace & 255) == 0 && workspace_bytes >= need),
+                "%s: workspace of %llu bytes at %p, needs %llu aligned to 256", who, (unsigned long long)workspace_bytes, workspace, (unsigned long long)need);
+    const int shares = preference_shares(p);
+    PreferenceParams k = {};
+    k.y = p->queries, k.ref = p->reference, k.ld_y = p->ld_queries, k.ld_ref = p->ld_reference;
+    k.offsets = p->offsets, k.chosen = p->chosen, k.rejected = p->rejected, k.weights = p->weights;
+    k.loss = p->loss, k.margin = p->margin, k.grad = p->grad, k.ld_grad = p->ld_grad, k.n_pairs = p->n_pairs;
+    k.rows = rows, k.ld_rows = ld_rows, k.n_rows = n_rows, k.dim = dim;
+    k.beta = p->beta, k.smoothing = p->label_smoothing, k.default_weight = p->n_pairs > 0 ? (float)(1.0 / (double)p->n_pairs) : 0.0f;
+    k.per_block = 16;
+    if (shares > 1) {
+        WorkspaceCut w(workspace);
+        k.part_vec = w.take<float>((uint64_t)p->n_queries * shares * dim * 4);
+        k.part_num = w.take<float>((uint64_t)p->n_queries * shares * 4);
+    }
+#define ROWS(Q_)                                                                             \
+    (rows_dtype == HVS_F32 ? run_preference<Q_, HVS_F32>(st, k, p->n_queries, shares)        \
+                           : rows_dtype == HVS_F16 ? run_preference<Q_, HVS_F16>(st, k, p->n_queries, shares) \
+                                                   : run_preference<Q_, HVS_BF16>(st, k, p->n_queries, shares))
+    if (p->query_dtype == HVS_F32) return ROWS(HVS_F32);
+    if (p->query_dtype == HVS_F16) return ROWS(HVS_F16);
+    return ROWS(HVS_BF16);
+#undef ROWS
+}
+
+extern "C" int hvs_preference_loss(int device_id, void *stream, const hvs_preference *p, const void *rows, int rows_dtype, int dim, int64_t ld_rows,
+                                   int64_t n_rows, void *workspace, uint64_t workspace_bytes) {
+    const char *who = "hvs_preference_loss";
+    HVS_TRY(check_preference(who, p, dim));
+    HVS_REQUIRE(learn_dtype_ok(rows_dtype), "%s: unknown row dtype %d", who, rows_dtype);
+    if (p->n_queries == 0) {
+        HVS_REQUIRE(p->n_pairs == 0, "%s: %lld pairs but no query", who, (long long)p->n_pairs);
+        return 0;
+    }
+    DeviceGuard guard(device_id);
+    HVS_HIP(guard.status);
+    return preference_core(who, (hipStream_t)stream, p, rows, rows_dtype, dim, ld_rows, n_rows, workspace, workspace_bytes);
+}
+
+// `to` waits for the work `from` holds now
+static int stream_after(hipStream_t to, hipStream_t from) {
+    hipEvent_t ev;
+    HVS_HIP(hipEventCreateWithFlags(&ev, hipEventDisableTiming));
+    hipError_t e = hipEventRecord(ev, from);
+    if (e == hipSuccess) e = hipStreamWaitEvent(to, ev, 0);
+    (void)hipEventDestroy(ev);  // released once the wait is done
+    HVS_HIP(e);
+    return 0;
+}
+
+extern "C" int hvs_index_preference_loss(hvs_index *idx, void *stream, const hvs_preference *p, void *workspace, uint64_t workspace_bytes) {
+    const char *who = "hvs_index_preference_loss";
+    HVS_REQUIRE(idx != nullptr, "%s: idx is NULL", who);
+    HVS_TRY(check_preference(who, p, idx->dim));
+    if (p->n_queries == 0) {
+        HVS_REQUIRE(p->n_pairs == 0, "%s: %lld pairs but no query", who, (long long)p->n_pairs);
+        return 0;
+    }
+    DeviceGuard guard(idx->device);
+    HVS_HIP(guard.status);
+    hipStream_t st = (hipStream_t)stream;
+    hipStreamCaptureStatus capturing = hipStreamCaptureStatusNone;
+    if (st != nullptr) HVS_HIP(hipStreamIsCapturing(st, &capturing));
+    HVS_REQUIRE(capturing == hipStreamCaptureStatusNone, "%s: the stream is being captured; a graph would keep the address of rows the table may move", who);
+    if (st != idx->stream) HVS_TRY(stream_after(st, idx->stream));
+    HVS_TRY(preference_core(who, st, p, idx->rows, idx->dtype, idx->dim, idx->ld, idx->n, workspace, workspace_bytes));
+    if (st != idx->stream) HVS_TRY(stream_after(idx->stream, st));
+    return 0;
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// global norm and clipping
+// ---------------------------------------------------------------------------------------------------------------
+#define CLIP_BATCH 64      // tensors per launch: their table travels in the kernel's arguments
+#define CLIP_CHUNK 8192    // elements a block takes at a time
+#define CLIP_BLOCKS 1024   // blocks of a norm launch, one partial sum each
+
+struct ClipTable {
+    const void *data[CLIP_BATCH];
+    void *out[CLIP_BATCH];
+    int64_t numel[CLIP_BATCH];
+    uint32_t first_chunk[CLIP_BATCH + 1];
+    int32_t dtype[CLIP_BATCH];
+    int n;
+};
+
+// two partial results of a norm: sums of squares add up, largest values do not, a NaN stays
+__device__ __forceinline__ double norm_join(double a, double b, bool inf_norm) {
+    if (!inf_norm) return a + b;
+    return a != a || b != b ? __builtin_nan("") : (a > b ? a : b);
+}
+__device__ __forceinline__ double block_join(double v, bool inf_norm, double *lds) {
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) v = norm_join(v, __shfl_xor(v, o), inf_norm);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return norm_join(norm_join(lds[0], lds[1], inf_norm), norm_join(lds[2], lds[3], inf_norm), inf_norm);
+}
+
+__device__ __forceinline__ int clip_tensor_of(const ClipTable &t, uint32_t chunk) {
+    int lo = 0, hi = t.n;  // the last tensor whose first chunk is not past this one
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (t.first_chunk[mid] <= chunk) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+template <int DT> __device__ __forceinline__ double chunk_norm(const void *data, int64_t begin, int64_t end, bool inf_norm) {
+    typedef typename Elem<DT>::type E;
+    constexpr int EPC = Elem<DT>::EPC;
+    const E *p = reinterpret_cast<const E *>(data);
+    double acc = 0.0;
+    auto add = [&](float v) { acc = inf_norm ? norm_join(acc, (double)fabsf(v), true) : fma((double)v, (double)v, acc); };
+    int64_t i = begin;
+    if (((uintptr_t)data & 15) == 0) {
+        const int64_t whole = begin + ((end - begin) / EPC) * EPC;
+        for (i = begin + threadIdx.x * EPC; i < whole; i += 256 * EPC) {
+            float v[EPC];
+            chunk_to_float<DT>(*reinterpret_cast<const f32x4 *>(p + i), v);
+#pragma unroll
+            for (int e = 0; e < EPC; e++) add(v[e]);
+        }
+        i = whole;
+    }
+    for (i += threadIdx.x; i < end; i += 256) add(learn_to_float(p[i]));
+    return acc;
+}
+
+__global__ __launch_bounds__(256) void clip_norm_kernel(ClipTable t, int inf_norm, double *__restrict__ partial) {
+    __shared__ double lds[4];
+    double acc = 0.0;
+    for (uint32_t c = blockIdx.x; c < t.first_chunk[t.n]; c += gridDim.x) {
+        const int k = clip_tensor_of(t, c);
+        const int64_t begin = (int64_t)(c - t.first_chunk[k]) * CLIP_CHUNK;
+        const int64_t end = begin + CLIP_CHUNK < t.numel[k] ? begin + CLIP_CHUNK : t.numel[k];
+        const double v = t.dtype[k] == HVS_F32   ? chunk_norm<HVS_F32>(t.data[k], begin, end, inf_norm)
+                         : t.dtype[k] == HVS_F16 ? chunk_norm<HVS_F16>(t.data[k], begin, end, inf_norm)
+                                                 : chunk_norm<HVS_BF16>(t.data[k], begin, end, inf_norm);
+        acc = norm_join(acc, v, inf_norm);
+    }
+    acc = block_join(acc, inf_norm, lds);
+    if (threadIdx.x == 0) partial[blockIdx.x] = acc;
+}
+
+template <int DT> __device__ __forceinline__ void chunk_scale(const void *data, void *out, int64_t begin, int64_t end, float f) {
+    typedef typename Elem<DT>::type E;
+    constexpr int EPC = Elem<DT>::EPC;
+    typedef E vec __attribute__((ext_vector_type(EPC)));
+    const E *p = reinterpret_cast<const E *>(data);
+    E *o = reinterpret_cast<E *>(out);
+    int64_t i = begin;
+    if (((uintptr_t)data & 15) == 0 && ((uintptr_t)out & 15) == 0) {
+        const int64_t whole = begin + ((end - begin) / EPC) * EPC;
+        for (i = begin + threadIdx.x * EPC; i < whole; i += 256 * EPC) {
+            float v[EPC];
+            chunk_to_float<DT>(*reinterpret_cast<const f32x4 *>(p + i), v);
+            vec r;
+#pragma unroll
+            for (int e = 0; e < EPC; e++) r[e] = learn_from_float<E>(v[e] * f);
+            *reinterpret_cast<vec *>(o + i) = r;
+        }
+        i = whole;
+    }
+    for (i += threadIdx.x; i < end; i += 256) o[i] = learn_from_float<E>(learn_to_float(p[i]) * f);
+}
+
+// Every block adds up the partial sums itself (the same order everywhere), then scales its chunks.
+__global__ __launch_bounds__(256) void clip_scale_kernel(ClipTable t, int inf_norm, const double *__restrict__ partial, int n_partial, double max_norm,
+                                                         float *__restrict__ norm_out, int write_norm) {
+    __shared__ double lds[4];
+    double acc = 0.0;
+    for (int i = threadIdx.x; i < n_partial; i += 256) acc = norm_join(acc, partial[i], inf_norm);
+    acc = block_join(acc, inf_norm, lds);
+    const float norm = (float)(inf_norm ? acc : sqrt(acc));
+    if (write_norm && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = norm;
+    float f = norm != norm ? norm : (max_norm < __builtin_inf() ? (float)fmin(max_norm / ((double)norm + 1e-6), 1.0) : 1.0f);
+    for (uint32_t c = blockIdx.x; c < t.first_chunk[t.n]; c += gridDim.x) {
+        const int k = clip_tensor_of(t, c);
+        if (f == 1.0f && t.out[k] == t.data[k]) continue;  // in place and nothing to clip: the tensor is its own result
+        const int64_t begin = (int64_t)(c - t.first_chunk[k]) * CLIP_CHUNK;
+        const int64_t end = begin + CLIP_CHUNK < t.numel[k] ? begin + CLIP_CHUNK : t.numel[k];
+        if (t.dtype[k] == HVS_F32) chunk_scale<HVS_F32>(t.data[k], t.out[k], begin, end, f);
+        else if (t.dtype[k] == HVS_F16) chunk_scale<HVS_F16>(t.data[k], t.out[k], begin, end, f);
+        else chunk_scale<HVS_BF16>(t.data[k], t.out[k], begin, end, f);
+    }
+}
+
+static int check_tensors(const char *who, const hvs_tensor *t, int n) {
+    HVS_REQUIRE(n >= 0 && (n == 0 || t), "%s: negative tensor count or NULL argument", who);
+    for (int i = 0; i < n; i++) {
+        HVS_REQUIRE(learn_dtype_ok(t[i].dtype), "%s: tensor %d: unknown dtype %d", who, i, t[i].dtype);
+        HVS_REQUIRE(t[i].numel >= 0 && t[i].numel <= (int64_t)1 << 40, "%s: tensor %d: %lld elements, must be in [0, 2^40]", who, i, (long long)t[i].numel);
+        if (t[i].numel == 0) continue;
+        const int es = hvs_elem_size(t[i].dtype);
+        HVS_REQUIRE(t[i].data && t[i].out, "%s: tensor %d is NULL", who, i);
+        HVS_REQUIRE((uintptr_t)t[i].data % es == 0 && (uintptr_t)t[i].out % es == 0, "%s: tensor %d is not aligned to its elements", who, i);
+        HVS_REQUIRE(t[i].data == t[i].out || !learn_overlap(t[i].data, 1, 0, t[i].numel * es, t[i].out, 1, 0, t[i].numel * es),
+                    "%s: tensor %d: out overlaps data without being data", who, i);
+    }
+    return 0;
+}
+
+// No tensor may be written while another one is read or written: a tensor named twice would be scaled twice.
+struct ClipRange {
+    uintptr_t begin, end;
+    bool written;
+};
+static int check_apart(const char *who, const hvs_tensor *t, int n) {
+    std::vector<ClipRange> r;
+    try {
+        r.reserve(2 * (size_t)n);
+    } catch (const std::bad_alloc &) {
+        hvs_set_error("%s: out of host memory", who);
+        return 1;
+    }
+    for (int i = 0; i < n; i++) {
+        const uintptr_t bytes = (uintptr_t)t[i].numel * hvs_elem_size(t[i].dtype);
+        if (bytes == 0) continue;
+        r.push_back({(uintptr_t)t[i].out, (uintptr_t)t[i].out + bytes, true});
+        if (t[i].data != t[i].out) r.push_back({(uintptr_t)t[i].data, (uintptr_t)t[i].data + bytes, false});
+    }
+    std::sort(r.begin(), r.end(), [](const ClipRange &a, const ClipRange &b) { return a.begin < b.begin; });
+    uintptr_t any_end = 0, written_end = 0;  // how far the ranges so far reach
+    for (const ClipRange &c : r) {
+        HVS_REQUIRE(c.begin >= (c.written ? any_end : written_end), "%s: two tensors share memory", who);
+        any_end = any_end > c.end ? any_end : c.end;
+        if (c.written) written_end = written_end > c.end ? written_end : c.end;
+    }
+    return 0;
+}
+
+// chunks of the tensors of one launch; at most 64 x 2^27, so they are counted in 64 bits and the caller splits the launch
+static int fill_table(const hvs_tensor *t, int n, int at, ClipTable *tab) {
+    tab->n = 0;
+    tab->first_chunk[0] = 0;
+    while (at < n && tab->n < CLIP_BATCH) {
+        const uint64_t chunks = ((uint64_t)t[at].numel + CLIP_CHUNK - 1) / CLIP_CHUNK;
+        const uint64_t end = tab->first_chunk[tab->n] + chunks;
+        if (end > 0x7FFFFFFFull) break;  // 2^40 elements are 2^27 chunks: at least one tensor always fits
+        tab->data[tab->n] = t[at].data, tab->out[tab->n] = t[at].out, tab->numel[tab->n] = t[at].numel, tab->dtype[tab->n] = t[at].dtype;
+        tab->first_chunk[++tab->n] = (uint32_t)end;
+        at++;
+    }
+    return at;
+}
+
+extern "C" int hvs_clip_workspace(const hvs_tensor *tensors, int n_tensors, uint64_t *out_bytes) {
+    HVS_TRY(check_tensors("hvs_clip_workspace", tensors, n_tensors));
+    HVS_REQUIRE(out_bytes != nullptr, "hvs_clip_workspace: NULL argument");
+    ClipTable tab;
+    uint64_t partials = 0;
+    for (int at = 0; at < n_tensors;) {
+        at = fill_table(tensors, n_tensors, at, &tab);
+        partials += tab.first_chunk[tab.n] < CLIP_BLOCKS ? tab.first_chunk[tab.n] : CLIP_BLOCKS;
+    }
+    *out_bytes = (partials ? partials : 1) * sizeof(double);
+    return 0;
+}
+
+extern "C" int hvs_clip_grad_norm(int device_id, void *stream, const hvs_tensor *tensors, int n_tensors, double max_norm, int infinity_norm, float *norm,
+                                  void *workspace, uint64_t workspace_bytes) {
+    const char *who = "hvs_clip_grad_norm";
+    uint64_t need = 0;
+    HVS_TRY(hvs_clip_workspace(tensors, n_tensors, &need));
+    HVS_TRY(check_apart(who, tensors, n_tensors));
+    HVS_REQUIRE(norm != nullptr, "%s: norm is NULL", who);
+    HVS_REQUIRE(max_norm >= 0.0, "%s: max_norm %g must not be negative or NaN", who, max_norm);
+    HVS_REQUIRE(workspace && ((uintptr_t)workspace & 255) == 0 && workspace_bytes >= need, "%s: workspace of %llu bytes at %p, needs %llu aligned to 256", who,
+                (unsigned long long)workspace_bytes, workspace, (unsigned long long)need);
+    DeviceGuard guard(device_id);
+    HVS_HIP(guard.status);
+    hipStream_t st = (hipStream_t)stream;
+    double *partial = (double *)workspace;
+    ClipTable tab;
+    int n_partial = 0;
+    for (int at = 0; at < n_tensors;) {
+        at = fill_table(tensors, n_tensors, at, &tab);
+        const int blocks = (int)(tab.first_chunk[tab.n] < CLIP_BLOCKS ? tab.first_chunk[tab.n] : CLIP_BLOCKS);
+        if (blocks == 0) continue;
+        clip_norm_kernel<<<blocks, 256, 0, st>>>(tab, infinity_norm != 0, partial + n_partial);
+        HVS_HIP(hipGetLastError());
+        n_partial += blocks;
+    }
+    bool first = true;
+    for (int at = 0; at < n_tensors || first; first = false) {
+        at = fill_table(tensors, n_tensors, at, &tab);
+        const uint32_t chunks = tab.first_chunk[tab.n];
+        if (chunks == 0 && !first) continue;
+        clip_scale_kernel<<<(int)(chunks < 1 ? 1 : (chunks < 2048 ? chunks : 2048)), 256, 0, st>>>(tab, infinity_norm != 0, partial, n_partial, max_norm, norm, first);
+        HVS_HIP(hipGetLastError());
+    }
+    return 0;
+}

@@ -1,0 +1,106 @@
+// Device and host helpers shared by the learning kernels (hvs_adapters.hip, hvs_feedback.hip): element access for the
+// three dtypes, 16-byte chunks with guards, wave sums, the current-device guard.
+#pragma once
+#include "hvs_gemm_tile.h"
+
+template <int DT> struct Elem;
+template <> struct Elem<HVS_F32> {
+    typedef float type;
+    static constexpr int EPC = 4;  // elements per 16-byte chunk
+};
+template <> struct Elem<HVS_F16> {
+    typedef _Float16 type;
+    static constexpr int EPC = 8;
+};
+template <> struct Elem<HVS_BF16> {
+    typedef __bf16 type;
+    static constexpr int EPC = 8;
+};
+
+__device__ __forceinline__ float learn_to_float(float v) { return v; }
+__device__ __forceinline__ float learn_to_float(_Float16 v) { return (float)v; }
+__device__ __forceinline__ float learn_to_float(__bf16 v) { return hvs_bf16_to_float(__builtin_bit_cast(uint16_t, v)); }
+template <typename E> __device__ __forceinline__ E learn_from_float(float v);
+template <> __device__ __forceinline__ float learn_from_float<float>(float v) { return v; }
+template <> __device__ __forceinline__ _Float16 learn_from_float<_Float16>(float v) { return (_Float16)v; }
+template <> __device__ __forceinline__ __bf16 learn_from_float<__bf16>(float v) { return __builtin_bit_cast(__bf16, hvs_float_to_bf16(v)); }
+
+// elements k .. k + EPC - 1 of a row of K elements, zeros past its end.  ALIGNED: the row starts on 16 bytes, K and k are
+// multiples of EPC (one 16-byte load); otherwise element by element.
+template <int DT, bool ALIGNED> __device__ __forceinline__ f32x4 load_chunk(const void *row, int k, int K) {
+    typedef typename Elem<DT>::type E;
+    constexpr int EPC = Elem<DT>::EPC;
+    const E *p = reinterpret_cast<const E *>(row);
+    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (ALIGNED) {
+        if (k < K) v = *reinterpret_cast<const f32x4 *>(p + k);
+    } else {
+        E e[EPC];
+#pragma unroll
+        for (int i = 0; i < EPC; i++) e[i] = k + i < K ? p[k + i] : (E)0.0f;
+        v = __builtin_bit_cast(f32x4, *reinterpret_cast<const f32x4 *>(e));
+    }
+    return v;
+}
+
+template <int DT> __device__ __forceinline__ void chunk_to_float(const f32x4 &c, float *out) {
+    typedef typename Elem<DT>::type E;
+    constexpr int EPC = Elem<DT>::EPC;
+    typedef E vec __attribute__((ext_vector_type(EPC)));
+    const vec v = __builtin_bit_cast(vec, c);
+#pragma unroll
+    for (int i = 0; i < EPC; i++) out[i] = learn_to_float((E)v[i]);
+}
+
+// D(16 x 16) += A(16 x 4 EPC) B(16 x 4 EPC)^T: lane (m = lane & 15, g = lane >> 4) holds the chunk k = EPC g .. of row m of
+// both operands; D: row 4 g + reg (an A row), column lane & 15 (a B row).  fp32: four 16x16x4 steps pair element j of the chunks.
+template <int DT> __device__ __forceinline__ f32x4 mfma_chunk(const f32x4 &a, const f32x4 &b, f32x4 c) {
+    if (DT == HVS_F16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    if (DT == HVS_BF16) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+#pragma unroll
+    for (int j = 0; j < 4; j++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], c, 0, 0, 0);
+    return c;
+}
+
+__device__ __forceinline__ float learn_wave_sum(float v) {
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o);
+    return v;
+}
+
+// Makes `device` current for a call and the caller's device current again after it.
+struct DeviceGuard {
+    int before = -1;
+    hipError_t status;
+    explicit DeviceGuard(int device) {
+        status = hipGetDevice(&before);
+        if (status == hipSuccess && device != before) status = hipSetDevice(device);
+        else before = -1;
+    }
+    ~DeviceGuard() {
+        if (before >= 0) (void)hipSetDevice(before);
+    }
+};
+
+static inline bool learn_dtype_ok(int dt) { return dt == HVS_F32 || dt == HVS_F16 || dt == HVS_BF16; }
+static inline bool learn_aligned(const void *p, int64_t ld_bytes, int64_t row_bytes) {
+    return ((uintptr_t)p & 15) == 0 && (ld_bytes & 15) == 0 && (row_bytes & 15) == 0;
+}
+// [a, a + rows of row_bytes at pitch ld_bytes) and the same of b share a byte (conservatively: their hulls do)
+static inline bool learn_overlap(const void *a, int64_t rows_a, int64_t ld_a, int64_t row_a, const void *b, int64_t rows_b, int64_t ld_b, int64_t row_b) {
+    if (rows_a <= 0 || rows_b <= 0) return false;
+    const uintptr_t a0 = (uintptr_t)a, a1 = a0 + (uintptr_t)((rows_a - 1) * ld_a + row_a);
+    const uintptr_t b0 = (uintptr_t)b, b1 = b0 + (uintptr_t)((rows_b - 1) * ld_b + row_b);
+    return a0 < b1 && b0 < a1;
+}
+// sizes of a workspace carved in 256-byte steps
+struct WorkspaceCut {
+    char *base;
+    uint64_t used = 0;
+    explicit WorkspaceCut(void *p) : base((char *)p) {}
+    template <typename P> P *take(uint64_t bytes) {
+        P *p = reinterpret_cast<P *>(base + used);
+        used += (bytes + 255) & ~(uint64_t)255;
+        return p;
+    }
+};

@@ -338,6 +338,23 @@ class HvsIndex:
             check(self._lib.hvs_gather(self._h, _np_ptr(pos), len(pos), _np_ptr(out), 0))
         return out
 
+    def preference_loss(self, queries, chosen, rejected, offsets, reference=None, beta: float = 20.0, label_smoothing: float = 0.0, weights=None):
+        """``adapters.preference_loss`` over this table's rows, read in place: ``chosen`` / ``rejected`` are row positions as
+        in ``gather``.  Torch tensors on this GPU; runs on torch's current stream after the work already given to the table,
+        and the table's later work runs after it.  Refused while that stream is captured into a graph (the table may move its
+        rows)."""
+        from .adapters import _need_tensor, _preference
+
+        _need_tensor("queries", queries)
+        if (queries.device.index or 0) != self.device:
+            raise ValueError("device tensors must live on the index's GPU")
+
+        def launch(st, stream, ws, size):
+            with self._lock:
+                return self._lib.hvs_index_preference_loss(self._h, stream, st, ws, size)
+
+        return _preference(queries, self.dim, chosen, rejected, offsets, reference, beta, label_smoothing, weights, launch)
+
     def kmeans_assign(self, centroids, want_sums: bool = True):
         """One E-step (+ M-step partial sums).  numpy in -> numpy out; torch in -> torch out."""
         if _is_torch(centroids):

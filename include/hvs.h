@@ -443,6 +443,122 @@ int hvs_graph_scores(hvs_graph *g, int64_t first, int64_t n, double *out, int on
  */
 int hvs_graph_top_chunks(hvs_graph *g, int k, int32_t *out_nodes, double *out_scores, int *out_count);
 
+/*
+ * ---- learning from feedback: query adapters, the loss they are trained with, gradient clipping ----
+ * No reference counterpart (the reference sends every query embedding to the search as the embedding service returns
+ * it).  Every tenant -- a (workspaceId, knowledgeBaseId) pair, the WHERE of PGVector.query, pgvector.py:577-580 -- may
+ * have a low-rank adapter that moves its query embeddings, beside one projection that all tenants share; the stored rows
+ * stay as they are.  The adapters are learned from pairs of rows, one preferred over the other for a query.
+ *
+ * All buffers of these calls are device memory of device_id unless said otherwise; work is submitted to `stream` (a
+ * hipStream_t, NULL = the default stream) and nothing waits for it; nothing is allocated, so the calls may be captured
+ * into a HIP graph.  `workspace` is scratch memory of the size the matching ..._workspace call reports, aligned to 256
+ * bytes; its contents mean nothing before and after, and calls that may overlap (two streams, two captured graphs) need
+ * one each.  The calling thread's current device is left as it was.
+ */
+
+/*
+ * The weights.  Row-major, without padding, all of one dtype (HVS_F32 / HVS_F16 / HVS_BF16) except scale:
+ *     y = W x + scale[c] B[c] (A[c] x)        for a row x with adapter code c
+ */
+typedef struct hvs_adapters {
+    const void *projection; /* W [d_out, d_in], shared */
+    const void *a;          /* A [n_adapters, rank, d_in] */
+    const void *b;          /* B [n_adapters, d_out, rank] */
+    const float *scale;     /* [n_adapters] */
+    int32_t dtype;
+    int32_t d_in, d_out;    /* 1 .. HVS_MAX_ADAPTER_DIM */
+    int32_t rank;           /* 1 .. HVS_MAX_ADAPTER_RANK */
+    int32_t n_adapters;     /* 1 .. HVS_MAX_ADAPTERS */
+} hvs_adapters;
+#define HVS_MAX_ADAPTER_DIM 16384
+#define HVS_MAX_ADAPTER_RANK 128
+#define HVS_MAX_ADAPTERS 16382
+
+/* bytes of workspace that hvs_adapters_apply (backward = 0) or hvs_adapters_backward (1) needs for n rows whose row
+ * pitches are at most max_ld elements */
+int hvs_adapters_workspace(const hvs_adapters *ad, int64_t n, int64_t max_ld, int backward, uint64_t *out_bytes);
+
+/*
+ * Apply the adapters to n rows at once, each row with its own: x [n, d_in] (row pitch ld_x elements), codes int32 [n]; out
+ * [n, d_out] (row pitch ld_out), of the weights' dtype, rounded once from fp32 sums.  A code < 0 means no adapter (W x
+ * alone); a code >= n_adapters makes the row NaN.  hidden: float [n, rank] or NULL, receives A[c] x (0 without adapter),
+ * which hvs_adapters_backward takes.  out must not overlap the inputs.
+ */
+int hvs_adapters_apply(int device_id, void *stream, const hvs_adapters *ad, const void *x, int64_t ld_x,
+                       const int32_t *codes, int64_t n, void *out, int64_t ld_out, float *hidden,
+                       void *workspace, uint64_t workspace_bytes);
+
+/*
+ * Gradients of hvs_adapters_apply for the gradient grad [n, d_out] of its output; the projection is frozen and gets none.
+ *     v = scale[c] B[c]^T grad,  grad_x = W^T grad + A[c]^T v,  grad_a[c] = sum v x^T,  grad_b[c] = sum scale[c] grad hidden^T
+ * grad_x [n, d_in] (the weights' dtype, row pitch ld_gx) or NULL; grad_a float [n_adapters, rank, d_in], grad_b float
+ * [n_adapters, d_out, rank]: overwritten, zero for adapters no row uses.  Sums run in a fixed order: the same call gives
+ * the same bits.  Rows with a code >= n_adapters get a NaN grad_x row and add nothing to grad_a and grad_b.
+ */
+int hvs_adapters_backward(int device_id, void *stream, const hvs_adapters *ad, const void *grad, int64_t ld_grad,
+                          const void *x, int64_t ld_x, const int32_t *codes, const float *hidden, int64_t n,
+                          void *grad_x, int64_t ld_gx, float *grad_a, float *grad_b,
+                          void *workspace, uint64_t workspace_bytes);
+
+/*
+ * Preference loss of n_pairs pairs (chosen, rejected) of rows, n_queries queries, with the gradient for the queries.  With
+ * cos(q, r) the cosine similarity (0 where a norm is 0), and a policy that picks rows by softmax(beta cos(q, row)), the log
+ * ratio of a pair needs no normaliser:
+ *     margin = (cos(q, chosen) - cos(q, rejected)) - (cos(q0, chosen) - cos(q0, rejected))
+ *     loss   = -(1 - label_smoothing) log sigmoid(beta margin) - label_smoothing log sigmoid(-beta margin)
+ * q0 = the reference policy's query (the embedding before adaptation); reference NULL: its term is 0.  Pairs
+ * offsets[i] .. offsets[i + 1] - 1 belong to query i (int64 [n_queries + 1], ascending from 0 to n_pairs; a query may have
+ * none).  chosen / rejected: int64 row positions.  A pair with a negative position is left out (loss and margin 0, no
+ * gradient); one with a position past the last row gets a NaN loss and margin and makes its query's gradient NaN.
+ * grad [n_queries, dim], the queries' dtype: gradient of sum_p weights[p] loss[p]; weights NULL = 1 / n_pairs each (the
+ * mean).  A query of norm 0 gets gradient 0.  Sums run in a fixed order.
+ */
+typedef struct hvs_preference {
+    const void *queries;    /* [n_queries, dim] */
+    int64_t ld_queries;     /* row pitch in elements */
+    const void *reference;  /* [n_queries, dim] of the same dtype, or NULL */
+    int64_t ld_reference;
+    const int64_t *offsets; /* [n_queries + 1] */
+    const int64_t *chosen;  /* [n_pairs] */
+    const int64_t *rejected;
+    const float *weights;   /* [n_pairs] or NULL */
+    float *loss;            /* [n_pairs] out */
+    float *margin;          /* [n_pairs] out */
+    void *grad;             /* [n_queries, dim] out */
+    int64_t ld_grad;
+    int64_t n_queries, n_pairs;
+    int32_t query_dtype;    /* HVS_F32 / HVS_F16 / HVS_BF16: queries, reference, grad */
+    float beta;             /* > 0 */
+    float label_smoothing;  /* 0 .. 0.5 */
+} hvs_preference;
+
+int hvs_preference_workspace(const hvs_preference *p, int dim, uint64_t *out_bytes);
+/* over any row matrix [n_rows, dim] of rows_dtype, row pitch ld_rows elements */
+int hvs_preference_loss(int device_id, void *stream, const hvs_preference *p, const void *rows, int rows_dtype, int dim,
+                        int64_t ld_rows, int64_t n_rows, void *workspace, uint64_t workspace_bytes);
+/* over the rows of a table (positions as in hvs_gather; deleted rows count as rows).  Runs on `stream`, after the work the
+ * table's own stream holds, and the table's later work runs after it.  A captured graph would keep the address of rows
+ * that the table may move, so a stream under capture is refused. */
+int hvs_index_preference_loss(hvs_index *idx, void *stream, const hvs_preference *p, void *workspace, uint64_t workspace_bytes);
+
+/*
+ * Global norm over many tensors and the clipped tensors: norm = sqrt(sum of squares over all elements), or the largest
+ * absolute value with infinity_norm; out = data * min(1, max_norm / (norm + 1e-6)), rounded once.  The sum of squares is
+ * held in double precision.  out may be data itself (in place) or separate memory of the same type; tensors may differ in
+ * type; what is written shares no memory with any other tensor of the call.  tensors is a HOST array, read before the call returns; norm (device float) receives the norm before clipping.  A
+ * NaN anywhere makes the norm and every output NaN; an infinite norm makes the factor 0.
+ */
+typedef struct hvs_tensor {
+    const void *data;
+    void *out;
+    int64_t numel;
+    int32_t dtype;
+} hvs_tensor;
+int hvs_clip_workspace(const hvs_tensor *tensors, int n_tensors, uint64_t *out_bytes);
+int hvs_clip_grad_norm(int device_id, void *stream, const hvs_tensor *tensors, int n_tensors, double max_norm,
+                       int infinity_norm, float *norm, void *workspace, uint64_t workspace_bytes);
+
 /* Per-kernel device time, measured with HIP events on the index's stream. */
 int hvs_profile_enable(hvs_index *idx, int on);
 int hvs_profile_get(hvs_index *idx, int which, double *total_ms, int64_t *launches);

@@ -1,0 +1,376 @@
+"""GPU tier: low-rank query adapters (forward, backward) against float64."""
+
+import numpy as np
+import pytest
+
+from oracle import learn_oracle as lo
+
+pytestmark = pytest.mark.gpu
+
+DT = {"f32": "float32", "f16": "float16", "bf16": "bfloat16"}
+
+
+@pytest.fixture(scope="module")
+def env():
+    import torch
+
+    import hirag_prod_amd as hvs
+
+    class Env:
+        pass
+
+    e = Env()
+    e.torch, e.hvs, e.dev = torch, hvs, torch.device("cuda", 0)
+    return e
+
+
+def np64(t):
+    return t.detach().double().cpu().numpy()
+
+
+def make(env, dtype, n, d_in, d_out, rank, adapters, seed=0, codes=None):
+    torch = env.torch
+    gen = torch.Generator().manual_seed(seed)
+    t = getattr(torch, DT[dtype])
+    rnd = lambda *s: torch.randn(*s, generator=gen)
+    x = rnd(n, d_in).to(env.dev, t)
+    w = (rnd(d_out, d_in) / d_in**0.5).to(env.dev, t)
+    a = (rnd(adapters, rank, d_in) / d_in**0.5).to(env.dev, t)
+    b = (rnd(adapters, d_out, rank) / rank**0.5).to(env.dev, t)
+    scale = (0.5 + torch.rand(adapters, generator=gen)).to(env.dev)
+    if codes is None:
+        codes = torch.randint(-1, adapters, (n,), generator=gen)
+    codes = torch.as_tensor(codes).to(env.dev, torch.int32)
+    return env.hvs.QueryAdapters(w, a, b, scale), x, codes, gen
+
+
+def weights64(ad):
+    return np64(ad.projection), np64(ad.a), np64(ad.b), np64(ad.scale)
+
+
+def check(got, want, tol, what):
+    got = np64(got)
+    assert got.shape == want.shape, what
+    nan = np.isnan(want)
+    assert np.array_equal(np.isnan(got), nan), f"{what}: NaN in other places"
+    bad = ~(np.abs(got - want) <= tol) & ~nan
+    assert not bad.any(), f"{what}: {bad.sum()} of {bad.size} off, worst {np.nanmax(np.abs(got - want) / tol):.2f} tolerances at {np.argwhere(bad)[:3].tolist()}"
+
+
+def check_apply(env, ad, x, codes, dtype, what="y"):
+    y, hidden = ad.apply(x, codes, return_hidden=True)
+    cn = codes.cpu().numpy()
+    want, tol, u, u_tol = lo.adapters_apply_tolerance(np64(x), cn, *weights64(ad), dtype)
+    check(hidden, u, u_tol, "hidden")
+    check(y, want, tol, what)
+    return y, hidden
+
+
+SIZES = [
+    # n, d_in, d_out, rank, adapters
+    (1, 8, 8, 1, 1),
+    (1, 1536, 1536, 16, 64),
+    (3, 100, 60, 5, 2),
+    (16, 64, 16, 16, 3),
+    (17, 257, 33, 17, 40),
+    (63, 768, 512, 8, 63),
+    (64, 1536, 768, 64, 7),
+    (65, 64, 64, 8, 3),
+    (65, 1, 1, 1, 1),
+    (130, 200, 130, 33, 4),
+    (300, 1001, 770, 13, 5),
+    (1024, 256, 256, 16, 300),
+    (1025, 96, 200, 32, 2),
+    (2500, 512, 520, 128, 11),
+]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n,d_in,d_out,rank,adapters", SIZES)
+def test_apply(env, dtype, n, d_in, d_out, rank, adapters):
+    ad, x, codes, _ = make(env, dtype, n, d_in, d_out, rank, adapters)
+    check_apply(env, ad, x, codes, dtype)
+
+
+def test_apply_largest_tile(env):
+    """Enough rows and columns for the 256 x 256 tile."""
+    for dtype in ("f16", "bf16"):
+        ad, x, codes, _ = make(env, dtype, 8200, 128, 2050, 16, 9)
+        check_apply(env, ad, x, codes, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n", [5, 200])
+@pytest.mark.parametrize("kind", ["none", "one", "each", "past"])
+def test_codes(env, dtype, n, kind):
+    codes = {"none": [-1] * n, "one": [2] * n, "each": list(range(n)), "past": [(-3, 0, n, 2**31 - 1)[i % 4] for i in range(n)]}[kind]
+    ad, x, codes, _ = make(env, dtype, n, 72, 80, 6, n, codes=codes)
+    y, hidden = check_apply(env, ad, x, codes, dtype)
+    if kind == "none":
+        assert bool((hidden == 0).all())
+
+
+def test_codes_beyond_32_bits(env):
+    torch = env.torch
+    ad, x, _, _ = make(env, "f32", 4, 16, 16, 2, 3)
+    codes = torch.tensor([0, 2**32, -(2**32), 2**32 + 1], dtype=torch.int64, device=env.dev)
+    y = ad.apply(x, codes)
+    assert bool(y[1].isnan().all()) and bool(y[3].isnan().all())
+    same = ad.apply(x, torch.tensor([0, -1, -1, -1], dtype=torch.int32, device=env.dev))
+    assert torch.equal(y[[0, 2]], same[[0, 2]])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("n", [10, 150])
+def test_strides_and_neighbours(env, dtype, n):
+    """Rows inside a wider tensor whose other columns are NaN, unaligned; the output's other columns stay as they were."""
+    torch = env.torch
+    for d_in, d_out, left in ((64, 64, 8), (100, 40, 4), (99, 41, 3)):
+        ad, x, codes, _ = make(env, dtype, n, d_in, d_out, 8, 3)
+        wide = torch.full((n, d_in + 2 * left), float("nan"), dtype=x.dtype, device=env.dev)
+        wide[:, left : left + d_in] = x
+        out = torch.full((n, d_out + 2 * left), 7.0, dtype=x.dtype, device=env.dev)
+        ad.apply(wide[:, left : left + d_in], codes, out=out[:, left : left + d_out])
+        want = ad.apply(x, codes)
+        assert torch.equal(out[:, left : left + d_out], want)
+        assert bool((out[:, :left] == 7).all()) and bool((out[:, left + d_out :] == 7).all())
+        # a transposed view has no contiguous rows: it is copied
+        assert torch.equal(ad.apply(x.t().contiguous().t(), codes), want)
+        assert torch.equal(ad.apply(x[:1].expand(n, d_in), codes[:1].expand(n)), ad.apply(x[:1].repeat(n, 1), codes[:1].repeat(n)))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n", [20, 140])
+def test_what_is_not_finite_stays_with_its_tenant(env, dtype, n):
+    torch = env.torch
+    ad, x, codes, _ = make(env, dtype, n, 72, 80, 8, 4, codes=[(i * 7) % 5 - 1 for i in range(n)])
+    want = ad.apply(x, codes)
+    ad.a[1, 2, 3] = float("nan")
+    ad.b[2, 5, 1] = float("inf")
+    x[7] = float("inf")
+    y = ad.apply(x, codes)
+    clean = (codes != 1) & (codes != 2)
+    clean[7] = False
+    assert torch.equal(y[clean], want[clean])
+    assert bool(y[codes == 1].isnan().all()) and bool((~y[7].isfinite()).any())
+
+
+def test_large_values_in_half_precision(env):
+    """A x beyond the largest fp16 number, brought back by B: the middle is held in fp32."""
+    torch = env.torch
+    for n in (8, 100):
+        ad, x, codes, _ = make(env, "f16", n, 64, 64, 16, 2, codes=[i % 2 for i in range(n)])
+        ad.a.mul_(512.0)
+        x.mul_(1024.0)
+        ad.b.mul_(1.0 / 4096.0)
+        y, hidden = check_apply(env, ad, x, codes, "f16")
+        assert float(hidden.abs().max()) > 65504 and bool(y.isfinite().all())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n,d_in,d_out,rank,adapters", [(1, 8, 8, 1, 1), (2, 100, 60, 5, 3), (64, 256, 128, 16, 5), (96, 768, 768, 8, 12), (333, 257, 130, 33, 7),
+                                                       (1030, 200, 96, 16, 40), (3000, 64, 72, 70, 2), (1500, 128, 64, 128, 3)])
+def test_backward(env, dtype, n, d_in, d_out, rank, adapters):
+    torch = env.torch
+    ad, x, codes, gen = make(env, dtype, n, d_in, d_out, rank, adapters)
+    g = torch.randn(n, d_out, generator=gen).to(env.dev, x.dtype)
+    _, hidden = ad.apply(x, codes, return_hidden=True)
+    dx, da, db = ad.backward(g, x, codes, hidden)
+    check_backward(ad, g, x, codes, hidden, dtype, dx, da, db)
+    # a fixed order of sums: the same bits again, and without grad_x
+    dx2, da2, db2 = ad.backward(g, x, codes, hidden)
+    assert torch.equal(dx, dx2) and torch.equal(da, da2) and torch.equal(db, db2)
+    none, da3, db3 = ad.backward(g, x, codes, hidden, input_grad=False)
+    assert none is None and torch.equal(da, da3) and torch.equal(db, db3)
+
+
+def check_backward(ad, g, x, codes, hidden, dtype, dx, da, db):
+    w, a, b, scale = weights64(ad)
+    g64, x64, h64, cn = np64(g), np64(x), np64(hidden), codes.cpu().numpy()
+    wx, wa, wb, v = lo.adapters_backward(g64, x64, cn, h64, w, a, b, scale)
+    # grad_x is the forward with the transposed weights
+    _, tol, v_, v_tol = lo.adapters_apply_tolerance(g64, cn, w.T.copy(), b.transpose(0, 2, 1).copy(), a.transpose(0, 2, 1).copy(), scale, dtype)
+    check(dx, wx, tol, "grad_x")
+    tol_a, tol_b = np.zeros_like(a), np.zeros_like(b)
+    for c in range(len(a)):
+        at = np.flatnonzero(cn == c)
+        m = len(at)
+        s = scale[c]
+        tol_a[c] = s * (sum_tol(v[at], x64[at], m) + v_tol[at].T @ np.abs(x64[at])) + 2 * 2.0**-24 * np.abs(wa[c])
+        tol_b[c] = s * sum_tol(g64[at], h64[at], m) + 2 * 2.0**-24 * np.abs(wb[c])
+    check(da, wa, tol_a, "grad_a")
+    check(db, wb, tol_b, "grad_b")
+    for c in range(len(a)):
+        if not (cn == c).any():
+            assert not da[c].any() and not db[c].any()
+
+
+def sum_tol(p, q, count):
+    return lo.sum_error(np.sqrt((p * p).T @ (q * q)), max(count, 1)) if count else np.zeros((p.shape[1], q.shape[1]))
+
+
+def test_gradient_against_differences(env):
+    """d sum(G y) / d theta by central differences of the float64 formula the kernels are checked against."""
+    ad, x, codes, gen = make(env, "f32", 70, 24, 20, 4, 3)
+    g = env.torch.randn(70, 20, generator=gen).to(env.dev)
+    _, hidden = ad.apply(x, codes, return_hidden=True)
+    dx, da, db = (np64(t) for t in ad.backward(g, x, codes, hidden))
+    w, a, b, scale = weights64(ad)
+    cn, x64, g64 = codes.cpu().numpy(), np64(x), np64(g)
+    f = lambda x_, a_, b_: (lo.adapters_apply(x_, cn, w, a_, b_, scale)[0] * g64).sum()
+    rng = np.random.default_rng(0)
+    for _ in range(5):
+        # the function is bilinear: a central difference along one argument is exact up to float64 rounding
+        for k, (arg, grad) in enumerate(((x64, dx), (a, da), (b, db))):
+            step = rng.standard_normal(arg.shape)
+            args = [x64, a, b]
+            hi, lo_ = list(args), list(args)
+            hi[k], lo_[k] = arg + step, arg - step
+            want, got = (f(*hi) - f(*lo_)) / 2, (grad * step).sum()
+            # each of the gradient's elements is off by at most ~70 * 2^-24 of the size of its terms
+            assert abs(got - want) <= 1e-5 * np.abs(grad * step).sum() + 1e-9, (k, got, want)
+
+
+def test_backward_isolates_and_skips(env):
+    """Rows without an adapter, or with a code past the last one, add nothing; their inputs may hold anything."""
+    torch = env.torch
+    n = 200
+    codes = [(i * 11) % 6 - 1 for i in range(n)]  # -1 .. 4 over 4 adapters: code 4 is past the last
+    ad, x, codes, gen = make(env, "f32", n, 40, 48, 5, 4, codes=codes)
+    g = torch.randn(n, 48, generator=gen).to(env.dev)
+    _, hidden = ad.apply(x, codes, return_hidden=True)
+    _, da, db = ad.backward(g, x, codes, hidden)
+    out = (codes < 0) | (codes >= 4)
+    x[out] = float("nan")
+    g2 = g.clone()
+    g2[out] = float("inf")
+    dx2, da2, db2 = ad.backward(g2, x, codes, hidden)
+    assert torch.equal(da, da2) and torch.equal(db, db2)
+    assert bool(dx2[codes >= 4].isnan().all()) and bool(dx2[~out].isfinite().all())
+
+
+@pytest.mark.parametrize("n", [0, 1])
+def test_empty(env, n):
+    torch = env.torch
+    ad, x, codes, _ = make(env, "f32", n, 16, 12, 3, 2, codes=[-1] * n)
+    y, hidden = ad.apply(x, codes, return_hidden=True)
+    assert y.shape == (n, 12) and hidden.shape == (n, 3)
+    dx, da, db = ad.backward(torch.ones(n, 12, device=env.dev), x, codes, hidden)
+    assert dx.shape == (n, 16) and not da.any() and not db.any()
+
+
+def test_chunks_of_rows(env):
+    """More rows than one pass takes (65 536): the same rows give the same results, and gradients add up over the passes."""
+    torch = env.torch
+    n = 65536 + 700
+    ad, x, codes, gen = make(env, "bf16", n, 64, 64, 4, 6)
+    y = ad.apply(x, codes)
+    assert torch.equal(y[-700:], ad.apply(x[-700:], codes[-700:]))
+    assert torch.equal(y[:65536], ad.apply(x[:65536], codes[:65536]))
+    g = torch.randn(n, 64, generator=gen).to(env.dev, x.dtype)
+    _, hidden = ad.apply(x, codes, return_hidden=True)
+    dx, da, db = ad.backward(g, x, codes, hidden)
+    g64, x64, cn = g.double(), x.double(), codes
+    for c in range(6):
+        at = (cn == c).nonzero()[:, 0]
+        m = len(at)
+        s = float(ad.scale[c])
+        v = g64[at] @ ad.b[c].double()
+        want_a, want_b = s * (v.t() @ x64[at]), s * (g64[at].t() @ hidden[at].double())
+        size_a = ((v * v).t() @ (x64[at] * x64[at])).sqrt()
+        size_b = ((g64[at] ** 2).t() @ (hidden[at].double() ** 2)).sqrt()
+        assert bool(((da[c] - want_a).abs() <= s * lo.sum_error(1.0, m + 64) * size_a * 2 + 1e-6 * want_a.abs()).all())
+        assert bool(((db[c] - want_b).abs() <= s * lo.sum_error(1.0, m) * size_b + 1e-6 * want_b.abs()).all())
+
+
+def test_many_adapters(env):
+    """The largest stack: more bins than one round of the grouping scan, several digits."""
+    torch = env.torch
+    s = 16382
+    gen = torch.Generator().manual_seed(3)
+    codes = torch.randint(-1, s + 1, (5000,), generator=gen)
+    ad, x, codes, _ = make(env, "f32", 5000, 16, 8, 2, s, codes=codes)
+    check_apply(env, ad, x, codes, "f32")
+    _, hidden = ad.apply(x, codes, return_hidden=True)
+    g = torch.randn(5000, 8, generator=gen).to(env.dev)
+    dx, da, db = ad.backward(g, x, codes, hidden)
+    check_backward(ad, g, x, codes, hidden, "f32", dx, da, db)
+
+
+def test_other_stream_and_graph(env):
+    """On a stream of the caller's, and captured: every replay gives what the eager call gives, with eager work between."""
+    torch = env.torch
+    for n in (5, 300):
+        ad, x, codes, gen = make(env, "bf16", n, 128, 96, 8, 5)
+        g = torch.randn(n, 96, generator=gen).to(env.dev, x.dtype)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            y, hidden = ad.apply(x, codes, return_hidden=True)
+            grads = ad.backward(g, x, codes, hidden)
+        side.synchronize()
+        assert torch.equal(y, ad.apply(x, codes))
+
+        def both():
+            y_, h_ = ad.apply(x, codes, return_hidden=True)
+            return (y_,) + ad.backward(g, x, codes, h_)
+
+        graphs = []
+        for _ in range(2):  # two graphs of the same adapters
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                outs = both()
+            graphs.append((graph, outs))
+        for turn in range(4):
+            x.copy_(torch.randn(n, 128, generator=gen).to(env.dev, x.dtype))
+            codes.copy_(torch.randint(-1, 5, (n,), generator=gen).to(env.dev, torch.int32))
+            want = both()
+            for graph, outs in graphs:
+                graph.replay()
+            torch.cuda.synchronize()
+            for graph, outs in graphs:
+                assert all(torch.equal(o, w_) for o, w_ in zip(outs, want)), turn
+        del grads
+
+
+def test_weights_changed_in_place_and_numpy(env):
+    torch = env.torch
+    ad, x, codes, _ = make(env, "f16", 6, 32, 32, 4, 2)
+    before = ad.apply(x, codes)
+    ad.b.zero_()
+    want = ad.apply(x, torch.full_like(codes, -1))
+    assert torch.equal(ad.apply(x, codes), want) and not torch.equal(before, want)
+    host = ad.apply(x.float().cpu().numpy(), codes.tolist())
+    assert host.dtype == np.float32 and np.array_equal(host, want.float().cpu().numpy())
+    fresh = env.hvs.QueryAdapters.create(24, 3, rank=4)
+    q = torch.randn(5, 24, device=env.dev)
+    assert torch.equal(fresh.apply(q, torch.tensor([0, 1, 2, -1, 1], device=env.dev)), q)
+
+
+def test_refusals(env):
+    torch, hvs = env.torch, env.hvs
+    ad, x, codes, _ = make(env, "f32", 6, 32, 24, 4, 2)
+    hidden = torch.zeros(6, 4, device=env.dev)
+    grad = torch.zeros(6, 24, device=env.dev)
+    for bad in (x[:, :31], x.half(), x[0], x.cpu()):
+        with pytest.raises(ValueError):
+            ad.apply(bad, codes)
+    for bad in (codes[:5], codes.float(), codes.cpu(), codes[None], [0.5] * 6):
+        with pytest.raises(ValueError):
+            ad.apply(x, bad)
+    square, xs, cs, _ = make(env, "f32", 6, 32, 32, 4, 2)
+    with pytest.raises(hvs.HvsError, match="overlaps"):
+        square.apply(xs, cs, out=xs)
+    with pytest.raises(ValueError):
+        ad.apply(x, codes, out=torch.empty(24, 6, device=env.dev).t())
+    with pytest.raises(ValueError):
+        ad.apply(x, codes, out=torch.empty(6, 24, device=env.dev, dtype=torch.float16))
+    for args in ((grad[:, :3], x, codes, hidden), (grad, x, codes, hidden[:, :2]), (grad, x, codes, hidden.double()), (grad[:3], x, codes, hidden)):
+        with pytest.raises(ValueError):
+            ad.backward(*args)
+    w, a, b, s = ad.projection, ad.a, ad.b, ad.scale
+    for bad in ((w, a, b, s.double()), (w, a[:1], b, s), (w.t(), a, b, s), (w, a.half(), b, s), (w, a, b[:, :5].contiguous(), s), (w.cpu(), a, b, s), (w.double(), a.double(), b.double(), s)):
+        with pytest.raises(ValueError):
+            hvs.QueryAdapters(*bad)
+    with pytest.raises(ValueError):
+        hvs.QueryAdapters.create(16, 2, rank=129)

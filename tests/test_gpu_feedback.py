@@ -1,0 +1,416 @@
+"""GPU tier: the preference loss with its gradient, gradient clipping, and a training step through all of them, against float64."""
+
+import math
+
+import numpy as np
+import pytest
+
+from oracle import learn_oracle as lo
+
+pytestmark = pytest.mark.gpu
+
+DT = {"f32": "float32", "f16": "float16", "bf16": "bfloat16"}
+
+
+@pytest.fixture(scope="module")
+def env():
+    import torch
+
+    import hirag_prod_amd as hvs
+
+    class Env:
+        pass
+
+    e = Env()
+    e.torch, e.hvs, e.dev = torch, hvs, torch.device("cuda", 0)
+    return e
+
+
+def np64(t):
+    return t.detach().double().cpu().numpy()
+
+
+def make(env, qdt, rdt, nq, dim, n_rows, counts, seed=0):
+    torch = env.torch
+    gen = torch.Generator().manual_seed(seed)
+    t = lambda name: getattr(torch, DT[name])
+    rows = torch.randn(n_rows, dim, generator=gen).to(env.dev, t(rdt))
+    q = torch.randn(nq, dim, generator=gen).to(env.dev, t(qdt))
+    ref = (q.float().cpu() + 0.2 * torch.randn(nq, dim, generator=gen)).to(env.dev, t(qdt))
+    counts = torch.as_tensor(counts) if counts is not None else torch.randint(0, 7, (nq,), generator=gen)
+    offsets = torch.zeros(nq + 1, dtype=torch.int64)
+    offsets[1:] = counts.cumsum(0)
+    pairs = int(offsets[-1])
+    chosen = torch.randint(0, n_rows, (pairs,), generator=gen)
+    rejected = torch.randint(0, n_rows, (pairs,), generator=gen)
+    return q, ref, rows, chosen.to(env.dev), rejected.to(env.dev), offsets.to(env.dev)
+
+
+def check(got, want, tol, what):
+    got = np64(got)
+    assert got.shape == want.shape, what
+    nan = np.isnan(want)
+    assert np.array_equal(np.isnan(got), nan), f"{what}: NaN in other places"
+    bad = ~(np.abs(got - want) <= tol) & ~nan
+    assert not bad.any(), f"{what}: {bad.sum()} of {bad.size} off, worst {np.nanmax(np.abs(got - want) / tol):.2f} tolerances at {np.argwhere(bad)[:3].tolist()}"
+
+
+def check_preference(q, ref, rows, chosen, rejected, offsets, got, qdt, beta, smoothing, weights=None):
+    q64, r64 = np64(q), np64(rows)
+    ref64 = None if ref is None else np64(ref)
+    loss, margin, grad, pull = lo.preference(q64, r64, chosen.cpu().numpy(), rejected.cpu().numpy(), offsets.cpu().numpy(), ref64, beta, smoothing,
+                                             None if weights is None else np64(weights))
+    dim = q64.shape[1]
+    # a cosine is a sum of dim products of norm at most 1, divided by two roots of such sums: relative 2^-22 each at most;
+    # a margin holds four of them
+    cos_tol = lo.sum_error(1.0, dim) + 8 * 2.0**-24 + 2 * lo.sum_error(1.0, dim)
+    margin_tol = 4 * cos_tol
+    check(got[1], margin, np.full_like(margin, margin_tol), "margin")
+    # |d loss / d margin| <= beta
+    check(got[0], loss, beta * margin_tol + 8 * 2.0**-24 * (1 + np.abs(loss)), "loss")
+    # the slope changes by at most beta^2 / 4 per unit of margin; every term has length at most 3 pull, element errors of the
+    # unit rows 2 cos_tol, and the sum over the pairs rounds once per pair
+    pairs_of = np.diff(offsets.cpu().numpy())
+    ylen = np.sqrt((q64 * q64).sum(1))
+    w = np.full(len(loss), 1.0 / max(len(loss), 1)) if weights is None else np.abs(np64(weights))
+    w_sum = np.array([w[a:b].sum() for a, b in zip(offsets.cpu().numpy()[:-1], offsets.cpu().numpy()[1:])])
+    inv = np.divide(1.0, ylen, out=np.zeros_like(ylen), where=ylen > 0)
+    tol = (inv * w_sum * beta * (beta / 4 * margin_tol * 3 + 3 * cos_tol) + pull * (pairs_of + 8) * 3 * 2.0**-24)[:, None]
+    check(got[2], grad, tol + lo.HALF_STEP[qdt] * np.abs(grad) + lo.TINY[qdt], "grad")
+
+
+@pytest.mark.parametrize("qdt,rdt", [(q, r) for q in DT for r in DT])
+@pytest.mark.parametrize("dim", [7, 256, 520, 1536, 2049])
+def test_preference(env, qdt, rdt, dim):
+    q, ref, rows, c, r, off = make(env, qdt, rdt, 37, dim, 90, None, seed=dim)
+    for reference, beta, smoothing in ((ref, 20.0, 0.0), (None, 5.0, 0.1)):
+        got = env.hvs.preference_loss(q, rows, c, r, off, reference=reference, beta=beta, label_smoothing=smoothing)
+        check_preference(q, reference, rows, c, r, off, got, qdt, beta, smoothing)
+        again = env.hvs.preference_loss(q, rows, c, r, off, reference=reference, beta=beta, label_smoothing=smoothing)
+        assert all(env.torch.equal(a, b) for a, b in zip(got, again))
+
+
+@pytest.mark.parametrize("dim", [1, 768, 8192, 8193, 16384])
+@pytest.mark.parametrize("counts", [[1], [16], [17], [500], [0, 70, 1, 0], [40, 0, 33]])
+def test_few_queries_many_pairs(env, dim, counts):
+    q, ref, rows, c, r, off = make(env, "f32", "f16", len(counts), dim, 50, counts, seed=dim + len(counts))
+    weights = env.torch.rand(len(c), device=env.dev)
+    got = env.hvs.preference_loss(q, rows, c, r, off, reference=ref, beta=10.0, weights=weights)
+    check_preference(q, ref, rows, c, r, off, got, "f32", 10.0, 0.0, weights)
+
+
+def test_many_queries(env):
+    q, ref, rows, c, r, off = make(env, "bf16", "f32", 700, 100, 300, None, seed=5)
+    got = env.hvs.preference_loss(q, rows, c, r, off, reference=ref, beta=20.0)
+    check_preference(q, ref, rows, c, r, off, got, "bf16", 20.0, 0.0)
+
+
+def test_left_out_pairs_and_bad_positions(env):
+    torch = env.torch
+    q, ref, rows, c, r, off = make(env, "f32", "f16", 40, 64, 30, None, seed=9)
+    n = len(c)
+    c[torch.arange(0, n, 3, device=env.dev)] = -1
+    r[torch.arange(1, n, 7, device=env.dev)] = -(2**40)
+    got = env.hvs.preference_loss(q, rows, c, r, off, reference=ref)
+    check_preference(q, ref, rows, c, r, off, got, "f32", 20.0, 0.0)
+    left = (c < 0) | (r < 0)
+    assert not got[0][left].any() and not got[1][left].any()
+    c[5], r[8] = 30, 2**40  # one past the last row, and far past it
+    got = env.hvs.preference_loss(q, rows, c, r, off, reference=ref)
+    check_preference(q, ref, rows, c, r, off, got, "f32", 20.0, 0.0)
+    c.fill_(-1)
+    got = env.hvs.preference_loss(q, rows, c, r, off, reference=ref)
+    assert not any(t.any() for t in got)
+
+
+def test_zero_norms_and_same_rows(env):
+    torch = env.torch
+    for nq in (3, 600):
+        q, ref, rows, c, r, off = make(env, "f32", "f32", nq, 40, 20, [4] * nq, seed=2)
+        rows[3] = 0
+        c[0], r[1] = 3, 3
+        c[4] = r[4] = 7  # chosen and rejected alike: margin 0
+        q[2] = 0
+        ref[0] = 0
+        got = env.hvs.preference_loss(q, rows, c, r, off, reference=ref, beta=4.0)
+        check_preference(q, ref, rows, c, r, off, got, "f32", 4.0, 0.0)
+        assert not got[2][2].any() and float(got[1][4]) == 0.0
+        assert all(bool(t.isfinite().all()) for t in got)
+
+
+def test_extreme_margins(env):
+    """Losses of thousands and slopes of zero, without overflow."""
+    torch = env.torch
+    q = torch.tensor([[1.0, 0.0], [1.0, 0.0]], device=env.dev)
+    rows = torch.tensor([[1.0, 0.0], [-1.0, 0.0]], device=env.dev)
+    off = torch.tensor([0, 1, 2], device=env.dev)
+    loss, margin, grad = env.hvs.preference_loss(q, rows, torch.tensor([0, 1], device=env.dev), torch.tensor([1, 0], device=env.dev), off, beta=1000.0)
+    assert margin.tolist() == [2.0, -2.0] and loss.tolist() == [0.0, 2000.0]
+    assert bool(grad.isfinite().all())
+
+
+def test_gradient_against_differences(env):
+    q, ref, rows, c, r, off = make(env, "f32", "f32", 6, 24, 30, [3, 0, 5, 1, 2, 4], seed=4)
+    w = env.torch.rand(len(c), device=env.dev)
+    _, _, grad = env.hvs.preference_loss(q, rows, c, r, off, reference=ref, beta=8.0, label_smoothing=0.1, weights=w)
+    args = (np64(rows), c.cpu().numpy(), r.cpu().numpy(), off.cpu().numpy(), np64(ref), 8.0, 0.1, np64(w))
+    f = lambda x: (lo.preference(x, *args)[0] * args[-1]).sum()
+    rng = np.random.default_rng(0)
+    q64, g = np64(q), np64(grad)
+    for _ in range(6):
+        step = rng.standard_normal(q64.shape)
+        h = 1e-4
+        want = (f(q64 + h * step) - f(q64 - h * step)) / (2 * h)
+        # the difference quotient is off by h^2 / 6 times a third derivative of order beta^3, far below 1e-5 of the terms
+        assert abs((g * step).sum() - want) <= 1e-4 * np.abs(g * step).sum() + 1e-7
+
+
+def test_strides(env):
+    torch = env.torch
+    q, ref, rows, c, r, off = make(env, "f16", "f16", 9, 64, 40, None, seed=8)
+    want = env.hvs.preference_loss(q, rows, c, r, off, reference=ref)
+    for left in (8, 3):  # rows that start on 16 bytes, and rows that do not
+        wide = lambda t: torch.cat([torch.full_like(t[:, :left], float("nan")), t, torch.full_like(t[:, :left], float("nan"))], 1)[:, left : left + 64]
+        got = env.hvs.preference_loss(wide(q), wide(rows), c.int(), r.int(), off.int(), reference=wide(ref))
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_table(env):
+    """Over the rows of an index: dims that its rows are padded to, after work on the index's own stream, and before."""
+    torch = env.torch
+    for dtype, dim in (("f16", 100), ("f32", 257), ("bf16", 768)):
+        q, ref, rows, c, r, off = make(env, "f32", dtype, 20, dim, 60, None, seed=dim)
+        idx = env.hvs.HvsIndex(dim, dtype, device=0)
+        idx.add(rows[:30])
+        idx.add(rows[30:])
+        want = env.hvs.preference_loss(q, rows, c, r, off, reference=ref)
+        got = idx.preference_loss(q, c, r, off, reference=ref)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            got = idx.preference_loss(q, c, r, off, reference=ref)
+        idx.add(rows)  # grows, and so moves, the table behind the call
+        side.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        with pytest.raises(ValueError):
+            idx.preference_loss(q[:, :5], c, r, off)
+        graph = torch.cuda.CUDAGraph()
+        refused = []
+        with torch.cuda.graph(graph):
+            try:
+                idx.preference_loss(q, c, r, off, reference=ref)
+            except env.hvs.HvsError as e:
+                refused.append(str(e))
+        assert refused and "captured" in refused[0]
+        idx.close()
+
+
+def test_preference_empty_and_refusals(env):
+    torch, hvs = env.torch, env.hvs
+    q, ref, rows, c, r, off = make(env, "f32", "f32", 4, 16, 10, [1, 2, 0, 1])
+    none = torch.zeros(0, dtype=torch.int64, device=env.dev)
+    loss, margin, grad = hvs.preference_loss(q, rows, none, none, torch.zeros(5, dtype=torch.int64, device=env.dev))
+    assert len(loss) == 0 and len(margin) == 0 and not grad.any()
+    loss, margin, grad = hvs.preference_loss(q[:0], rows, none, none, torch.zeros(1, dtype=torch.int64, device=env.dev))
+    assert grad.shape == (0, 16)
+    nan = hvs.preference_loss(q, rows[:0], c, r, off)
+    assert bool(nan[0].isnan().all())
+    for kw in (dict(beta=0.0), dict(beta=-1.0), dict(beta=math.nan), dict(beta=math.inf), dict(label_smoothing=-0.1), dict(label_smoothing=0.6)):
+        with pytest.raises(hvs.HvsError):
+            hvs.preference_loss(q, rows, c, r, off, **kw)
+    for args in ((q, rows[:, :8], c, r, off), (q.double(), rows, c, r, off), (q, rows, c[:2], r, off), (q, rows, c, r, off[:-1]), (q, rows.cpu(), c, r, off),
+                 (q, rows, c.float(), r, off), (q[0], rows, c, r, off)):
+        with pytest.raises(ValueError):
+            hvs.preference_loss(*args)
+    with pytest.raises(ValueError):
+        hvs.preference_loss(q, rows, c, r, off, reference=ref.half())
+    with pytest.raises(ValueError):
+        hvs.preference_loss(q, rows, c, r, off, weights=torch.ones(3, device=env.dev))
+
+
+def test_preference_graph(env):
+    torch = env.torch
+    q, ref, rows, c, r, off = make(env, "f32", "f16", 5, 128, 60, [30, 2, 0, 50, 1], seed=3)
+    call = lambda: env.hvs.preference_loss(q, rows, c, r, off, reference=ref)
+    graphs = []
+    call()
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = call()
+        graphs.append((graph, outs))
+    for turn in range(4):
+        q.copy_(torch.randn(5, 128, generator=torch.Generator().manual_seed(turn)).to(env.dev))
+        want = call()
+        for graph, _ in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for _, outs in graphs:
+            assert all(torch.equal(o, w) for o, w in zip(outs, want)), turn
+
+
+# -- clipping ----------------------------------------------------------------------------------------------------
+
+
+def check_clip(env, grads, max_norm, infinity, norm, outs):
+    g64 = [np64(g) for g in grads]
+    want_norm, want = lo.clip(g64, max_norm, infinity)
+    # double sums, one rounding to fp32
+    assert abs(float(norm) - want_norm) <= 2 * 2.0**-24 * want_norm
+    name = {env.torch.float32: "f32", env.torch.float16: "f16", env.torch.bfloat16: "bf16"}
+    for g, o, w in zip(grads, outs, want):
+        assert o.dtype == g.dtype and o.shape == g.shape
+        half = lo.HALF_STEP[name[g.dtype]]
+        # the factor and the product in fp32 (four roundings), then one rounding to the type
+        assert bool((np.abs(np64(o) - w) <= (4 * 2.0**-24 + half) * np.abs(w) + lo.TINY[name[g.dtype]]).all())
+
+
+@pytest.mark.parametrize("infinity", [False, True])
+@pytest.mark.parametrize("max_norm", [0.0, 0.3, 1e9])
+@pytest.mark.parametrize("sizes", [[1], [3, 0, 8191, 8192, 8193], [100000, 7], list(range(1, 200))])
+def test_clip(env, sizes, max_norm, infinity):
+    torch = env.torch
+    gen = torch.Generator().manual_seed(len(sizes))
+    types = [torch.float32, torch.bfloat16, torch.float16]
+    grads = [torch.randn(n, generator=gen).to(env.dev, types[i % 3]) for i, n in enumerate(sizes)]
+    kind = math.inf if infinity else 2.0
+    outs = [torch.full_like(g, 5.0) for g in grads]
+    norm = env.hvs.clip_grad_norm(grads, max_norm, norm_type=kind, out=outs)
+    check_clip(env, grads, max_norm, infinity, norm, outs)
+    inplace = [g.clone() for g in grads]
+    norm2 = env.hvs.clip_grad_norm(inplace, max_norm, norm_type=kind)
+    assert torch.equal(norm, norm2) and all(torch.equal(a, b) for a, b in zip(inplace, outs))
+
+
+def test_clip_unaligned_views_and_neighbours(env):
+    torch = env.torch
+    for t in (torch.float32, torch.float16, torch.bfloat16):
+        base = torch.randn(20001, device=env.dev).to(t)
+        want = base.clone()
+        out = torch.zeros(20001, device=env.dev, dtype=t)
+        view = base[3:20000]
+        norm = env.hvs.clip_grad_norm([view], 2.0, out=[out[1:19998]])
+        check_clip(env, [view], 2.0, False, norm, [out[1:19998]])
+        assert torch.equal(base, want) and float(out[0]) == 0 and float(out[-1]) == 0
+        halves = [base[:10000].view(100, 100), base[10000:20000]]
+        env.hvs.clip_grad_norm(halves, 1.0)
+        assert torch.equal(base[20000], want[20000])
+
+
+def test_clip_range_and_not_finite(env):
+    torch = env.torch
+    # squares beyond and below fp32
+    for size in (1e25, 1e-30):
+        g = torch.full((1000,), size, device=env.dev)
+        norm = env.hvs.clip_grad_norm([g], math.inf)
+        assert abs(float(norm) - size * math.sqrt(1000)) <= 1e-6 * size * math.sqrt(1000)
+        assert bool((g == torch.full((), size, device=env.dev)).all())
+    for infinity in (2.0, math.inf):
+        g = torch.ones(9000, device=env.dev)
+        h = torch.ones(10, device=env.dev, dtype=torch.float16)
+        g[8500] = float("nan")
+        norm = env.hvs.clip_grad_norm([h, g], 1.0, norm_type=infinity)
+        assert math.isnan(float(norm)) and bool(g.isnan().all()) and bool(h.isnan().all())
+        g = torch.ones(9000, device=env.dev)
+        g[1] = float("-inf")
+        norm = env.hvs.clip_grad_norm([g], 1.0, norm_type=infinity)
+        assert float(norm) == math.inf and float(g[0]) == 0.0 and math.isnan(float(g[1]))
+
+
+def test_clip_refusals(env):
+    torch, hvs = env.torch, env.hvs
+    g = torch.ones(64, device=env.dev)
+    for bad in ([], [g.cpu()], [g.double()], [g.view(8, 8).t()], [[1.0]]):
+        with pytest.raises(ValueError):
+            hvs.clip_grad_norm(bad, 1.0)
+    for kw in (dict(norm_type=1.0), dict(out=[]), dict(out=[g.half()]), dict(out=[torch.ones(63, device=env.dev)])):
+        with pytest.raises(ValueError):
+            hvs.clip_grad_norm([g], 1.0, **kw)
+    for bad in (-1.0, math.nan):
+        with pytest.raises(hvs.HvsError):
+            hvs.clip_grad_norm([g], bad)
+    # a tensor named twice would be scaled twice
+    with pytest.raises(hvs.HvsError, match="share memory"):
+        hvs.clip_grad_norm([g, g], 0.1)
+    with pytest.raises(hvs.HvsError, match="share memory"):
+        hvs.clip_grad_norm([g[:40], g[30:]], 0.1)
+    with pytest.raises(hvs.HvsError, match="overlaps"):
+        hvs.clip_grad_norm([g[:40]], 0.1, out=[g[10:50]])
+    with pytest.raises(hvs.HvsError, match="share memory"):
+        hvs.clip_grad_norm([g[:10], g[20:30]], 0.1, out=[g[20:30], torch.ones(10, device=env.dev)])
+    assert bool((g == 1).all())
+    # reading one tensor twice is fine
+    outs = [torch.zeros_like(g), torch.zeros_like(g)]
+    norm = hvs.clip_grad_norm([g, g], 1e9, out=outs)
+    assert abs(float(norm) - math.sqrt(128)) < 1e-5 and all(torch.equal(o, g) for o in outs)
+
+
+def test_clip_graph(env):
+    torch = env.torch
+    grads = [torch.ones(30000, device=env.dev), torch.ones(77, device=env.dev, dtype=torch.bfloat16)]
+    outs = [torch.zeros_like(g) for g in grads]
+    env.hvs.clip_grad_norm(grads, 1.0, out=outs)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        norm = env.hvs.clip_grad_norm(grads, 1.0, out=outs)
+    for turn in range(4):
+        for g in grads:
+            g.copy_(torch.randn(g.shape, device=env.dev))
+        graph.replay()
+        torch.cuda.synchronize()
+        check_clip(env, grads, 1.0, False, norm, outs)
+        want = [torch.zeros_like(g) for g in grads]
+        assert torch.equal(norm, env.hvs.clip_grad_norm(grads, 1.0, out=want)) and all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+# -- together ----------------------------------------------------------------------------------------------------
+
+
+def test_training_step_and_search(env):
+    """The gradients of a whole step against differences of the float64 loss, and the adapted queries in a search."""
+    torch = env.torch
+    gen = torch.Generator().manual_seed(1)
+    dim, n_rows, nq, s, r = 32, 200, 12, 3, 4
+    rows = torch.randn(n_rows, dim, generator=gen)
+    idx = env.hvs.HvsIndex(dim, "f32", device=0)
+    idx.add(rows.numpy())
+    w = torch.eye(dim) + 0.1 * torch.randn(dim, dim, generator=gen)
+    a = torch.randn(s, r, dim, generator=gen) / dim**0.5
+    b = 0.3 * torch.randn(s, dim, r, generator=gen)
+    ad = env.hvs.QueryAdapters(w.to(env.dev), a.to(env.dev), b.to(env.dev), torch.tensor([1.0, 0.5, 2.0], device=env.dev))
+    x = torch.randn(nq, dim, generator=gen).to(env.dev)
+    codes = torch.tensor([0, 1, 2, -1] * 3, device=env.dev)
+    off = torch.arange(0, 3 * nq + 1, 3, device=env.dev)
+    c = torch.randint(0, n_rows, (3 * nq,), generator=gen).to(env.dev)
+    rej = torch.randint(0, n_rows, (3 * nq,), generator=gen).to(env.dev)
+    step = ad.feedback_gradients(idx, x, codes, c, rej, off, beta=6.0)
+    tensor_step = ad.feedback_gradients(rows.to(env.dev), x, codes, c, rej, off, beta=6.0)
+    assert all(torch.equal(p, q) for p, q in zip(step, tensor_step))
+    w64, a64, b64, s64 = np64(ad.projection), np64(ad.a), np64(ad.b), np64(ad.scale)
+    x64, cn = np64(x), codes.cpu().numpy()
+    ref = x64 @ w64.T
+    pref = (rows.double().numpy(), c.cpu().numpy(), rej.cpu().numpy(), off.cpu().numpy(), ref, 6.0, 0.0)
+    f = lambda a_, b_: lo.preference(lo.adapters_apply(x64, cn, w64, a_, b_, s64)[0], *pref)[0].mean()
+    assert abs(float(step.loss.mean()) - f(a64, b64)) < 1e-5
+    rng = np.random.default_rng(0)
+    h = 1e-4
+    for _ in range(4):
+        da, db = rng.standard_normal(a64.shape), rng.standard_normal(b64.shape)
+        want = (f(a64 + h * da, b64 + h * db) - f(a64 - h * da, b64 - h * db)) / (2 * h)
+        ga, gb = np64(step.grad_a), np64(step.grad_b)
+        size = np.abs(ga * da).sum() + np.abs(gb * db).sum()
+        assert abs((ga * da).sum() + (gb * db).sum() - want) <= 1e-4 * size
+    norm = math.sqrt((np64(step.grad_a) ** 2).sum() + (np64(step.grad_b) ** 2).sum())
+    assert abs(float(step.norm) - norm) <= 1e-5 * norm
+    clipped = ad.feedback_gradients(idx, x, codes, c, rej, off, beta=6.0, max_norm=norm / 4)
+    got = math.sqrt((np64(clipped.grad_a) ** 2).sum() + (np64(clipped.grad_b) ** 2).sum())
+    assert abs(got - norm / 4) <= 1e-4 * norm and abs(float(clipped.norm) - norm) <= 1e-5 * norm
+    # adapted queries go into a search as they are
+    y = ad.apply(x, codes)
+    dist, ids, cnt = idx.search(y, k=5)
+    y64 = np64(y)
+    full = 1 - lo.unit(y64)[0] @ lo.unit(rows.double().numpy())[0].T
+    best = np.sort(full, 1)[:, :5]
+    assert np.abs(np64(dist) - best).max() < 1e-5
+    idx.close()
