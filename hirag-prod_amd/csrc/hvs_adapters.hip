@@ -5,18 +5,19 @@
 //
 // Two routes.  Few rows (FEW_ROWS): every 16-column slice of W is read once by its own block, bound by the latency of
 // reading W; rows stay in arrival order.  Many rows: rows are ordered by code (a stable counting sort), so that a tile of
-// rows meets few adapters; the low-rank term is put into the accumulators of the tile product first and W x is added by
-// the same matrix-pipe loop as the searches use, so y is rounded and written once.
+// rows meets few adapters; W x comes from the matrix-pipe loop the searches use, the low-rank term is added in its
+// accumulators, and y is rounded and written once.
 //
 // u = A_c x is held in fp32.  For 16-bit weights the product with B runs on the 16-bit pipe: u is divided by a power of
 // two that brings its largest element to [0.5, 1) (no overflow in fp16 whatever the inputs), split into two 16-bit parts
-// hi + lo (relative error 2^-16 for bf16, 2^-22 for fp16: far below the output's own rounding), and the accumulators are
-// multiplied by that power and by s_c before W x is added.
+// hi + lo (relative error 2^-16 for bf16, 2^-22 for fp16: far below the output's own rounding), and the product is
+// multiplied by that power and by s_c as it is added to W x.
 #include "hvs_learn.h"
 
 #define FEW_ROWS 64
 #define GROUP_CHUNK 1024  // rows per block of the grouping kernels
 #define MAX_CHUNK_ROWS 65536
+#define SHRINK_WIDE_ROWS 16384  // rows from which u = A x is taken 32 rows a wave instead of 16 a block
 
 // ---------------------------------------------------------------------------------------------------------------
 // grouping: rows ordered by adapter, equal codes in row order
@@ -35,36 +36,66 @@ __global__ __launch_bounds__(GROUP_CHUNK) void group_count_kernel(const int32_t 
     for (int b = threadIdx.x; b < nb; b += GROUP_CHUNK) counts[(size_t)blockIdx.x * nb + b] = hist[b];
 }
 
-// Every block adds up the counts of all chunks itself (bins in rounds of 1024: a block scan with a carry) and places its
-// own rows: the 16 waves take turns, and inside a wave lanes of one bin find each other with one ballot per bit of the bin.
+// Every block finds the first place of each bin and how many of the bin's rows lie before its own, and places its rows; nothing
+// depends on timing.  Up to GROUP_SELF chunks it counts all rows itself (4096 rows: 5 us instead of 6 + 4 with a counting
+// launch); beyond, it adds up the counts of group_count_kernel, a wave per bin with a lane per chunk.
+// FEW_BINS: the waves' counts per bin lie side by side in LDS and one barrier ranks the rows of the block; with more bins the
+// 16 waves take turns.  Inside a wave lanes of one bin find each other with one ballot per bit of the bin.
+#define GROUP_SELF 8
+#define GROUP_FEW_BINS 512
+template <bool FEW_BINS>
 __global__ __launch_bounds__(GROUP_CHUNK) void group_place_kernel(const int32_t *__restrict__ codes, int n, int S, int bits, int chunks,
                                                                   const uint32_t *__restrict__ counts, uint32_t *__restrict__ order,
                                                                   int32_t *__restrict__ scodes, uint32_t *__restrict__ seg_begin) {
-    extern __shared__ uint32_t next[];  // [S + 2] next free place of every bin
-    __shared__ uint32_t wave_sum[GROUP_CHUNK / 64];
-    const int nb = S + 2, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int i = blockIdx.x * GROUP_CHUNK + tid;
+    constexpr int WAVES = GROUP_CHUNK / 64;
+    extern __shared__ uint32_t next[];  // [S + 2] next free place of every bin; [S + 2] its rows before this block's
+    __shared__ uint32_t wave_sum[WAVES];
+    __shared__ uint16_t by_wave[FEW_BINS ? WAVES : 1][FEW_BINS ? GROUP_FEW_BINS : 1];
+    const int nb = S + 2, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, me = blockIdx.x;
+    uint32_t *before = next + nb;
+    const int i = me * GROUP_CHUNK + tid;
     const int32_t code = i < n ? codes[i] : 0;
     const uint32_t bin = i < n ? group_bin(code, S) : 0;
-    if (chunks == 1) {  // no counting launch: count here
-        for (int b = tid; b < nb; b += GROUP_CHUNK) next[b] = 0;
+    if (chunks <= GROUP_SELF) {
+        for (int b = tid; b < 2 * nb; b += GROUP_CHUNK) next[b] = 0;
         __syncthreads();
-        if (i < n) atomicAdd(&next[bin], 1u);
-        __syncthreads();
-    }
-    uint32_t carry = 0;
-    for (int b0 = 0; b0 < nb; b0 += GROUP_CHUNK) {
-        const int b = b0 + tid;
-        uint32_t total = 0, before = 0;
-        if (b < nb) {
-            if (chunks == 1) total = next[b];
-            else
-                for (int k = 0; k < chunks; k++) {
-                    const uint32_t v = counts[(size_t)k * nb + b];
-                    total += v;
-                    before += k < (int)blockIdx.x ? v : 0u;
-                }
+        for (int k = 0; k < chunks; k++) {
+            const int at = k * GROUP_CHUNK + tid;
+            if (at < n) {
+                const uint32_t q = k == me ? bin : group_bin(codes[at], S);
+                atomicAdd(&next[q], 1u);  // whole numbers: the order does not matter
+                if (k < me) atomicAdd(&before[q], 1u);
+            }
         }
+    } else if (FEW_BINS) {
+        for (int b = wave; b < nb; b += WAVES) {
+            const uint32_t v = lane < chunks ? counts[(size_t)lane * nb + b] : 0;  // at most 64 chunks
+            uint32_t all = v, mine = lane < me ? v : 0;
+#pragma unroll
+            for (int o = 32; o >= 1; o >>= 1) {
+                all += __shfl_xor(all, o);
+                mine += __shfl_xor(mine, o);
+            }
+            if (lane == 0) next[b] = all, before[b] = mine;
+        }
+    } else {
+        for (int b = tid; b < nb; b += GROUP_CHUNK) {
+            uint32_t all = 0, mine = 0;
+            for (int k = 0; k < chunks; k++) {
+                const uint32_t v = counts[(size_t)k * nb + b];
+                all += v;
+                mine += k < me ? v : 0u;
+            }
+            next[b] = all, before[b] = mine;
+        }
+    }
+    if (FEW_BINS)
+        for (int b = tid; b < WAVES * GROUP_FEW_BINS; b += GROUP_CHUNK) (&by_wave[0][0])[b] = 0;
+    __syncthreads();
+    uint32_t carry = 0;
+    for (int b0 = 0; b0 < nb; b0 += GROUP_CHUNK) {  // exclusive scan over the bins
+        const int b = b0 + tid;
+        const uint32_t total = b < nb ? next[b] : 0;
         uint32_t inc = total;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
@@ -75,14 +106,14 @@ __global__ __launch_bounds__(GROUP_CHUNK) void group_place_kernel(const int32_t 
         __syncthreads();
         uint32_t base = carry, all = 0;
 #pragma unroll
-        for (int w = 0; w < GROUP_CHUNK / 64; w++) {
+        for (int w = 0; w < WAVES; w++) {
             if (w < wave) base += wave_sum[w];
             all += wave_sum[w];
         }
         const uint32_t start = base + inc - total;
         if (b < nb) {
-            next[b] = start + before;
-            if (blockIdx.x == 0 && b >= 1) seg_begin[b - 1] = start;  // seg_begin[S] = end of the last adapter's rows
+            next[b] = start + before[b];
+            if (me == 0 && b >= 1) seg_begin[b - 1] = start;  // seg_begin[S] = end of the last adapter's rows
         }
         carry += all;
         __syncthreads();
@@ -93,16 +124,28 @@ __global__ __launch_bounds__(GROUP_CHUNK) void group_place_kernel(const int32_t 
         const uint64_t m = __ballot(one);
         peers &= one ? m : ~m;
     }
-    const uint64_t below = (1ull << lane) - 1ull;
-    for (int w = 0; w < GROUP_CHUNK / 64; w++) {
-        if (w == wave && i < n) {
-            const uint32_t place = next[bin] + (uint32_t)__popcll(peers & below);
+    const uint32_t rank = (uint32_t)__popcll(peers & ((1ull << lane) - 1ull)), here = (uint32_t)__popcll(peers);
+    const bool highest = i < n && (peers >> lane) == 1ull;
+    if (FEW_BINS) {
+        if (highest) by_wave[wave][bin] = (uint16_t)here;
+        __syncthreads();
+        if (i < n) {
+            uint32_t place = next[bin] + rank;
+            for (int w = 0; w < wave; w++) place += by_wave[w][bin];
             order[place] = (uint32_t)i;
             scodes[place] = code;
         }
-        __syncthreads();
-        if (w == wave && i < n && (peers >> lane) == 1ull) next[bin] += (uint32_t)__popcll(peers);  // the highest of its peers
-        __syncthreads();
+    } else {
+        for (int w = 0; w < WAVES; w++) {
+            if (w == wave && i < n) {
+                const uint32_t place = next[bin] + rank;
+                order[place] = (uint32_t)i;
+                scodes[place] = code;
+            }
+            __syncthreads();
+            if (w == wave && highest) next[bin] += here;
+            __syncthreads();
+        }
     }
 }
 
@@ -119,20 +162,44 @@ struct ShrinkParams {
     int n, K, r, rp, S;     // rp: r rounded up to 16
     float *hidden;          // [n][r] by row, or NULL
     void *u_hi, *u_lo;      // [n][rp] in the order of `order` (fp32: u_hi alone), or NULL
-    float *factor;          // [n] likewise: what the tile product multiplies the low-rank sums by
+    float *factor;          // [n] likewise: what the tile product multiplies the low-rank sums by (0 without adapter)
     const float *scale;
 };
 
 #define SHRINK_WAVES 8
 // One block per 16 rows (and per share blockIdx.y of the adapters among them): D[rank][row] on 16x16 matrix tiles, the
-// block's waves split K and add up through LDS.  Every adapter that occurs is read once per tile of rows that uses it;
-// loads go straight to registers (a lane's 16 bytes are a fragment).
+// block's waves split K and add up through LDS.  Loads go straight to registers (a lane's 16 bytes are a fragment).
+// what the sums u of one row, spread over the lanes that hold them, become: the caller's fp32 copy, and the two 16-bit parts
+// (fp32 weights: u itself) with the factor of their product.  `largest` = max |u| of the row; 4 ranks j .. j + 3 per call
+template <int DT> __device__ __forceinline__ void shrink_store(const ShrinkParams &p, int64_t at, int j, const float *u, float largest, int32_t c) {
+    typedef typename Elem<DT>::type E;
+    const bool known = c >= 0 && c < p.S;
+    if (p.hidden) {
+        float *out = p.hidden + (p.order ? (int64_t)p.order[at] : at) * p.r;
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (j + e < p.r) out[j + e] = c < p.S ? u[e] : __builtin_nanf("");
+    }
+    if (!p.u_hi || j >= p.rp) return;
+    typedef E vec __attribute__((ext_vector_type(4)));
+    const int e2 = largest > 0.0f && largest < __builtin_inff() ? ilogbf(largest) + 1 : 0;
+    vec hi, lo;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const float v = known ? (DT == HVS_F32 ? u[e] : ldexpf(u[e], -e2)) : 0.0f;
+        hi[e] = learn_from_float<E>(v);
+        lo[e] = learn_from_float<E>(v - learn_to_float((E)hi[e]));
+    }
+    *reinterpret_cast<vec *>(reinterpret_cast<E *>(p.u_hi) + at * p.rp + j) = hi;
+    if (DT != HVS_F32) *reinterpret_cast<vec *>(reinterpret_cast<E *>(p.u_lo) + at * p.rp + j) = lo;
+    if (j == 0) p.factor[at] = known ? (DT == HVS_F32 ? p.scale[c] : ldexpf(p.scale[c], e2)) : 0.0f;
+}
+
 template <int DT, int RT, bool ALIGNED>
 __global__ __launch_bounds__(64 * SHRINK_WAVES) void shrink_kernel(ShrinkParams p) {
     typedef typename Elem<DT>::type E;
     constexpr int EPC = Elem<DT>::EPC, STEP = 4 * EPC;
-    __shared__ float part[SHRINK_WAVES][RT * 16][17];
-    __shared__ float row_max[16];
+    __shared__ float part[SHRINK_WAVES][16][RT * 16 + 4];  // [wave][row][rank]
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int m = lane & 15, g = lane >> 4;
     const int at = blockIdx.x * 16 + m;
@@ -142,18 +209,16 @@ __global__ __launch_bounds__(64 * SHRINK_WAVES) void shrink_kernel(ShrinkParams 
     const E *x = reinterpret_cast<const E *>(p.x) + (int64_t)row * p.ld_x;
     uint32_t todo = (uint32_t)__ballot(valid) & 0xFFFFu;
     for (int ordinal = 0; todo; ordinal++) {
-        const int lead = __builtin_ctz(todo);
-        const int32_t c = __builtin_amdgcn_readlane(code, lead);
+        const int32_t c = __builtin_amdgcn_readlane(code, __builtin_ctz(todo));
         const uint32_t members = (uint32_t)__ballot(valid && code == c) & 0xFFFFu;
         todo &= ~members;
         if (ordinal % (int)gridDim.y != (int)blockIdx.y) continue;
         f32x4 acc[RT];
 #pragma unroll
-        for (int t = 0; t < RT; t++) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        const bool known = c >= 0 && c < p.S;
-        if (known) {
+        for (int q = 0; q < RT; q++) acc[q] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (c >= 0 && c < p.S) {
             const E *a = reinterpret_cast<const E *>(p.a) + (int64_t)c * p.r * p.lda;
-            constexpr int UNROLL = RT <= 2 ? 4 : 2;
+            constexpr int UNROLL = RT == 1 ? 6 : (RT == 2 ? 4 : 2);
             for (int k0 = wave * STEP; k0 < p.K; k0 += SHRINK_WAVES * STEP * UNROLL) {
                 f32x4 fx[UNROLL], fa[UNROLL][RT];
 #pragma unroll
@@ -161,70 +226,107 @@ __global__ __launch_bounds__(64 * SHRINK_WAVES) void shrink_kernel(ShrinkParams 
                     const int k = k0 + s * SHRINK_WAVES * STEP + g * EPC;
                     fx[s] = load_chunk<DT, ALIGNED>(x, k, valid ? p.K : 0);
 #pragma unroll
-                    for (int t = 0; t < RT; t++) {
-                        const int j = t * 16 + m;
-                        fa[s][t] = load_chunk<DT, ALIGNED>(a + (int64_t)(j < p.r ? j : 0) * p.lda, k, j < p.r ? p.K : 0);
+                    for (int q = 0; q < RT; q++) {
+                        const int j = q * 16 + m;
+                        fa[s][q] = load_chunk<DT, ALIGNED>(a + (int64_t)(j < p.r ? j : 0) * p.lda, k, j < p.r ? p.K : 0);
                     }
                 }
 #pragma unroll
                 for (int s = 0; s < UNROLL; s++)
 #pragma unroll
-                    for (int t = 0; t < RT; t++) acc[t] = mfma_chunk<DT>(fa[s][t], fx[s], acc[t]);
+                    for (int q = 0; q < RT; q++) acc[q] = mfma_chunk<DT>(fa[s][q], fx[s], acc[q]);
             }
         }
 #pragma unroll
-        for (int t = 0; t < RT; t++)
+        for (int q = 0; q < RT; q++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) part[wave][t * 16 + 4 * g + e][m] = acc[t][e];
+            for (int e = 0; e < 4; e++) part[wave][m][q * 16 + 4 * g + e] = acc[q][e];
         __syncthreads();
-        // thread (j, m') owns rank j of row m': the waves' sums in wave order
-        for (int q = tid; q < RT * 256; q += 64 * SHRINK_WAVES) {
-            float s = 0.0f;
+        // 4 RT lanes of one wave per row, 4 ranks each: the waves' sums in wave order
+        if (tid < 64 * RT) {
+            const int mm = tid / (4 * RT), j = tid % (4 * RT) * 4;
+            float u[4] = {0.0f, 0.0f, 0.0f, 0.0f}, mx = 0.0f;
 #pragma unroll
-            for (int w = 0; w < SHRINK_WAVES; w++) s += part[w][q >> 4][q & 15];
-            part[0][q >> 4][q & 15] = c < p.S ? s : __builtin_nanf("");  // (its own cell: nobody else reads it before the barrier)
+            for (int w = 0; w < SHRINK_WAVES; w++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) u[e] += part[w][mm][j + e];
+#pragma unroll
+            for (int e = 0; e < 4; e++) mx = fmaxf(mx, fabsf(u[e]));
+#pragma unroll
+            for (int o = 2 * RT; o >= 1; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
+            if (members >> mm & 1) shrink_store<DT>(p, (int64_t)blockIdx.x * 16 + mm, j, u, mx, c);
         }
         __syncthreads();
-        if (tid < 16) {
+    }
+}
+
+// Many rows: a wave takes 32 rows and all of K, so that nothing is added up across waves and an adapter is read once per 32
+// rows of it.  Bound by reading x.
+template <int DT, int RT, bool ALIGNED> __global__ __launch_bounds__(256) void shrink_wide_kernel(ShrinkParams p) {
+    typedef typename Elem<DT>::type E;
+    constexpr int EPC = Elem<DT>::EPC, STEP = 4 * EPC;
+    const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+    const int row0 = (blockIdx.x * 4 + (threadIdx.x >> 6)) * 32;
+    const bool valid = lane < 32 && row0 + lane < p.n;
+    const int32_t code = valid ? p.codes[row0 + lane] : -1;
+    const E *x[2];
+#pragma unroll
+    for (int t = 0; t < 2; t++) {
+        const int at = row0 + t * 16 + m;
+        x[t] = reinterpret_cast<const E *>(p.x) + (int64_t)p.order[at < p.n ? at : p.n - 1] * p.ld_x;
+    }
+    uint32_t todo = (uint32_t)__ballot(valid);
+    while (todo) {
+        const int32_t c = __builtin_amdgcn_readlane(code, __builtin_ctz(todo));
+        const uint32_t members = (uint32_t)__ballot(valid && code == c);
+        todo &= ~members;
+        f32x4 acc[2][RT];
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int q = 0; q < RT; q++) acc[t][q] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (c >= 0 && c < p.S) {
+            const E *a = reinterpret_cast<const E *>(p.a) + (int64_t)c * p.r * p.lda;
+            constexpr int UNROLL = RT == 1 ? 6 : (RT == 2 ? 4 : (RT == 4 ? 2 : 1));
+            for (int k0 = 0; k0 < p.K; k0 += STEP * UNROLL) {
+                f32x4 fx[UNROLL][2], fa[UNROLL][RT];
+#pragma unroll
+                for (int s = 0; s < UNROLL; s++) {
+                    const int k = k0 + s * STEP + g * EPC;
+#pragma unroll
+                    for (int q = 0; q < RT; q++) {
+                        const int j = q * 16 + m;
+                        fa[s][q] = load_chunk<DT, ALIGNED>(a + (int64_t)(j < p.r ? j : 0) * p.lda, k, j < p.r ? p.K : 0);
+                    }
+#pragma unroll
+                    for (int t = 0; t < 2; t++) fx[s][t] = load_chunk<DT, ALIGNED>(x[t], k, members >> (16 * t) & 0xFFFFu ? p.K : 0);
+                }
+#pragma unroll
+                for (int s = 0; s < UNROLL; s++)
+#pragma unroll
+                    for (int t = 0; t < 2; t++)
+#pragma unroll
+                        for (int q = 0; q < RT; q++) acc[t][q] = mfma_chunk<DT>(fa[s][q], fx[s][t], acc[t][q]);
+            }
+        }
+        // lane (m, g): ranks q 16 + 4 g .. + 3 of row m
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
             float mx = 0.0f;
-            for (int j = 0; j < p.r; j++) mx = fmaxf(mx, fabsf(part[0][j][tid]));
-            row_max[tid] = mx;
-        }
-        __syncthreads();
-        if (p.hidden)
-            for (int q = tid; q < 16 * p.r; q += 64 * SHRINK_WAVES) {
-                const int mm = q / p.r, j = q - mm * p.r;
-                if (members >> mm & 1) {
-                    const int64_t out_row = p.order ? (int64_t)p.order[blockIdx.x * 16 + mm] : (int64_t)blockIdx.x * 16 + mm;
-                    p.hidden[out_row * p.r + j] = part[0][j][mm];
+#pragma unroll
+            for (int q = 0; q < RT; q++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) mx = fmaxf(mx, fabsf(acc[t][q][e]));
+            mx = fmaxf(mx, __shfl_xor(mx, 16));
+            mx = fmaxf(mx, __shfl_xor(mx, 32));
+            if (members >> (16 * t + m) & 1) {
+#pragma unroll
+                for (int q = 0; q < RT; q++) {
+                    const float u[4] = {acc[t][q][0], acc[t][q][1], acc[t][q][2], acc[t][q][3]};
+                    shrink_store<DT>(p, row0 + t * 16 + m, q * 16 + 4 * g, u, mx, c);
                 }
-            }
-        if (p.u_hi) {
-            for (int q = tid; q < 16 * p.rp; q += 64 * SHRINK_WAVES) {
-                const int mm = q / p.rp, j = q - mm * p.rp;
-                if (!(members >> mm & 1)) continue;
-                const int64_t o = ((int64_t)blockIdx.x * 16 + mm) * p.rp + j;
-                float u = j < p.r && known ? part[0][j < RT * 16 ? j : 0][mm] : 0.0f;
-                if (DT == HVS_F32) reinterpret_cast<float *>(p.u_hi)[o] = u;
-                else {
-                    const float mx = row_max[mm];
-                    if (mx > 0.0f && mx < __builtin_inff()) u = ldexpf(u, -ilogbf(mx) - 1);
-                    const E hi = learn_from_float<E>(u);
-                    reinterpret_cast<E *>(p.u_hi)[o] = hi;
-                    reinterpret_cast<E *>(p.u_lo)[o] = learn_from_float<E>(u - learn_to_float(hi));
-                }
-            }
-            if (tid < 16 && (members >> tid & 1)) {
-                float f = c >= p.S ? __builtin_nanf("") : 1.0f;
-                if (known) {
-                    const float mx = row_max[tid];
-                    f = p.scale[c];
-                    if (DT != HVS_F32 && mx > 0.0f && mx < __builtin_inff()) f = ldexpf(f, ilogbf(mx) + 1);
-                }
-                p.factor[blockIdx.x * 16 + tid] = f;
             }
         }
-        __syncthreads();
     }
 }
 
@@ -248,7 +350,7 @@ struct ProjectParams {
     int64_t ld_out;
     int n, K, N, r, rp, S;
     int b_aligned;   // rows of b start on 16 bytes and r is a whole number of chunks
-    int out_vec;     // four consecutive outputs may be stored at once
+    int out_vec;     // rows of out start on 16 bytes
 };
 
 #define FEW_WAVES 8
@@ -341,6 +443,16 @@ template <class T> __device__ __forceinline__ void adapter_src_tail(TileSrcT<T::
     }
 }
 
+// swaps the upper half of a with the lower half of b: a keeps its lower lanes and gets b's lower lanes above them, b gets a's
+// upper lanes below its own
+__device__ __forceinline__ void swap_halves(uint32_t &a, uint32_t &b) {
+    const auto r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+    a = r[0];
+    b = r[1];
+}
+
+// A block walks a range of tiles, columns first, and fetches the first k-step of the next tile while it finishes the last
+// one, so that only the block's first tile waits for memory before it can start.
 template <int DT, class T>
 __global__ __launch_bounds__(T::GT, T::GT <= 256 ? 2 : 1) void project_tile_kernel(ProjectParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)  // device-only types (buffer descriptors) inside
@@ -351,122 +463,157 @@ __global__ __launch_bounds__(T::GT, T::GT <= 256 ? 2 : 1) void project_tile_kern
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave / T::WN, wn = wave % T::WN;
     const int l32 = lane & 31, h = lane >> 5;
-    // blocks of one XCD (dispatched round robin) take consecutive tiles, columns first: they share rows of x and all of W
-    const int CT = (p.N + T::BM - 1) / T::BM;
-    const int total = gridDim.x, xcd = blockIdx.x & 7, q8 = total >> 3, rem = total & 7;
-    const int tile = xcd * q8 + (xcd < rem ? xcd : rem) + (blockIdx.x >> 3);
-    const int rt = tile / CT, ct = tile - rt * CT;
-    const int row0 = rt * T::BN, col0 = ct * T::BM;
+    // blocks of one XCD (dispatched round robin) take consecutive ranges: they share rows of x and all of W
+    const int CT = (p.N + T::BM - 1) / T::BM, tiles = CT * ((p.n + T::BN - 1) / T::BN);
+    const int blocks = gridDim.x, xcd = blockIdx.x & 7, q8 = blocks >> 3, rem = blocks & 7;
+    const int at = xcd * q8 + (xcd < rem ? xcd : rem) + (blockIdx.x >> 3);
+    const int tile_lo = (int)((int64_t)tiles * at / blocks), tile_hi = (int)((int64_t)tiles * (at + 1) / blocks);
+    if (tile_lo >= tile_hi) return;
 
     TileSrcT<T::DMA_N> srcA, srcB;
     const int k_bytes = p.K * (int)sizeof(E);
     const int nks = (k_bytes + KB - 1) / KB, tail = (k_bytes % KB) / 16;
-    {
-        const int rows_a = p.N - col0;
+    auto init_src = [&](int tile) {
+        const int rt = tile / CT, col0 = (tile - rt * CT) * T::BM;
+        const int cols = p.N - col0, last = cols < T::BM ? cols : T::BM;
         const char *wbase = reinterpret_cast<const char *>(p.w) + (int64_t)col0 * p.ldw * sizeof(E);
-        const int last = rows_a < T::BM ? rows_a : T::BM;
         adapter_src_init<T>(srcA, wbase, nullptr, 0, last, p.ldw * sizeof(E), (int64_t)(last - 1) * p.ldw * sizeof(E) + k_bytes, tid);
-        adapter_src_init<T>(srcB, p.x, p.order, row0, p.n, p.ld_x * sizeof(E), (int64_t)(p.n - 1) * p.ld_x * sizeof(E) + k_bytes, tid);
-    }
+        adapter_src_init<T>(srcB, p.x, p.order, rt * T::BN, p.n, p.ld_x * sizeof(E), (int64_t)(p.n - 1) * p.ld_x * sizeof(E) + k_bytes, tid);
+    };
     auto before_step = [&](int ks) {  // the sources of step ks are about to be used
         if (tail && ks == nks - 1) {
             adapter_src_tail<T>(srcA, tail, tid);
             adapter_src_tail<T>(srcB, tail, tid);
         }
     };
+    init_src(tile_lo);
     before_step(0);
     dma_tiles<T>(srcA, srcB, smem, koff_plain(0), wave);
-
-    f32x16 acc[MT][NT];
-    zero_acc(acc);
-    // low-rank term of this wave's columns and rows, adapter by adapter
-    const int wcol = col0 + wm * (MT * 32), wrow = row0 + wn * (NT * 32);
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
-        const int j = wrow + nt * 32 + l32;
-        const bool valid = j < p.n;
-        const int32_t code = valid ? p.codes[j] : -1;
-        const bool use = code >= 0 && code < p.S;
-        uint32_t todo = (uint32_t)__ballot(use);
-        while (todo) {
-            const int32_t c = __builtin_amdgcn_readlane(code, __builtin_ctz(todo));
-            const bool mine = use && code == c;
-            todo &= ~(uint32_t)__ballot(mine);
-            const E *b = reinterpret_cast<const E *>(p.b) + (int64_t)c * p.N * p.ldb;
-            // sums of their own, taken over only by the rows of this adapter: a weight that is not finite stays with its tenant
-            f32x16 low[MT];
-#pragma unroll
-            for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) low[mt][e] = 0.0f;
-            for (int k0 = 0; k0 < p.rp; k0 += 2 * EPC) {
-                const int k = k0 + h * EPC;
-                f32x4 ub = {0.0f, 0.0f, 0.0f, 0.0f}, ul = ub;
-                if (mine) {
-                    ub = *reinterpret_cast<const f32x4 *>(reinterpret_cast<const E *>(p.u_hi) + (int64_t)j * p.rp + k);
-                    if (DT != HVS_F32) ul = *reinterpret_cast<const f32x4 *>(reinterpret_cast<const E *>(p.u_lo) + (int64_t)j * p.rp + k);
-                }
-#pragma unroll
-                for (int mt = 0; mt < MT; mt++) {
-                    const int col = wcol + mt * 32 + l32;
-                    const int r_here = col < p.N ? p.r : 0;
-                    const E *brow = b + (int64_t)(col < p.N ? col : 0) * p.ldb;
-                    const f32x4 fb = p.b_aligned ? load_chunk<DT, true>(brow, k, r_here) : load_chunk<DT, false>(brow, k, r_here);
-                    if (DT == HVS_F32) {
-#pragma unroll
-                        for (int e = 0; e < 4; e++) low[mt] = __builtin_amdgcn_mfma_f32_32x32x2f32(fb[e], ub[e], low[mt], 0, 0, 0);
-                    } else {
-                        low[mt] = mfma16<DT>(fb, ub, low[mt]);
-                        low[mt] = mfma16<DT>(fb, ul, low[mt]);
-                    }
-                }
-            }
-#pragma unroll
-            for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) acc[mt][nt][e] = mine ? low[mt][e] : acc[mt][nt][e];
-        }
-        const float f = valid ? p.factor[j] : 1.0f;
-#pragma unroll
-        for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-            for (int e = 0; e < 16; e++) acc[mt][nt][e] *= f;
-    }
     __syncthreads();
 
     int cur = 0;
-    for (int ks = 0; ks < nks; ks++) {
-        // the step after the last one fetches that one again; the stage it fills is never read
-        const int next = ks + 1 < nks ? ks + 1 : ks;
-        if (ks + 1 < nks) before_step(next);
-        compute_step<DT, T>(acc, smem + cur * T::STAGE_BYTES, wm, wn, lane, srcA, srcB, smem + (cur ^ 1) * T::STAGE_BYTES, koff_plain(next), wave);
-        __syncthreads();
+    for (int tile = tile_lo; tile < tile_hi; tile++) {
+        const int rt = tile / CT;
+        const int wcol = (tile - rt * CT) * T::BM + wm * (MT * 32), wrow = rt * T::BN + wn * (NT * 32);
+        int32_t codes[NT];
+        float factor[NT];
+        uint32_t out_row[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {  // wanted after the product: on their way during it
+            const int j = wrow + nt * 32 + l32;
+            codes[nt] = j < p.n ? p.codes[j] : -1;
+            factor[nt] = j < p.n ? p.factor[j] : 0.0f;
+            out_row[nt] = j < p.n ? p.order[j] : 0;
+        }
+        f32x16 acc[MT][NT];
+        zero_acc(acc);
+        for (int ks = 0; ks + 1 < nks; ks++) {
+            before_step(ks + 1);
+            compute_step<DT, T>(acc, smem + cur * T::STAGE_BYTES, wm, wn, lane, srcA, srcB, smem + (cur ^ 1) * T::STAGE_BYTES, koff_plain(ks + 1), wave);
+            __syncthreads();
+            cur ^= 1;
+        }
+        // the last step fetches the next tile's first one (after the last tile: its own again, which nothing reads)
+        init_src(tile + 1 < tile_hi ? tile + 1 : tile);
+        before_step(0);
+        compute_step<DT, T>(acc, smem + cur * T::STAGE_BYTES, wm, wn, lane, srcA, srcB, smem + (cur ^ 1) * T::STAGE_BYTES, koff_plain(0), wave);
         cur ^= 1;
-    }
 
-    // accumulator element e of lane (l32, h): column 8 (e / 4) + 4 h + e % 4 of its 32, row l32
 #pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
-        const int j = wrow + nt * 32 + l32;
-        if (j >= p.n) continue;
-        E *out = reinterpret_cast<E *>(p.out) + (int64_t)p.order[j] * p.ld_out;
+        for (int nt = 0; nt < NT; nt++) {
+            const int j = wrow + nt * 32 + l32;
+            const bool valid = j < p.n;
+            const int32_t code = codes[nt];
+            const float f = factor[nt];
+            const bool use = code >= 0 && code < p.S;
+            // low-rank term, adapter by adapter, in sums of its own that only the rows of the adapter take over: a weight
+            // that is not finite stays with its tenant.  KC matrix steps of ranks at a time: their u fragments serve every
+            // adapter among the rows, and the fragments of b for all columns are in flight together
+            constexpr int KC = 2;
+            for (int k0 = 0; k0 < p.rp; k0 += KC * 2 * EPC) {
+                f32x4 ub[KC], ul[KC];
 #pragma unroll
-        for (int mt = 0; mt < MT; mt++)
+                for (int s = 0; s < KC; s++) {
+                    const int k = k0 + s * 2 * EPC + h * EPC;
+                    ub[s] = ul[s] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                    if (use && k < p.rp) {
+                        ub[s] = *reinterpret_cast<const f32x4 *>(reinterpret_cast<const E *>(p.u_hi) + (int64_t)j * p.rp + k);
+                        if (DT != HVS_F32) ul[s] = *reinterpret_cast<const f32x4 *>(reinterpret_cast<const E *>(p.u_lo) + (int64_t)j * p.rp + k);
+                    }
+                }
+                uint32_t todo = (uint32_t)__ballot(use);
+                while (todo) {
+                    const int32_t c = __builtin_amdgcn_readlane(code, __builtin_ctz(todo));
+                    const bool mine = use && code == c;
+                    todo &= ~(uint32_t)__ballot(mine);
+                    const E *b = reinterpret_cast<const E *>(p.b) + (int64_t)c * p.N * p.ldb;
+                    f32x4 fb[MT][KC];
 #pragma unroll
-            for (int e4 = 0; e4 < 4; e4++) {
-                const int col = wcol + mt * 32 + 8 * e4 + 4 * h;
-                E v[4];
+                    for (int mt = 0; mt < MT; mt++) {
+                        const int col = wcol + mt * 32 + l32;
+                        const E *brow = b + (int64_t)(col < p.N ? col : 0) * p.ldb;
 #pragma unroll
-                for (int e = 0; e < 4; e++) v[e] = learn_from_float<E>(acc[mt][nt][4 * e4 + e]);
-                if (p.out_vec && col + 3 < p.N) {
-                    typedef E vec __attribute__((ext_vector_type(4)));
-                    *reinterpret_cast<vec *>(out + col) = vec{v[0], v[1], v[2], v[3]};
-                } else {
+                        for (int s = 0; s < KC; s++) {
+                            const int k = k0 + s * 2 * EPC + h * EPC, r_here = col < p.N ? p.r : 0;
+                            fb[mt][s] = p.b_aligned ? load_chunk<DT, true>(brow, k, r_here) : load_chunk<DT, false>(brow, k, r_here);
+                        }
+                    }
 #pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        if (col + e < p.N) out[col + e] = v[e];
+                    for (int mt = 0; mt < MT; mt++) {
+                        f32x16 low;
+#pragma unroll
+                        for (int e = 0; e < 16; e++) low[e] = 0.0f;
+#pragma unroll
+                        for (int s = 0; s < KC; s++) {
+                            if (DT == HVS_F32) {
+#pragma unroll
+                                for (int e = 0; e < 4; e++) low = __builtin_amdgcn_mfma_f32_32x32x2f32(fb[mt][s][e], ub[s][e], low, 0, 0, 0);
+                            } else {
+                                low = mfma16<DT>(fb[mt][s], ub[s], low);
+                                low = mfma16<DT>(fb[mt][s], ul[s], low);
+                            }
+                        }
+#pragma unroll
+                        for (int e = 0; e < 16; e++) acc[mt][nt][e] = mine ? fmaf(f, low[e], acc[mt][nt][e]) : acc[mt][nt][e];
+                    }
                 }
             }
+            const bool lost = valid && code >= p.S;  // a code past the last adapter
+            E *out = reinterpret_cast<E *>(p.out) + (int64_t)out_row[nt] * p.ld_out;
+            // accumulator element e of lane (l32, h): column 8 (e / 4) + 4 h + e % 4 of its 32, row l32
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++) {
+                E v[16];
+#pragma unroll
+                for (int e = 0; e < 16; e++) v[e] = learn_from_float<E>(lost ? __builtin_nanf("") : acc[mt][nt][e]);
+                if (DT != HVS_F32 && p.out_vec && wcol + mt * 32 + 32 <= p.N) {
+                    // the two halves trade quarters, so that a lane holds 8 columns in a row: 16-byte stores
+                    uint32_t w[8];
+#pragma unroll
+                    for (int i = 0; i < 8; i++) w[i] = __builtin_bit_cast(uint32_t, *reinterpret_cast<uint32_t *>(v + 2 * i));
+#pragma unroll
+                    for (int i = 0; i < 8; i += 4) {
+                        swap_halves(w[i], w[i + 2]);
+                        swap_halves(w[i + 1], w[i + 3]);
+                        typedef uint32_t vec __attribute__((ext_vector_type(4)));
+                        if (valid) *reinterpret_cast<vec *>(out + wcol + mt * 32 + i * 4 + h * 8) = vec{w[i], w[i + 1], w[i + 2], w[i + 3]};
+                    }
+                } else {
+#pragma unroll
+                    for (int e4 = 0; e4 < 4; e4++) {
+                        const int col = wcol + mt * 32 + 8 * e4 + 4 * h;
+                        typedef E vec __attribute__((ext_vector_type(4)));
+                        if (valid && p.out_vec && col + 3 < p.N) *reinterpret_cast<vec *>(out + col) = vec{v[4 * e4], v[4 * e4 + 1], v[4 * e4 + 2], v[4 * e4 + 3]};
+                        else if (valid) {
+#pragma unroll
+                            for (int e = 0; e < 4; e++)
+                                if (col + e < p.N) out[col + e] = v[4 * e4 + e];
+                        }
+                    }
+                }
+            }
+        }
+        __syncthreads();  // the next tile's first step has landed for every wave
     }
 #endif
 }
@@ -690,7 +837,7 @@ static uint64_t cut_workspace(const hvs_adapters *ad, int64_t nc, int backward, 
     ws->order = w.take<uint32_t>(nc * 4);
     ws->scodes = w.take<int32_t>(nc * 4);
     ws->seg_begin = w.take<uint32_t>(((uint64_t)ad->n_adapters + 1) * 4);
-    ws->counts = w.take<uint32_t>(chunks > 1 ? (uint64_t)chunks * (ad->n_adapters + 2) * 4 : 0);
+    ws->counts = w.take<uint32_t>(chunks > GROUP_SELF ? (uint64_t)chunks * (ad->n_adapters + 2) * 4 : 0);
     ws->factor = w.take<float>(nc * 4);
     ws->u_hi = w.take<char>(nc * rp * es);
     ws->u_lo = w.take<char>(ad->dtype == HVS_F32 ? 0 : nc * rp * es);
@@ -724,12 +871,17 @@ static int launch_group(hipStream_t st, const int32_t *codes, int n, int S, cons
     const size_t lds = (size_t)(S + 2) * 4;
     int bits = 1;
     while ((1 << bits) < S + 2) bits++;
-    if (lds > 48 * 1024) {
-        HVS_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(&group_count_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-        HVS_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(&group_place_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+    if (chunks > GROUP_SELF) {
+        if (lds > 48 * 1024) HVS_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(&group_count_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+        group_count_kernel<<<chunks, GROUP_CHUNK, lds, st>>>(codes, n, S, ws.counts);
     }
-    if (chunks > 1) group_count_kernel<<<chunks, GROUP_CHUNK, lds, st>>>(codes, n, S, ws.counts);
-    group_place_kernel<<<chunks, GROUP_CHUNK, lds, st>>>(codes, n, S, bits, chunks, ws.counts, ws.order, ws.scodes, ws.seg_begin);
+    if (S + 2 <= GROUP_FEW_BINS) {
+        group_place_kernel<true><<<chunks, GROUP_CHUNK, 2 * lds, st>>>(codes, n, S, bits, chunks, ws.counts, ws.order, ws.scodes, ws.seg_begin);
+    } else {
+        if (2 * lds > 48 * 1024)
+            HVS_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(&group_place_kernel<false>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)(2 * lds)));
+        group_place_kernel<false><<<chunks, GROUP_CHUNK, 2 * lds, st>>>(codes, n, S, bits, chunks, ws.counts, ws.order, ws.scodes, ws.seg_begin);
+    }
     HVS_HIP(hipGetLastError());
     return 0;
 }
@@ -737,9 +889,15 @@ static int launch_group(hipStream_t st, const int32_t *codes, int n, int S, cons
 template <int DT> static int launch_shrink(hipStream_t st, const ShrinkParams &p, int shares) {
     const int es = hvs_elem_size(DT);
     const bool al = learn_aligned(p.x, p.ld_x * es, (int64_t)p.K * es) && learn_aligned(p.a, p.lda * es, (int64_t)p.K * es);
-    const dim3 grid((p.n + 15) / 16, shares);
-#define SHRINK(RT_) \
-    (al ? shrink_kernel<DT, RT_, true><<<grid, 64 * SHRINK_WAVES, 0, st>>>(p) : shrink_kernel<DT, RT_, false><<<grid, 64 * SHRINK_WAVES, 0, st>>>(p))
+    const bool wide = p.order && p.n >= SHRINK_WIDE_ROWS;
+    const dim3 grid((p.n + 15) / 16, shares), wgrid((p.n + 127) / 128);
+#define SHRINK(RT_)                                                                                          \
+    do {                                                                                                     \
+        if (wide && al) shrink_wide_kernel<DT, RT_, true><<<wgrid, 256, 0, st>>>(p);                         \
+        else if (wide) shrink_wide_kernel<DT, RT_, false><<<wgrid, 256, 0, st>>>(p);                         \
+        else if (al) shrink_kernel<DT, RT_, true><<<grid, 64 * SHRINK_WAVES, 0, st>>>(p);                    \
+        else shrink_kernel<DT, RT_, false><<<grid, 64 * SHRINK_WAVES, 0, st>>>(p);                           \
+    } while (0)
     if (p.r <= 16) SHRINK(1);
     else if (p.r <= 32) SHRINK(2);
     else if (p.r <= 64) SHRINK(4);
@@ -767,7 +925,8 @@ template <int DT, class T> static int launch_tile(hipStream_t st, const ProjectP
     const int tiles = ((p.N + T::BM - 1) / T::BM) * ((p.n + T::BN - 1) / T::BN);
     const size_t lds = 2 * T::STAGE_BYTES;
     HVS_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(&project_tile_kernel<DT, T>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-    project_tile_kernel<DT, T><<<tiles, T::GT, lds, st>>>(p);
+    const int resident = 256 * (T::GT <= 256 ? 2 : 1);  // blocks the chip holds at once
+    project_tile_kernel<DT, T><<<tiles < resident ? tiles : resident, T::GT, lds, st>>>(p);
     HVS_HIP(hipGetLastError());
     return 0;
 }
@@ -846,7 +1005,7 @@ static int run_direction(hipStream_t st, const hvs_adapters *ad, const Direction
     p.K = round_up(d.K, epc);  // whole chunks: K itself where rows were taken as they are, their padded width where they were packed
     p.codes = ws.scodes, p.order = ws.order, p.u_hi = ws.u_hi, p.u_lo = ws.u_lo, p.factor = ws.factor;
     p.b_aligned = learn_aligned(d.b, d.ldb * es, 0) && (d.b_padded || s.r % epc == 0);
-    p.out_vec = ((uintptr_t)d.out % (4 * es)) == 0 && (d.ld_out * es) % (4 * es) == 0;
+    p.out_vec = learn_aligned(d.out, d.ld_out * es, 0);
     if (DT == HVS_F32) return launch_tile<DT, Tile128>(st, p);
     // the largest tile that still gives every CU one: a larger tile reads less per product, idle CUs cost more
     auto tiles = [&](int t) { return (int64_t)((p.N + t - 1) / t) * ((n + t - 1) / t); };

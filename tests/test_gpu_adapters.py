@@ -99,6 +99,14 @@ def test_apply_largest_tile(env):
         check_apply(env, ad, x, codes, dtype)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("d_in,rank,adapters", [(72, 16, 5), (41, 21, 700), (64, 50, 3), (96, 128, 33)])
+def test_apply_many_rows(env, dtype, d_in, rank, adapters):
+    """Rows enough for the wide form of A x, and more than the grouping counts by itself."""
+    ad, x, codes, _ = make(env, dtype, 16500, d_in, 24, rank, adapters)
+    check_apply(env, ad, x, codes, dtype)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("n", [5, 200])
 @pytest.mark.parametrize("kind", ["none", "one", "each", "past"])
