@@ -6,14 +6,17 @@
 template <int DT> struct Elem;
 template <> struct Elem<HVS_F32> {
     typedef float type;
+    typedef f32x4 loose __attribute__((aligned(4)));  // 16 bytes at an element's address
     static constexpr int EPC = 4;  // elements per 16-byte chunk
 };
 template <> struct Elem<HVS_F16> {
     typedef _Float16 type;
+    typedef f32x4 loose __attribute__((aligned(2)));
     static constexpr int EPC = 8;
 };
 template <> struct Elem<HVS_BF16> {
     typedef __bf16 type;
+    typedef f32x4 loose __attribute__((aligned(2)));
     static constexpr int EPC = 8;
 };
 
@@ -26,19 +29,23 @@ template <> __device__ __forceinline__ _Float16 learn_from_float<_Float16>(float
 template <> __device__ __forceinline__ __bf16 learn_from_float<__bf16>(float v) { return __builtin_bit_cast(__bf16, hvs_float_to_bf16(v)); }
 
 // elements k .. k + EPC - 1 of a row of K elements, zeros past its end.  ALIGNED: the row starts on 16 bytes, K and k are
-// multiples of EPC (one 16-byte load); otherwise element by element.
+// multiples of EPC; otherwise the same 16-byte load from an address that is a multiple of the element's size only (global
+// memory takes those), and the row's end element by element.
 template <int DT, bool ALIGNED> __device__ __forceinline__ f32x4 load_chunk(const void *row, int k, int K) {
     typedef typename Elem<DT>::type E;
     constexpr int EPC = Elem<DT>::EPC;
+    typedef typename Elem<DT>::loose loose;
     const E *p = reinterpret_cast<const E *>(row);
     f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
     if (ALIGNED) {
         if (k < K) v = *reinterpret_cast<const f32x4 *>(p + k);
-    } else {
+    } else if (k + EPC <= K) {
+        v = *reinterpret_cast<const loose *>(p + k);
+    } else if (k < K) {
         E e[EPC];
 #pragma unroll
         for (int i = 0; i < EPC; i++) e[i] = k + i < K ? p[k + i] : (E)0.0f;
-        v = __builtin_bit_cast(f32x4, *reinterpret_cast<const f32x4 *>(e));
+        __builtin_memcpy(&v, e, 16);
     }
     return v;
 }
@@ -60,6 +67,20 @@ template <int DT> __device__ __forceinline__ f32x4 mfma_chunk(const f32x4 &a, co
 #pragma unroll
     for (int j = 0; j < 4; j++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], c, 0, 0, 0);
     return c;
+}
+
+// A 16-row, 64-byte piece of a row matrix on its way to mfma_chunk.  Lane l LOADS chunk l & 3 of row l >> 2 (four lanes cover 64
+// bytes of a row: the vector memory path takes such a quad in one cycle; fragment order, 16 rows next to each other, costs
+// it four) and the lanes trade their chunks through 1 KB of LDS of their wave's own.  No barrier: a wave's LDS accesses stay in order.
+__device__ __forceinline__ int turn_row(int lane) { return lane >> 2; }
+template <int DT> __device__ __forceinline__ int turn_k(int lane) { return (lane & 3) * Elem<DT>::EPC; }
+__device__ __forceinline__ void turn_put(char *lds, const f32x4 &v, int lane) {
+    const int r = lane >> 2;
+    *reinterpret_cast<f32x4 *>(lds + (r * 4 + ((lane & 3) ^ (r >> 2))) * 16) = v;
+}
+__device__ __forceinline__ f32x4 turn_get(const char *lds, int lane) {
+    const int m = lane & 15;
+    return *reinterpret_cast<const f32x4 *>(lds + (m * 4 + ((lane >> 4) ^ (m >> 2))) * 16);
 }
 
 __device__ __forceinline__ float learn_wave_sum(float v) {
