@@ -19,31 +19,28 @@ are what ``backward`` and ``preference_loss`` return.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from typing import NamedTuple, Optional, Sequence
 
 import numpy as np
+import torch
 
 from . import _lib
 from ._lib import DTYPE_CODE, HvsAdaptersStruct, HvsPreferenceStruct, HvsTensorStruct, check, load_library
 
-
-def _torch():
-    import torch
-
-    return torch
+_CODE_OF = {torch.float32: _lib.HVS_F32, torch.float16: _lib.HVS_F16, torch.bfloat16: _lib.HVS_BF16}
 
 
 def _dtype_code(t) -> int:
-    torch = _torch()
-    code = {torch.float32: _lib.HVS_F32, torch.float16: _lib.HVS_F16, torch.bfloat16: _lib.HVS_BF16}.get(t.dtype)
+    code = _CODE_OF.get(t.dtype)
     if code is None:
         raise ValueError(f"unsupported tensor dtype {t.dtype}")
     return code
 
 
 def _need_tensor(name: str, t, device=None) -> None:
-    if not isinstance(t, _torch().Tensor):
+    if not isinstance(t, torch.Tensor):
         raise ValueError(f"{name} must be a torch tensor")
     if t.device.type != "cuda" or (device is not None and t.device != device):
         raise ValueError(f"{name} must live on {'a GPU' if device is None else device}, not on {t.device}")
@@ -75,7 +72,6 @@ def _out_rows(name: str, t, n: int, width: int, dtype, device):
 
 def _numbers(name: str, values, n: Optional[int], dtype, device):
     """Whole numbers, one per row or pair, on the GPU."""
-    torch = _torch()
     if not isinstance(values, torch.Tensor):
         values = torch.as_tensor(np.ascontiguousarray(values), device=device)
     _need_tensor(name, values, device)
@@ -91,12 +87,24 @@ def _numbers(name: str, values, n: Optional[int], dtype, device):
 
 
 def _scratch(nbytes: int, device):
-    torch = _torch()
-    return torch.empty(max(int(nbytes), 1), dtype=torch.uint8, device=device)
+    """Scratch memory and its address; None where none is needed."""
+    if not nbytes:
+        return None, None
+    t = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    return t, t.data_ptr()
 
 
-def _stream(device) -> ctypes.c_void_p:
-    return ctypes.c_void_p(_torch().cuda.current_stream(device).cuda_stream)
+def _stream(device) -> int:
+    """torch's current stream of a GPU (the raw handle: building a Stream object costs more than a small launch)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+@functools.lru_cache(maxsize=4096)
+def _adapters_workspace(code: int, d_in: int, d_out: int, rank: int, n_adapters: int, n: int, max_ld: int, backward: int) -> int:
+    need = ctypes.c_uint64(0)
+    st = HvsAdaptersStruct(None, None, None, None, code, d_in, d_out, rank, n_adapters)
+    check(load_library().hvs_adapters_workspace(ctypes.byref(st), n, max_ld, backward, ctypes.byref(need)))
+    return need.value
 
 
 class FeedbackGradients(NamedTuple):
@@ -119,7 +127,6 @@ class QueryAdapters:
     """
 
     def __init__(self, projection, a, b, scale):
-        torch = _torch()
         _need_tensor("projection", projection)
         device = projection.device
         for name, t, dim in (("projection", projection, 2), ("a", a, 3), ("b", b, 3), ("scale", scale, 1)):
@@ -149,7 +156,6 @@ class QueryAdapters:
     def create(cls, dim: int, n_adapters: int, rank: int = 16, dtype: str = "f32", device: int = 0, scale: float = 1.0, seed: int = 0) -> "QueryAdapters":
         """Adapters that change nothing yet: ``W`` the identity, ``B`` zero, ``A`` random (normal, 1 / sqrt(dim)), so that the
         first gradient reaches ``B``."""
-        torch = _torch()
         if dtype not in DTYPE_CODE:
             raise ValueError(f"dtype must be one of {sorted(DTYPE_CODE)}, got {dtype!r}")
         t = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}[dtype]
@@ -163,10 +169,10 @@ class QueryAdapters:
         return HvsAdaptersStruct(self.projection.data_ptr(), self.a.data_ptr(), self.b.data_ptr(), self.scale.data_ptr(), self._code, self.d_in,
                                  self.d_out, self.rank, self.n_adapters)
 
-    def _workspace(self, st, n: int, max_ld: int, backward: int):
-        need = ctypes.c_uint64(0)
-        check(self._lib.hvs_adapters_workspace(ctypes.byref(st), n, max_ld, backward, ctypes.byref(need)))
-        return _scratch(need.value, self.device), need.value
+    def _workspace(self, n: int, max_ld: int, backward: int):
+        size = _adapters_workspace(self._code, self.d_in, self.d_out, self.rank, self.n_adapters, n, max_ld, backward)
+        ws, ptr = _scratch(size, self.device)
+        return ws, ptr, size
 
     def apply(self, x, codes, out=None, return_hidden: bool = False):
         """``x`` [n, d_in] and one adapter code per row -> [n, d_out]; every row may use another adapter.
@@ -174,7 +180,6 @@ class QueryAdapters:
         A torch tensor of the adapters' dtype gives a torch tensor (``out``, when given); with ``return_hidden`` also the
         float32 [n, rank] values ``A[c] x`` that ``backward`` takes.  A numpy array (float32, from an embedding service)
         gives a float32 numpy array.  A code past the last adapter makes its row NaN.  ``out`` must not overlap ``x``."""
-        torch = _torch()
         if not isinstance(x, torch.Tensor):
             if out is not None or return_hidden:
                 raise ValueError("out and return_hidden need device tensors")
@@ -190,10 +195,9 @@ class QueryAdapters:
             out, ld_out = _out_rows("out", out, n, self.d_out, self.dtype, self.device)
         hidden = torch.empty((n, self.rank), dtype=torch.float32, device=self.device) if return_hidden else None
         if n:
-            st = self._struct()
-            ws, size = self._workspace(st, n, max(ld_x, ld_out), 0)
-            check(self._lib.hvs_adapters_apply(self.device.index, _stream(self.device), ctypes.byref(st), x.data_ptr(), ld_x, codes.data_ptr(), n,
-                                               out.data_ptr(), ld_out, hidden.data_ptr() if return_hidden else None, ws.data_ptr(), size))
+            ws, ws_ptr, size = self._workspace(n, max(ld_x, ld_out), 0)
+            check(self._lib.hvs_adapters_apply(self.device.index, _stream(self.device), ctypes.byref(self._struct()), x.data_ptr(), ld_x, codes.data_ptr(), n,
+                                               out.data_ptr(), ld_out, hidden.data_ptr() if return_hidden else None, ws_ptr, size))
         return (out, hidden) if return_hidden else out
 
     def backward(self, grad, x, codes, hidden, input_grad: bool = True):
@@ -202,7 +206,6 @@ class QueryAdapters:
         -> ``(grad_x, grad_a, grad_b)``: grad_x [n, d_in] in the adapters' dtype (None without ``input_grad``), grad_a and
         grad_b float32 in the shapes of ``a`` and ``b``, zero for adapters no row uses.  The projection is frozen.  The same
         call gives the same bits."""
-        torch = _torch()
         x, ld_x = _rows("x", x, self.d_in, self.dtype, self.device)
         n = x.shape[0]
         grad, ld_grad = _rows("grad", grad, self.d_out, self.dtype, self.device, n)
@@ -212,11 +215,10 @@ class QueryAdapters:
         grad_x = torch.empty((n, self.d_in), dtype=self.dtype, device=self.device) if input_grad else None
         grad_a = torch.empty(self.a.shape, dtype=torch.float32, device=self.device)
         grad_b = torch.empty(self.b.shape, dtype=torch.float32, device=self.device)
-        st = self._struct()
-        ws, size = self._workspace(st, n, max(ld_x, ld_grad), 1)
-        check(self._lib.hvs_adapters_backward(self.device.index, _stream(self.device), ctypes.byref(st), grad.data_ptr(), ld_grad, x.data_ptr(), ld_x,
-                                              codes.data_ptr(), hidden.data_ptr(), n, grad_x.data_ptr() if input_grad and n else None, self.d_in,
-                                              grad_a.data_ptr(), grad_b.data_ptr(), ws.data_ptr(), size))
+        ws, ws_ptr, size = self._workspace(n, max(ld_x, ld_grad), 1)
+        check(self._lib.hvs_adapters_backward(self.device.index, _stream(self.device), ctypes.byref(self._struct()), grad.data_ptr(), ld_grad, x.data_ptr(),
+                                              ld_x, codes.data_ptr(), hidden.data_ptr(), n, grad_x.data_ptr() if input_grad and n else None, self.d_in,
+                                              grad_a.data_ptr(), grad_b.data_ptr(), ws_ptr, size))
         return grad_x, grad_a, grad_b
 
     def feedback_gradients(self, table, x, codes, chosen, rejected, offsets, beta: float = 20.0, label_smoothing: float = 0.0,
@@ -224,7 +226,6 @@ class QueryAdapters:
         """The gradients of one training step on rated answers: adapt the queries ``x``, take the preference loss of their
         pairs of rows of ``table`` (an ``HvsIndex``, or a tensor of rows) against the unadapted projection ``W x`` as the
         reference policy, go back to the adapters and clip.  Apply them with any optimizer, in place."""
-        torch = _torch()
         y, hidden = self.apply(x, codes, return_hidden=True)
         reference = self.apply(x, torch.full((len(y),), -1, dtype=torch.int32, device=self.device))
         args = dict(reference=reference, beta=beta, label_smoothing=label_smoothing, weights=weights)
@@ -239,7 +240,6 @@ class QueryAdapters:
 
 def _preference(queries, dim, chosen, rejected, offsets, reference, beta, label_smoothing, weights, launch):
     """The part ``preference_loss`` and ``HvsIndex.preference_loss`` share; ``launch(struct, stream, workspace, size)``."""
-    torch = _torch()
     _need_tensor("queries", queries)
     device = queries.device
     code = _dtype_code(queries)
@@ -265,8 +265,8 @@ def _preference(queries, dim, chosen, rejected, offsets, reference, beta, label_
                              grad.data_ptr(), dim, nq, pairs, code, float(beta), float(label_smoothing))
     need = ctypes.c_uint64(0)
     check(load_library().hvs_preference_workspace(ctypes.byref(st), dim, ctypes.byref(need)))
-    ws = _scratch(need.value, device) if need.value else None
-    check(launch(ctypes.byref(st), _stream(device), None if ws is None else ws.data_ptr(), need.value))
+    ws, ws_ptr = _scratch(need.value, device)
+    check(launch(ctypes.byref(st), _stream(device), ws_ptr, need.value))
     return loss, margin, grad
 
 
@@ -300,7 +300,6 @@ def clip_grad_norm(grads: Sequence, max_norm: float, norm_type: float = 2.0, out
     largest absolute value (``math.inf``).  The tensors are contiguous, of float32, float16 or bfloat16 in any mix, on one
     GPU, at least one; they are scaled in place, or into ``out`` (tensors of the same shapes and dtypes).  ``max_norm`` inf
     scales nothing.  A NaN anywhere makes the norm and every element NaN."""
-    torch = _torch()
     grads = list(grads)
     if not grads:
         raise ValueError("clip_grad_norm needs at least one tensor")
@@ -325,9 +324,9 @@ def clip_grad_norm(grads: Sequence, max_norm: float, norm_type: float = 2.0, out
     norm = torch.empty((), dtype=torch.float32, device=device)
     need = ctypes.c_uint64(0)
     check(lib.hvs_clip_workspace(table, len(grads), ctypes.byref(need)))
-    ws = _scratch(need.value, device)
-    check(lib.hvs_clip_grad_norm(device.index, _stream(device), table, len(grads), float(max_norm), int(norm_type == math.inf), norm.data_ptr(),
-                                 ws.data_ptr(), need.value))
+    ws, ws_ptr = _scratch(need.value, device)
+    check(lib.hvs_clip_grad_norm(device.index, _stream(device), table, len(grads), float(max_norm), int(norm_type == math.inf), norm.data_ptr(), ws_ptr,
+                                 need.value))
     return norm
 
 

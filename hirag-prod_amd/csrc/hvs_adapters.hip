@@ -21,6 +21,9 @@
 #define FEW_ROWS_16 768
 #define GROUP_CHUNK 1024  // rows per block of the grouping kernels
 #define MAX_CHUNK_ROWS 65536
+#define OUTER_BLOCKS 1024    // blocks the gradients of the stacks aim at,
+#define OUTER_MIN_ROWS 32    // ... with tiles of at least so many rows
+#define OUTER_MAX_ROWS 2048  // ... and at most so many
 #define SHRINK_WIDE_ROWS 16384  // rows from which u = A x is taken 32 rows a wave instead of 16 a block
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -824,39 +827,59 @@ __global__ __launch_bounds__(256) void pack_rows_kernel(const E *__restrict__ sr
     }
 }
 
-// dst[z][c][r] = src[z][r][c] for matrices of R x C; dst rows have pitch ld (>= R), filled with zeros past R
-template <typename E>
-__global__ __launch_bounds__(256) void transpose_kernel(const E *__restrict__ src, int R, int C, int ld, E *__restrict__ dst) {
+// dst[z][c][r] = src[z][r][c] for `count` matrices of R x C; dst rows have pitch ld (>= R), filled with zeros past R
+struct TransposeJob {
+    const void *src;
+    void *dst;
+    int R, C, ld, tiles_c, tiles_r;
+    int64_t blocks;  // tiles_c tiles_r count
+};
+struct TransposeJobs {
+    TransposeJob job[3];
+};
+// all transposed weights of a backward pass in one launch: a block per 64 x 64 tile, jobs one after the other
+template <typename E> __global__ __launch_bounds__(256) void transpose_kernel(TransposeJobs jobs) {
     __shared__ E tile[64][65];
-    const int64_t z = blockIdx.z;
-    const E *s = src + z * (int64_t)R * C;
-    E *d = dst + z * (int64_t)C * ld;
-    const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;
+    int64_t at = blockIdx.x;
+    int which = 0;
+    while (which < 2 && at >= jobs.job[which].blocks) at -= jobs.job[which++].blocks;
+    const TransposeJob &t = jobs.job[which];
+    const int64_t z = at / (t.tiles_c * t.tiles_r);
+    const int rest = (int)(at - z * (t.tiles_c * t.tiles_r));
+    const E *s = reinterpret_cast<const E *>(t.src) + z * (int64_t)t.R * t.C;
+    E *d = reinterpret_cast<E *>(t.dst) + z * (int64_t)t.C * t.ld;
+    const int r0 = rest / t.tiles_c * 64, c0 = rest % t.tiles_c * 64;
+#pragma unroll 8
     for (int i = threadIdx.x; i < 4096; i += 256) {
         const int r = r0 + (i >> 6), c = c0 + (i & 63);
-        tile[i >> 6][i & 63] = r < R && c < C ? s[(int64_t)r * C + c] : (E)0.0f;
+        tile[i >> 6][i & 63] = r < t.R && c < t.C ? s[(int64_t)r * t.C + c] : (E)0.0f;
     }
     __syncthreads();
+#pragma unroll 8
     for (int i = threadIdx.x; i < 4096; i += 256) {
         const int c = c0 + (i >> 6), r = r0 + (i & 63);
-        if (c < C && r < ld) d[(int64_t)c * ld + r] = tile[i & 63][i >> 6];
+        if (c < t.C && r < t.ld) d[(int64_t)c * t.ld + r] = tile[i & 63][i >> 6];
     }
 }
 
 // ---------------------------------------------------------------------------------------------------------------
 // gradients of the stacks: G_c[j][col] = s_c sum over the rows of adapter c of q[row][j] X[row][col]
 // ---------------------------------------------------------------------------------------------------------------
-struct OuterParams {
+struct OuterProblem {
     const float *q;  // [n][r] by row
     const void *x;   // [n][d], pitch ld_x
     int64_t ld_x;
+    float *out;      // [S][r][d], or [S][d][r] when transposed
+    float *partial;  // [2 tiles][r d], each laid out as out
+    int d, transposed, cols;  // cols: blocks over d
+};
+struct OuterParams {
+    OuterProblem problem[2];  // grad_a: q = v, X = x;  grad_b: q = hidden, X = grad
     const int32_t *scodes;
     const uint32_t *order;
     const uint32_t *seg_begin;  // [S + 1]
     const float *scale;
-    float *out;      // [S][r][d], or [S][d][r] when transposed
-    float *partial;  // [2 tiles][r][d]
-    int n, d, r, S, rows_per, transposed, accumulate;
+    int n, r, S, rows_per, accumulate;
 };
 
 // Rows are cut into tiles of rows_per (in code order).  A block walks the adapters of its tile, for 16 chunks of columns;
@@ -865,21 +888,29 @@ struct OuterParams {
 // `partial` (slot 0: it began in an earlier tile, slot 1: it begins here), and outer_join_kernel adds those in tile order.
 template <int DT, int RT, bool ALIGNED> __global__ __launch_bounds__(256) void outer_kernel(OuterParams p) {
     typedef typename Elem<DT>::type E;
-    constexpr int EPC = Elem<DT>::EPC, CC = 16 * EPC;
-    __shared__ float red[RT * 16][CC + 1];
+    constexpr int EPC = Elem<DT>::EPC, CC = 16 * EPC, COPIES = RT <= 2 ? 4 : 2;
+    __shared__ float red[COPIES][RT * 16][CC + 1];
+    __shared__ uint32_t rows[OUTER_MAX_ROWS];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int m = lane & 15, g = lane >> 4;
+    const bool second = (int)blockIdx.y >= p.problem[0].cols;
+    const OuterProblem &o = p.problem[second ? 1 : 0];
     const int lo = blockIdx.x * p.rows_per, hi = lo + p.rows_per < p.n ? lo + p.rows_per : p.n;
-    const int c0 = blockIdx.y * CC, j0 = blockIdx.z * (RT * 16);
+    const int c0 = ((int)blockIdx.y - (second ? p.problem[0].cols : 0)) * CC, j0 = blockIdx.z * (RT * 16);
+    for (int i = lo + tid; i < hi; i += 256) rows[i - lo] = p.order[i];
     int i = lo;
+    int32_t c = p.scodes[lo];
+    __syncthreads();
     while (i < hi) {
-        const int32_t c = p.scodes[i];
         if (c < 0 || c >= p.S) {  // rows without an adapter come first, codes past the last one come last
             i = c < 0 ? ((int)p.seg_begin[0] < hi ? (int)p.seg_begin[0] : hi) : hi;
+            if (i < hi) c = p.scodes[i];
             continue;
         }
         const int seg_lo = (int)p.seg_begin[c], seg_hi = (int)p.seg_begin[c + 1];
+        const float s = p.scale[c];
         const int end = seg_hi < hi ? seg_hi : hi;
+        const int32_t next_c = end < hi ? p.scodes[end] : -1;
         f32x4 acc[RT][EPC];
 #pragma unroll
         for (int t = 0; t < RT; t++)
@@ -890,85 +921,86 @@ template <int DT, int RT, bool ALIGNED> __global__ __launch_bounds__(256) void o
             f32x4 fx[UNROLL];
             float fq[UNROLL][RT];
 #pragma unroll
-            for (int s = 0; s < UNROLL; s++) {
-                const int at = b + 16 * s + g;
+            for (int u = 0; u < UNROLL; u++) {
+                const int at = b + 16 * u + g;
                 const bool ok = at < end;
-                const int64_t row = p.order[ok ? at : i];
-                fx[s] = load_chunk<DT, ALIGNED>(reinterpret_cast<const E *>(p.x) + row * p.ld_x, c0 + m * EPC, ok ? p.d : 0);
+                const int64_t row = rows[(ok ? at : i) - lo];
+                fx[u] = load_chunk<DT, ALIGNED>(reinterpret_cast<const E *>(o.x) + row * o.ld_x, c0 + m * EPC, ok ? o.d : 0);
 #pragma unroll
                 for (int t = 0; t < RT; t++) {
                     const int j = j0 + t * 16 + m;
-                    fq[s][t] = ok && j < p.r ? p.q[row * p.r + j] : 0.0f;
+                    fq[u][t] = ok && j < p.r ? o.q[row * p.r + j] : 0.0f;
                 }
             }
 #pragma unroll
-            for (int s = 0; s < UNROLL; s++) {
+            for (int u = 0; u < UNROLL; u++) {
                 float v[EPC];
-                chunk_to_float<DT>(fx[s], v);
+                chunk_to_float<DT>(fx[u], v);
 #pragma unroll
                 for (int t = 0; t < RT; t++)
 #pragma unroll
-                    for (int e = 0; e < EPC; e++) acc[t][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(fq[s][t], v[e], acc[t][e], 0, 0, 0);
+                    for (int e = 0; e < EPC; e++) acc[t][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(fq[u][t], v[e], acc[t][e], 0, 0, 0);
             }
         }
-        // the four waves' sums, in wave order
-        for (int w = 0; w < 4; w++) {
-            if (w == wave) {
+        // the four waves' sums, in a fixed order: each in its own copy, or the upper two added onto the lower two's
+        auto put = [&](int copy, bool add) {
 #pragma unroll
-                for (int t = 0; t < RT; t++)
+            for (int t = 0; t < RT; t++)
 #pragma unroll
-                    for (int e = 0; e < EPC; e++)
+                for (int e = 0; e < EPC; e++)
 #pragma unroll
-                        for (int k = 0; k < 4; k++) {
-                            float *cell = &red[t * 16 + 4 * g + k][m * EPC + e];
-                            *cell = w == 0 ? acc[t][e][k] : *cell + acc[t][e][k];
-                        }
-            }
+                    for (int k = 0; k < 4; k++) {
+                        float *cell = &red[copy][t * 16 + 4 * g + k][m * EPC + e];
+                        *cell = add ? *cell + acc[t][e][k] : acc[t][e][k];
+                    }
+        };
+        if (COPIES == 4) put(wave, false);
+        else {
+            if (wave >= 2) put(wave - 2, false);
             __syncthreads();
+            if (wave < 2) put(wave, true);
         }
+        __syncthreads();
         const bool whole = seg_lo >= lo && seg_hi <= hi;
-        const float s = p.scale[c];
-        float *part = p.partial + (int64_t)(2 * blockIdx.x + (seg_lo < lo ? 0 : 1)) * p.r * p.d;
-        const int rn = p.r - j0 < RT * 16 ? p.r - j0 : RT * 16, cn = p.d - c0 < CC ? p.d - c0 : CC;
-        if (whole && p.transposed) {
-            float *out = p.out + (int64_t)c * p.r * p.d;
-            for (int k = tid; k < rn * cn; k += 256) {
-                const int col = k / rn, j = k - col * rn;
-                float *o = out + (int64_t)(c0 + col) * p.r + j0 + j;
-                *o = s * red[j][col] + (p.accumulate ? *o : 0.0f);
-            }
-        } else {
-            float *out = whole ? p.out + (int64_t)c * p.r * p.d : part;
-            for (int k = tid; k < rn * cn; k += 256) {
-                const int j = k / cn, col = k - j * cn;
-                float *o = out + (int64_t)(j0 + j) * p.d + c0 + col;
-                *o = whole ? s * red[j][col] + (p.accumulate ? *o : 0.0f) : red[j][col];
-            }
+        const int64_t size = (int64_t)p.r * o.d;
+        float *out = whole ? o.out + (int64_t)c * size : o.partial + (int64_t)(2 * blockIdx.x + (seg_lo < lo ? 0 : 1)) * size;
+        const int rn = p.r - j0 < RT * 16 ? p.r - j0 : RT * 16, cn = o.d - c0 < CC ? o.d - c0 : CC;
+        for (int k = tid; k < RT * 16 * CC; k += 256) {
+            const int j = o.transposed ? k % (RT * 16) : k / CC, col = o.transposed ? k / (RT * 16) : k % CC;
+            if (j >= rn || col >= cn) continue;
+            float v = red[0][j][col];
+#pragma unroll
+            for (int w = 1; w < COPIES; w++) v += red[w][j][col];
+            float *cell = out + (o.transposed ? (int64_t)(c0 + col) * p.r + j0 + j : (int64_t)(j0 + j) * o.d + c0 + col);
+            *cell = whole ? s * v + (p.accumulate ? *cell : 0.0f) : v;
         }
         __syncthreads();
         i = end;
+        c = next_c;
     }
 }
 
 // adapters without rows: zero; adapters over several tiles: their partial sums in tile order
-__global__ __launch_bounds__(256) void outer_join_kernel(OuterParams p) {
+template <int VEC> __global__ __launch_bounds__(256) void outer_join_kernel(OuterParams p) {
+    typedef float vec __attribute__((ext_vector_type(VEC)));
     const int c = blockIdx.x;
     const int lo = (int)p.seg_begin[c], hi = (int)p.seg_begin[c + 1];
-    const int64_t size = (int64_t)p.r * p.d;
-    float *out = p.out + (int64_t)c * size;
-    if (lo == hi) {
-        if (!p.accumulate)
-            for (int64_t k = blockIdx.y * 256ll + threadIdx.x; k < size; k += gridDim.y * 256ll) out[k] = 0.0f;
-        return;
-    }
-    const int t0 = lo / p.rows_per, t1 = (hi - 1) / p.rows_per;
-    if (t0 == t1) return;
+    const int t0 = lo / p.rows_per, t1 = hi > lo ? (hi - 1) / p.rows_per : t0;
+    if (hi > lo ? t0 == t1 : p.accumulate) return;
+    const OuterProblem &o = p.problem[blockIdx.z];
+    const int64_t size = (int64_t)p.r * o.d / VEC;
+    vec *out = reinterpret_cast<vec *>(o.out) + (int64_t)c * size;
+    const vec *part = reinterpret_cast<const vec *>(o.partial);
     const float s = p.scale[c];
     for (int64_t k = blockIdx.y * 256ll + threadIdx.x; k < size; k += gridDim.y * 256ll) {
-        const int64_t at = p.transposed ? (k % p.r) * p.d + k / p.r : k;
-        float v = p.partial[(int64_t)(2 * t0 + 1) * size + at];
-        for (int t = t0 + 1; t <= t1; t++) v += p.partial[(int64_t)(2 * t) * size + at];
-        out[k] = s * v + (p.accumulate ? out[k] : 0.0f);
+        if (hi == lo) {
+            out[k] = (vec)0.0f;
+            continue;
+        }
+        vec v = part[(int64_t)(2 * t0 + 1) * size + k];
+#pragma unroll 4
+        for (int t = t0 + 1; t <= t1; t++) v += part[(int64_t)(2 * t) * size + k];
+        out[k] = p.accumulate ? s * v + out[k] : s * v;
     }
 }
 
@@ -988,6 +1020,7 @@ static int check_adapters(const char *who, const hvs_adapters *ad) {
     HVS_REQUIRE(ad->n_adapters >= 1 && ad->n_adapters <= HVS_MAX_ADAPTERS, "%s: %d adapters, must be in [1, %d]", who, ad->n_adapters, HVS_MAX_ADAPTERS);
     return 0;
 }
+static bool once(int64_t n, int rank) { return n <= ONCE_ROWS && rank <= 64; }
 static int few_rows(int dtype) { return dtype == HVS_F32 ? FEW_ROWS_F32 : FEW_ROWS_16; }
 static int round_up(int v, int to) { return (v + to - 1) / to * to; }
 static int elems_per_chunk(int dtype) { return dtype == HVS_F32 ? 4 : 8; }
@@ -1004,22 +1037,23 @@ static int64_t chunk_rows(int64_t n, int64_t max_ld, int es) {
 struct AdapterWs {
     uint32_t *order, *seg_begin, *counts;
     int32_t *scodes;
-    float *factor, *hidden, *partial;
+    float *factor, *hidden, *partial_a, *partial_b;
     char *u_hi, *u_lo, *packed_w, *packed_x, *w_t, *a_t, *b_t;
 };
 
-// rows of a tile of the stack gradients: about OUTER_BLOCKS blocks, at least OUTER_MIN_ROWS rows each
-#define OUTER_BLOCKS 1024
-#define OUTER_MIN_ROWS 32
+// rows of a tile of the stack gradients, for both of them
 static int outer_cols(int d, int dtype) { return (d + 16 * elems_per_chunk(dtype) - 1) / (16 * elems_per_chunk(dtype)); }
-static int outer_rows_per(int n, int d, int dtype) {
-    const int rows = (int)(((int64_t)n * outer_cols(d, dtype) + OUTER_BLOCKS - 1) / OUTER_BLOCKS);
-    return round_up(rows < OUTER_MIN_ROWS ? OUTER_MIN_ROWS : rows, 16);
+static int outer_rows_per(int64_t n, const hvs_adapters *ad) {
+    const int cols = outer_cols(ad->d_in, ad->dtype) + outer_cols(ad->d_out, ad->dtype);
+    const int64_t rows = (n * cols + OUTER_BLOCKS - 1) / OUTER_BLOCKS;
+    return (int)(rows < OUTER_MIN_ROWS ? OUTER_MIN_ROWS : (rows > OUTER_MAX_ROWS ? OUTER_MAX_ROWS : (rows + 15) / 16 * 16));
 }
 // the most tiles n rows or fewer are cut into (fewer rows may be cut into more tiles than n, by rounding)
-static int64_t outer_max_tiles(int64_t n, int d, int dtype) {
-    const int64_t by_blocks = (OUTER_BLOCKS + outer_cols(d, dtype) - 1) / outer_cols(d, dtype), by_rows = (n + OUTER_MIN_ROWS - 1) / OUTER_MIN_ROWS;
-    return by_blocks < by_rows ? by_blocks : by_rows;
+static int64_t outer_max_tiles(int64_t n, const hvs_adapters *ad) {
+    const int cols = outer_cols(ad->d_in, ad->dtype) + outer_cols(ad->d_out, ad->dtype);
+    const int64_t by_blocks = (OUTER_BLOCKS + cols - 1) / cols, by_max = (n + OUTER_MAX_ROWS - 1) / OUTER_MAX_ROWS;
+    const int64_t by_min = (n + OUTER_MIN_ROWS - 1) / OUTER_MIN_ROWS, most = by_blocks > by_max ? by_blocks : by_max;
+    return most < by_min ? most : by_min;
 }
 
 static uint64_t cut_workspace(const hvs_adapters *ad, int64_t nc, int backward, void *base, AdapterWs *ws) {
@@ -1041,12 +1075,9 @@ static uint64_t cut_workspace(const hvs_adapters *ad, int64_t nc, int backward, 
         ws->w_t = w.take<char>((uint64_t)ad->d_in * round_up(ad->d_out, epc) * es);
         ws->b_t = w.take<char>((uint64_t)ad->n_adapters * ad->rank * round_up(ad->d_out, epc) * es);
         ws->a_t = w.take<char>((uint64_t)ad->n_adapters * ad->d_in * rp * es);
-        uint64_t part = 0;
-        for (int d : {ad->d_in, ad->d_out}) {
-            const uint64_t b = 2ull * outer_max_tiles(nc, d, ad->dtype) * ad->rank * d * 4;
-            part = b > part ? b : part;
-        }
-        ws->partial = w.take<float>(part);
+        const uint64_t slots = 2ull * outer_max_tiles(nc, ad) * ad->rank;
+        ws->partial_a = w.take<float>(slots * ad->d_in * 4);
+        ws->partial_b = w.take<float>(slots * ad->d_out * 4);
     }
     return w.used;
 }
@@ -1056,7 +1087,7 @@ extern "C" int hvs_adapters_workspace(const hvs_adapters *ad, int64_t n, int64_t
     HVS_REQUIRE(n >= 0 && out_bytes, "hvs_adapters_workspace: negative row count or NULL argument");
     const int64_t nc = chunk_rows(n, max_ld > 0 ? max_ld : 1, hvs_elem_size(ad->dtype));
     AdapterWs ws;
-    *out_bytes = cut_workspace(ad, nc, backward, nullptr, &ws);
+    *out_bytes = n == 0 || (!backward && once(n, ad->rank)) ? 0 : cut_workspace(ad, nc, backward, nullptr, &ws);
     return 0;
 }
 
@@ -1167,16 +1198,12 @@ template <int DT> static int launch_pack(hipStream_t st, const void *src, int64_
     return 0;
 }
 
-template <int DT> static int launch_transpose(hipStream_t st, const void *src, int64_t count, int R, int C, int ld, void *dst) {
-    typedef typename Elem<DT>::type E;
-    // the last row tile covers the pitch, so that the padding is written
-    for (int64_t z0 = 0; z0 < count; z0 += 65535) {
-        const int64_t zn = count - z0 < 65535 ? count - z0 : 65535;
-        const dim3 grid((C + 63) / 64, (ld + 63) / 64, (unsigned)zn);
-        transpose_kernel<E><<<grid, 256, 0, st>>>((const E *)src + z0 * R * C, R, C, ld, (E *)dst + z0 * C * ld);
-    }
-    HVS_HIP(hipGetLastError());
-    return 0;
+static TransposeJob transpose_job(const void *src, int64_t count, int R, int C, int ld, void *dst) {
+    TransposeJob t = {};
+    t.src = src, t.dst = dst, t.R = R, t.C = C, t.ld = ld;
+    t.tiles_c = (C + 63) / 64, t.tiles_r = (ld + 63) / 64;  // the row tiles cover the pitch, so that the padding is written
+    t.blocks = count * t.tiles_c * t.tiles_r;
+    return t;
 }
 
 // One direction for one chunk of rows: u = A x into hidden, y = W x + s B u into out.  A: [S][r] rows of K, pitch lda;
@@ -1217,7 +1244,7 @@ static int run_direction(hipStream_t st, const hvs_adapters *ad, const Direction
     p.x = dd.x, p.ld_x = dd.ld_x, p.w = dd.w, p.ldw = dd.ldw, p.b = d.b, p.ldb = d.ldb, p.scale = ad->scale;
     p.out = d.out, p.ld_out = d.ld_out, p.n = n, p.K = d.K, p.N = d.N, p.r = s.r, p.rp = s.rp, p.S = s.S;
     if (few) {
-        if (d.out && n <= ONCE_ROWS && p.r <= 64) {
+        if (d.out && once(n, p.r)) {
             p.codes = codes;
             return launch_once<DT>(st, p, hidden, d.a, d.lda);
         }
@@ -1262,7 +1289,7 @@ static int check_rows(const char *who, const char *what, const void *p, int64_t 
 static int check_workspace(const char *who, const hvs_adapters *ad, int64_t n, int64_t max_ld, int backward, const void *ws, uint64_t bytes) {
     uint64_t need = 0;
     HVS_TRY(hvs_adapters_workspace(ad, n, max_ld, backward, &need));
-    HVS_REQUIRE(ws != nullptr && ((uintptr_t)ws & 255) == 0 && bytes >= need, "%s: workspace of %llu bytes at %p, needs %llu aligned to 256", who,
+    HVS_REQUIRE(need == 0 || (ws != nullptr && ((uintptr_t)ws & 255) == 0 && bytes >= need), "%s: workspace of %llu bytes at %p, needs %llu aligned to 256", who,
                 (unsigned long long)bytes, ws, (unsigned long long)need);
     return 0;
 }
@@ -1305,11 +1332,14 @@ extern "C" int hvs_adapters_apply(int device_id, void *stream, const hvs_adapter
     return 0;
 }
 
-template <int DT> static int launch_outer(hipStream_t st, OuterParams p) {
-    constexpr int EPC = Elem<DT>::EPC;
+template <int DT> static int launch_outer(hipStream_t st, const OuterParams &p) {
     const int es = hvs_elem_size(DT);
-    const bool al = learn_aligned(p.x, p.ld_x * es, (int64_t)p.d * es);
-    const int tiles = (p.n + p.rows_per - 1) / p.rows_per, cols = (p.d + 16 * EPC - 1) / (16 * EPC);
+    bool al = true, vec = true;
+    for (const OuterProblem &o : p.problem) {
+        al = al && learn_aligned(o.x, o.ld_x * es, (int64_t)o.d * es);
+        vec = vec && (int64_t)p.r * o.d % 4 == 0 && (uintptr_t)o.out % 16 == 0;
+    }
+    const int tiles = (p.n + p.rows_per - 1) / p.rows_per, cols = p.problem[0].cols + p.problem[1].cols;
 #define OUTER(RT_)                                                                                                           \
     do {                                                                                                                     \
         const dim3 grid(tiles, cols, (p.r + 16 * RT_ - 1) / (16 * RT_));                                                     \
@@ -1320,9 +1350,11 @@ template <int DT> static int launch_outer(hipStream_t st, OuterParams p) {
     else if (p.r <= 32) OUTER(2);
     else OUTER(4);
 #undef OUTER
-    const int64_t size = (int64_t)p.r * p.d;
-    const int by = (int)(size / 1024 < 1 ? 1 : (size / 1024 > 64 ? 64 : size / 1024));
-    outer_join_kernel<<<dim3(p.S, by), 256, 0, st>>>(p);
+    const int wide = p.problem[0].d > p.problem[1].d ? p.problem[0].d : p.problem[1].d;
+    const int64_t by = (int64_t)p.r * wide / 1024;
+    const dim3 grid(p.S, (unsigned)(by < 1 ? 1 : (by > 64 ? 64 : by)), 2);
+    if (vec) outer_join_kernel<4><<<grid, 256, 0, st>>>(p);
+    else outer_join_kernel<1><<<grid, 256, 0, st>>>(p);
     HVS_HIP(hipGetLastError());
     return 0;
 }
@@ -1333,11 +1365,17 @@ static int run_backward(hipStream_t st, const hvs_adapters *ad, const void *grad
     const int es = hvs_elem_size(DT), epc = Elem<DT>::EPC, rp = round_up(ad->rank, 16);
     const int dop = round_up(ad->d_out, epc);
     // the weights of the transposed product; frozen W too is laid out by every call, so that nothing can be out of date
+    TransposeJobs jobs = {};
+    int k = 0;
+    jobs.job[k++] = transpose_job(ad->b, ad->n_adapters, ad->d_out, ad->rank, dop, ws.b_t);
     if (grad_x) {
-        HVS_TRY(launch_transpose<DT>(st, ad->projection, 1, ad->d_out, ad->d_in, dop, ws.w_t));
-        HVS_TRY(launch_transpose<DT>(st, ad->a, ad->n_adapters, ad->rank, ad->d_in, rp, ws.a_t));
+        jobs.job[k++] = transpose_job(ad->projection, 1, ad->d_out, ad->d_in, dop, ws.w_t);
+        jobs.job[k++] = transpose_job(ad->a, ad->n_adapters, ad->rank, ad->d_in, rp, ws.a_t);
     }
-    HVS_TRY(launch_transpose<DT>(st, ad->b, ad->n_adapters, ad->d_out, ad->rank, dop, ws.b_t));
+    const int64_t blocks = jobs.job[0].blocks + jobs.job[1].blocks + jobs.job[2].blocks;
+    HVS_REQUIRE(blocks <= 0x7FFFFFFF, "hvs_adapters_backward: %d adapters of %d x %d x %d are too many for one launch", ad->n_adapters, ad->rank, ad->d_in, ad->d_out);
+    transpose_kernel<typename Elem<DT>::type><<<(unsigned)blocks, 256, 0, st>>>(jobs);
+    HVS_HIP(hipGetLastError());
     for (int64_t r0 = 0; r0 < n; r0 += nc) {
         const int rows = (int)(n - r0 < nc ? n - r0 : nc);
         HVS_TRY(launch_group(st, codes + r0, rows, ad->n_adapters, ws));
@@ -1348,13 +1386,11 @@ static int run_backward(hipStream_t st, const hvs_adapters *ad, const void *grad
         d.out = grad_x ? (char *)grad_x + r0 * ld_gx * es : nullptr, d.ld_out = ld_gx;
         HVS_TRY(run_direction<DT>(st, ad, d, codes + r0, rows, ws.hidden, ws, true));
         OuterParams o = {};
-        o.scodes = ws.scodes, o.order = ws.order, o.seg_begin = ws.seg_begin, o.scale = ad->scale, o.partial = ws.partial;
-        o.n = rows, o.r = ad->rank, o.S = ad->n_adapters, o.accumulate = r0 > 0;
-        o.q = ws.hidden, o.x = (const char *)x + r0 * ld_x * es, o.ld_x = ld_x, o.d = ad->d_in, o.out = grad_a, o.transposed = 0;
-        o.rows_per = outer_rows_per(rows, o.d, DT);
-        HVS_TRY(launch_outer<DT>(st, o));
-        o.q = hidden + r0 * ad->rank, o.x = d.x, o.ld_x = ld_grad, o.d = ad->d_out, o.out = grad_b, o.transposed = 1;
-        o.rows_per = outer_rows_per(rows, o.d, DT);
+        o.scodes = ws.scodes, o.order = ws.order, o.seg_begin = ws.seg_begin, o.scale = ad->scale;
+        o.n = rows, o.r = ad->rank, o.S = ad->n_adapters, o.accumulate = r0 > 0, o.rows_per = outer_rows_per(rows, ad);
+        const char *xr = (const char *)x + r0 * ld_x * es;
+        o.problem[0] = {ws.hidden, xr, ld_x, grad_a, ws.partial_a, ad->d_in, 0, outer_cols(ad->d_in, DT)};
+        o.problem[1] = {hidden + r0 * ad->rank, d.x, ld_grad, grad_b, ws.partial_b, ad->d_out, 1, outer_cols(ad->d_out, DT)};
         HVS_TRY(launch_outer<DT>(st, o));
     }
     return 0;
