@@ -12,8 +12,6 @@
 // two that brings its largest element to [0.5, 1) (no overflow in fp16 whatever the inputs), split into two 16-bit parts
 // hi + lo (relative error 2^-16 for bf16, 2^-22 for fp16: far below the output's own rounding), and the product is
 // multiplied by that power and by s_c as it is added to W x.
-#include <atomic>
-
 #include "hvs_learn.h"
 
 #define ONCE_ROWS 2  // rows up to which one launch does all
@@ -1097,14 +1095,13 @@ static int launch_group(hipStream_t st, const int32_t *codes, int n, int S, cons
     int bits = 1;
     while ((1 << bits) < S + 2) bits++;
     if (chunks > GROUP_SELF) {
-        if (lds > 48 * 1024) HVS_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(&group_count_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+        HVS_TRY((learn_allow_lds<group_count_kernel>((int)lds)));
         group_count_kernel<<<chunks, GROUP_CHUNK, lds, st>>>(codes, n, S, ws.counts);
     }
     if (S + 2 <= GROUP_FEW_BINS) {
         group_place_kernel<true><<<chunks, GROUP_CHUNK, 2 * lds, st>>>(codes, n, S, bits, chunks, ws.counts, ws.order, ws.scodes, ws.seg_begin);
     } else {
-        if (2 * lds > 48 * 1024)
-            HVS_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(&group_place_kernel<false>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)(2 * lds)));
+        HVS_TRY((learn_allow_lds<group_place_kernel<false>>((int)(2 * lds))));
         group_place_kernel<false><<<chunks, GROUP_CHUNK, 2 * lds, st>>>(codes, n, S, bits, chunks, ws.counts, ws.order, ws.scodes, ws.seg_begin);
     }
     HVS_HIP(hipGetLastError());
@@ -1150,19 +1147,6 @@ template <int DT> static int launch_few(hipStream_t st, const ProjectParams &p) 
     return 0;
 }
 
-// Lets a kernel have `lds` bytes of LDS on the current device; asked once per kernel and device (the request costs a
-// microsecond, and the answer does not change).
-template <auto *KERNEL> static int allow_lds(int lds) {
-    static std::atomic<uint64_t> done{0};
-    int device = 0;
-    HVS_HIP(hipGetDevice(&device));
-    const uint64_t bit = device < 64 ? 1ull << device : 0;
-    if (done.load(std::memory_order_relaxed) & bit) return 0;
-    HVS_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(KERNEL), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
-    done.fetch_or(bit, std::memory_order_relaxed);
-    return 0;
-}
-
 template <int DT> static int launch_once(hipStream_t st, const ProjectParams &p, float *hidden, const void *a, int64_t lda) {
     const int es = hvs_elem_size(DT), grid = (p.N + 15) / 16;
     const int64_t row = (int64_t)p.K * es;
@@ -1183,7 +1167,7 @@ template <int DT> static int launch_once(hipStream_t st, const ProjectParams &p,
 template <int DT, class T> static int launch_tile(hipStream_t st, const ProjectParams &p) {
     const int tiles = ((p.N + T::BM - 1) / T::BM) * ((p.n + T::BN - 1) / T::BN);
     const size_t lds = 2 * T::STAGE_BYTES;
-    HVS_TRY((allow_lds<project_tile_kernel<DT, T>>((int)lds)));
+    HVS_TRY((learn_allow_lds<project_tile_kernel<DT, T>>((int)lds)));
     const int resident = 256 * (512 / T::GT);  // blocks the chip holds at once
     project_tile_kernel<DT, T><<<tiles < resident ? tiles : resident, T::GT, lds, st>>>(p);
     HVS_HIP(hipGetLastError());

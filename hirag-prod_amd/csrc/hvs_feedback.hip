@@ -30,13 +30,21 @@ struct PreferenceParams {
     int per_block;    // pairs a block takes before a second one joins in
 };
 
-// eight consecutive elements of a row as fp32, zeros past its end
-template <int DT, bool ALIGNED> __device__ __forceinline__ void load8(const void *base, int64_t row, int64_t ld, int k, int dim, float *out) {
+// eight consecutive elements of a row as they lie in memory, zeros past its end, and as fp32
+template <int DT> struct Raw8 {
+    f32x4 c[8 / Elem<DT>::EPC];
+};
+template <int DT, bool ALIGNED> __device__ __forceinline__ void load8(const void *base, int64_t row, int64_t ld, int k, int dim, Raw8<DT> &out) {
     typedef typename Elem<DT>::type E;
     constexpr int EPC = Elem<DT>::EPC;
     const E *p = reinterpret_cast<const E *>(base) + row * ld;
 #pragma unroll
-    for (int i = 0; i < 8; i += EPC) chunk_to_float<DT>(load_chunk<DT, ALIGNED>(p, k + i, dim), out + i);
+    for (int i = 0; i < 8 / EPC; i++) out.c[i] = load_chunk<DT, ALIGNED>(p, k + i * EPC, dim);
+}
+template <int DT> __device__ __forceinline__ void raw8_to_float(const Raw8<DT> &r, float *out) {
+    constexpr int EPC = Elem<DT>::EPC;
+#pragma unroll
+    for (int i = 0; i < 8 / EPC; i++) chunk_to_float<DT>(r.c[i], out + i * EPC);
 }
 
 __device__ __forceinline__ float softplus(float z) { return fmaxf(z, 0.0f) + log1pf(expf(-fabsf(z))); }
@@ -61,13 +69,15 @@ __device__ __forceinline__ void pair_share(const PreferenceParams &p, int64_t q,
     used = len > 0 ? (int)((len + per - 1) / per) : 1;
 }
 
-// A team of TW waves holds a whole row in registers, CH x 8 elements a lane: the query, the reference query, the two rows
-// of the pair at hand and the gradient sum.  The block's teams take the pairs of its share in turn and add up in team order.
+// A team of TW waves holds the rows of a pair, CH x 8 elements a lane, as they lie in memory, and the gradient sum in fp32;
+// the rows of the team's next pair are on their way meanwhile.  Teams of one wave read the query and the reference query
+// from LDS (registers then allow four waves per SIMD), larger teams hold their part.  The block's teams take the pairs of
+// its share in turn and are added up in team order.  Bound by reading the rows.
 template <int QDT, int RDT, int CH, int TW, int WAVES, bool ALIGNED>
 __global__ __launch_bounds__(64 * WAVES) void preference_kernel(PreferenceParams p) {
     typedef typename Elem<QDT>::type Q;
-    constexpr int TEAMS = WAVES / TW, NE = CH * 8;
-    extern __shared__ float vec[];  // [dim]
+    constexpr int TEAMS = WAVES / TW, SPAN = CH * TW * 512;  // SPAN: dim rounded up to what a team covers
+    extern __shared__ __attribute__((aligned(16))) float smem[];  // TW 1: [2][SPAN] the queries, then [TEAMS][SPAN]; else [dim]
     __shared__ float sums[WAVES][8];
     __shared__ float num[TEAMS];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -80,111 +90,179 @@ __global__ __launch_bounds__(64 * WAVES) void preference_kernel(PreferenceParams
     if (z >= used) return;
     const int64_t lo = b0 + z * per, hi = lo + per < b1 ? lo + per : b1;
 
-    // sums over a team's elements, the same value in every lane
-    auto team_sum = [&](float *v, int count) {
-#pragma unroll 8
-        for (int i = 0; i < count; i++) v[i] = learn_wave_sum(v[i]);
+    // eight sums over a team's elements, the same in every lane
+    auto team_sum = [&](const float *v, float *s) {
+        learn_wave_sum8(v, s);
         if (TW > 1) {
             __syncthreads();
             if (lane == 0)
-                for (int i = 0; i < count; i++) sums[wave][i] = v[i];
-            __syncthreads();
-            for (int i = 0; i < count; i++) {
-                v[i] = 0.0f;
 #pragma unroll
-                for (int w = 0; w < TW; w++) v[i] += sums[team * TW + w][i];
+                for (int i = 0; i < 8; i++) sums[wave][i] = s[i];
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                s[i] = 0.0f;
+#pragma unroll
+                for (int w = 0; w < TW; w++) s[i] += sums[team * TW + w][i];
             }
         }
     };
+    auto left_out = [&](int64_t a, int64_t b) { return a < 0 || b < 0 || a >= p.n_rows || b >= p.n_rows; };
 
-    float y[NE], f[NE], g[NE];
-    float norms[2] = {0.0f, 0.0f};
-#pragma unroll
-    for (int c = 0; c < CH; c++) {
-        const int k = (c * TW * 64 + tl) * 8;
-        load8<QDT, ALIGNED>(p.y, q, p.ld_y, k, p.dim, y + c * 8);
-        if (p.ref) load8<QDT, ALIGNED>(p.ref, q, p.ld_ref, k, p.dim, f + c * 8);
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            if (!p.ref) f[c * 8 + i] = 0.0f;
-            norms[0] = fmaf(y[c * 8 + i], y[c * 8 + i], norms[0]);
-            norms[1] = fmaf(f[c * 8 + i], f[c * 8 + i], norms[1]);
-            g[c * 8 + i] = 0.0f;
-        }
-    }
-    team_sum(norms, 2);
-    const float inv_y = inverse_norm(norms[0]), inv_f = inverse_norm(norms[1]);
-    float total = 0.0f;  // sum of g_p s_p
-
-    for (int64_t i = lo + team; i < hi; i += TEAMS) {
-        const int64_t a = p.chosen[i], b = p.rejected[i];
-        if (a < 0 || b < 0 || a >= p.n_rows || b >= p.n_rows) {
-            const bool left_out = a < 0 || b < 0;
-            const float v = left_out ? 0.0f : __builtin_nanf("");
-            if (tl == 0) p.loss[i] = p.margin[i] = v;
-            total += v;
-            continue;
-        }
-        float ra[NE], rb[NE];
+    // the first pair's positions and rows
+    int64_t i = lo + team, a = -1, b = -1, a_next = -1, b_next = -1;
+    if (i < hi) a = p.chosen[i], b = p.rejected[i];
+    if (i + TEAMS < hi) a_next = p.chosen[i + TEAMS], b_next = p.rejected[i + TEAMS];
+    Raw8<RDT> ra[CH], rb[CH];
+    auto fetch = [&](int64_t ka, int64_t kb) {
+        if (left_out(ka, kb)) return;
 #pragma unroll
         for (int c = 0; c < CH; c++) {
             const int k = (c * TW * 64 + tl) * 8;
-            load8<RDT, ALIGNED>(p.rows, a, p.ld_rows, k, p.dim, ra + c * 8);
-            load8<RDT, ALIGNED>(p.rows, b, p.ld_rows, k, p.dim, rb + c * 8);
+            load8<RDT, ALIGNED>(p.rows, ka, p.ld_rows, k, p.dim, ra[c]);
+            load8<RDT, ALIGNED>(p.rows, kb, p.ld_rows, k, p.dim, rb[c]);
         }
-        float s[6] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+    };
+    fetch(a, b);
+
+    float y_own[TW > 1 ? CH * 8 : 1], f_own[TW > 1 ? CH * 8 : 1], g[CH * 8];
+    float inv_y, inv_f;
+    {
+        float part[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f}, s[8];
 #pragma unroll
-        for (int e = 0; e < NE; e++) {
-            s[0] = fmaf(y[e], ra[e], s[0]);
-            s[1] = fmaf(y[e], rb[e], s[1]);
-            s[2] = fmaf(ra[e], ra[e], s[2]);
-            s[3] = fmaf(rb[e], rb[e], s[3]);
-            s[4] = fmaf(f[e], ra[e], s[4]);
-            s[5] = fmaf(f[e], rb[e], s[5]);
-        }
-        team_sum(s, 6);
-        const float ia = inverse_norm(s[2]), ib = inverse_norm(s[3]);
-        const float cos = inv_y * product_difference(s[0], ia, s[1], ib);
-        const float m = product_difference(1.0f, cos, inv_f, product_difference(s[4], ia, s[5], ib));
-        const float h = p.beta * m, e = p.smoothing;
-        const float up = 1.0f / (1.0f + expf(-h)), down = 1.0f / (1.0f + expf(h));  // sigma(h), sigma(-h): each without cancellation
-        if (tl == 0) {
-            p.loss[i] = (1.0f - e) * softplus(-h) + e * softplus(h);
-            p.margin[i] = m;
-        }
-        const float w = (p.weights ? p.weights[i] : p.default_weight) * p.beta * (e * up - (1.0f - e) * down);
-        total = fmaf(w, cos, total);
-        const float wa = w * ia, wb = w * ib;
+        for (int c = 0; c < CH; c++) {
+            const int k = (c * TW * 64 + tl) * 8;
+            Raw8<QDT> raw;
+            float yv[8], fv[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+            load8<QDT, ALIGNED>(p.y, q, p.ld_y, k, p.dim, raw);
+            raw8_to_float<QDT>(raw, yv);
+            if (p.ref) {
+                load8<QDT, ALIGNED>(p.ref, q, p.ld_ref, k, p.dim, raw);
+                raw8_to_float<QDT>(raw, fv);
+            }
 #pragma unroll
-        for (int k = 0; k < NE; k++) g[k] = fmaf(wa, ra[k], fmaf(-wb, rb[k], g[k]));
+            for (int e = 0; e < 8; e++) {
+                part[0] = fmaf(yv[e], yv[e], part[0]);
+                part[1] = fmaf(fv[e], fv[e], part[1]);
+                g[c * 8 + e] = 0.0f;
+                if (TW > 1) y_own[c * 8 + e] = yv[e], f_own[c * 8 + e] = fv[e];
+            }
+            if (TW == 1 && team == c % TEAMS) {  // every wave has loaded all of both: one of them puts each piece down
+                f32x4 *yl = reinterpret_cast<f32x4 *>(smem + k), *fl = reinterpret_cast<f32x4 *>(smem + SPAN + k);
+                yl[0] = f32x4{yv[0], yv[1], yv[2], yv[3]}, yl[1] = f32x4{yv[4], yv[5], yv[6], yv[7]};
+                fl[0] = f32x4{fv[0], fv[1], fv[2], fv[3]}, fl[1] = f32x4{fv[4], fv[5], fv[6], fv[7]};
+            }
+        }
+        team_sum(part, s);
+        inv_y = inverse_norm(s[0]);
+        inv_f = inverse_norm(s[1]);
+    }
+    if (TW == 1) __syncthreads();
+    auto query8 = [&](int which, int c, float *out) {  // this lane's piece c of the query (0) or the reference (1)
+        if (TW > 1) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) out[e] = which ? f_own[c * 8 + e] : y_own[c * 8 + e];
+        } else {
+            const f32x4 *l = reinterpret_cast<const f32x4 *>(smem + which * SPAN + (c * 64 + tl) * 8);
+            const f32x4 v0 = l[0], v1 = l[1];
+#pragma unroll
+            for (int e = 0; e < 4; e++) out[e] = v0[e], out[4 + e] = v1[e];
+        }
+    };
+
+    float total = 0.0f;  // sum of g_p s_p
+    for (; i < hi; i += TEAMS) {
+        if (left_out(a, b)) {
+            const float v = a < 0 || b < 0 ? 0.0f : __builtin_nanf("");
+            if (tl == 0) p.loss[i] = p.margin[i] = v;
+            total += v;
+        } else {
+            float part[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f}, s[8];
+#pragma unroll
+            for (int c = 0; c < CH; c++) {
+                float av[8], bv[8], yv[8];
+                raw8_to_float<RDT>(ra[c], av);
+                raw8_to_float<RDT>(rb[c], bv);
+                query8(0, c, yv);
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    part[0] = fmaf(yv[e], av[e], part[0]);
+                    part[1] = fmaf(yv[e], bv[e], part[1]);
+                    part[2] = fmaf(av[e], av[e], part[2]);
+                    part[3] = fmaf(bv[e], bv[e], part[3]);
+                }
+                if (p.ref) {
+                    query8(1, c, yv);
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        part[4] = fmaf(yv[e], av[e], part[4]);
+                        part[5] = fmaf(yv[e], bv[e], part[5]);
+                    }
+                }
+            }
+            team_sum(part, s);
+            const float ia = inverse_norm(s[2]), ib = inverse_norm(s[3]);
+            const float cos = inv_y * product_difference(s[0], ia, s[1], ib);
+            const float m = product_difference(1.0f, cos, inv_f, product_difference(s[4], ia, s[5], ib));
+            const float h = p.beta * m, e = p.smoothing;
+            const float up = 1.0f / (1.0f + expf(-h)), down = 1.0f / (1.0f + expf(h));  // sigma(h), sigma(-h): each without cancellation
+            if (tl == 0) {
+                p.loss[i] = (1.0f - e) * softplus(-h) + e * softplus(h);
+                p.margin[i] = m;
+            }
+            const float w = (p.weights ? p.weights[i] : p.default_weight) * p.beta * (e * up - (1.0f - e) * down);
+            total = fmaf(w, cos, total);
+            const float wa = w * ia, wb = w * ib;
+#pragma unroll
+            for (int c = 0; c < CH; c++) {
+                if (RDT != HVS_F32)  // convert the rows again rather than keep them twice as wide across the sums
+#pragma unroll
+                    for (int k = 0; k < 8 / Elem<RDT>::EPC; k++) asm volatile("" : "+v"(ra[c].c[k]), "+v"(rb[c].c[k]));
+                float av[8], bv[8];
+                raw8_to_float<RDT>(ra[c], av);
+                raw8_to_float<RDT>(rb[c], bv);
+#pragma unroll
+                for (int k = 0; k < 8; k++) g[c * 8 + k] = fmaf(wa, av[k], fmaf(-wb, bv[k], g[c * 8 + k]));
+            }
+        }
+        a = a_next, b = b_next;
+        fetch(a, b);
+        a_next = b_next = -1;
+        if (i + 2 * TEAMS < hi) a_next = p.chosen[i + 2 * TEAMS], b_next = p.rejected[i + 2 * TEAMS];
     }
 
     // the teams that had pairs, in team order
     const int busy = TEAMS == 1 ? 1 : (hi - lo < TEAMS ? (hi - lo > 0 ? (int)(hi - lo) : 1) : TEAMS);
+    float *vec = smem + (TW == 1 ? 2 * SPAN : 0);
     if (tl == 0) num[team] = total;
-    for (int t = 0; t < busy; t++) {
-        if (team == t) {
+    if (team < busy) {
 #pragma unroll
-            for (int c = 0; c < CH; c++) {
-                const int k = (c * TW * 64 + tl) * 8;
+        for (int c = 0; c < CH; c++) {
+            const int k = (c * TW * 64 + tl) * 8;
+            if (TW == 1) {
+                f32x4 *l = reinterpret_cast<f32x4 *>(vec + team * SPAN + k);
+                l[0] = f32x4{g[c * 8], g[c * 8 + 1], g[c * 8 + 2], g[c * 8 + 3]};
+                l[1] = f32x4{g[c * 8 + 4], g[c * 8 + 5], g[c * 8 + 6], g[c * 8 + 7]};
+            } else {
 #pragma unroll
-                for (int i = 0; i < 8; i++)
-                    if (k + i < p.dim) vec[k + i] = t == 0 ? g[c * 8 + i] : vec[k + i] + g[c * 8 + i];
+                for (int e = 0; e < 8; e++)
+                    if (k + e < p.dim) vec[k + e] = g[c * 8 + e];
             }
         }
-        __syncthreads();
     }
+    __syncthreads();
     float sum = 0.0f;
     for (int t = 0; t < busy; t++) sum += num[t];
-    if (used == 1) {
-        const Q *yr = reinterpret_cast<const Q *>(p.y) + q * p.ld_y;
-        Q *out = reinterpret_cast<Q *>(p.grad) + q * p.ld_grad;
-        for (int k = tid; k < p.dim; k += 64 * WAVES) out[k] = learn_from_float<Q>(inv_y * (vec[k] - sum * inv_y * learn_to_float(yr[k])));
-    } else {
-        float *pv = p.part_vec + (q * shares + z) * p.dim;
-        for (int k = tid; k < p.dim; k += 64 * WAVES) pv[k] = vec[k];
-        if (tid == 0) p.part_num[q * shares + z] = sum;
+    const Q *yr = reinterpret_cast<const Q *>(p.y) + q * p.ld_y;
+    Q *out = reinterpret_cast<Q *>(p.grad) + q * p.ld_grad;
+    float *pv = used == 1 ? nullptr : p.part_vec + (q * shares + z) * p.dim;
+    for (int k = tid; k < p.dim; k += 64 * WAVES) {
+        float v = vec[k];
+        for (int t = 1; t < busy; t++) v += vec[t * SPAN + k];
+        if (used == 1) out[k] = learn_from_float<Q>(inv_y * (v - sum * inv_y * (TW == 1 ? smem[k] : learn_to_float(yr[k]))));
+        else pv[k] = v;
     }
+    if (used > 1 && tid == 0) p.part_num[q * shares + z] = sum;
 }
 
 // queries whose pairs several blocks shared: their sums in share order
@@ -216,15 +294,18 @@ template <int QDT> __global__ __launch_bounds__(256) void preference_join_kernel
     }
 }
 
-#define PREF_FEW 512      // queries up to which a block has 16 waves and several blocks may share a query's pairs
-#define PREF_BLOCKS 1024  // ... so that about this many blocks are launched
-#define PREF_WAVE_DIM 2048
+#define PREF_FEW 512         // queries up to which several blocks may share a query's pairs,
+#define PREF_BLOCKS 1024     // ... about this many blocks in all,
+#define PREF_SHARE_PAIRS 16  // ... with this many pairs each
+#define PREF_WAVE_DIM 2048   // columns up to which a wave takes a pair by itself
 
 static int preference_shares(const hvs_preference *p) {
-    if (p->n_queries < 1 || p->n_queries >= PREF_FEW || p->n_pairs <= 16) return 1;
-    const int64_t by_blocks = PREF_BLOCKS / p->n_queries, by_pairs = (p->n_pairs + 15) / 16;
-    return (int)(by_blocks < by_pairs ? by_blocks : by_pairs);
+    if (p->n_queries < 1 || p->n_queries >= PREF_FEW) return 1;
+    const int64_t by_blocks = PREF_BLOCKS / p->n_queries, each = PREF_SHARE_PAIRS * p->n_queries, by_pairs = (p->n_pairs + each - 1) / each;
+    return (int)(by_pairs < 1 ? 1 : (by_blocks < by_pairs ? by_blocks : by_pairs));
 }
+// 16 waves a block where few queries have many pairs each, so that one query's pairs are in flight together; else 4
+static bool preference_wide(const hvs_preference *p) { return p->n_queries < PREF_FEW && p->n_pairs > 8 * p->n_queries; }
 
 static int check_preference(const char *who, const hvs_preference *p, int dim) {
     HVS_REQUIRE(p != nullptr, "%s: NULL argument", who);
@@ -253,23 +334,19 @@ extern "C" int hvs_preference_workspace(const hvs_preference *p, int dim, uint64
 template <int QDT, int RDT, int CH, int TW, int WAVES>
 static int launch_preference(hipStream_t st, const PreferenceParams &p, int64_t nq, int shares, bool aligned) {
     const dim3 grid((unsigned)nq, shares);
-    const size_t lds = (size_t)p.dim * 4;
+    const size_t lds = (TW == 1 ? (size_t)(2 + WAVES) * CH * 512 : (size_t)p.dim) * 4;
     if (aligned) {
-        if (lds > 48 * 1024)
-            HVS_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(&preference_kernel<QDT, RDT, CH, TW, WAVES, true>),
-                                        hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+        HVS_TRY((learn_allow_lds<preference_kernel<QDT, RDT, CH, TW, WAVES, true>>((int)lds)));
         preference_kernel<QDT, RDT, CH, TW, WAVES, true><<<grid, 64 * WAVES, lds, st>>>(p);
     } else {
-        if (lds > 48 * 1024)
-            HVS_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(&preference_kernel<QDT, RDT, CH, TW, WAVES, false>),
-                                        hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+        HVS_TRY((learn_allow_lds<preference_kernel<QDT, RDT, CH, TW, WAVES, false>>((int)lds)));
         preference_kernel<QDT, RDT, CH, TW, WAVES, false><<<grid, 64 * WAVES, lds, st>>>(p);
     }
     HVS_HIP(hipGetLastError());
     return 0;
 }
 
-template <int QDT, int RDT> static int run_preference(hipStream_t st, const PreferenceParams &p, int64_t nq, int shares) {
+template <int QDT, int RDT> static int run_preference(hipStream_t st, const PreferenceParams &p, int64_t nq, int shares, bool wide) {
     const int qs = hvs_elem_size(QDT), rs = hvs_elem_size(RDT);
     const bool al = p.dim % 8 == 0 && learn_aligned(p.y, p.ld_y * qs, 0) && (!p.ref || learn_aligned(p.ref, p.ld_ref * qs, 0)) &&
                     learn_aligned(p.rows, p.ld_rows * rs, 0);
@@ -277,8 +354,7 @@ template <int QDT, int RDT> static int run_preference(hipStream_t st, const Pref
     else if (p.dim > PREF_WAVE_DIM) HVS_TRY((launch_preference<QDT, RDT, 1, 16, 16>(st, p, nq, shares, al)));
     else {
         const int ch = (p.dim + 511) / 512;
-        // few queries: 16 waves a block, so that the pairs of one query are in flight together
-#define PREF(CH_) (nq < PREF_FEW ? launch_preference<QDT, RDT, CH_, 1, 16>(st, p, nq, shares, al) : launch_preference<QDT, RDT, CH_, 1, 4>(st, p, nq, shares, al))
+#define PREF(CH_) (wide ? launch_preference<QDT, RDT, CH_, 1, 16>(st, p, nq, shares, al) : launch_preference<QDT, RDT, CH_, 1, 4>(st, p, nq, shares, al))
         if (ch == 1) HVS_TRY(PREF(1));
         else if (ch == 2) HVS_TRY(PREF(2));
         else if (ch == 3) HVS_TRY(PREF(3));
@@ -317,16 +393,16 @@ static int preference_core(const char *who, hipStream_t st, const hvs_preference
     k.loss = p->loss, k.margin = p->margin, k.grad = p->grad, k.ld_grad = p->ld_grad, k.n_pairs = p->n_pairs;
     k.rows = rows, k.ld_rows = ld_rows, k.n_rows = n_rows, k.dim = dim;
     k.beta = p->beta, k.smoothing = p->label_smoothing, k.default_weight = p->n_pairs > 0 ? (float)(1.0 / (double)p->n_pairs) : 0.0f;
-    k.per_block = 16;
+    k.per_block = PREF_SHARE_PAIRS;
     if (shares > 1) {
         WorkspaceCut w(workspace);
         k.part_vec = w.take<float>((uint64_t)p->n_queries * shares * dim * 4);
         k.part_num = w.take<float>((uint64_t)p->n_queries * shares * 4);
     }
 #define ROWS(Q_)                                                                             \
-    (rows_dtype == HVS_F32 ? run_preference<Q_, HVS_F32>(st, k, p->n_queries, shares)        \
-                           : rows_dtype == HVS_F16 ? run_preference<Q_, HVS_F16>(st, k, p->n_queries, shares) \
-                                                   : run_preference<Q_, HVS_BF16>(st, k, p->n_queries, shares))
+    (rows_dtype == HVS_F32 ? run_preference<Q_, HVS_F32>(st, k, p->n_queries, shares, preference_wide(p))        \
+                           : rows_dtype == HVS_F16 ? run_preference<Q_, HVS_F16>(st, k, p->n_queries, shares, preference_wide(p)) \
+                                                   : run_preference<Q_, HVS_BF16>(st, k, p->n_queries, shares, preference_wide(p)))
     if (p->query_dtype == HVS_F32) return ROWS(HVS_F32);
     if (p->query_dtype == HVS_F16) return ROWS(HVS_F16);
     return ROWS(HVS_BF16);

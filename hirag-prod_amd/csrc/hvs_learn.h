@@ -1,6 +1,9 @@
 // Device and host helpers shared by the learning kernels (hvs_adapters.hip, hvs_feedback.hip): element access for the
 // three dtypes, 16-byte chunks with guards, wave sums, the current-device guard.
 #pragma once
+#include <atomic>
+#include <mutex>
+
 #include "hvs_gemm_tile.h"
 
 template <int DT> struct Elem;
@@ -89,6 +92,32 @@ __device__ __forceinline__ float learn_wave_sum(float v) {
     return v;
 }
 
+template <int CTRL> __device__ __forceinline__ float learn_dpp(float v) {
+    return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), CTRL, 0xF, 0xF, true));
+}
+// Eight sums over the wave at once, in vector registers alone: halves trade places with the next value's, then quarters, so
+// that every step works on two values; a row of 16 lanes then holds one value and adds up by rotation.  s[i] becomes the
+// sum of v[i], the same in every lane.
+__device__ __forceinline__ void learn_wave_sum8(const float *v, float *s) {
+    float u[4], w[2];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[2 * i]), __float_as_uint(v[2 * i + 1]), false, false);
+        u[i] = __uint_as_float(r[0]) + __uint_as_float(r[1]);  // lanes 0-31: v[2 i], lanes 32-63: v[2 i + 1]
+    }
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(u[2 * i]), __float_as_uint(u[2 * i + 1]), false, false);
+        w[i] = __uint_as_float(r[0]) + __uint_as_float(r[1]);  // rows of 16: v[4 i], v[4 i + 2], v[4 i + 1], v[4 i + 3]
+        w[i] += learn_dpp<0x128>(w[i]);  // rotations by 8, 4, 2, 1
+        w[i] += learn_dpp<0x124>(w[i]);
+        w[i] += learn_dpp<0x122>(w[i]);
+        w[i] += learn_dpp<0x121>(w[i]);
+#pragma unroll
+        for (int k = 0; k < 4; k++) s[4 * i + k] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w[i]), (k & 1) * 32 + (k >> 1) * 16));
+    }
+}
+
 // Makes `device` current for a call and the caller's device current again after it.
 struct DeviceGuard {
     int before = -1;
@@ -102,6 +131,23 @@ struct DeviceGuard {
         if (before >= 0) (void)hipSetDevice(before);
     }
 };
+
+// Lets a kernel have `lds` bytes of dynamic LDS on the current device.  Below 48 KB nothing is asked; the request (a microsecond)
+// is made again only where the kernel has not been allowed as much on that device yet.
+template <auto *KERNEL> static int learn_allow_lds(int lds) {
+    static std::atomic<int> allowed[16];
+    static std::mutex asking;  // a request for less must not follow one for more
+    if (lds <= 48 * 1024) return 0;
+    int device = 0;
+    HVS_HIP(hipGetDevice(&device));
+    HVS_REQUIRE(device < 16, "device %d: at most 16 are served", device);
+    if (allowed[device].load(std::memory_order_acquire) >= lds) return 0;
+    const std::lock_guard<std::mutex> lock(asking);
+    if (allowed[device].load(std::memory_order_acquire) >= lds) return 0;
+    HVS_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(KERNEL), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+    allowed[device].store(lds, std::memory_order_release);
+    return 0;
+}
 
 static inline bool learn_dtype_ok(int dt) { return dt == HVS_F32 || dt == HVS_F16 || dt == HVS_BF16; }
 static inline bool learn_aligned(const void *p, int64_t ld_bytes, int64_t row_bytes) {
