@@ -48,6 +48,9 @@ def _need_tensor(name: str, t, device=None) -> None:
 
 def _rows(name: str, t, width: int, dtype, device, n: Optional[int] = None):
     """A [n, width] tensor whose rows are contiguous and do not overlap -> (tensor, row pitch in elements)."""
+    if (type(t) is torch.Tensor and t.dtype is dtype and t.dim() == 2 and t.is_contiguous() and t.device == device and t.shape[1] == width
+            and (n is None or t.shape[0] == n)):
+        return t, width
     _need_tensor(name, t, device)
     if t.dim() != 2 or t.shape[1] != width or (n is not None and t.shape[0] != n):
         raise ValueError(f"{name} must be [{'n' if n is None else n}, {width}], got {tuple(t.shape)}")
@@ -72,6 +75,9 @@ def _out_rows(name: str, t, n: int, width: int, dtype, device):
 
 def _numbers(name: str, values, n: Optional[int], dtype, device):
     """Whole numbers, one per row or pair, on the GPU."""
+    if (type(values) is torch.Tensor and values.dtype is dtype and values.dim() == 1 and values.is_contiguous() and values.device == device
+            and (n is None or values.shape[0] == n)):
+        return values
     if not isinstance(values, torch.Tensor):
         values = torch.as_tensor(np.ascontiguousarray(values), device=device)
     _need_tensor(name, values, device)
@@ -104,6 +110,14 @@ def _adapters_workspace(code: int, d_in: int, d_out: int, rank: int, n_adapters:
     need = ctypes.c_uint64(0)
     st = HvsAdaptersStruct(None, None, None, None, code, d_in, d_out, rank, n_adapters)
     check(load_library().hvs_adapters_workspace(ctypes.byref(st), n, max_ld, backward, ctypes.byref(need)))
+    return need.value
+
+
+@functools.lru_cache(maxsize=4096)
+def _preference_workspace(nq: int, pairs: int, dim: int) -> int:
+    need = ctypes.c_uint64(0)
+    st = HvsPreferenceStruct(n_queries=nq, n_pairs=pairs, query_dtype=_lib.HVS_F32, beta=1.0, label_smoothing=0.0)
+    check(load_library().hvs_preference_workspace(ctypes.byref(st), dim, ctypes.byref(need)))
     return need.value
 
 
@@ -257,16 +271,14 @@ def _preference(queries, dim, chosen, rejected, offsets, reference, beta, label_
         if weights.dtype != torch.float32 or tuple(weights.shape) != (pairs,):
             raise ValueError(f"weights must hold {pairs} float32 entries")
         weights = weights.contiguous()
-    loss = torch.empty(pairs, dtype=torch.float32, device=device)
-    margin = torch.empty(pairs, dtype=torch.float32, device=device)
+    loss, margin = torch.empty((2, pairs), dtype=torch.float32, device=device)
     grad = torch.empty((nq, dim), dtype=queries.dtype, device=device)
     st = HvsPreferenceStruct(queries.data_ptr(), ld, None if reference is None else reference.data_ptr(), ld_ref, offsets.data_ptr(), chosen.data_ptr(),
                              rejected.data_ptr(), None if weights is None else weights.data_ptr(), loss.data_ptr(), margin.data_ptr(),
                              grad.data_ptr(), dim, nq, pairs, code, float(beta), float(label_smoothing))
-    need = ctypes.c_uint64(0)
-    check(load_library().hvs_preference_workspace(ctypes.byref(st), dim, ctypes.byref(need)))
-    ws, ws_ptr = _scratch(need.value, device)
-    check(launch(ctypes.byref(st), _stream(device), ws_ptr, need.value))
+    size = _preference_workspace(nq, pairs, dim)
+    ws, ws_ptr = _scratch(size, device)
+    check(launch(ctypes.byref(st), _stream(device), ws_ptr, size))
     return loss, margin, grad
 
 
@@ -310,16 +322,19 @@ def clip_grad_norm(grads: Sequence, max_norm: float, norm_type: float = 2.0, out
         raise ValueError(f"out holds {len(outs)} tensors for {len(grads)}")
     _need_tensor("grads[0]", grads[0])
     device = grads[0].device
-    table = (HvsTensorStruct * len(grads))()
+    entries = []
     for i, (g, o) in enumerate(zip(grads, outs)):
-        _need_tensor(f"grads[{i}]", g, device)
+        if not isinstance(g, torch.Tensor) or g.device != device:
+            _need_tensor(f"grads[{i}]", g, device)
         if not g.is_contiguous():
             raise ValueError(f"grads[{i}] must be contiguous")
         if o is not g:
-            _need_tensor(f"out[{i}]", o, device)
+            if not isinstance(o, torch.Tensor) or o.device != device:
+                _need_tensor(f"out[{i}]", o, device)
             if o.shape != g.shape or o.dtype != g.dtype or not o.is_contiguous():
                 raise ValueError(f"out[{i}] must be contiguous, {tuple(g.shape)} of {g.dtype}")
-        table[i] = (g.data_ptr(), o.data_ptr(), g.numel(), _dtype_code(g))
+        entries.append((g.data_ptr(), o.data_ptr(), g.numel(), _dtype_code(g)))
+    table = (HvsTensorStruct * len(entries))(*entries)
     lib = load_library()
     norm = torch.empty((), dtype=torch.float32, device=device)
     need = ctypes.c_uint64(0)

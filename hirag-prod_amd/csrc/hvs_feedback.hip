@@ -9,9 +9,11 @@
 // ---------------------------------------------------------------------------------------------------------------
 // preference loss
 // ---------------------------------------------------------------------------------------------------------------
-// With c^ = c / |c| etc. and s = cos(y, c) - cos(y, r):  d s / d y = (c^ - r^ - s y^) / |y|, so the gradient of a query is
-//     (sum_p g_p (c^_p - r^_p)  -  (sum_p g_p s_p) y^) / |y|,   g_p = w_p beta (e sigma(h_p) - (1 - e) sigma(-h_p)):
-// one vector and one number are kept over the pairs of a query, and every row is read once.
+// With c^ = c / |c| etc., e_p = c^ - r^ and s_p = y^ . e_p (the difference of the cosines):  d s / d y = (e - s y^) / |y|, so the
+// gradient of a query is
+//     (sum_p g_p e_p  -  (sum_p g_p s_p) y^) / |y|,   g_p = w_p beta (eps sigma(h_p) - (1 - eps) sigma(-h_p)):
+// one vector and one number are kept over the pairs of a query, and every row is read once.  The margin, the small difference
+// of two such differences, is summed as (y^ - y0^) . e_p: both differences are taken element by element, before the sum.
 struct PreferenceParams {
     const void *y, *ref;
     int64_t ld_y, ld_ref;
@@ -47,15 +49,17 @@ template <int DT> __device__ __forceinline__ void raw8_to_float(const Raw8<DT> &
     for (int i = 0; i < 8 / EPC; i++) chunk_to_float<DT>(r.c[i], out + i * EPC);
 }
 
+// 16-bit rows are converted again for every use rather than kept twice as wide across the sums
+template <int DT, int CH> __device__ __forceinline__ void keep_raw(Raw8<DT> (&a)[CH], Raw8<DT> (&b)[CH]) {
+    if (DT == HVS_F32) return;
+#pragma unroll
+    for (int c = 0; c < CH; c++)
+#pragma unroll
+        for (int k = 0; k < 8 / Elem<DT>::EPC; k++) asm volatile("" : "+v"(a[c].c[k]), "+v"(b[c].c[k]));
+}
+
 __device__ __forceinline__ float softplus(float z) { return fmaxf(z, 0.0f) + log1pf(expf(-fabsf(z))); }
 __device__ __forceinline__ float inverse_norm(float sum_of_squares) { return sum_of_squares == 0.0f ? 0.0f : 1.0f / sqrtf(sum_of_squares); }
-
-// a x - b y with each product rounded by itself: equal pairs give exactly 0, which a fused multiply-add would not
-__device__ __forceinline__ float product_difference(float a, float x, float b, float y) {
-#pragma clang fp contract(off)
-    const float ax = a * x, by = b * y;
-    return ax - by;
-}
 
 // how the pairs [b0, b1) of a query are shared out; the same on every side that asks
 __device__ __forceinline__ void pair_share(const PreferenceParams &p, int64_t q, int shares, int64_t &b0, int64_t &b1, int64_t &per, int &used) {
@@ -78,7 +82,7 @@ __global__ __launch_bounds__(64 * WAVES) void preference_kernel(PreferenceParams
     typedef typename Elem<QDT>::type Q;
     constexpr int TEAMS = WAVES / TW, SPAN = CH * TW * 512;  // SPAN: dim rounded up to what a team covers
     extern __shared__ __attribute__((aligned(16))) float smem[];  // TW 1: [2][SPAN] the queries, then [TEAMS][SPAN]; else [dim]
-    __shared__ float sums[WAVES][8];
+    __shared__ float sums[WAVES][2];
     __shared__ float num[TEAMS];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int team = wave / TW, tl = (wave % TW) * 64 + lane;
@@ -90,21 +94,16 @@ __global__ __launch_bounds__(64 * WAVES) void preference_kernel(PreferenceParams
     if (z >= used) return;
     const int64_t lo = b0 + z * per, hi = lo + per < b1 ? lo + per : b1;
 
-    // eight sums over a team's elements, the same in every lane
-    auto team_sum = [&](const float *v, float *s) {
-        learn_wave_sum8(v, s);
+    // two sums over a team's elements, the same in every lane
+    auto team_sum = [&](float &a, float &b) {
+        learn_wave_sum2(a, b);
         if (TW > 1) {
             __syncthreads();
-            if (lane == 0)
-#pragma unroll
-                for (int i = 0; i < 8; i++) sums[wave][i] = s[i];
+            if (lane == 0) sums[wave][0] = a, sums[wave][1] = b;
             __syncthreads();
+            a = b = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                s[i] = 0.0f;
-#pragma unroll
-                for (int w = 0; w < TW; w++) s[i] += sums[team * TW + w][i];
-            }
+            for (int w = 0; w < TW; w++) a += sums[team * TW + w][0], b += sums[team * TW + w][1];
         }
     };
     auto left_out = [&](int64_t a, int64_t b) { return a < 0 || b < 0 || a >= p.n_rows || b >= p.n_rows; };
@@ -125,43 +124,56 @@ __global__ __launch_bounds__(64 * WAVES) void preference_kernel(PreferenceParams
     };
     fetch(a, b);
 
-    float y_own[TW > 1 ? CH * 8 : 1], f_own[TW > 1 ? CH * 8 : 1], g[CH * 8];
+    // y^ and y^ - y0^ (without a reference: y^), which the sums over a pair are taken with
+    float y_own[TW > 1 ? CH * 8 : 1], d_own[TW > 1 ? CH * 8 : 1], g[CH * 8];
     float inv_y, inv_f;
     {
-        float part[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f}, s[8];
+        Raw8<QDT> ry[CH], rf[CH];
+        float yy = 0.0f, ff = 0.0f;
 #pragma unroll
         for (int c = 0; c < CH; c++) {
             const int k = (c * TW * 64 + tl) * 8;
-            Raw8<QDT> raw;
-            float yv[8], fv[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-            load8<QDT, ALIGNED>(p.y, q, p.ld_y, k, p.dim, raw);
-            raw8_to_float<QDT>(raw, yv);
+            float v[8];
+            load8<QDT, ALIGNED>(p.y, q, p.ld_y, k, p.dim, ry[c]);
+            raw8_to_float<QDT>(ry[c], v);
+#pragma unroll
+            for (int e = 0; e < 8; e++) yy = fmaf(v[e], v[e], yy);
             if (p.ref) {
-                load8<QDT, ALIGNED>(p.ref, q, p.ld_ref, k, p.dim, raw);
-                raw8_to_float<QDT>(raw, fv);
+                load8<QDT, ALIGNED>(p.ref, q, p.ld_ref, k, p.dim, rf[c]);
+                raw8_to_float<QDT>(rf[c], v);
+#pragma unroll
+                for (int e = 0; e < 8; e++) ff = fmaf(v[e], v[e], ff);
             }
+#pragma unroll
+            for (int e = 0; e < 8; e++) g[c * 8 + e] = 0.0f;
+        }
+        team_sum(yy, ff);
+        inv_y = inverse_norm(yy);
+        inv_f = inverse_norm(ff);
+#pragma unroll
+        for (int c = 0; c < CH; c++) {
+            const int k = (c * TW * 64 + tl) * 8;
+            float yv[8], dv[8];
+            raw8_to_float<QDT>(ry[c], yv);
+            if (p.ref) raw8_to_float<QDT>(rf[c], dv);
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                part[0] = fmaf(yv[e], yv[e], part[0]);
-                part[1] = fmaf(fv[e], fv[e], part[1]);
-                g[c * 8 + e] = 0.0f;
-                if (TW > 1) y_own[c * 8 + e] = yv[e], f_own[c * 8 + e] = fv[e];
+                dv[e] = p.ref ? fmaf(yv[e], inv_y, -(dv[e] * inv_f)) : yv[e] * inv_y;
+                yv[e] *= inv_y;
+                if (TW > 1) y_own[c * 8 + e] = yv[e], d_own[c * 8 + e] = dv[e];
             }
-            if (TW == 1 && team == c % TEAMS) {  // every wave has loaded all of both: one of them puts each piece down
-                f32x4 *yl = reinterpret_cast<f32x4 *>(smem + k), *fl = reinterpret_cast<f32x4 *>(smem + SPAN + k);
+            if (TW == 1 && team == c % TEAMS) {  // every wave has all of both: one of them puts each piece down
+                f32x4 *yl = reinterpret_cast<f32x4 *>(smem + k), *dl = reinterpret_cast<f32x4 *>(smem + SPAN + k);
                 yl[0] = f32x4{yv[0], yv[1], yv[2], yv[3]}, yl[1] = f32x4{yv[4], yv[5], yv[6], yv[7]};
-                fl[0] = f32x4{fv[0], fv[1], fv[2], fv[3]}, fl[1] = f32x4{fv[4], fv[5], fv[6], fv[7]};
+                dl[0] = f32x4{dv[0], dv[1], dv[2], dv[3]}, dl[1] = f32x4{dv[4], dv[5], dv[6], dv[7]};
             }
         }
-        team_sum(part, s);
-        inv_y = inverse_norm(s[0]);
-        inv_f = inverse_norm(s[1]);
     }
     if (TW == 1) __syncthreads();
-    auto query8 = [&](int which, int c, float *out) {  // this lane's piece c of the query (0) or the reference (1)
+    auto query8 = [&](int which, int c, float *out) {  // this lane's piece c of y^ (0) or of the difference (1)
         if (TW > 1) {
 #pragma unroll
-            for (int e = 0; e < 8; e++) out[e] = which ? f_own[c * 8 + e] : y_own[c * 8 + e];
+            for (int e = 0; e < 8; e++) out[e] = which ? d_own[c * 8 + e] : y_own[c * 8 + e];
         } else {
             const f32x4 *l = reinterpret_cast<const f32x4 *>(smem + which * SPAN + (c * 64 + tl) * 8);
             const f32x4 v0 = l[0], v1 = l[1];
@@ -177,33 +189,35 @@ __global__ __launch_bounds__(64 * WAVES) void preference_kernel(PreferenceParams
             if (tl == 0) p.loss[i] = p.margin[i] = v;
             total += v;
         } else {
-            float part[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f}, s[8];
+            float ia = 0.0f, ib = 0.0f, cos = 0.0f, m = 0.0f;
 #pragma unroll
             for (int c = 0; c < CH; c++) {
-                float av[8], bv[8], yv[8];
+                float av[8], bv[8];
+                raw8_to_float<RDT>(ra[c], av);
+                raw8_to_float<RDT>(rb[c], bv);
+#pragma unroll
+                for (int e = 0; e < 8; e++) ia = fmaf(av[e], av[e], ia), ib = fmaf(bv[e], bv[e], ib);
+            }
+            team_sum(ia, ib);
+            // a row against itself is no preference: exactly 0, whatever the roundings below
+            ia = a == b ? 0.0f : inverse_norm(ia);
+            ib = a == b ? 0.0f : inverse_norm(ib);
+            keep_raw(ra, rb);
+#pragma unroll
+            for (int c = 0; c < CH; c++) {
+                float av[8], bv[8], yv[8], dv[8];
                 raw8_to_float<RDT>(ra[c], av);
                 raw8_to_float<RDT>(rb[c], bv);
                 query8(0, c, yv);
+                query8(1, c, dv);
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
-                    part[0] = fmaf(yv[e], av[e], part[0]);
-                    part[1] = fmaf(yv[e], bv[e], part[1]);
-                    part[2] = fmaf(av[e], av[e], part[2]);
-                    part[3] = fmaf(bv[e], bv[e], part[3]);
-                }
-                if (p.ref) {
-                    query8(1, c, yv);
-#pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        part[4] = fmaf(yv[e], av[e], part[4]);
-                        part[5] = fmaf(yv[e], bv[e], part[5]);
-                    }
+                    const float d = fmaf(av[e], ia, -(bv[e] * ib));
+                    cos = fmaf(yv[e], d, cos);
+                    m = fmaf(dv[e], d, m);
                 }
             }
-            team_sum(part, s);
-            const float ia = inverse_norm(s[2]), ib = inverse_norm(s[3]);
-            const float cos = inv_y * product_difference(s[0], ia, s[1], ib);
-            const float m = product_difference(1.0f, cos, inv_f, product_difference(s[4], ia, s[5], ib));
+            team_sum(cos, m);
             const float h = p.beta * m, e = p.smoothing;
             const float up = 1.0f / (1.0f + expf(-h)), down = 1.0f / (1.0f + expf(h));  // sigma(h), sigma(-h): each without cancellation
             if (tl == 0) {
@@ -213,11 +227,9 @@ __global__ __launch_bounds__(64 * WAVES) void preference_kernel(PreferenceParams
             const float w = (p.weights ? p.weights[i] : p.default_weight) * p.beta * (e * up - (1.0f - e) * down);
             total = fmaf(w, cos, total);
             const float wa = w * ia, wb = w * ib;
+            keep_raw(ra, rb);
 #pragma unroll
             for (int c = 0; c < CH; c++) {
-                if (RDT != HVS_F32)  // convert the rows again rather than keep them twice as wide across the sums
-#pragma unroll
-                    for (int k = 0; k < 8 / Elem<RDT>::EPC; k++) asm volatile("" : "+v"(ra[c].c[k]), "+v"(rb[c].c[k]));
                 float av[8], bv[8];
                 raw8_to_float<RDT>(ra[c], av);
                 raw8_to_float<RDT>(rb[c], bv);
@@ -259,7 +271,7 @@ __global__ __launch_bounds__(64 * WAVES) void preference_kernel(PreferenceParams
     for (int k = tid; k < p.dim; k += 64 * WAVES) {
         float v = vec[k];
         for (int t = 1; t < busy; t++) v += vec[t * SPAN + k];
-        if (used == 1) out[k] = learn_from_float<Q>(inv_y * (v - sum * inv_y * (TW == 1 ? smem[k] : learn_to_float(yr[k]))));
+        if (used == 1) out[k] = learn_from_float<Q>(inv_y * (v - sum * (TW == 1 ? smem[k] : inv_y * learn_to_float(yr[k]))));
         else pv[k] = v;
     }
     if (used > 1 && tid == 0) p.part_num[q * shares + z] = sum;
@@ -290,7 +302,7 @@ template <int QDT> __global__ __launch_bounds__(256) void preference_join_kernel
     for (int k = threadIdx.x; k < p.dim; k += 256) {
         float v = 0.0f;
         for (int z = 0; z < used; z++) v += p.part_vec[(q * shares + z) * p.dim + k];
-        out[k] = learn_from_float<Q>(inv_y * (v - sum * inv_y * learn_to_float(y[k])));
+        out[k] = learn_from_float<Q>(inv_y * (v - sum * (inv_y * learn_to_float(y[k]))));
     }
 }
 
@@ -368,8 +380,8 @@ template <int QDT, int RDT> static int run_preference(hipStream_t st, const Pref
     return 0;
 }
 
-static int preference_core(const char *who, hipStream_t st, const hvs_preference *p, const void *rows, int rows_dtype, int dim, int64_t ld_rows,
-                           int64_t n_rows, void *workspace, uint64_t workspace_bytes) {
+static int check_preference_buffers(const char *who, const hvs_preference *p, const void *rows, int rows_dtype, int dim, int64_t ld_rows, int64_t n_rows,
+                                    const void *workspace, uint64_t workspace_bytes) {
     const int qs = hvs_elem_size(p->query_dtype);
     HVS_REQUIRE(p->queries && p->grad && p->offsets, "%s: queries, grad or offsets is NULL", who);
     HVS_REQUIRE(p->n_pairs == 0 || (p->chosen && p->rejected && p->loss && p->margin), "%s: chosen, rejected, loss or margin is NULL", who);
@@ -386,6 +398,10 @@ static int preference_core(const char *who, hipStream_t st, const hvs_preference
     HVS_TRY(hvs_preference_workspace(p, dim, &need));
     HVS_REQUIRE(need == 0 || (workspace && ((uintptr_t)workspace & 255) == 0 && workspace_bytes >= need),
                 "%s: workspace of %llu bytes at %p, needs %llu aligned to 256", who, (unsigned long long)workspace_bytes, workspace, (unsigned long long)need);
+    return 0;
+}
+
+static int preference_core(hipStream_t st, const hvs_preference *p, const void *rows, int rows_dtype, int dim, int64_t ld_rows, int64_t n_rows, void *workspace) {
     const int shares = preference_shares(p);
     PreferenceParams k = {};
     k.y = p->queries, k.ref = p->reference, k.ld_y = p->ld_queries, k.ld_ref = p->ld_reference;
@@ -418,20 +434,10 @@ extern "C" int hvs_preference_loss(int device_id, void *stream, const hvs_prefer
         HVS_REQUIRE(p->n_pairs == 0, "%s: %lld pairs but no query", who, (long long)p->n_pairs);
         return 0;
     }
+    HVS_TRY(check_preference_buffers(who, p, rows, rows_dtype, dim, ld_rows, n_rows, workspace, workspace_bytes));
     DeviceGuard guard(device_id);
     HVS_HIP(guard.status);
-    return preference_core(who, (hipStream_t)stream, p, rows, rows_dtype, dim, ld_rows, n_rows, workspace, workspace_bytes);
-}
-
-// `to` waits for the work `from` holds now
-static int stream_after(hipStream_t to, hipStream_t from) {
-    hipEvent_t ev;
-    HVS_HIP(hipEventCreateWithFlags(&ev, hipEventDisableTiming));
-    hipError_t e = hipEventRecord(ev, from);
-    if (e == hipSuccess) e = hipStreamWaitEvent(to, ev, 0);
-    (void)hipEventDestroy(ev);  // released once the wait is done
-    HVS_HIP(e);
-    return 0;
+    return preference_core((hipStream_t)stream, p, rows, rows_dtype, dim, ld_rows, n_rows, workspace);
 }
 
 extern "C" int hvs_index_preference_loss(hvs_index *idx, void *stream, const hvs_preference *p, void *workspace, uint64_t workspace_bytes) {
@@ -442,15 +448,26 @@ extern "C" int hvs_index_preference_loss(hvs_index *idx, void *stream, const hvs
         HVS_REQUIRE(p->n_pairs == 0, "%s: %lld pairs but no query", who, (long long)p->n_pairs);
         return 0;
     }
+    HVS_TRY(check_preference_buffers(who, p, idx->rows, idx->dtype, idx->dim, idx->ld, idx->n, workspace, workspace_bytes));
     DeviceGuard guard(idx->device);
     HVS_HIP(guard.status);
     hipStream_t st = (hipStream_t)stream;
     hipStreamCaptureStatus capturing = hipStreamCaptureStatusNone;
     if (st != nullptr) HVS_HIP(hipStreamIsCapturing(st, &capturing));
     HVS_REQUIRE(capturing == hipStreamCaptureStatusNone, "%s: the stream is being captured; a graph would keep the address of rows the table may move", who);
-    if (st != idx->stream) HVS_TRY(stream_after(st, idx->stream));
-    HVS_TRY(preference_core(who, st, p, idx->rows, idx->dtype, idx->dim, idx->ld, idx->n, workspace, workspace_bytes));
-    if (st != idx->stream) HVS_TRY(stream_after(idx->stream, st));
+    if (st == idx->stream) return preference_core(st, p, idx->rows, idx->dtype, idx->dim, idx->ld, idx->n, workspace);
+    if (idx->ev_reader == nullptr) HVS_HIP(hipEventCreateWithFlags(&idx->ev_reader, hipEventDisableTiming | hipEventDisableSystemFence));
+    // after the work the table's stream holds: mostly it holds none, and then there is nothing to wait for
+    const hipError_t idle = hipStreamQuery(idx->stream);
+    if (idle == hipErrorNotReady) {
+        (void)hipGetLastError();  // an answer, not an error to be found by the next launch
+        HVS_HIP(hipEventRecord(idx->ev_reader, idx->stream));
+        HVS_HIP(hipStreamWaitEvent(st, idx->ev_reader, 0));
+    } else HVS_HIP(idle);
+    HVS_TRY(preference_core(st, p, idx->rows, idx->dtype, idx->dim, idx->ld, idx->n, workspace));
+    // what the table does next may move the rows: it waits for this read
+    HVS_HIP(hipEventRecord(idx->ev_reader, st));
+    HVS_HIP(hipStreamWaitEvent(idx->stream, idx->ev_reader, 0));
     return 0;
 }
 
@@ -458,7 +475,8 @@ extern "C" int hvs_index_preference_loss(hvs_index *idx, void *stream, const hvs
 // global norm and clipping
 // ---------------------------------------------------------------------------------------------------------------
 #define CLIP_BATCH 64      // tensors per launch: their table travels in the kernel's arguments
-#define CLIP_CHUNK 8192    // elements a block takes at a time
+#define CLIP_CHUNK 8192    // most elements a block takes at a time,
+#define CLIP_CHUNK_MIN 1024  // ... and fewest: small sets are spread over as many blocks as that gives
 #define CLIP_BLOCKS 1024   // blocks of a norm launch, one partial sum each
 
 struct ClipTable {
@@ -467,7 +485,7 @@ struct ClipTable {
     int64_t numel[CLIP_BATCH];
     uint32_t first_chunk[CLIP_BATCH + 1];
     int32_t dtype[CLIP_BATCH];
-    int n;
+    int n, chunk;  // chunk: elements a block takes at a time
 };
 
 // two partial results of a norm: sums of squares add up, largest values do not, a NaN stays
@@ -520,8 +538,8 @@ __global__ __launch_bounds__(256) void clip_norm_kernel(ClipTable t, int inf_nor
     double acc = 0.0;
     for (uint32_t c = blockIdx.x; c < t.first_chunk[t.n]; c += gridDim.x) {
         const int k = clip_tensor_of(t, c);
-        const int64_t begin = (int64_t)(c - t.first_chunk[k]) * CLIP_CHUNK;
-        const int64_t end = begin + CLIP_CHUNK < t.numel[k] ? begin + CLIP_CHUNK : t.numel[k];
+        const int64_t begin = (int64_t)(c - t.first_chunk[k]) * t.chunk;
+        const int64_t end = begin + t.chunk < t.numel[k] ? begin + t.chunk : t.numel[k];
         const double v = t.dtype[k] == HVS_F32   ? chunk_norm<HVS_F32>(t.data[k], begin, end, inf_norm)
                          : t.dtype[k] == HVS_F16 ? chunk_norm<HVS_F16>(t.data[k], begin, end, inf_norm)
                                                  : chunk_norm<HVS_BF16>(t.data[k], begin, end, inf_norm);
@@ -553,7 +571,8 @@ template <int DT> __device__ __forceinline__ void chunk_scale(const void *data, 
     for (i += threadIdx.x; i < end; i += 256) o[i] = learn_from_float<E>(learn_to_float(p[i]) * f);
 }
 
-// Every block adds up the partial sums itself (the same order everywhere), then scales its chunks.
+// Every block adds up the partial sums itself (the same order everywhere), then scales its chunks, the last ones first: they
+// are what the norm pass has left in the caches.
 __global__ __launch_bounds__(256) void clip_scale_kernel(ClipTable t, int inf_norm, const double *__restrict__ partial, int n_partial, double max_norm,
                                                          float *__restrict__ norm_out, int write_norm) {
     __shared__ double lds[4];
@@ -563,11 +582,13 @@ __global__ __launch_bounds__(256) void clip_scale_kernel(ClipTable t, int inf_no
     const float norm = (float)(inf_norm ? acc : sqrt(acc));
     if (write_norm && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = norm;
     float f = norm != norm ? norm : (max_norm < __builtin_inf() ? (float)fmin(max_norm / ((double)norm + 1e-6), 1.0) : 1.0f);
-    for (uint32_t c = blockIdx.x; c < t.first_chunk[t.n]; c += gridDim.x) {
+    const uint32_t chunks = t.first_chunk[t.n];
+    for (uint32_t i = blockIdx.x; i < chunks; i += gridDim.x) {
+        const uint32_t c = chunks - 1 - i;
         const int k = clip_tensor_of(t, c);
         if (f == 1.0f && t.out[k] == t.data[k]) continue;  // in place and nothing to clip: the tensor is its own result
-        const int64_t begin = (int64_t)(c - t.first_chunk[k]) * CLIP_CHUNK;
-        const int64_t end = begin + CLIP_CHUNK < t.numel[k] ? begin + CLIP_CHUNK : t.numel[k];
+        const int64_t begin = (int64_t)(c - t.first_chunk[k]) * t.chunk;
+        const int64_t end = begin + t.chunk < t.numel[k] ? begin + t.chunk : t.numel[k];
         if (t.dtype[k] == HVS_F32) chunk_scale<HVS_F32>(t.data[k], t.out[k], begin, end, f);
         else if (t.dtype[k] == HVS_F16) chunk_scale<HVS_F16>(t.data[k], t.out[k], begin, end, f);
         else chunk_scale<HVS_BF16>(t.data[k], t.out[k], begin, end, f);
@@ -618,14 +639,24 @@ static int check_apart(const char *who, const hvs_tensor *t, int n) {
     return 0;
 }
 
-// chunks of the tensors of one launch; at most 64 x 2^27, so they are counted in 64 bits and the caller splits the launch
-static int fill_table(const hvs_tensor *t, int n, int at, ClipTable *tab) {
+// elements a block takes at a time: about 2048 chunks in all, within the limits
+static int clip_chunk(const hvs_tensor *t, int n) {
+    int64_t total = 0;
+    for (int i = 0; i < n && total < (int64_t)CLIP_CHUNK << 11; i++) total += t[i].numel;
+    int chunk = CLIP_CHUNK_MIN;
+    while (chunk < CLIP_CHUNK && (int64_t)chunk << 11 < total) chunk *= 2;
+    return chunk;
+}
+// The tensors of one launch, from number `at` on; returns the number of the first one left over.  2^40 elements are at most
+// 2^30 chunks, so at least one tensor always fits.
+static int fill_table(const hvs_tensor *t, int n, int at, int chunk, ClipTable *tab) {
     tab->n = 0;
+    tab->chunk = chunk;
     tab->first_chunk[0] = 0;
     while (at < n && tab->n < CLIP_BATCH) {
-        const uint64_t chunks = ((uint64_t)t[at].numel + CLIP_CHUNK - 1) / CLIP_CHUNK;
+        const uint64_t chunks = ((uint64_t)t[at].numel + chunk - 1) / chunk;
         const uint64_t end = tab->first_chunk[tab->n] + chunks;
-        if (end > 0x7FFFFFFFull) break;  // 2^40 elements are 2^27 chunks: at least one tensor always fits
+        if (end > 0x7FFFFFFFull) break;
         tab->data[tab->n] = t[at].data, tab->out[tab->n] = t[at].out, tab->numel[tab->n] = t[at].numel, tab->dtype[tab->n] = t[at].dtype;
         tab->first_chunk[++tab->n] = (uint32_t)end;
         at++;
@@ -637,9 +668,10 @@ extern "C" int hvs_clip_workspace(const hvs_tensor *tensors, int n_tensors, uint
     HVS_TRY(check_tensors("hvs_clip_workspace", tensors, n_tensors));
     HVS_REQUIRE(out_bytes != nullptr, "hvs_clip_workspace: NULL argument");
     ClipTable tab;
+    const int chunk = clip_chunk(tensors, n_tensors);
     uint64_t partials = 0;
     for (int at = 0; at < n_tensors;) {
-        at = fill_table(tensors, n_tensors, at, &tab);
+        at = fill_table(tensors, n_tensors, at, chunk, &tab);
         partials += tab.first_chunk[tab.n] < CLIP_BLOCKS ? tab.first_chunk[tab.n] : CLIP_BLOCKS;
     }
     *out_bytes = (partials ? partials : 1) * sizeof(double);
@@ -661,9 +693,10 @@ extern "C" int hvs_clip_grad_norm(int device_id, void *stream, const hvs_tensor 
     hipStream_t st = (hipStream_t)stream;
     double *partial = (double *)workspace;
     ClipTable tab;
+    const int chunk = clip_chunk(tensors, n_tensors);
     int n_partial = 0;
     for (int at = 0; at < n_tensors;) {
-        at = fill_table(tensors, n_tensors, at, &tab);
+        at = fill_table(tensors, n_tensors, at, chunk, &tab);
         const int blocks = (int)(tab.first_chunk[tab.n] < CLIP_BLOCKS ? tab.first_chunk[tab.n] : CLIP_BLOCKS);
         if (blocks == 0) continue;
         clip_norm_kernel<<<blocks, 256, 0, st>>>(tab, infinity_norm != 0, partial + n_partial);
@@ -672,7 +705,7 @@ extern "C" int hvs_clip_grad_norm(int device_id, void *stream, const hvs_tensor 
     }
     bool first = true;
     for (int at = 0; at < n_tensors || first; first = false) {
-        at = fill_table(tensors, n_tensors, at, &tab);
+        at = fill_table(tensors, n_tensors, at, chunk, &tab);
         const uint32_t chunks = tab.first_chunk[tab.n];
         if (chunks == 0 && !first) continue;
         clip_scale_kernel<<<(int)(chunks < 1 ? 1 : (chunks < 2048 ? chunks : 2048)), 256, 0, st>>>(tab, infinity_norm != 0, partial, n_partial, max_norm, norm, first);

@@ -632,6 +632,7 @@ extern "C" int hvs_index_destroy(hvs_index *idx) {
     hipEventDestroy(idx->ev1);
     hipEventDestroy(idx->tm0);
     hipEventDestroy(idx->tm1);
+    if (idx->ev_reader) hipEventDestroy(idx->ev_reader);
     if (idx->own_stream) hipStreamDestroy(idx->stream);
     delete idx;
     return 0;

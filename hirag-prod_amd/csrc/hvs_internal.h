@@ -108,6 +108,7 @@ struct hvs_index {
     int64_t prof_launches[HVS_PROF_COUNT] = {0};
     hipEvent_t ev0 = nullptr, ev1 = nullptr;  // profiling pair
     hipEvent_t tm0 = nullptr, tm1 = nullptr;  // user timer pair
+    hipEvent_t ev_reader = nullptr;           // orders reads of the rows on a caller's stream against this index's own (hvs_index_preference_loss)
 };
 
 int hvs_ws_get(hvs_index *idx, int slot, size_t bytes, void **out);

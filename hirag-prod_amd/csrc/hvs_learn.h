@@ -95,27 +95,19 @@ __device__ __forceinline__ float learn_wave_sum(float v) {
 template <int CTRL> __device__ __forceinline__ float learn_dpp(float v) {
     return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), CTRL, 0xF, 0xF, true));
 }
-// Eight sums over the wave at once, in vector registers alone: halves trade places with the next value's, then quarters, so
-// that every step works on two values; a row of 16 lanes then holds one value and adds up by rotation.  s[i] becomes the
-// sum of v[i], the same in every lane.
-__device__ __forceinline__ void learn_wave_sum8(const float *v, float *s) {
-    float u[4], w[2];
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[2 * i]), __float_as_uint(v[2 * i + 1]), false, false);
-        u[i] = __uint_as_float(r[0]) + __uint_as_float(r[1]);  // lanes 0-31: v[2 i], lanes 32-63: v[2 i + 1]
-    }
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(u[2 * i]), __float_as_uint(u[2 * i + 1]), false, false);
-        w[i] = __uint_as_float(r[0]) + __uint_as_float(r[1]);  // rows of 16: v[4 i], v[4 i + 2], v[4 i + 1], v[4 i + 3]
-        w[i] += learn_dpp<0x128>(w[i]);  // rotations by 8, 4, 2, 1
-        w[i] += learn_dpp<0x124>(w[i]);
-        w[i] += learn_dpp<0x122>(w[i]);
-        w[i] += learn_dpp<0x121>(w[i]);
-#pragma unroll
-        for (int k = 0; k < 4; k++) s[4 * i + k] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w[i]), (k & 1) * 32 + (k >> 1) * 16));
-    }
+// Two sums over the wave at once, in vector registers alone: the halves trade places, so that each works on one value; rows of
+// 16 lanes add up by rotation, then the two rows of a half.  a and b become the sums, the same in every lane.
+__device__ __forceinline__ void learn_wave_sum2(float &a, float &b) {
+    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+    float u = __uint_as_float(r[0]) + __uint_as_float(r[1]);  // lanes 0-31: a, lanes 32-63: b
+    u += learn_dpp<0x128>(u);                                 // rotations by 8, 4, 2, 1
+    u += learn_dpp<0x124>(u);
+    u += learn_dpp<0x122>(u);
+    u += learn_dpp<0x121>(u);
+    r = __builtin_amdgcn_permlane16_swap(__float_as_uint(u), __float_as_uint(u), false, false);
+    const uint32_t s = __float_as_uint(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+    a = __uint_as_float(__builtin_amdgcn_readlane(s, 0));
+    b = __uint_as_float(__builtin_amdgcn_readlane(s, 32));
 }
 
 // Makes `device` current for a call and the caller's device current again after it.

@@ -409,6 +409,9 @@ class HipVectorStore(BaseVDB):
         self._group_codes: Dict[tuple, int] = {}
         self._lock = asyncio.Lock()
         self._coalescer = _SearchCoalescer(self._search_batch) if coalesce_queries else None
+        self._adapters = None  # set_query_adapters
+        self._adapter_codes: Dict[tuple, int] = {}
+        self._adapt_coalescer = _SearchCoalescer(self._adapt_batch) if coalesce_queries else None
         self.search_copy = bool(search_copy)
         self._copy_logged: Dict[str, int] = {}
         self.auto_partition = bool(auto_partition)
@@ -762,6 +765,8 @@ class HipVectorStore(BaseVDB):
         q = np.asarray([self._to_list(e) for e in q_embs], dtype=np.float32)
         if q.ndim != 2 or q.shape[0] == 0:
             return []
+        if self._adapters is not None:
+            q = await self._adapt(q, workspace_id, knowledge_base_id)
 
         scored: List[dict] = []
         if table.index is not None and len(table.rows):
@@ -797,6 +802,36 @@ class HipVectorStore(BaseVDB):
                 break
         logger.info(f"[query] Retrieved {len(scored)} records from '{table_name}', elapsed={time.perf_counter() - start:.3f}s")
         return scored
+
+    def set_query_adapters(self, adapters, codes: Optional[Dict[tuple, int]] = None) -> None:
+        """Send the embeddings of every ``query`` through ``adapters`` (a ``QueryAdapters``, or None to stop) before the
+        search.  ``codes``: (workspace id, knowledge base id) -> adapter number; pairs that are not named go through the
+        shared projection alone.  The stored rows stay as they are, so this may change at any time; a query uses the
+        adapters that are set when its embedding arrives.  Not part of ``save``: the weights are the caller's."""
+        codes = {(str(w), str(k)): int(c) for (w, k), c in (codes or {}).items()}
+        if adapters is not None:
+            bad = [c for c in codes.values() if not 0 <= c < adapters.n_adapters]
+            if bad:
+                raise ValueError(f"adapter number {bad[0]} is not in [0, {adapters.n_adapters})")
+        self._adapters, self._adapter_codes = adapters, codes
+
+    async def _adapt(self, q: np.ndarray, workspace_id, knowledge_base_id) -> np.ndarray:
+        """The query embeddings of one request after its tenant's adapter; requests that wait together share one call,
+        whatever their tenants."""
+        adapters, code = self._adapters, self._adapter_codes.get((str(workspace_id), str(knowledge_base_id)), -1)
+        if q.shape[1] != adapters.d_in:
+            raise ValueError(f"query embeddings have {q.shape[1]} columns, the query adapters take {adapters.d_in}")
+        key = ("query adapters", adapters)
+        if self._adapt_coalescer is not None:
+            return await self._adapt_coalescer.submit(key, (q, code))
+        return (await asyncio.to_thread(self._adapt_batch, key, [(q, code)]))[0]
+
+    @staticmethod
+    def _adapt_batch(key: tuple, requests: List[tuple]) -> List[np.ndarray]:
+        """Blocking part of ``_adapt``: the embeddings of many requests, each with its own adapter, in one call."""
+        counts = [len(q) for q, _ in requests]
+        y = key[1].apply(np.concatenate([q for q, _ in requests], axis=0), np.repeat(np.array([c for _, c in requests], dtype=np.int32), counts))
+        return np.split(y, np.cumsum(counts)[:-1])
 
     def _search_batch(self, key: tuple, queries: List[np.ndarray]) -> List[List[tuple]]:
         """Blocking part of coalesced ``query`` calls: requests with the same key in one launch."""

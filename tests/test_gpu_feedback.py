@@ -414,3 +414,38 @@ def test_training_step_and_search(env):
     best = np.sort(full, 1)[:, :5]
     assert np.abs(np64(dist) - best).max() < 1e-5
     idx.close()
+
+
+def test_store_queries_through_adapters(env):
+    """Requests of several tenants in flight together, each through its own adapter, on the real index."""
+    import asyncio
+
+    import hirag_prod_amd.store as st
+    from tests import store_cases
+
+    torch = env.torch
+    dim = store_cases.DIM
+    gen = torch.Generator().manual_seed(11)
+    a = torch.randn(2, 4, dim, generator=gen) / dim**0.5
+    b = torch.randn(2, dim, 4, generator=gen) / 2
+    ad = env.hvs.QueryAdapters(torch.eye(dim, device=env.dev), a.to(env.dev), b.to(env.dev), torch.ones(2, device=env.dev))
+    s = st.HipVectorStore.create(store_cases.make_embedding_func(), vector_type="vector")
+
+    async def scenario():
+        tenants = [("ws1", "kb1", 0), ("ws1", "kb2", -1), ("ws2", "kb1", 1)]
+        for w, k, _ in tenants:
+            props = [store_cases.chunk_props(i, w, k) for i in range(20)]
+            await s.upsert_texts([p["text"] for p in props], props, "Chunks")
+        s.set_query_adapters(ad, {("ws1", "kb1"): 0, ("ws2", "kb1"): 1})
+        asked = [(i, t) for i in range(5) for t in tenants]
+        got = await asyncio.gather(*[s.query(f"question {i}", w, k, "Chunks", topk=5, topn=3, distance_threshold=3.0) for i, (w, k, _) in asked])
+        for hits, (i, (w, k, c)) in zip(got, asked):
+            q = store_cases.embed_text(f"question {i}").astype(np.float32).astype(np.float64)
+            y = q if c < 0 else q + np64(b[c]) @ (np64(a[c]) @ q)
+            rows = np.stack([store_cases.embed_text(f"text {w} {k} {j}") for j in range(20)])
+            dist = 1 - (rows @ y) / np.linalg.norm(rows, axis=1) / np.linalg.norm(y)
+            order = np.argsort(dist, kind="stable")[:5]
+            store_cases.same_hits([h["documentKey"] for h in hits], [f"chunk-{w}-{k}-{j}" for j in order], dist[order], [h["distance"] for h in hits])
+
+    asyncio.run(scenario())
+    s.close()
