@@ -15,20 +15,37 @@
 #include "hvs_learn.h"
 
 #define ONCE_ROWS 2  // rows up to which one launch does all
+// rows up to which blocks of few outputs take the rows in arrival order; a whole call with 1536 x 1536 weights, this route
+// against the grouped tiles: fp32 1024 rows 99 / 112 us, 1536 rows 145 / 112; bf16 512 rows 24 / 36 us, 777 rows 34 / 34
 #define FEW_ROWS_F32 1024
 #define FEW_ROWS_16 768
 #define GROUP_CHUNK 1024  // rows per block of the grouping kernels
 #define MAX_CHUNK_ROWS 65536
-#define OUTER_BLOCKS 1024    // blocks the gradients of the stacks aim at,
-#define OUTER_MIN_ROWS 32    // ... with tiles of at least so many rows
-#define OUTER_MAX_ROWS 2048  // ... and at most so many
 #define SHRINK_WIDE_ROWS 16384  // rows from which u = A x is taken 32 rows a wave instead of 16 a block
+#define SHRINK_WAVES 8
+#define SHRINK_SHARES 4  // blocks that share the adapters among 16 rows in code order (1, 2, 4, 8: 11.2, 9.5, 8.9, 9.6 us, mean of three sizes)
+#define OUTER_ROWS 512       // rows whose numbers a block of the stack gradients holds at a time
+#define OUTER_PARTIAL_BYTES (128ll << 20)  // what their partial sums may take
 
 // ---------------------------------------------------------------------------------------------------------------
 // grouping: rows ordered by adapter, equal codes in row order
 // ---------------------------------------------------------------------------------------------------------------
 // bin 0: no adapter, bin c + 1: adapter c, bin S + 1: codes past the last adapter
 __device__ __forceinline__ int group_bin(int32_t code, int S) { return code < 0 ? 0 : (code >= S ? S + 1 : code + 1); }
+
+// The rows of every adapter cut into pieces of `rows` rows (one piece, an empty one, for an adapter without rows): what a
+// block of the stack gradients works on.
+struct Piece {
+    int32_t adapter;
+    uint32_t begin, end;  // rows, in code order
+    int32_t slot;         // place of its partial sums, -1 when it is all of its adapter's rows
+};
+struct PieceTable {
+    Piece *piece;     // [S + n / rows]; NULL: no table wanted
+    uint32_t *slot;   // [S] first slot of an adapter of several pieces
+    uint32_t *count;  // [1]
+    int rows;
+};
 
 __global__ __launch_bounds__(GROUP_CHUNK) void group_count_kernel(const int32_t *__restrict__ codes, int n, int S, uint32_t *__restrict__ counts) {
     extern __shared__ uint32_t hist[];  // [S + 2]
@@ -51,7 +68,7 @@ __global__ __launch_bounds__(GROUP_CHUNK) void group_count_kernel(const int32_t 
 template <bool FEW_BINS>
 __global__ __launch_bounds__(GROUP_CHUNK) void group_place_kernel(const int32_t *__restrict__ codes, int n, int S, int bits, int chunks,
                                                                   const uint32_t *__restrict__ counts, uint32_t *__restrict__ order,
-                                                                  int32_t *__restrict__ scodes, uint32_t *__restrict__ seg_begin) {
+                                                                  int32_t *__restrict__ scodes, uint32_t *__restrict__ seg_begin, PieceTable pieces) {
     constexpr int WAVES = GROUP_CHUNK / 64;
     extern __shared__ uint32_t next[];  // [S + 2] next free place of every bin; [S + 2] its rows before this block's
     __shared__ uint32_t wave_sum[WAVES];
@@ -97,15 +114,13 @@ __global__ __launch_bounds__(GROUP_CHUNK) void group_place_kernel(const int32_t 
     if (FEW_BINS)
         for (int b = tid; b < WAVES * GROUP_FEW_BINS; b += GROUP_CHUNK) (&by_wave[0][0])[b] = 0;
     __syncthreads();
-    uint32_t carry = 0;
-    for (int b0 = 0; b0 < nb; b0 += GROUP_CHUNK) {  // exclusive scan over the bins
-        const int b = b0 + tid;
-        const uint32_t total = b < nb ? next[b] : 0;
-        uint32_t inc = total;
+    // exclusive sum over the bins of a round of 1024, on top of what came before
+    auto block_scan = [&](uint32_t v, uint32_t &carry) {
+        uint32_t inc = v;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
-            const uint32_t v = __shfl_up(inc, o);
-            if (lane >= o) inc += v;
+            const uint32_t u = __shfl_up(inc, o);
+            if (lane >= o) inc += u;
         }
         if (lane == 63) wave_sum[wave] = inc;
         __syncthreads();
@@ -115,14 +130,34 @@ __global__ __launch_bounds__(GROUP_CHUNK) void group_place_kernel(const int32_t 
             if (w < wave) base += wave_sum[w];
             all += wave_sum[w];
         }
-        const uint32_t start = base + inc - total;
+        carry += all;
+        __syncthreads();
+        return base + inc - v;
+    };
+    uint32_t carry = 0, cut_carry = 0;
+    for (int b0 = 0; b0 < nb; b0 += GROUP_CHUNK) {
+        const int b = b0 + tid;
+        const uint32_t total = b < nb ? next[b] : 0;
+        const uint32_t start = block_scan(total, carry);
         if (b < nb) {
             next[b] = start + before[b];
             if (me == 0 && b >= 1) seg_begin[b - 1] = start;  // seg_begin[S] = end of the last adapter's rows
         }
-        carry += all;
-        __syncthreads();
+        if (me == 0 && pieces.piece) {
+            // pieces in the low half, slots for partial sums in the high half: fewer than 2^16 of each
+            const bool is_adapter = b >= 1 && b <= S;
+            const uint32_t np = is_adapter ? (total > 0 ? (total + pieces.rows - 1) / pieces.rows : 1) : 0;
+            const uint32_t at = block_scan(np + (np > 1 ? np << 16 : 0), cut_carry);
+            if (is_adapter) {
+                pieces.slot[b - 1] = at >> 16;
+                for (uint32_t k = 0; k < np; k++) {
+                    const uint32_t lo = k * pieces.rows, hi = lo + pieces.rows < total ? lo + pieces.rows : total;
+                    pieces.piece[(at & 0xFFFFu) + k] = Piece{b - 1, start + lo, start + hi, np > 1 ? (int32_t)((at >> 16) + k) : -1};
+                }
+            }
+        }
     }
+    if (me == 0 && tid == 0 && pieces.piece) *pieces.count = cut_carry & 0xFFFFu;
     uint64_t peers = __ballot(i < n);
     for (int bit = 0; bit < bits; bit++) {
         const bool one = (bin >> bit) & 1u;
@@ -199,11 +234,10 @@ template <int DT> __device__ __forceinline__ void shrink_store(const ShrinkParam
     if (j == 0) p.factor[at] = known ? (DT == HVS_F32 ? p.scale[c] : ldexpf(p.scale[c], e2)) : 0.0f;
 }
 
-template <int RT> constexpr int shrink_waves() { return RT <= 2 ? 16 : 8; }
 template <int DT, int RT, bool ALIGNED>
-__global__ __launch_bounds__(64 * shrink_waves<RT>()) void shrink_kernel(ShrinkParams p) {
+__global__ __launch_bounds__(64 * SHRINK_WAVES) void shrink_kernel(ShrinkParams p) {
     typedef typename Elem<DT>::type E;
-    constexpr int SHRINK_WAVES = shrink_waves<RT>(), EPC = Elem<DT>::EPC, STEP = 4 * EPC;
+    constexpr int EPC = Elem<DT>::EPC, STEP = 4 * EPC;
     constexpr int UNROLL = RT == 1 ? 3 : (RT == 2 ? 2 : 1);
     __shared__ float part[SHRINK_WAVES][16][RT * 16 + 4];  // [wave][row][rank]
     __shared__ __attribute__((aligned(16))) char turn[SHRINK_WAVES][(1 + RT) * 1024];
@@ -460,14 +494,23 @@ __global__ __launch_bounds__(64 * WAVES, 4) void project_few_kernel(ProjectParam
             for (int t = 0; t < MT; t++) turn_put(turn + t * 1024, fw[s][t], lane);
 #pragma unroll
             for (int t = 0; t < NT; t++) turn_put(turn + (MT + t) * 1024, fx[s][t], lane);
-            f32x4 aw[MT];
+            f32x4 aw[MT], bx[NT];
 #pragma unroll
             for (int a = 0; a < MT; a++) aw[a] = turn_get(turn + a * 1024, lane);
 #pragma unroll
-            for (int t = 0; t < NT; t++) {
-                const f32x4 bx = turn_get(turn + (MT + t) * 1024, lane);
+            for (int t = 0; t < NT; t++) bx[t] = turn_get(turn + (MT + t) * 1024, lane);
+            if (DT == HVS_F32) {  // the sums take turns: a product does not wait for the one before it
 #pragma unroll
-                for (int a = 0; a < MT; a++) acc[a][t] = mfma_chunk<DT>(aw[a], bx, acc[a][t]);
+                for (int j = 0; j < 4; j++)
+#pragma unroll
+                    for (int a = 0; a < MT; a++)
+#pragma unroll
+                        for (int t = 0; t < NT; t++) acc[a][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(aw[a][j], bx[t][j], acc[a][t], 0, 0, 0);
+            } else {
+#pragma unroll
+                for (int a = 0; a < MT; a++)
+#pragma unroll
+                    for (int t = 0; t < NT; t++) acc[a][t] = mfma_chunk<DT>(aw[a], bx[t], acc[a][t]);
             }
         }
         k0 += WAVES * STEP * UNROLL;
@@ -713,35 +756,44 @@ __global__ __launch_bounds__(T::GT, 2) void project_tile_kernel(ProjectParams p)
         compute_step<DT, T>(acc, smem + cur * T::STAGE_BYTES, wm, wn, lane, srcA, srcB, smem + (cur ^ 1) * T::STAGE_BYTES, koff_plain(0), wave);
         cur ^= 1;
 
+        // low-rank term, adapter by adapter, in sums of its own that only the rows of the adapter take over: a weight that is
+        // not finite stays with its tenant.  KC matrix steps of ranks at a time, GROUPS row groups together: their u fragments
+        // serve every adapter among the rows, an adapter's fragments of b serve all its rows, and with registers to spare
+        // the next adapter's are on their way meanwhile
+        constexpr int KC = 2, GROUPS = MT <= 2 ? NT : 1;
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
-            const int j = wrow + nt * 32 + l32;
-            const bool valid = j < p.n;
-            const int32_t code = codes[nt];
-            const float f = factor[nt];
-            const bool use = code >= 0 && code < p.S;
-            // low-rank term, adapter by adapter, in sums of its own that only the rows of the adapter take over: a weight
-            // that is not finite stays with its tenant.  KC matrix steps of ranks at a time: their u fragments serve every
-            // adapter among the rows, and the fragments of b for all columns are in flight together
-            constexpr int KC = 2;
+        for (int n0 = 0; n0 < NT; n0 += GROUPS)
             for (int k0 = 0; k0 < p.rp; k0 += KC * 2 * EPC) {
-                f32x4 ub[KC], ul[KC];
+                f32x4 ub[GROUPS][KC], ul[GROUPS][KC];
+                uint32_t todo[GROUPS];
 #pragma unroll
-                for (int s = 0; s < KC; s++) {
-                    const int k = k0 + s * 2 * EPC + h * EPC;
-                    ub[s] = ul[s] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-                    if (use && k < p.rp) {
-                        ub[s] = *reinterpret_cast<const f32x4 *>(reinterpret_cast<const E *>(p.u_hi) + (int64_t)j * p.rp + k);
-                        if (DT != HVS_F32) ul[s] = *reinterpret_cast<const f32x4 *>(reinterpret_cast<const E *>(p.u_lo) + (int64_t)j * p.rp + k);
+                for (int t = 0; t < GROUPS; t++) {
+                    const int32_t code = codes[n0 + t];
+                    const bool use = code >= 0 && code < p.S;
+                    todo[t] = (uint32_t)__ballot(use);
+                    const int64_t u_row = (int64_t)(wrow + (n0 + t) * 32 + l32) * p.rp;
+#pragma unroll
+                    for (int s = 0; s < KC; s++) {
+                        const int k = k0 + s * 2 * EPC + h * EPC;
+                        ub[t][s] = ul[t][s] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                        if (use && k < p.rp) {
+                            ub[t][s] = *reinterpret_cast<const f32x4 *>(reinterpret_cast<const E *>(p.u_hi) + u_row + k);
+                            if (DT != HVS_F32) ul[t][s] = *reinterpret_cast<const f32x4 *>(reinterpret_cast<const E *>(p.u_lo) + u_row + k);
+                        }
                     }
                 }
-                uint32_t todo = (uint32_t)__ballot(use);
-                while (todo) {
-                    const int32_t c = __builtin_amdgcn_readlane(code, __builtin_ctz(todo));
-                    const bool mine = use && code == c;
-                    todo &= ~(uint32_t)__ballot(mine);
+                auto take = [&]() {  // the next adapter among the rows, -1 when there is none
+                    int32_t c = -1;
+#pragma unroll
+                    for (int t = GROUPS - 1; t >= 0; t--)
+                        if (todo[t]) c = __builtin_amdgcn_readlane(codes[n0 + t], __builtin_ctz(todo[t]));
+#pragma unroll
+                    for (int t = 0; t < GROUPS; t++)
+                        if (c >= 0) todo[t] &= ~(uint32_t)__ballot(codes[n0 + t] == c);
+                    return c;
+                };
+                auto fetch = [&](int32_t c, f32x4 (&fb)[MT][KC]) {
                     const E *b = reinterpret_cast<const E *>(p.b) + (int64_t)c * p.N * p.ldb;
-                    f32x4 fb[MT][KC];
 #pragma unroll
                     for (int mt = 0; mt < MT; mt++) {
                         const int col = wcol + mt * 32 + l32;
@@ -752,26 +804,52 @@ __global__ __launch_bounds__(T::GT, 2) void project_tile_kernel(ProjectParams p)
                             fb[mt][s] = p.b_aligned ? load_chunk<DT, true>(brow, k, r_here) : load_chunk<DT, false>(brow, k, r_here);
                         }
                     }
+                };
+                f32x4 fb[MT][KC], fb_next[GROUPS > 1 ? MT : 1][KC];
+                int32_t c = take();
+                if (c >= 0) fetch(c, fb);
+                while (c >= 0) {
+                    const int32_t next = take();
+                    if constexpr (GROUPS > 1)
+                        if (next >= 0) fetch(next, fb_next);
 #pragma unroll
-                    for (int mt = 0; mt < MT; mt++) {
-                        f32x16 low;
+                    for (int t = 0; t < GROUPS; t++) {
+                        const bool mine = codes[n0 + t] == c;
+                        if (!__ballot(mine)) continue;
+                        const float f = factor[n0 + t];
 #pragma unroll
-                        for (int e = 0; e < 16; e++) low[e] = 0.0f;
+                        for (int mt = 0; mt < MT; mt++) {
+                            f32x16 low;
 #pragma unroll
-                        for (int s = 0; s < KC; s++) {
-                            if (DT == HVS_F32) {
+                            for (int e = 0; e < 16; e++) low[e] = 0.0f;
 #pragma unroll
-                                for (int e = 0; e < 4; e++) low = __builtin_amdgcn_mfma_f32_32x32x2f32(fb[mt][s][e], ub[s][e], low, 0, 0, 0);
-                            } else {
-                                low = mfma16<DT>(fb[mt][s], ub[s], low);
-                                low = mfma16<DT>(fb[mt][s], ul[s], low);
+                            for (int s = 0; s < KC; s++) {
+                                if (DT == HVS_F32) {
+#pragma unroll
+                                    for (int e = 0; e < 4; e++) low = __builtin_amdgcn_mfma_f32_32x32x2f32(fb[mt][s][e], ub[t][s][e], low, 0, 0, 0);
+                                } else {
+                                    low = mfma16<DT>(fb[mt][s], ub[t][s], low);
+                                    low = mfma16<DT>(fb[mt][s], ul[t][s], low);
+                                }
                             }
-                        }
 #pragma unroll
-                        for (int e = 0; e < 16; e++) acc[mt][nt][e] = mine ? fmaf(f, low[e], acc[mt][nt][e]) : acc[mt][nt][e];
+                            for (int e = 0; e < 16; e++) acc[mt][n0 + t][e] = mine ? fmaf(f, low[e], acc[mt][n0 + t][e]) : acc[mt][n0 + t][e];
+                        }
                     }
+                    c = next;
+                    if constexpr (GROUPS > 1) {
+#pragma unroll
+                        for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                            for (int s = 0; s < KC; s++) fb[mt][s] = fb_next[mt][s];
+                    } else if (c >= 0) fetch(c, fb);
                 }
             }
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            const int j = wrow + nt * 32 + l32;
+            const bool valid = j < p.n;
+            const int32_t code = codes[nt];
             const bool lost = valid && code >= p.S;  // a code past the last adapter
             E *out = reinterpret_cast<E *>(p.out) + (int64_t)out_row[nt] * p.ld_out;
             // accumulator element e of lane (l32, h): column 8 (e / 4) + 4 h + e % 4 of its 32, row l32
@@ -829,34 +907,41 @@ __global__ __launch_bounds__(256) void pack_rows_kernel(const E *__restrict__ sr
 struct TransposeJob {
     const void *src;
     void *dst;
-    int R, C, ld, tiles_c, tiles_r;
-    int64_t blocks;  // tiles_c tiles_r count
+    int R, C, ld, tiles_c, tiles_r, log_c;  // tiles of 4096 elements, 2^log_c columns wide: narrow matrices get narrow tiles
+    int64_t blocks;                         // tiles_c tiles_r count
 };
 struct TransposeJobs {
     TransposeJob job[3];
 };
-// all transposed weights of a backward pass in one launch: a block per 64 x 64 tile, jobs one after the other
+// all transposed weights of a backward pass in one launch: a block per tile, jobs one after the other
 template <typename E> __global__ __launch_bounds__(256) void transpose_kernel(TransposeJobs jobs) {
-    __shared__ E tile[64][65];
+    __shared__ E tile[256 * 17];  // rows of 2^log_c + 1 elements: 256 x 17, 64 x 65 or 16 x 257
     int64_t at = blockIdx.x;
     int which = 0;
     while (which < 2 && at >= jobs.job[which].blocks) at -= jobs.job[which++].blocks;
     const TransposeJob &t = jobs.job[which];
     const int64_t z = at / (t.tiles_c * t.tiles_r);
     const int rest = (int)(at - z * (t.tiles_c * t.tiles_r));
+    const int log_c = t.log_c, log_r = 12 - log_c, pitch = (1 << log_c) + 1;
     const E *s = reinterpret_cast<const E *>(t.src) + z * (int64_t)t.R * t.C;
     E *d = reinterpret_cast<E *>(t.dst) + z * (int64_t)t.C * t.ld;
-    const int r0 = rest / t.tiles_c * 64, c0 = rest % t.tiles_c * 64;
-#pragma unroll 8
-    for (int i = threadIdx.x; i < 4096; i += 256) {
-        const int r = r0 + (i >> 6), c = c0 + (i & 63);
-        tile[i >> 6][i & 63] = r < t.R && c < t.C ? s[(int64_t)r * t.C + c] : (E)0.0f;
+    const int r0 = rest / t.tiles_c << log_r, c0 = rest % t.tiles_c << log_c;
+    E v[16];
+#pragma unroll
+    for (int k = 0; k < 16; k++) {
+        const int i = threadIdx.x + 256 * k, r = r0 + (i >> log_c), c = c0 + (i & ((1 << log_c) - 1));
+        v[k] = r < t.R && c < t.C ? s[(int64_t)r * t.C + c] : (E)0.0f;
+    }
+#pragma unroll
+    for (int k = 0; k < 16; k++) {
+        const int i = threadIdx.x + 256 * k;
+        tile[(i >> log_c) * pitch + (i & ((1 << log_c) - 1))] = v[k];
     }
     __syncthreads();
-#pragma unroll 8
-    for (int i = threadIdx.x; i < 4096; i += 256) {
-        const int c = c0 + (i >> 6), r = r0 + (i & 63);
-        if (c < t.C && r < t.ld) d[(int64_t)c * t.ld + r] = tile[i & 63][i >> 6];
+#pragma unroll
+    for (int k = 0; k < 16; k++) {
+        const int i = threadIdx.x + 256 * k, c = i >> log_r, r = i & ((1 << log_r) - 1);
+        if (c0 + c < t.C && r0 + r < t.ld) d[(int64_t)(c0 + c) * t.ld + r0 + r] = tile[r * pitch + c];
     }
 }
 
@@ -868,61 +953,58 @@ struct OuterProblem {
     const void *x;   // [n][d], pitch ld_x
     int64_t ld_x;
     float *out;      // [S][r][d], or [S][d][r] when transposed
-    float *partial;  // [2 tiles][r d], each laid out as out
+    float *partial;  // [slots][r d], each laid out as out
     int d, transposed, cols;  // cols: blocks over d
 };
 struct OuterParams {
     OuterProblem problem[2];  // grad_a: q = v, X = x;  grad_b: q = hidden, X = grad
-    const int32_t *scodes;
     const uint32_t *order;
     const uint32_t *seg_begin;  // [S + 1]
+    PieceTable pieces;
     const float *scale;
-    int n, r, S, rows_per, accumulate;
+    int r, S, accumulate;
 };
 
-// Rows are cut into tiles of rows_per (in code order).  A block walks the adapters of its tile, for 16 chunks of columns;
-// fp32 matrix products (16x16x4: lane = (rank or column chunk, row), so q needs no rounding and X no transposition).  An
-// adapter whose rows all lie in the tile is written out; one that goes on in a neighbouring tile leaves its sum in
-// `partial` (slot 0: it began in an earlier tile, slot 1: it begins here), and outer_join_kernel adds those in tile order.
+// A block takes one piece of an adapter's rows and 16 chunks of columns; fp32 matrix products (16x16x4: lane = (rank or column
+// chunk, row), so q needs no rounding and X no transposition).  An adapter of one piece is written out, zeros where it has no
+// rows; one of several leaves its sums in `partial`, and outer_join_kernel adds them in order.  A block per adapter and
+// piece keeps the blocks alike whether there are few adapters or hundreds (96 rows, 256 adapters: cutting the rows alone, so
+// that a block met many adapters one after the other, took twice as long).
 template <int DT, int RT, bool ALIGNED> __global__ __launch_bounds__(256) void outer_kernel(OuterParams p) {
     typedef typename Elem<DT>::type E;
-    constexpr int EPC = Elem<DT>::EPC, CC = 16 * EPC, COPIES = RT <= 2 ? 4 : 2;
+    constexpr int EPC = Elem<DT>::EPC, CC = 16 * EPC, COPIES = 2;
     __shared__ float red[COPIES][RT * 16][CC + 1];
-    __shared__ uint32_t rows[OUTER_MAX_ROWS];
+    __shared__ uint32_t rows[OUTER_ROWS];
+    const Piece piece = p.pieces.piece[blockIdx.x];
+    if (blockIdx.x >= *p.pieces.count) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int m = lane & 15, g = lane >> 4;
     const bool second = (int)blockIdx.y >= p.problem[0].cols;
     const OuterProblem &o = p.problem[second ? 1 : 0];
-    const int lo = blockIdx.x * p.rows_per, hi = lo + p.rows_per < p.n ? lo + p.rows_per : p.n;
     const int c0 = ((int)blockIdx.y - (second ? p.problem[0].cols : 0)) * CC, j0 = blockIdx.z * (RT * 16);
-    for (int i = lo + tid; i < hi; i += 256) rows[i - lo] = p.order[i];
-    int i = lo;
-    int32_t c = p.scodes[lo];
-    __syncthreads();
-    while (i < hi) {
-        if (c < 0 || c >= p.S) {  // rows without an adapter come first, codes past the last one come last
-            i = c < 0 ? ((int)p.seg_begin[0] < hi ? (int)p.seg_begin[0] : hi) : hi;
-            if (i < hi) c = p.scodes[i];
-            continue;
-        }
-        const int seg_lo = (int)p.seg_begin[c], seg_hi = (int)p.seg_begin[c + 1];
-        const float s = p.scale[c];
-        const int end = seg_hi < hi ? seg_hi : hi;
-        const int32_t next_c = end < hi ? p.scodes[end] : -1;
-        f32x4 acc[RT][EPC];
+    const int32_t c = piece.adapter;
+    const int lo = (int)piece.begin, hi = (int)piece.end;
+    const bool whole = piece.slot < 0;
+    if (lo >= hi && p.accumulate) return;
+    const float s = p.scale[c];
+    f32x4 acc[RT][EPC];
 #pragma unroll
-        for (int t = 0; t < RT; t++)
+    for (int t = 0; t < RT; t++)
 #pragma unroll
-            for (int e = 0; e < EPC; e++) acc[t][e] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int e = 0; e < EPC; e++) acc[t][e] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int base = lo; base < hi; base += OUTER_ROWS) {
+        const int end = base + OUTER_ROWS < hi ? base + OUTER_ROWS : hi;
+        for (int i = base + tid; i < end; i += 256) rows[i - base] = p.order[i];
+        __syncthreads();
         constexpr int UNROLL = RT <= 2 ? 4 : 2;
-        for (int b = i + 4 * wave; b < end; b += 16 * UNROLL) {
+        for (int b = base + 4 * wave; b < end; b += 16 * UNROLL) {
             f32x4 fx[UNROLL];
             float fq[UNROLL][RT];
 #pragma unroll
             for (int u = 0; u < UNROLL; u++) {
                 const int at = b + 16 * u + g;
                 const bool ok = at < end;
-                const int64_t row = rows[(ok ? at : i) - lo];
+                const int64_t row = rows[ok ? at - base : 0];
                 fx[u] = load_chunk<DT, ALIGNED>(reinterpret_cast<const E *>(o.x) + row * o.ld_x, c0 + m * EPC, ok ? o.d : 0);
 #pragma unroll
                 for (int t = 0; t < RT; t++) {
@@ -940,64 +1022,51 @@ template <int DT, int RT, bool ALIGNED> __global__ __launch_bounds__(256) void o
                     for (int e = 0; e < EPC; e++) acc[t][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(fq[u][t], v[e], acc[t][e], 0, 0, 0);
             }
         }
-        // the four waves' sums, in a fixed order: each in its own copy, or the upper two added onto the lower two's
-        auto put = [&](int copy, bool add) {
-#pragma unroll
-            for (int t = 0; t < RT; t++)
-#pragma unroll
-                for (int e = 0; e < EPC; e++)
-#pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        float *cell = &red[copy][t * 16 + 4 * g + k][m * EPC + e];
-                        *cell = add ? *cell + acc[t][e][k] : acc[t][e][k];
-                    }
-        };
-        if (COPIES == 4) put(wave, false);
-        else {
-            if (wave >= 2) put(wave - 2, false);
-            __syncthreads();
-            if (wave < 2) put(wave, true);
-        }
         __syncthreads();
-        const bool whole = seg_lo >= lo && seg_hi <= hi;
-        const int64_t size = (int64_t)p.r * o.d;
-        float *out = whole ? o.out + (int64_t)c * size : o.partial + (int64_t)(2 * blockIdx.x + (seg_lo < lo ? 0 : 1)) * size;
-        const int rn = p.r - j0 < RT * 16 ? p.r - j0 : RT * 16, cn = o.d - c0 < CC ? o.d - c0 : CC;
-        for (int k = tid; k < RT * 16 * CC; k += 256) {
-            const int j = o.transposed ? k % (RT * 16) : k / CC, col = o.transposed ? k / (RT * 16) : k % CC;
-            if (j >= rn || col >= cn) continue;
-            float v = red[0][j][col];
+    }
+    // the four waves' sums, in a fixed order: the upper two put theirs down, the lower two add to them
+    auto put = [&](int copy, bool add) {
 #pragma unroll
-            for (int w = 1; w < COPIES; w++) v += red[w][j][col];
-            float *cell = out + (o.transposed ? (int64_t)(c0 + col) * p.r + j0 + j : (int64_t)(j0 + j) * o.d + c0 + col);
-            *cell = whole ? s * v + (p.accumulate ? *cell : 0.0f) : v;
-        }
-        __syncthreads();
-        i = end;
-        c = next_c;
+        for (int t = 0; t < RT; t++)
+#pragma unroll
+            for (int e = 0; e < EPC; e++)
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    float *cell = &red[copy][t * 16 + 4 * g + k][m * EPC + e];
+                    *cell = add ? *cell + acc[t][e][k] : acc[t][e][k];
+                }
+    };
+    if (wave >= 2) put(wave - 2, false);
+    __syncthreads();
+    if (wave < 2) put(wave, true);
+    __syncthreads();
+    const int64_t size = (int64_t)p.r * o.d;
+    float *out = whole ? o.out + (int64_t)c * size : o.partial + (int64_t)piece.slot * size;
+    const int rn = p.r - j0 < RT * 16 ? p.r - j0 : RT * 16, cn = o.d - c0 < CC ? o.d - c0 : CC;
+    for (int k = tid; k < RT * 16 * CC; k += 256) {
+        const int j = o.transposed ? k % (RT * 16) : k / CC, col = o.transposed ? k / (RT * 16) : k % CC;
+        if (j >= rn || col >= cn) continue;
+        const float v = red[0][j][col] + red[1][j][col];
+        float *cell = out + (o.transposed ? (int64_t)(c0 + col) * p.r + j0 + j : (int64_t)(j0 + j) * o.d + c0 + col);
+        *cell = whole ? s * v + (p.accumulate ? *cell : 0.0f) : v;
     }
 }
 
-// adapters without rows: zero; adapters over several tiles: their partial sums in tile order
+// adapters of several pieces: their partial sums in order
 template <int VEC> __global__ __launch_bounds__(256) void outer_join_kernel(OuterParams p) {
     typedef float vec __attribute__((ext_vector_type(VEC)));
-    const int c = blockIdx.x;
-    const int lo = (int)p.seg_begin[c], hi = (int)p.seg_begin[c + 1];
-    const int t0 = lo / p.rows_per, t1 = hi > lo ? (hi - 1) / p.rows_per : t0;
-    if (hi > lo ? t0 == t1 : p.accumulate) return;
+    const int c = blockIdx.x, n = (int)(p.seg_begin[c + 1] - p.seg_begin[c]);
+    if (n <= p.pieces.rows) return;
+    const int np = (n + p.pieces.rows - 1) / p.pieces.rows;
     const OuterProblem &o = p.problem[blockIdx.z];
     const int64_t size = (int64_t)p.r * o.d / VEC;
     vec *out = reinterpret_cast<vec *>(o.out) + (int64_t)c * size;
-    const vec *part = reinterpret_cast<const vec *>(o.partial);
+    const vec *part = reinterpret_cast<const vec *>(o.partial) + (int64_t)p.pieces.slot[c] * size;
     const float s = p.scale[c];
     for (int64_t k = blockIdx.y * 256ll + threadIdx.x; k < size; k += gridDim.y * 256ll) {
-        if (hi == lo) {
-            out[k] = (vec)0.0f;
-            continue;
-        }
-        vec v = part[(int64_t)(2 * t0 + 1) * size + k];
+        vec v = part[k];
 #pragma unroll 4
-        for (int t = t0 + 1; t <= t1; t++) v += part[(int64_t)(2 * t) * size + k];
+        for (int t = 1; t < np; t++) v += part[t * size + k];
         out[k] = p.accumulate ? s * v + out[k] : s * v;
     }
 }
@@ -1037,24 +1106,20 @@ struct AdapterWs {
     int32_t *scodes;
     float *factor, *hidden, *partial_a, *partial_b;
     char *u_hi, *u_lo, *packed_w, *packed_x, *w_t, *a_t, *b_t;
+    PieceTable pieces;
 };
 
-// rows of a tile of the stack gradients, for both of them
+// Rows in a piece of the stack gradients, for passes of up to n rows: 256, in large passes 512, more where the partial sums would
+// take too much.  Adapters of several pieces have at most 2 n / rows of them.
+static int piece_rows(int64_t n, const hvs_adapters *ad) {
+    int64_t rows = n <= 16384 ? 256 : 512;
+    while (rows < MAX_CHUNK_ROWS && 2 * ((n + rows - 1) / rows) * ad->rank * (ad->d_in + ad->d_out) * 4 > OUTER_PARTIAL_BYTES) rows *= 2;
+    return (int)rows;
+}
 static int outer_cols(int d, int dtype) { return (d + 16 * elems_per_chunk(dtype) - 1) / (16 * elems_per_chunk(dtype)); }
-static int outer_rows_per(int64_t n, const hvs_adapters *ad) {
-    const int cols = outer_cols(ad->d_in, ad->dtype) + outer_cols(ad->d_out, ad->dtype);
-    const int64_t rows = (n * cols + OUTER_BLOCKS - 1) / OUTER_BLOCKS;
-    return (int)(rows < OUTER_MIN_ROWS ? OUTER_MIN_ROWS : (rows > OUTER_MAX_ROWS ? OUTER_MAX_ROWS : (rows + 15) / 16 * 16));
-}
-// the most tiles n rows or fewer are cut into (fewer rows may be cut into more tiles than n, by rounding)
-static int64_t outer_max_tiles(int64_t n, const hvs_adapters *ad) {
-    const int cols = outer_cols(ad->d_in, ad->dtype) + outer_cols(ad->d_out, ad->dtype);
-    const int64_t by_blocks = (OUTER_BLOCKS + cols - 1) / cols, by_max = (n + OUTER_MAX_ROWS - 1) / OUTER_MAX_ROWS;
-    const int64_t by_min = (n + OUTER_MIN_ROWS - 1) / OUTER_MIN_ROWS, most = by_blocks > by_max ? by_blocks : by_max;
-    return most < by_min ? most : by_min;
-}
 
 static uint64_t cut_workspace(const hvs_adapters *ad, int64_t nc, int backward, void *base, AdapterWs *ws) {
+    *ws = {};
     WorkspaceCut w(base);
     const int es = hvs_elem_size(ad->dtype), epc = elems_per_chunk(ad->dtype), rp = round_up(ad->rank, 16);
     const int64_t chunks = (nc + GROUP_CHUNK - 1) / GROUP_CHUNK;
@@ -1073,7 +1138,11 @@ static uint64_t cut_workspace(const hvs_adapters *ad, int64_t nc, int backward, 
         ws->w_t = w.take<char>((uint64_t)ad->d_in * round_up(ad->d_out, epc) * es);
         ws->b_t = w.take<char>((uint64_t)ad->n_adapters * ad->rank * round_up(ad->d_out, epc) * es);
         ws->a_t = w.take<char>((uint64_t)ad->n_adapters * ad->d_in * rp * es);
-        const uint64_t slots = 2ull * outer_max_tiles(nc, ad) * ad->rank;
+        ws->pieces.rows = piece_rows(nc, ad);
+        const uint64_t several = (nc + ws->pieces.rows - 1) / ws->pieces.rows, slots = nc > ws->pieces.rows ? 2 * several * ad->rank : 0;
+        ws->pieces.piece = w.take<Piece>(((uint64_t)ad->n_adapters + several) * sizeof(Piece));
+        ws->pieces.slot = w.take<uint32_t>((uint64_t)ad->n_adapters * 4);
+        ws->pieces.count = w.take<uint32_t>(4);
         ws->partial_a = w.take<float>(slots * ad->d_in * 4);
         ws->partial_b = w.take<float>(slots * ad->d_out * 4);
     }
@@ -1099,10 +1168,10 @@ static int launch_group(hipStream_t st, const int32_t *codes, int n, int S, cons
         group_count_kernel<<<chunks, GROUP_CHUNK, lds, st>>>(codes, n, S, ws.counts);
     }
     if (S + 2 <= GROUP_FEW_BINS) {
-        group_place_kernel<true><<<chunks, GROUP_CHUNK, 2 * lds, st>>>(codes, n, S, bits, chunks, ws.counts, ws.order, ws.scodes, ws.seg_begin);
+        group_place_kernel<true><<<chunks, GROUP_CHUNK, 2 * lds, st>>>(codes, n, S, bits, chunks, ws.counts, ws.order, ws.scodes, ws.seg_begin, ws.pieces);
     } else {
         HVS_TRY((learn_allow_lds<group_place_kernel<false>>((int)(2 * lds))));
-        group_place_kernel<false><<<chunks, GROUP_CHUNK, 2 * lds, st>>>(codes, n, S, bits, chunks, ws.counts, ws.order, ws.scodes, ws.seg_begin);
+        group_place_kernel<false><<<chunks, GROUP_CHUNK, 2 * lds, st>>>(codes, n, S, bits, chunks, ws.counts, ws.order, ws.scodes, ws.seg_begin, ws.pieces);
     }
     HVS_HIP(hipGetLastError());
     return 0;
@@ -1117,8 +1186,8 @@ template <int DT> static int launch_shrink(hipStream_t st, const ShrinkParams &p
     do {                                                                                                     \
         if (wide && al) shrink_wide_kernel<DT, RT_, true><<<wgrid, 256, 0, st>>>(p);                         \
         else if (wide) shrink_wide_kernel<DT, RT_, false><<<wgrid, 256, 0, st>>>(p);                         \
-        else if (al) shrink_kernel<DT, RT_, true><<<grid, 64 * shrink_waves<RT_>(), 0, st>>>(p);                    \
-        else shrink_kernel<DT, RT_, false><<<grid, 64 * shrink_waves<RT_>(), 0, st>>>(p);                           \
+        else if (al) shrink_kernel<DT, RT_, true><<<grid, 64 * SHRINK_WAVES, 0, st>>>(p);                    \
+        else shrink_kernel<DT, RT_, false><<<grid, 64 * SHRINK_WAVES, 0, st>>>(p);                           \
     } while (0)
     if (p.r <= 16) SHRINK(1);
     else if (p.r <= 32) SHRINK(2);
@@ -1185,7 +1254,9 @@ template <int DT> static int launch_pack(hipStream_t st, const void *src, int64_
 static TransposeJob transpose_job(const void *src, int64_t count, int R, int C, int ld, void *dst) {
     TransposeJob t = {};
     t.src = src, t.dst = dst, t.R = R, t.C = C, t.ld = ld;
-    t.tiles_c = (C + 63) / 64, t.tiles_r = (ld + 63) / 64;  // the row tiles cover the pitch, so that the padding is written
+    t.log_c = C <= 32 ? 4 : (ld <= 32 ? 8 : 6);
+    const int tc = 1 << t.log_c, tr = 4096 >> t.log_c;
+    t.tiles_c = (C + tc - 1) / tc, t.tiles_r = (ld + tr - 1) / tr;  // the row tiles cover the pitch, so that the padding is written
     t.blocks = count * t.tiles_c * t.tiles_r;
     return t;
 }
@@ -1243,7 +1314,7 @@ static int run_direction(hipStream_t st, const hvs_adapters *ad, const Direction
     if (!grouped) HVS_TRY(launch_group(st, codes, n, s.S, ws));
     s.codes = ws.scodes, s.order = ws.order;
     if (d.out) s.u_hi = ws.u_hi, s.u_lo = ws.u_lo, s.factor = ws.factor;
-    HVS_TRY(launch_shrink<DT>(st, s, 2));
+    HVS_TRY(launch_shrink<DT>(st, s, SHRINK_SHARES));
     if (!d.out) return 0;
     p.K = round_up(d.K, epc);  // whole chunks: K itself where rows were taken as they are, their padded width where they were packed
     p.codes = ws.scodes, p.order = ws.order, p.u_hi = ws.u_hi, p.u_lo = ws.u_lo, p.factor = ws.factor;
@@ -1252,7 +1323,9 @@ static int run_direction(hipStream_t st, const hvs_adapters *ad, const Direction
     // the largest tile that still gives every CU one: a larger tile reads less per product, idle CUs cost more
     // (4096 x 1536 x 1536 bf16: 384 tiles of 128 48 us a call, 1536 of 64 59 us; 2048 rows: 192 of 128 39 us, 768 of 64 33 us)
     auto tiles = [&](int t) { return (int64_t)((p.N + t - 1) / t) * ((n + t - 1) / t); };
-    if (DT != HVS_F32 && tiles(256) >= 256) return launch_tile<DT, Tile256>(st, p);
+    if constexpr (DT != HVS_F32) {
+        if (tiles(256) >= 256) return launch_tile<DT, Tile256>(st, p);
+    }
     if (tiles(128) >= 256) return launch_tile<DT, Tile128>(st, p);
     return launch_tile<DT, Tile64>(st, p);
 }
@@ -1316,17 +1389,19 @@ extern "C" int hvs_adapters_apply(int device_id, void *stream, const hvs_adapter
     return 0;
 }
 
-template <int DT> static int launch_outer(hipStream_t st, const OuterParams &p) {
+template <int DT> static int launch_outer(hipStream_t st, const OuterParams &p, int64_t n) {
     const int es = hvs_elem_size(DT);
     bool al = true, vec = true;
     for (const OuterProblem &o : p.problem) {
         al = al && learn_aligned(o.x, o.ld_x * es, (int64_t)o.d * es);
         vec = vec && (int64_t)p.r * o.d % 4 == 0 && (uintptr_t)o.out % 16 == 0;
     }
-    const int tiles = (p.n + p.rows_per - 1) / p.rows_per, cols = p.problem[0].cols + p.problem[1].cols;
+    // (the table says how many pieces there are; the launch has room for the most there can be)
+    const int64_t most = p.S + (n + p.pieces.rows - 1) / p.pieces.rows;
+    const int cols = p.problem[0].cols + p.problem[1].cols;
 #define OUTER(RT_)                                                                                                           \
     do {                                                                                                                     \
-        const dim3 grid(tiles, cols, (p.r + 16 * RT_ - 1) / (16 * RT_));                                                     \
+        const dim3 grid((unsigned)most, cols, (p.r + 16 * RT_ - 1) / (16 * RT_));                                            \
         if (al) outer_kernel<DT, RT_, true><<<grid, 256, 0, st>>>(p);                                                        \
         else outer_kernel<DT, RT_, false><<<grid, 256, 0, st>>>(p);                                                          \
     } while (0)
@@ -1334,6 +1409,8 @@ template <int DT> static int launch_outer(hipStream_t st, const OuterParams &p) 
     else if (p.r <= 32) OUTER(2);
     else OUTER(4);
 #undef OUTER
+    HVS_HIP(hipGetLastError());
+    if (n <= p.pieces.rows) return 0;
     const int wide = p.problem[0].d > p.problem[1].d ? p.problem[0].d : p.problem[1].d;
     const int64_t by = (int64_t)p.r * wide / 1024;
     const dim3 grid(p.S, (unsigned)(by < 1 ? 1 : (by > 64 ? 64 : by)), 2);
@@ -1370,12 +1447,12 @@ static int run_backward(hipStream_t st, const hvs_adapters *ad, const void *grad
         d.out = grad_x ? (char *)grad_x + r0 * ld_gx * es : nullptr, d.ld_out = ld_gx;
         HVS_TRY(run_direction<DT>(st, ad, d, codes + r0, rows, ws.hidden, ws, true));
         OuterParams o = {};
-        o.scodes = ws.scodes, o.order = ws.order, o.seg_begin = ws.seg_begin, o.scale = ad->scale;
-        o.n = rows, o.r = ad->rank, o.S = ad->n_adapters, o.accumulate = r0 > 0, o.rows_per = outer_rows_per(rows, ad);
+        o.order = ws.order, o.seg_begin = ws.seg_begin, o.pieces = ws.pieces, o.scale = ad->scale;
+        o.r = ad->rank, o.S = ad->n_adapters, o.accumulate = r0 > 0;
         const char *xr = (const char *)x + r0 * ld_x * es;
         o.problem[0] = {ws.hidden, xr, ld_x, grad_a, ws.partial_a, ad->d_in, 0, outer_cols(ad->d_in, DT)};
         o.problem[1] = {hidden + r0 * ad->rank, d.x, ld_grad, grad_b, ws.partial_b, ad->d_out, 1, outer_cols(ad->d_out, DT)};
-        HVS_TRY(launch_outer<DT>(st, o));
+        HVS_TRY(launch_outer<DT>(st, o, rows));
     }
     return 0;
 }

@@ -456,18 +456,21 @@ extern "C" int hvs_index_preference_loss(hvs_index *idx, void *stream, const hvs
     if (st != nullptr) HVS_HIP(hipStreamIsCapturing(st, &capturing));
     HVS_REQUIRE(capturing == hipStreamCaptureStatusNone, "%s: the stream is being captured; a graph would keep the address of rows the table may move", who);
     if (st == idx->stream) return preference_core(st, p, idx->rows, idx->dtype, idx->dim, idx->ld, idx->n, workspace);
-    if (idx->ev_reader == nullptr) HVS_HIP(hipEventCreateWithFlags(&idx->ev_reader, hipEventDisableTiming | hipEventDisableSystemFence));
-    // after the work the table's stream holds: mostly it holds none, and then there is nothing to wait for
+    hipEvent_t &ev = idx->ev_reader;
+    if (ev == nullptr) HVS_HIP(hipEventCreateWithFlags(&ev, hipEventDisableTiming | hipEventDisableSystemFence));
+    // the event is about to stand for this read: an earlier one on another stream is waited for by the table's stream now
+    if (idx->reader_pending && idx->reader_stream != st) HVS_HIP(hipStreamWaitEvent(idx->stream, ev, 0));
+    // after the work the table's stream holds; mostly it holds none, and then there is nothing to wait for
     const hipError_t idle = hipStreamQuery(idx->stream);
     if (idle == hipErrorNotReady) {
         (void)hipGetLastError();  // an answer, not an error to be found by the next launch
-        HVS_HIP(hipEventRecord(idx->ev_reader, idx->stream));
-        HVS_HIP(hipStreamWaitEvent(st, idx->ev_reader, 0));
+        HVS_HIP(hipEventRecord(ev, idx->stream));
+        HVS_HIP(hipStreamWaitEvent(st, ev, 0));
     } else HVS_HIP(idle);
     HVS_TRY(preference_core(st, p, idx->rows, idx->dtype, idx->dim, idx->ld, idx->n, workspace));
-    // what the table does next may move the rows: it waits for this read
-    HVS_HIP(hipEventRecord(idx->ev_reader, st));
-    HVS_HIP(hipStreamWaitEvent(idx->stream, idx->ev_reader, 0));
+    HVS_HIP(hipEventRecord(ev, st));
+    idx->reader_stream = st;
+    idx->reader_pending = true;
     return 0;
 }
 

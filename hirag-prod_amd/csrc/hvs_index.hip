@@ -615,6 +615,7 @@ extern "C" int hvs_index_create(hvs_index **out, int device_id, int dim, int dty
 extern "C" int hvs_index_destroy(hvs_index *idx) {
     if (!idx) return 0;
     (void)hipSetDevice(idx->device);
+    if (idx->reader_pending) (void)hipEventSynchronize(idx->ev_reader);
     (void)hipStreamSynchronize(idx->stream);
     hipFree(idx->rows);
     hipFree(idx->inv_norm);
@@ -651,11 +652,21 @@ static int grow(hvs_index *idx, P **ptr, size_t old_count, size_t new_count, boo
     return 0;
 }
 
+// Called before rows move, change or go: the table's stream waits for the reads of its rows that callers' streams still hold
+// (hvs_index_preference_loss).
+static int readers_wait(hvs_index *idx) {
+    if (!idx->reader_pending) return 0;
+    HVS_HIP(hipStreamWaitEvent(idx->stream, idx->ev_reader, 0));
+    idx->reader_pending = false;
+    return 0;
+}
+
 extern "C" int hvs_index_reserve(hvs_index *idx, int64_t capacity_rows) {
     HVS_REQUIRE(idx != nullptr, "hvs_index_reserve: idx is NULL");
     HVS_REQUIRE(capacity_rows < (int64_t)0xFFFFFFFFll, "hvs_index_reserve: at most 2^32-1 rows per index");
     if (capacity_rows <= idx->cap) return 0;
     HVS_HIP(hipSetDevice(idx->device));
+    HVS_TRY(readers_wait(idx));
     const size_t row_bytes = (size_t)idx->ld * idx->elem_size;
     {
         // Rows beyond n and HVS_ROWS_SLACK bytes after the last one are kept zero: the MFMA kernels fetch whole
@@ -808,6 +819,7 @@ extern "C" int hvs_index_update(hvs_index *idx, const int64_t *positions, const 
     HVS_REQUIRE(positions && rows, "hvs_index_update: NULL argument");
     HVS_REQUIRE(src_dtype == HVS_F32 || src_dtype == idx->dtype, "hvs_index_update: source dtype %d not accepted", src_dtype);
     HVS_HIP(hipSetDevice(idx->device));
+    HVS_TRY(readers_wait(idx));
     const size_t src_row_bytes = (size_t)idx->dim * hvs_elem_size(src_dtype);
     if (on_device) {
         HVS_TRY(validate_device_positions(idx, positions, n, "hvs_index_update"));
@@ -928,6 +940,7 @@ extern "C" int hvs_index_export(hvs_index *idx, int64_t first, int64_t n, void *
 // new arrays sized for them, the old ones released only when every copy has succeeded.  Tombstones are gone afterwards
 // (the caller lists live rows only).  renumber_ids: ids become the new positions.
 static int rebuild_rows(hvs_index *idx, const uint32_t *positions, int64_t n_live, int renumber_ids, const char *who) {
+    HVS_TRY(readers_wait(idx));
     const size_t pitch = (size_t)idx->ld * idx->elem_size;
     const int64_t cap = n_live > 1024 ? n_live : 1024;
     char *rows = nullptr;

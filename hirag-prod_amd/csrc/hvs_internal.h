@@ -108,7 +108,11 @@ struct hvs_index {
     int64_t prof_launches[HVS_PROF_COUNT] = {0};
     hipEvent_t ev0 = nullptr, ev1 = nullptr;  // profiling pair
     hipEvent_t tm0 = nullptr, tm1 = nullptr;  // user timer pair
-    hipEvent_t ev_reader = nullptr;           // orders reads of the rows on a caller's stream against this index's own (hvs_index_preference_loss)
+    // reads of the rows on a caller's stream (hvs_index_preference_loss): the last one, and whether this index's stream has yet
+    // to wait for it before rows move, change or go
+    hipEvent_t ev_reader = nullptr;
+    hipStream_t reader_stream = nullptr;
+    bool reader_pending = false;
 };
 
 int hvs_ws_get(hvs_index *idx, int slot, size_t bytes, void **out);
