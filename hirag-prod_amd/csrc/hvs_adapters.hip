@@ -1109,10 +1109,10 @@ struct AdapterWs {
     PieceTable pieces;
 };
 
-// Rows in a piece of the stack gradients, for passes of up to n rows: 256, in large passes 512, more where the partial sums would
-// take too much.  Adapters of several pieces have at most 2 n / rows of them.
+// Rows in a piece of the stack gradients, for passes of up to n rows: 128, in large passes 256, more where the partial sums would
+// take too much (8192 rows of 64 adapters, 128 / 256 / 512 / 1024 rows: 34, 38, 42, 52 us with the join).  Adapters of several pieces have at most 2 n / rows of them.
 static int piece_rows(int64_t n, const hvs_adapters *ad) {
-    int64_t rows = n <= 16384 ? 256 : 512;
+        int64_t rows = n <= 16384 ? 128 : 256;
     while (rows < MAX_CHUNK_ROWS && 2 * ((n + rows - 1) / rows) * ad->rank * (ad->d_in + ad->d_out) * 4 > OUTER_PARTIAL_BYTES) rows *= 2;
     return (int)rows;
 }
@@ -1320,13 +1320,19 @@ static int run_direction(hipStream_t st, const hvs_adapters *ad, const Direction
     p.codes = ws.scodes, p.order = ws.order, p.u_hi = ws.u_hi, p.u_lo = ws.u_lo, p.factor = ws.factor;
     p.b_aligned = learn_aligned(d.b, d.ldb * es, 0) && (d.b_padded || s.r % epc == 0);
     p.out_vec = learn_aligned(d.out, d.ld_out * es, 0);
-    // the largest tile that still gives every CU one: a larger tile reads less per product, idle CUs cost more
-    // (4096 x 1536 x 1536 bf16: 384 tiles of 128 48 us a call, 1536 of 64 59 us; 2048 rows: 192 of 128 39 us, 768 of 64 33 us)
-    auto tiles = [&](int t) { return (int64_t)((p.N + t - 1) / t) * ((n + t - 1) / t); };
+    // The tile whose rounds over the chip take least time, in units of a round of two 128-tiles per CU.  Four 64-tiles per CU
+    // take 0.55 of that (fp32 0.48) when they are all there is and 0.7 round after round, a single 128-tile per CU 0.7 (fp32
+    // 0.5), a 256-tile per CU 1.75 for four times the work.  With 1536 x 1536 bf16 weights, us a call: 2048 rows 64 / 128 33 / 39,
+    // 4096 rows 59 / 48; 8192 rows 64 / 128 / 256 83 / 77 / 68; 16 384 rows 128 / 256 120 / 135.
+    auto rounds = [&](int t, int slots) { return (((int64_t)(p.N + t - 1) / t) * ((n + t - 1) / t) + slots - 1) / slots; };
+    const bool f32 = DT == HVS_F32;
+    const double c64 = rounds(64, 1024) == 1 ? (f32 ? 0.48 : 0.55) : 0.7 * (double)rounds(64, 1024);
+    const double c128 = rounds(128, 256) == 1 ? (f32 ? 0.5 : 0.7) : (double)rounds(128, 512);
     if constexpr (DT != HVS_F32) {
-        if (tiles(256) >= 256) return launch_tile<DT, Tile256>(st, p);
+        const double c256 = 1.75 * (double)rounds(256, 256);
+        if (c256 <= c128 && c256 <= c64) return launch_tile<DT, Tile256>(st, p);
     }
-    if (tiles(128) >= 256) return launch_tile<DT, Tile128>(st, p);
+    if (c128 <= c64) return launch_tile<DT, Tile128>(st, p);
     return launch_tile<DT, Tile64>(st, p);
 }
 
