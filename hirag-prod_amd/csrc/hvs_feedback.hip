@@ -480,7 +480,7 @@ extern "C" int hvs_index_preference_loss(hvs_index *idx, void *stream, const hvs
 #define CLIP_BATCH 64      // tensors per launch: their table travels in the kernel's arguments
 #define CLIP_CHUNK 8192    // most elements a block takes at a time,
 #define CLIP_CHUNK_MIN 1024  // ... and fewest: small sets are spread over as many blocks as that gives
-#define CLIP_BLOCKS 1024   // blocks of a norm launch, one partial sum each
+#define CLIP_BLOCKS 2048   // blocks of a norm launch, one partial sum each
 
 struct ClipTable {
     const void *data[CLIP_BATCH];
@@ -524,7 +524,20 @@ template <int DT> __device__ __forceinline__ double chunk_norm(const void *data,
     int64_t i = begin;
     if (((uintptr_t)data & 15) == 0) {
         const int64_t whole = begin + ((end - begin) / EPC) * EPC;
-        for (i = begin + threadIdx.x * EPC; i < whole; i += 256 * EPC) {
+        i = begin + threadIdx.x * EPC;
+        for (; i + 3 * 256 * EPC < whole; i += 4 * 256 * EPC) {  // four loads in flight (118 -> 100 us)
+            f32x4 c[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) c[k] = *reinterpret_cast<const f32x4 *>(p + i + k * 256 * EPC);
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                float v[EPC];
+                chunk_to_float<DT>(c[k], v);
+#pragma unroll
+                for (int e = 0; e < EPC; e++) add(v[e]);
+            }
+        }
+        for (; i < whole; i += 256 * EPC) {
             float v[EPC];
             chunk_to_float<DT>(*reinterpret_cast<const f32x4 *>(p + i), v);
 #pragma unroll
@@ -561,13 +574,15 @@ template <int DT> __device__ __forceinline__ void chunk_scale(const void *data, 
     int64_t i = begin;
     if (((uintptr_t)data & 15) == 0 && ((uintptr_t)out & 15) == 0) {
         const int64_t whole = begin + ((end - begin) / EPC) * EPC;
+        // what is written is not read again here: kept out of the caches, it leaves them to what the next norm pass reads
+        // (565 MB of gradients: norm pass 139 -> 118 us).  Four loads in flight, as the norm pass has them, cost 10 us here.
         for (i = begin + threadIdx.x * EPC; i < whole; i += 256 * EPC) {
             float v[EPC];
             chunk_to_float<DT>(*reinterpret_cast<const f32x4 *>(p + i), v);
             vec r;
 #pragma unroll
             for (int e = 0; e < EPC; e++) r[e] = learn_from_float<E>(v[e] * f);
-            *reinterpret_cast<vec *>(o + i) = r;
+            __builtin_nontemporal_store(r, reinterpret_cast<vec *>(o + i));
         }
         i = whole;
     }
