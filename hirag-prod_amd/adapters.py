@@ -204,7 +204,7 @@ class QueryAdapters:
         n = x.shape[0]
         codes = _numbers("codes", codes, n, torch.int32, self.device)
         if out is None:
-            out, ld_out = torch.empty((n, self.d_out), dtype=self.dtype, device=self.device), self.d_out
+            out, ld_out = x.new_empty(n, self.d_out), self.d_out
         else:
             out, ld_out = _out_rows("out", out, n, self.d_out, self.dtype, self.device)
         hidden = torch.empty((n, self.rank), dtype=torch.float32, device=self.device) if return_hidden else None
@@ -226,7 +226,7 @@ class QueryAdapters:
         codes = _numbers("codes", codes, n, torch.int32, self.device)
         hidden, _ = _rows("hidden", hidden, self.rank, torch.float32, self.device, n)
         hidden = hidden.contiguous()
-        grad_x = torch.empty((n, self.d_in), dtype=self.dtype, device=self.device) if input_grad else None
+        grad_x = x.new_empty(n, self.d_in) if input_grad else None
         grad_a = torch.empty(self.a.shape, dtype=torch.float32, device=self.device)
         grad_b = torch.empty(self.b.shape, dtype=torch.float32, device=self.device)
         ws, ws_ptr, size = self._workspace(n, max(ld_x, ld_grad), 1)
@@ -271,8 +271,9 @@ def _preference(queries, dim, chosen, rejected, offsets, reference, beta, label_
         if weights.dtype != torch.float32 or tuple(weights.shape) != (pairs,):
             raise ValueError(f"weights must hold {pairs} float32 entries")
         weights = weights.contiguous()
-    loss, margin = torch.empty((2, pairs), dtype=torch.float32, device=device)
-    grad = torch.empty((nq, dim), dtype=queries.dtype, device=device)
+    loss = torch.empty(pairs, dtype=torch.float32, device=device)
+    margin = torch.empty(pairs, dtype=torch.float32, device=device)
+    grad = queries.new_empty(nq, dim)
     st = HvsPreferenceStruct(queries.data_ptr(), ld, None if reference is None else reference.data_ptr(), ld_ref, offsets.data_ptr(), chosen.data_ptr(),
                              rejected.data_ptr(), None if weights is None else weights.data_ptr(), loss.data_ptr(), margin.data_ptr(),
                              grad.data_ptr(), dim, nq, pairs, code, float(beta), float(label_smoothing))
