@@ -268,7 +268,7 @@ def check_clip(env, grads, max_norm, infinity, norm, outs):
 
 @pytest.mark.parametrize("infinity", [False, True])
 @pytest.mark.parametrize("max_norm", [0.0, 0.3, 1e9])
-@pytest.mark.parametrize("sizes", [[1], [3, 0, 8191, 8192, 8193], [100000, 7], list(range(1, 200))])
+@pytest.mark.parametrize("sizes", [[1], [0], [3, 0, 8191, 8192, 8193], [0, 65000, 535, 1], [65000, 536, 1], [100000, 7], list(range(1, 200))])
 def test_clip(env, sizes, max_norm, infinity):
     torch = env.torch
     gen = torch.Generator().manual_seed(len(sizes))
