@@ -176,6 +176,7 @@ __global__ __launch_bounds__(GROUP_CHUNK) void group_place_kernel(const int32_t 
             scodes[place] = code;
         }
     } else {
+        __syncthreads();  // the first places of the last round of bins are down
         for (int w = 0; w < WAVES; w++) {
             if (w == wave && i < n) {
                 const uint32_t place = next[bin] + rank;

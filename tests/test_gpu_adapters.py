@@ -382,3 +382,18 @@ def test_refusals(env):
             hvs.QueryAdapters(*bad)
     with pytest.raises(ValueError):
         hvs.QueryAdapters.create(16, 2, rank=129)
+
+
+@pytest.mark.parametrize("adapters", [510, 511, 1022, 1023, 5000, 16382])
+def test_grouping_over_many_bins(env, adapters):
+    """Rows of the last and of the first adapters, more bins than a round of the grouping takes: each row comes back to its
+    place, with its own adapter, and an adapter's gradient holds its rows alone."""
+    torch = env.torch
+    for n in (1500, 9000):
+        gen = torch.Generator().manual_seed(n)
+        pick = torch.tensor([-1, 0, 1, adapters - 2, adapters - 1])
+        codes = torch.where(torch.rand(n, generator=gen) < 0.5, pick[torch.randint(0, 5, (n,), generator=gen)], torch.randint(0, adapters, (n,), generator=gen))
+        ad, x, codes, _ = make(env, "f32", n, 12, 20, 2, adapters, codes=codes)
+        y, hidden = check_apply(env, ad, x, codes, "f32")
+        g = torch.randn(n, 20, device=env.dev)
+        check_backward(ad, g, x, codes, hidden, "f32", *ad.backward(g, x, codes, hidden))
