@@ -222,13 +222,15 @@ template <int DT> __device__ __forceinline__ void shrink_store(const ShrinkParam
     }
     if (!p.u_hi || j >= p.rp) return;
     typedef E vec __attribute__((ext_vector_type(4)));
-    const int e2 = largest > 0.0f && largest < __builtin_inff() ? ilogbf(largest) + 1 : 0;
+    // (within 64: the power times the scale must stay a number, and beyond 2^64 bf16 holds u as it is, fp16 has none)
+    const int e2 = largest > 0.0f && largest < __builtin_inff() ? min(max(ilogbf(largest) + 1, -64), 64) : 0;
     vec hi, lo;
 #pragma unroll
     for (int e = 0; e < 4; e++) {
         const float v = known ? (DT == HVS_F32 ? u[e] : ldexpf(u[e], -e2)) : 0.0f;
         hi[e] = learn_from_float<E>(v);
-        lo[e] = learn_from_float<E>(v - learn_to_float((E)hi[e]));
+        const float rest = v - learn_to_float((E)hi[e]);
+        lo[e] = learn_from_float<E>(largest < __builtin_inff() ? rest : 0.0f);  // inf - inf: the first part says it all
     }
     *reinterpret_cast<vec *>(reinterpret_cast<E *>(p.u_hi) + at * p.rp + j) = hi;
     if (DT != HVS_F32) *reinterpret_cast<vec *>(reinterpret_cast<E *>(p.u_lo) + at * p.rp + j) = lo;
@@ -1049,7 +1051,7 @@ template <int DT, int RT, bool ALIGNED> __global__ __launch_bounds__(256) void o
         if (j >= rn || col >= cn) continue;
         const float v = red[0][j][col] + red[1][j][col];
         float *cell = out + (o.transposed ? (int64_t)(c0 + col) * p.r + j0 + j : (int64_t)(j0 + j) * o.d + c0 + col);
-        *cell = whole ? s * v + (p.accumulate ? *cell : 0.0f) : v;
+        *cell = !whole ? v : (lo < hi ? s * v : 0.0f) + (p.accumulate ? *cell : 0.0f);  // no rows: 0, whatever s is
     }
 }
 
@@ -1113,7 +1115,7 @@ struct AdapterWs {
 // Rows in a piece of the stack gradients, for passes of up to n rows: 128, in large passes 256, more where the partial sums would
 // take too much (8192 rows of 64 adapters, 128 / 256 / 512 / 1024 rows: 34, 38, 42, 52 us with the join).  Adapters of several pieces have at most 2 n / rows of them.
 static int piece_rows(int64_t n, const hvs_adapters *ad) {
-        int64_t rows = n <= 16384 ? 128 : 256;
+    int64_t rows = n <= 16384 ? 128 : 256;
     while (rows < MAX_CHUNK_ROWS && 2 * ((n + rows - 1) / rows) * ad->rank * (ad->d_in + ad->d_out) * 4 > OUTER_PARTIAL_BYTES) rows *= 2;
     return (int)rows;
 }
@@ -1153,6 +1155,7 @@ static uint64_t cut_workspace(const hvs_adapters *ad, int64_t nc, int backward, 
 extern "C" int hvs_adapters_workspace(const hvs_adapters *ad, int64_t n, int64_t max_ld, int backward, uint64_t *out_bytes) {
     HVS_TRY(check_adapters("hvs_adapters_workspace", ad));
     HVS_REQUIRE(n >= 0 && out_bytes, "hvs_adapters_workspace: negative row count or NULL argument");
+    HVS_REQUIRE(max_ld <= 0x7FFFFFFF, "hvs_adapters_workspace: row pitch %lld is 2 GB or more", (long long)max_ld);
     const int64_t nc = chunk_rows(n, max_ld > 0 ? max_ld : 1, hvs_elem_size(ad->dtype));
     AdapterWs ws;
     *out_bytes = n == 0 || (!backward && once(n, ad->rank)) ? 0 : cut_workspace(ad, nc, backward, nullptr, &ws);
@@ -1376,6 +1379,7 @@ extern "C" int hvs_adapters_apply(int device_id, void *stream, const hvs_adapter
     HVS_TRY(check_rows(who, "x", x, ld_x, ad->d_in, es));
     HVS_TRY(check_rows(who, "out", out, ld_out, ad->d_out, es));
     HVS_REQUIRE(codes != nullptr, "%s: codes is NULL", who);
+    HVS_REQUIRE(((uintptr_t)codes | (uintptr_t)hidden) % 4 == 0, "%s: codes or hidden is not aligned to its elements", who);
     HVS_REQUIRE(!learn_overlap(x, n, ld_x * es, (int64_t)ad->d_in * es, out, n, ld_out * es, (int64_t)ad->d_out * es), "%s: out overlaps x", who);
     const int64_t max_ld = ld_x > ld_out ? ld_x : ld_out;
     HVS_TRY(check_workspace(who, ad, n, max_ld, 0, workspace, workspace_bytes));
@@ -1487,6 +1491,7 @@ extern "C" int hvs_adapters_backward(int device_id, void *stream, const hvs_adap
     HVS_TRY(check_rows(who, "grad", grad, ld_grad, ad->d_out, es));
     HVS_TRY(check_rows(who, "x", x, ld_x, ad->d_in, es));
     HVS_REQUIRE(codes && hidden, "%s: codes or hidden is NULL", who);
+    HVS_REQUIRE(((uintptr_t)codes | (uintptr_t)hidden) % 4 == 0, "%s: codes or hidden is not aligned to its elements", who);
     int64_t max_ld = ld_grad > ld_x ? ld_grad : ld_x;
     if (grad_x) {
         HVS_TRY(check_rows(who, "grad_x", grad_x, ld_gx, ad->d_in, es));

@@ -390,6 +390,9 @@ static int check_preference_buffers(const char *who, const hvs_preference *p, co
     HVS_REQUIRE((uintptr_t)p->queries % qs == 0 && (uintptr_t)p->reference % qs == 0 && (uintptr_t)p->grad % qs == 0 &&
                     (uintptr_t)rows % hvs_elem_size(rows_dtype) == 0,
                 "%s: a tensor is not aligned to its elements", who);
+    HVS_REQUIRE(((uintptr_t)p->offsets | (uintptr_t)p->chosen | (uintptr_t)p->rejected) % 8 == 0 &&
+                    ((uintptr_t)p->weights | (uintptr_t)p->loss | (uintptr_t)p->margin) % 4 == 0,
+                "%s: a list is not aligned to its elements", who);
     HVS_REQUIRE(!learn_overlap(p->queries, p->n_queries, p->ld_queries * qs, (int64_t)dim * qs, p->grad, p->n_queries, p->ld_grad * qs, (int64_t)dim * qs) &&
                     !(p->reference && learn_overlap(p->reference, p->n_queries, p->ld_reference * qs, (int64_t)dim * qs, p->grad, p->n_queries, p->ld_grad * qs,
                                                     (int64_t)dim * qs)),

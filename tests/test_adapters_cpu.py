@@ -241,3 +241,22 @@ def test_store_sends_queries_through_the_adapters(coalesce):
             await ask(0, "ws1", "kb1")
 
     asyncio.run(scenario())
+
+
+def test_lists_off_their_elements_and_wide_pitches_are_refused():
+    import hirag_prod_amd as hvs
+    from hirag_prod_amd._lib import HvsPreferenceStruct
+
+    lib, ad, need = hvs.load_library(), adapters(), ctypes.c_uint64(0)
+    apply = lambda codes, hidden: lib.hvs_adapters_apply(0, None, ctypes.byref(ad), P, 64, codes, 3, Q, 64, hidden, W, 1 << 30)
+    back = lambda codes, hidden: lib.hvs_adapters_backward(0, None, ctypes.byref(ad), P, 64, P, 64, codes, hidden, 3, None, 0, Q, R, W, 1 << 30)
+    for call in (apply, back):
+        refused(call(R + 2, R), "aligned")
+        refused(call(R, R + 1), "aligned")
+    for wide in (1 << 31, 1 << 62):
+        refused(lib.hvs_adapters_workspace(ctypes.byref(ad), 5, wide, 0, ctypes.byref(need)), "pitch")
+    ok = dict(queries=P, ld_queries=16, reference=None, ld_reference=0, offsets=P, chosen=P, rejected=P, weights=P, loss=R, margin=R, grad=Q, ld_grad=16, n_queries=4,
+              n_pairs=9, query_dtype=0, beta=2.0, label_smoothing=0.0)
+    for name, off in (("offsets", 4), ("chosen", 4), ("rejected", 1), ("weights", 2), ("loss", 2), ("margin", 1)):
+        p = HvsPreferenceStruct(**{**ok, name: ok[name] + off})
+        refused(lib.hvs_preference_loss(0, None, ctypes.byref(p), R, 1, 16, 16, 50, W, 1 << 30), "aligned")

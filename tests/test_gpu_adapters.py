@@ -397,3 +397,47 @@ def test_grouping_over_many_bins(env, adapters):
         y, hidden = check_apply(env, ad, x, codes, "f32")
         g = torch.randn(n, 20, device=env.dev)
         check_backward(ad, g, x, codes, hidden, "f32", *ad.backward(g, x, codes, hidden))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n", [1, 30, 1100])
+def test_hidden_past_the_largest_number(env, dtype, n):
+    """A x beyond fp32: the row's outputs are infinite in the sign of B, on every route; the other tenant's are finite."""
+    torch = env.torch
+    t = getattr(torch, DT[dtype])
+    w, a, b = torch.zeros(24, 64, dtype=t, device=env.dev), torch.ones(2, 3, 64, dtype=t, device=env.dev), torch.ones(2, 24, 3, dtype=t, device=env.dev)
+    b[:, ::2] = -1
+    codes = torch.arange(n, device=env.dev, dtype=torch.int32) % 2
+    x = torch.where(codes[:, None] == 0, 3e38, 1.0).expand(n, 64).to(t)
+    y, hidden = env.hvs.QueryAdapters(w, a, b, torch.ones(2, device=env.dev)).apply(x.contiguous(), codes, return_hidden=True)
+    sign = torch.ones(24, device=env.dev)
+    sign[::2] = -1
+    assert bool((hidden[0::2] == torch.inf).all()) and bool((hidden[1::2] == 64).all())
+    assert torch.equal(y[0::2].float(), (sign * torch.inf).expand(len(y[0::2]), 24)) and torch.equal(y[1::2].float(), (sign * 192).expand(len(y[1::2]), 24))
+
+
+@pytest.mark.parametrize("n", [3, 2000])
+def test_scale_that_is_not_finite_without_rows(env, n):
+    """An adapter without rows has zero gradients, whatever its scale is."""
+    torch = env.torch
+    codes = torch.zeros(n, dtype=torch.int32)
+    ad, x, codes, gen = make(env, "f32", n, 40, 24, 4, 3, codes=codes)
+    ad.scale[1], ad.scale[2] = torch.nan, torch.inf
+    g = torch.randn(n, 24, generator=gen).to(env.dev)
+    _, hidden = ad.apply(x, codes, return_hidden=True)
+    _, da, db = ad.backward(g, x, codes, hidden)
+    assert not da[1:].any() and not db[1:].any() and bool(da[0].isfinite().all()) and bool(db[0].isfinite().all())
+
+
+@pytest.mark.parametrize("n", [20, 1100])
+def test_hidden_near_the_ends_of_the_range(env, n):
+    """A x of 2^127.5 and of 2^-100, with weights that bring y back to ordinary size."""
+    torch = env.torch
+    for big, scale in ((2.0**120, 2.0**-90), (2.0**-100, 2.0**100)):
+        x = torch.full((n, 64), big, dtype=torch.bfloat16, device=env.dev)
+        a = torch.full((1, 1, 64), 2.82, dtype=torch.bfloat16, device=env.dev)
+        b = torch.full((1, 16, 1), 1.5 * 2.0**-40, dtype=torch.bfloat16, device=env.dev) if big > 1 else torch.full((1, 16, 1), 1.5, dtype=torch.bfloat16, device=env.dev)
+        w = torch.zeros(16, 64, dtype=torch.bfloat16, device=env.dev)
+        y = env.hvs.QueryAdapters(w, a, b, torch.full((1,), scale, device=env.dev)).apply(x, torch.zeros(n, dtype=torch.int32, device=env.dev))
+        want = scale * np64(b).max() * 64 * big * np64(a).max()
+        assert np.abs(np64(y) - want).max() <= (2.0**-8 + 2.0**-15) * want, (big, want)
