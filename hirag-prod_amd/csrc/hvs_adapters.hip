@@ -59,11 +59,12 @@ __global__ __launch_bounds__(GROUP_CHUNK) void group_count_kernel(const int32_t 
 }
 
 // Every block finds the first place of each bin and how many of the bin's rows lie before its own, and places its rows; nothing
-// depends on timing.  Up to GROUP_SELF chunks it counts all rows itself (4096 rows: 5 us instead of 6 + 4 with a counting
-// launch); beyond, it adds up the counts of group_count_kernel, a wave per bin with a lane per chunk.
+// depends on timing.  Up to GROUP_SELF chunks it counts all rows itself; beyond, it adds up the counts of group_count_kernel, a
+// wave per bin with a lane per chunk (a call with 64-column outputs, counting itself / adding up: 4096 rows 16 adapters 17.8 /
+// 19.5 us, 256 adapters 20 / 34; 16 384 rows 31.3 / 29, 33 / 41; 32 768 rows 40 / 33, 41 / 44; 65 536 rows 59 / 42, 61 / 54).
 // FEW_BINS: the waves' counts per bin lie side by side in LDS and one barrier ranks the rows of the block; with more bins the
 // 16 waves take turns.  Inside a wave lanes of one bin find each other with one ballot per bit of the bin.
-#define GROUP_SELF 8
+#define GROUP_SELF 16
 #define GROUP_FEW_BINS 512
 template <bool FEW_BINS>
 __global__ __launch_bounds__(GROUP_CHUNK) void group_place_kernel(const int32_t *__restrict__ codes, int n, int S, int bits, int chunks,

@@ -1,5 +1,6 @@
 // The loss that query adapters are trained with, and the clipping of their gradients (C ABI: include/hvs.h).
 #include <algorithm>
+#include <climits>
 #include <new>
 #include <utility>
 #include <vector>
@@ -29,6 +30,7 @@ struct PreferenceParams {
     float beta, smoothing, default_weight;
     float *part_vec;  // [n_queries][shares][dim] sums of queries that several blocks work on
     float *part_num;  // [n_queries][shares]
+    float *part_inv;  // [n_queries] 1 / |y|
     int per_block;    // pairs a block takes before a second one joins in
 };
 
@@ -274,50 +276,71 @@ __global__ __launch_bounds__(64 * WAVES) void preference_kernel(PreferenceParams
         if (used == 1) out[k] = learn_from_float<Q>(inv_y * (v - sum * (TW == 1 ? smem[k] : inv_y * learn_to_float(yr[k]))));
         else pv[k] = v;
     }
-    if (used > 1 && tid == 0) p.part_num[q * shares + z] = sum;
+    // pairs before the first query's and after the last one's are left out like those with a negative position
+    if (z == 0) {
+        if (q == 0)
+            for (int64_t k = tid; k < b0; k += 64 * WAVES) p.loss[k] = p.margin[k] = 0.0f;
+        if (q == (int64_t)gridDim.x - 1)
+            for (int64_t k = b1 + tid; k < p.n_pairs; k += 64 * WAVES) p.loss[k] = p.margin[k] = 0.0f;
+    }
+    if (used > 1 && tid == 0) {
+        p.part_num[q * shares + z] = sum;
+        if (z == 0) p.part_inv[q] = inv_y;
+    }
 }
 
-// queries whose pairs several blocks shared: their sums in share order
-template <int QDT> __global__ __launch_bounds__(256) void preference_join_kernel(PreferenceParams p, int shares) {
+// Queries whose pairs several blocks shared: their sums, a block per query and 64 columns.  Each of the waves adds its part of the
+// shares in order, then the waves are added in order.
+#define JOIN_WAVES 8
+template <int QDT> __global__ __launch_bounds__(64 * JOIN_WAVES) void preference_join_kernel(PreferenceParams p, int shares) {
     typedef typename Elem<QDT>::type Q;
-    __shared__ float part[4];
+    __shared__ float part[JOIN_WAVES][64];
     const int64_t q = blockIdx.x;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, k = blockIdx.y * 64 + lane;
     int64_t b0, b1, per;
     int used;
     pair_share(p, q, shares, b0, b1, per, used);
     if (used == 1) return;
-    const Q *y = reinterpret_cast<const Q *>(p.y) + q * p.ld_y;
-    Q *out = reinterpret_cast<Q *>(p.grad) + q * p.ld_grad;
-    float yy = 0.0f;
-    for (int k = threadIdx.x; k < p.dim; k += 256) {
-        const float v = learn_to_float(y[k]);
-        yy = fmaf(v, v, yy);
+    const float *vec = p.part_vec + q * shares * p.dim + k, *num = p.part_num + q * shares;
+    float v = 0.0f, sum = 0.0f;
+    if (k < p.dim) {
+#pragma unroll 8
+        for (int z = wave; z < used; z += JOIN_WAVES) v += vec[(int64_t)z * p.dim];
     }
-    yy = learn_wave_sum(yy);
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = yy;
+    part[wave][lane] = v;
     __syncthreads();
-    const float inv_y = inverse_norm(part[0] + part[1] + part[2] + part[3]);
-    float sum = 0.0f;
-    for (int z = 0; z < used; z++) sum += p.part_num[q * shares + z];
-    for (int k = threadIdx.x; k < p.dim; k += 256) {
-        float v = 0.0f;
-        for (int z = 0; z < used; z++) v += p.part_vec[(q * shares + z) * p.dim + k];
-        out[k] = learn_from_float<Q>(inv_y * (v - sum * (inv_y * learn_to_float(y[k]))));
-    }
+    if (wave) return;
+    for (int z = lane; z < used; z += 64) sum += num[z];
+    sum = learn_wave_sum(sum);
+    if (k >= p.dim) return;
+    v = part[0][lane];
+#pragma unroll
+    for (int w = 1; w < JOIN_WAVES; w++) v += part[w][lane];
+    const float inv_y = p.part_inv[q], y = learn_to_float(reinterpret_cast<const Q *>(p.y)[q * p.ld_y + k]);
+    reinterpret_cast<Q *>(p.grad)[q * p.ld_grad + k] = learn_from_float<Q>(inv_y * (v - sum * (inv_y * y)));
 }
 
-#define PREF_FEW 512         // queries up to which several blocks may share a query's pairs,
-#define PREF_BLOCKS 1024     // ... about this many blocks in all,
-#define PREF_SHARE_PAIRS 16  // ... with this many pairs each
-#define PREF_WAVE_DIM 2048   // columns up to which a wave takes a pair by itself
+#define PREF_WAVE_DIM 2048  // columns up to which a wave takes a pair by itself
 
-static int preference_shares(const hvs_preference *p) {
-    if (p->n_queries < 1 || p->n_queries >= PREF_FEW) return 1;
-    const int64_t by_blocks = PREF_BLOCKS / p->n_queries, each = PREF_SHARE_PAIRS * p->n_queries, by_pairs = (p->n_pairs + each - 1) / each;
-    return (int)(by_pairs < 1 ? 1 : (by_blocks < by_pairs ? by_blocks : by_pairs));
+// How the pairs are spread over the chip, by counts alone (the host does not see the offsets); 1536 columns, fp16 rows.
+struct PreferencePlan {
+    int shares;     // blocks a query's pairs may be shared by
+    int per_block;  // pairs a block takes before another one joins in
+    bool wide;      // 16 waves a block instead of 4
+};
+static PreferencePlan preference_plan(const hvs_preference *p) {
+    const int64_t nq = p->n_queries, pairs = p->n_pairs;
+    // queries enough for the chip: a block each
+    if (nq < 1 || nq > 512) return {1, INT_MAX, false};
+    // Few pairs each: a block each saves the join, which reads a vector per block (a block each / shared: 16 x 16 10.6 / 9.9 us,
+    // 64 x 64 22.9 / 15.0; 100 x 16 10.5 / 13.0, 100 x 64 23.3 / 22.1, 400 x 32 27.5 / 36).  16 waves where there is a CU for each
+    // block and more than one pair for a wave (4 waves / 16: 100 x 4 7.1 / 7.3, 250 x 8 9.1 / 8.7, 250 x 16 13.2 / 11.2, 400 x 16 17.4 / 22.8).
+    if (pairs <= (nq <= 64 ? 16 : 64) * nq) return {1, INT_MAX, nq <= 256 && pairs > 4 * nq};
+    // more: blocks of a pair for each of 4 waves, until they are 512; then more pairs each
+    // (4, 8, 16, 32 pairs a block: 1 x 64 10.9, 12.2, 15.8, 22.6 us; 64 x 64 16.9, 15.0, 16.5, 23.2)
+    const int64_t even = (pairs + 511) / 512, per = even < 4 ? 4 : (even + 3) / 4 * 4, most = 1024 / nq, shares = (pairs + per - 1) / per;
+    return {(int)(shares < most ? shares : most), (int)(per < INT_MAX ? per : INT_MAX), false};
 }
-// 16 waves a block where few queries have many pairs each, so that one query's pairs are in flight together; else 4
-static bool preference_wide(const hvs_preference *p) { return p->n_queries < PREF_FEW && p->n_pairs > 8 * p->n_queries; }
 
 static int check_preference(const char *who, const hvs_preference *p, int dim) {
     HVS_REQUIRE(p != nullptr, "%s: NULL argument", who);
@@ -333,11 +356,12 @@ static int check_preference(const char *who, const hvs_preference *p, int dim) {
 extern "C" int hvs_preference_workspace(const hvs_preference *p, int dim, uint64_t *out_bytes) {
     HVS_TRY(check_preference("hvs_preference_workspace", p, dim));
     HVS_REQUIRE(out_bytes != nullptr, "hvs_preference_workspace: NULL argument");
-    const int shares = preference_shares(p);
+    const int shares = preference_plan(p).shares;
     WorkspaceCut w(nullptr);
     if (shares > 1) {
         w.take<float>((uint64_t)p->n_queries * shares * dim * 4);
         w.take<float>((uint64_t)p->n_queries * shares * 4);
+        w.take<float>((uint64_t)p->n_queries * 4);
     }
     *out_bytes = w.used;
     return 0;
@@ -374,7 +398,7 @@ template <int QDT, int RDT> static int run_preference(hipStream_t st, const Pref
 #undef PREF
     }
     if (shares > 1) {
-        preference_join_kernel<QDT><<<(unsigned)nq, 256, 0, st>>>(p, shares);
+        preference_join_kernel<QDT><<<dim3((unsigned)nq, (p.dim + 63) / 64), 64 * JOIN_WAVES, 0, st>>>(p, shares);
         HVS_HIP(hipGetLastError());
     }
     return 0;
@@ -405,23 +429,25 @@ static int check_preference_buffers(const char *who, const hvs_preference *p, co
 }
 
 static int preference_core(hipStream_t st, const hvs_preference *p, const void *rows, int rows_dtype, int dim, int64_t ld_rows, int64_t n_rows, void *workspace) {
-    const int shares = preference_shares(p);
+    const PreferencePlan plan = preference_plan(p);
+    const int shares = plan.shares;
     PreferenceParams k = {};
     k.y = p->queries, k.ref = p->reference, k.ld_y = p->ld_queries, k.ld_ref = p->ld_reference;
     k.offsets = p->offsets, k.chosen = p->chosen, k.rejected = p->rejected, k.weights = p->weights;
     k.loss = p->loss, k.margin = p->margin, k.grad = p->grad, k.ld_grad = p->ld_grad, k.n_pairs = p->n_pairs;
     k.rows = rows, k.ld_rows = ld_rows, k.n_rows = n_rows, k.dim = dim;
     k.beta = p->beta, k.smoothing = p->label_smoothing, k.default_weight = p->n_pairs > 0 ? (float)(1.0 / (double)p->n_pairs) : 0.0f;
-    k.per_block = PREF_SHARE_PAIRS;
+    k.per_block = plan.per_block;
     if (shares > 1) {
         WorkspaceCut w(workspace);
         k.part_vec = w.take<float>((uint64_t)p->n_queries * shares * dim * 4);
         k.part_num = w.take<float>((uint64_t)p->n_queries * shares * 4);
+        k.part_inv = w.take<float>((uint64_t)p->n_queries * 4);
     }
-#define ROWS(Q_)                                                                             \
-    (rows_dtype == HVS_F32 ? run_preference<Q_, HVS_F32>(st, k, p->n_queries, shares, preference_wide(p))        \
-                           : rows_dtype == HVS_F16 ? run_preference<Q_, HVS_F16>(st, k, p->n_queries, shares, preference_wide(p)) \
-                                                   : run_preference<Q_, HVS_BF16>(st, k, p->n_queries, shares, preference_wide(p)))
+#define ROWS(Q_)                                                                                     \
+    (rows_dtype == HVS_F32 ? run_preference<Q_, HVS_F32>(st, k, p->n_queries, shares, plan.wide)        \
+                           : rows_dtype == HVS_F16 ? run_preference<Q_, HVS_F16>(st, k, p->n_queries, shares, plan.wide) \
+                                                   : run_preference<Q_, HVS_BF16>(st, k, p->n_queries, shares, plan.wide))
     if (p->query_dtype == HVS_F32) return ROWS(HVS_F32);
     if (p->query_dtype == HVS_F16) return ROWS(HVS_F16);
     return ROWS(HVS_BF16);

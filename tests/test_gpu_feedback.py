@@ -449,3 +449,24 @@ def test_store_queries_through_adapters(env):
 
     asyncio.run(scenario())
     s.close()
+
+
+@pytest.mark.parametrize("nq", [1, 3, 600])
+def test_pairs_of_no_query(env, nq):
+    """A padded list: pairs before the first query's and after the last one's are left out, the others are what they are alone."""
+    torch = env.torch
+    q, ref, rows, c, r, off = make(env, "f32", "f16", nq, 96, 30, [5] * nq, seed=nq)
+    pad = lambda t: torch.cat([torch.full((7,), 10**9, device=env.dev), t, torch.full((300,), 3, device=env.dev)])
+    weights = torch.rand(len(c), device=env.dev)
+    wpad = torch.cat([torch.full((7,), torch.nan, device=env.dev), weights, torch.full((300,), torch.nan, device=env.dev)])
+    loss, margin, grad = env.hvs.preference_loss(q, rows, pad(c), pad(r), off + 7, reference=ref, beta=10.0, weights=wpad)
+    assert all(not t[:7].any() and not t[7 + len(c) :].any() for t in (loss, margin))
+    check_preference(q, ref, rows, c, r, off, (loss[7 : 7 + len(c)], margin[7 : 7 + len(c)], grad), "f32", 10.0, 0.0, weights)
+
+
+def test_one_query_with_most_pairs(env):
+    """Counts that say little about a query: among a few, one has nearly all pairs."""
+    for counts in ([0] * 30 + [700], [900] + [1] * 99, [0, 3, 2000, 1], [0] * 300 + [9000]):
+        q, ref, rows, c, r, off = make(env, "f32", "bf16", len(counts), 200, 60, counts, seed=len(counts))
+        got = env.hvs.preference_loss(q, rows, c, r, off, reference=ref, beta=10.0)
+        check_preference(q, ref, rows, c, r, off, got, "f32", 10.0, 0.0)
