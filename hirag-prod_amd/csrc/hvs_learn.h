@@ -145,12 +145,16 @@ static inline bool learn_dtype_ok(int dt) { return dt == HVS_F32 || dt == HVS_F1
 static inline bool learn_aligned(const void *p, int64_t ld_bytes, int64_t row_bytes) {
     return ((uintptr_t)p & 15) == 0 && (ld_bytes & 15) == 0 && (row_bytes & 15) == 0;
 }
-// [a, a + rows of row_bytes at pitch ld_bytes) and the same of b share a byte (conservatively: their hulls do)
+// rows_a rows of row_a bytes at pitch ld_a and the same of b share a byte.  Columns of one wide tensor do not; rows of different
+// pitches count as sharing where the ranges they span do.
 static inline bool learn_overlap(const void *a, int64_t rows_a, int64_t ld_a, int64_t row_a, const void *b, int64_t rows_b, int64_t ld_b, int64_t row_b) {
     if (rows_a <= 0 || rows_b <= 0) return false;
     const uintptr_t a0 = (uintptr_t)a, a1 = a0 + (uintptr_t)((rows_a - 1) * ld_a + row_a);
     const uintptr_t b0 = (uintptr_t)b, b1 = b0 + (uintptr_t)((rows_b - 1) * ld_b + row_b);
-    return a0 < b1 && b0 < a1;
+    if (a0 >= b1 || b0 >= a1) return false;
+    if (ld_a != ld_b || ld_a <= 0) return true;
+    const int64_t ahead = (int64_t)(b0 - a0) % ld_a, d = ahead < 0 ? ahead + ld_a : ahead;  // from a row of a to the next row of b
+    return d < row_a || d + row_b > ld_a;
 }
 // sizes of a workspace carved in 256-byte steps
 struct WorkspaceCut {

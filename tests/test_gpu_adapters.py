@@ -441,3 +441,111 @@ def test_hidden_near_the_ends_of_the_range(env, n):
         y = env.hvs.QueryAdapters(w, a, b, torch.full((1,), scale, device=env.dev)).apply(x, torch.zeros(n, dtype=torch.int32, device=env.dev))
         want = scale * np64(b).max() * 64 * big * np64(a).max()
         assert np.abs(np64(y) - want).max() <= (2.0**-8 + 2.0**-15) * want, (big, want)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_graph_of_many_rows(env, dtype):
+    """The grouped routes, captured: counted by the blocks themselves (3000 rows) and by a launch of its own (17 000)."""
+    torch = env.torch
+    for n, adapters in ((3000, 5), (17000, 600)):
+        ad, x, codes, gen = make(env, dtype, n, 48, 40, 4, adapters)
+        g = torch.randn(n, 40, generator=gen).to(env.dev, x.dtype)
+
+        def both():
+            y_, h_ = ad.apply(x, codes, return_hidden=True)
+            return (y_,) + ad.backward(g, x, codes, h_)
+
+        both()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = both()
+        for turn in range(4):
+            x.copy_(torch.randn(n, 48, generator=gen).to(env.dev, x.dtype))
+            codes.copy_(torch.randint(-1, adapters, (n,), generator=gen).to(env.dev, torch.int32))
+            want = both()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(o, w_) for o, w_ in zip(outs, want)), turn
+
+
+def test_two_streams_at_once(env):
+    """Calls of one object on two streams, each with scratch memory of its own, give what they give one after the other."""
+    torch = env.torch
+    ad, x, codes, gen = make(env, "bf16", 6000, 256, 256, 8, 30)
+    parts = [(x[:4000], codes[:4000]), (x[1000:], codes[1000:]), (x[:100], codes[:100])]
+    g = torch.randn(6000, 256, generator=gen).to(env.dev, x.dtype)
+
+    def step(part):
+        xp, cp = part
+        y, h = ad.apply(xp, cp, return_hidden=True)
+        return (y,) + ad.backward(g[: len(xp)], xp, cp, h)
+
+    want = [step(p) for p in parts]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in parts]
+    got = [None] * len(parts)
+    for _ in range(5):
+        for k, (stream, part) in enumerate(zip(streams, parts)):
+            with torch.cuda.stream(stream):
+                got[k] = step(part)
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+def test_offsets_past_32_bits(env):
+    """Rows of a wide tensor, so far apart that the last ones lie past 2^32 bytes and 2^31 elements."""
+    torch = env.torch
+    n, width = 5000, 450000
+    wide = torch.empty(n, width, dtype=torch.float16, device=env.dev)
+    ad, x, codes, gen = make(env, "f16", n, 72, 40, 4, 5)
+    strided = wide[:, :72]
+    strided.copy_(x)
+    out = wide[:, -40:]
+    assert strided.stride(0) == width and n * width > 2**31
+    want, hidden = ad.apply(x, codes, return_hidden=True)
+    y, h = ad.apply(strided, codes, return_hidden=True)
+    # passes of other sizes may take other routes: both are right to their own last bits
+    check_apply(env, ad, x, codes, "f16")
+    want64, tol, u, u_tol = lo.adapters_apply_tolerance(np64(x), codes.cpu().numpy(), *weights64(ad), "f16")
+    check(y, want64, tol, "y")
+    check(h, u, u_tol, "hidden")
+    g = torch.randn(n, 40, generator=gen).to(env.dev, x.dtype)
+    out.copy_(g)
+    check_backward(ad, g, x, codes, hidden, "f16", *ad.backward(out, strided, codes, hidden))
+    few = ad.apply(strided[-3:], codes[-3:])
+    check(few, want64[-3:], tol[-3:], "last rows")
+
+
+def test_tensors_that_require_gradients(env):
+    """Parameters and views are taken as the numbers they hold; no graph is recorded."""
+    torch = env.torch
+    ad, x, codes, _ = make(env, "f32", 33, 40, 24, 4, 3)
+    par = env.hvs.QueryAdapters(ad.projection, torch.nn.Parameter(ad.a), torch.nn.Parameter(ad.b), ad.scale)
+    xp = torch.nn.Parameter(x)
+    y = par.apply(xp, codes)
+    assert not y.requires_grad and torch.equal(y, ad.apply(x, codes))
+    assert torch.equal(par.apply(x.t().contiguous().t(), codes), y) and torch.equal(par.apply(x[:1].expand(33, 40), codes), ad.apply(x[:1].repeat(33, 1), codes))
+    assert torch.equal(par.apply(x.flip(0), codes.flip(0)), y.flip(0))
+
+
+@pytest.mark.parametrize("n", [1, 40, 2000])
+def test_columns_of_one_tensor(env, n):
+    """Input and output side by side in one tensor are apart; a column in common, or other pitches over the same range, is not."""
+    torch = env.torch
+    ad, x, codes, gen = make(env, "f32", n, 24, 20, 4, 3)
+    want, tol, _, _ = lo.adapters_apply_tolerance(np64(x), codes.cpu().numpy(), *weights64(ad), "f32")
+    for x_at, out_at in ((0, 24), (20, 0), (1, 27)):
+        wide = torch.zeros(n, 48, device=env.dev)
+        wide[:, x_at : x_at + 24] = x
+        got = ad.apply(wide[:, x_at : x_at + 24], codes, out=wide[:, out_at : out_at + 20])
+        check(got, want, tol, "y")
+        assert torch.equal(wide[:, x_at : x_at + 24], x)
+        assert not wide[:, max(x_at + 24, out_at + 20) :].any()
+    wide = torch.zeros(n + 1, 48, device=env.dev)
+    for x_at, out_at in ((0, 23), (19, 0), (4, 4)):
+        with pytest.raises(env.hvs.HvsError, match="overlaps"):
+            ad.apply(wide[:n, x_at : x_at + 24], codes, out=wide[:n, out_at : out_at + 20])
+    if n > 1:
+        with pytest.raises(env.hvs.HvsError, match="overlaps"):
+            ad.apply(wide[:n, :24], codes, out=wide.view(-1)[24 : 24 + n * 20].view(n, 20))

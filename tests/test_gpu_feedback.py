@@ -470,3 +470,70 @@ def test_one_query_with_most_pairs(env):
         q, ref, rows, c, r, off = make(env, "f32", "bf16", len(counts), 200, 60, counts, seed=len(counts))
         got = env.hvs.preference_loss(q, rows, c, r, off, reference=ref, beta=10.0)
         check_preference(q, ref, rows, c, r, off, got, "f32", 10.0, 0.0)
+
+
+def test_table_read_by_two_streams_then_changed(env):
+    """Rows are read as they were when the call was made, whatever the table does next, on two streams in turn."""
+    torch = env.torch
+    q, ref, rows, c, r, off = make(env, "f32", "f16", 300, 512, 4000, [60] * 300, seed=3)
+    for change in ("update", "compact", "add"):
+        idx = env.hvs.HvsIndex(512, "f16", device=0)
+        idx.add(rows)
+        want = env.hvs.preference_loss(q, rows, c, r, off, reference=ref)
+        torch.cuda.synchronize()
+        streams = [torch.cuda.Stream() for _ in range(2)]
+        got = []
+        for turn in range(4):
+            with torch.cuda.stream(streams[turn % 2]):
+                got.append(idx.preference_loss(q, c, r, off, reference=ref))
+        if change == "update":
+            idx.update(np.arange(4000), np.zeros((4000, 512), dtype=np.float32))
+        elif change == "compact":
+            idx.set_deleted(np.arange(0, 4000, 2))
+            idx.compact()
+        else:
+            idx.add(rows)
+        torch.cuda.synchronize()
+        for one in got:
+            assert all(torch.equal(a, b) for a, b in zip(one, want)), change
+        idx.close()
+
+
+def test_rows_past_32_bits(env):
+    """Positions of rows that lie past 2^31 elements."""
+    torch = env.torch
+    n, dim = 2_200_000, 1024
+    rows = torch.empty(n, dim, dtype=torch.float16, device=env.dev)
+    q, ref, some, c, r, off = make(env, "bf16", "f16", 30, dim, 50, None, seed=21)
+    at = torch.cat([torch.arange(25), torch.arange(n - 25, n)]).to(env.dev)
+    rows[at] = some
+    got = env.hvs.preference_loss(q, rows, at[c], at[r], off, reference=ref)
+    want = env.hvs.preference_loss(q, some, c, r, off, reference=ref)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_clip_past_32_bits(env):
+    torch = env.torch
+    n = 2**31 + 4096 + 3
+    g = torch.zeros(n, dtype=torch.float16, device=env.dev)
+    at = torch.tensor([0, 5, 2**31 - 1, 2**31, n - 1], device=env.dev)
+    g[at] = 4.0
+    norm = env.hvs.clip_grad_norm([g, torch.zeros(3, device=env.dev)], 1.0)
+    want = (5 * 16) ** 0.5
+    assert abs(float(norm) - want) <= 2.0**-24 * want
+    half = 2.0**-11 + 2.0**-22
+    assert bool(((g[at].double() - 4.0 / (want + 1e-6)).abs() <= half * 4 / want).all()) and int((g != 0).sum()) == 5
+
+
+def test_clip_graph_of_one_launch(env):
+    torch = env.torch
+    g = torch.ones(500, device=env.dev)
+    graph = torch.cuda.CUDAGraph()
+    out = torch.zeros_like(g)
+    with torch.cuda.graph(graph):
+        norm = env.hvs.clip_grad_norm([g], 1.0, out=[out])
+    for turn in range(4):
+        g.copy_(torch.randn(500, device=env.dev))
+        graph.replay()
+        torch.cuda.synchronize()
+        check_clip(env, [g], 1.0, False, norm, [out])
