@@ -193,7 +193,8 @@ class QueryAdapters:
 
         A torch tensor of the adapters' dtype gives a torch tensor (``out``, when given); with ``return_hidden`` also the
         float32 [n, rank] values ``A[c] x`` that ``backward`` takes.  A numpy array (float32, from an embedding service)
-        gives a float32 numpy array.  A code past the last adapter makes its row NaN.  ``out`` must not overlap ``x``."""
+        gives a float32 numpy array.  A code past the last adapter makes its row NaN.  ``out`` must not overlap ``x``
+        (columns of one wide tensor do not)."""
         if not isinstance(x, torch.Tensor):
             if out is not None or return_hidden:
                 raise ValueError("out and return_hidden need device tensors")
@@ -286,8 +287,8 @@ def _preference(queries, dim, chosen, rejected, offsets, reference, beta, label_
 def preference_loss(queries, rows, chosen, rejected, offsets, reference=None, beta: float = 20.0, label_smoothing: float = 0.0, weights=None):
     """Preference loss of pairs of rows and its gradient for the queries, in one pass over the rows.
 
-    ``queries`` [nq, dim]; ``rows`` [n, dim]; pairs ``offsets[i] .. offsets[i + 1]`` (``offsets`` [nq + 1], ascending from 0)
-    belong to query i; ``chosen`` / ``rejected`` are row positions.  With a policy that picks rows by softmax(beta cos(query, row)),
+    ``queries`` [nq, dim]; ``rows`` [n, dim]; pairs ``offsets[i] .. offsets[i + 1]`` (``offsets`` [nq + 1], ascending)
+    belong to query i, and pairs outside all of them are left out; ``chosen`` / ``rejected`` are row positions.  With a policy that picks rows by softmax(beta cos(query, row)),
     ``margin = (cos(q, chosen) - cos(q, rejected)) - (cos(q0, chosen) - cos(q0, rejected))`` for the reference policy's
     queries q0 (``reference`` [nq, dim]; None: without that term) is the paired log ratio over beta, and
     ``loss = -(1 - s) log sigmoid(beta margin) - s log sigmoid(-beta margin)`` with ``s = label_smoothing`` in [0, 0.5].

@@ -807,7 +807,9 @@ class HipVectorStore(BaseVDB):
         """Send the embeddings of every ``query`` through ``adapters`` (a ``QueryAdapters``, or None to stop) before the
         search.  ``codes``: (workspace id, knowledge base id) -> adapter number; pairs that are not named go through the
         shared projection alone.  The stored rows stay as they are, so this may change at any time; a query uses the
-        adapters that are set when its embedding arrives.  Not part of ``save``: the weights are the caller's."""
+        adapters that are set when its embedding arrives.  Queries run on torch's default stream: weights that a training loop
+        changes in place should be changed there too, or be swapped for another object.  Not part of ``save``: the weights
+        are the caller's."""
         codes = {(str(w), str(k)): int(c) for (w, k), c in (codes or {}).items()}
         if adapters is not None:
             bad = [c for c in codes.values() if not 0 <= c < adapters.n_adapters]

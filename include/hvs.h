@@ -453,8 +453,9 @@ int hvs_graph_top_chunks(hvs_graph *g, int k, int32_t *out_nodes, double *out_sc
  * All buffers of these calls are device memory of device_id unless said otherwise; work is submitted to `stream` (a
  * hipStream_t, NULL = the default stream) and nothing waits for it; nothing is allocated, so the calls may be captured
  * into a HIP graph.  `workspace` is scratch memory of the size the matching ..._workspace call reports, aligned to 256
- * bytes; its contents mean nothing before and after, and calls that may overlap (two streams, two captured graphs) need
- * one each.  The calling thread's current device is left as it was.
+ * bytes (NULL where that size is 0); its contents mean nothing before and after, and calls that may overlap (two streams,
+ * two captured graphs) need one each.  Every buffer starts on a whole number of its elements.  The calling thread's current
+ * device is left as it was.
  */
 
 /*
@@ -483,7 +484,7 @@ int hvs_adapters_workspace(const hvs_adapters *ad, int64_t n, int64_t max_ld, in
  * Apply the adapters to n rows at once, each row with its own: x [n, d_in] (row pitch ld_x elements), codes int32 [n]; out
  * [n, d_out] (row pitch ld_out), of the weights' dtype, rounded once from fp32 sums.  A code < 0 means no adapter (W x
  * alone); a code >= n_adapters makes the row NaN.  hidden: float [n, rank] or NULL, receives A[c] x (0 without adapter),
- * which hvs_adapters_backward takes.  out must not overlap the inputs.
+ * which hvs_adapters_backward takes.  out must not overlap x (columns of one wide tensor, at one pitch, do not overlap).
  */
 int hvs_adapters_apply(int device_id, void *stream, const hvs_adapters *ad, const void *x, int64_t ld_x,
                        const int32_t *codes, int64_t n, void *out, int64_t ld_out, float *hidden,
@@ -508,8 +509,8 @@ int hvs_adapters_backward(int device_id, void *stream, const hvs_adapters *ad, c
  *     margin = (cos(q, chosen) - cos(q, rejected)) - (cos(q0, chosen) - cos(q0, rejected))
  *     loss   = -(1 - label_smoothing) log sigmoid(beta margin) - label_smoothing log sigmoid(-beta margin)
  * q0 = the reference policy's query (the embedding before adaptation); reference NULL: its term is 0.  Pairs
- * offsets[i] .. offsets[i + 1] - 1 belong to query i (int64 [n_queries + 1], ascending from 0 to n_pairs; a query may have
- * none).  chosen / rejected: int64 row positions.  A pair with a negative position is left out (loss and margin 0, no
+ * offsets[i] .. offsets[i + 1] - 1 belong to query i (int64 [n_queries + 1], ascending within 0 .. n_pairs; a query may
+ * have none, and pairs before offsets[0] and from offsets[n_queries] on are left out).  chosen / rejected: int64 row positions.  A pair with a negative position is left out (loss and margin 0, no
  * gradient); one with a position past the last row gets a NaN loss and margin and makes its query's gradient NaN.
  * grad [n_queries, dim], the queries' dtype: gradient of sum_p weights[p] loss[p]; weights NULL = 1 / n_pairs each (the
  * mean).  A query of norm 0 gets gradient 0.  Sums run in a fixed order.
@@ -546,8 +547,8 @@ int hvs_index_preference_loss(hvs_index *idx, void *stream, const hvs_preference
  * Global norm over many tensors and the clipped tensors: norm = sqrt(sum of squares over all elements), or the largest
  * absolute value with infinity_norm; out = data * min(1, max_norm / (norm + 1e-6)), rounded once.  The sum of squares is
  * held in double precision.  out may be data itself (in place) or separate memory of the same type; tensors may differ in
- * type; what is written shares no memory with any other tensor of the call.  tensors is a HOST array, read before the call returns; norm (device float) receives the norm before clipping.  A
- * NaN anywhere makes the norm and every output NaN; an infinite norm makes the factor 0.
+ * type; what is written shares no memory with any other tensor of the call.  tensors is a HOST array, read before the call
+ * returns; norm (device float) receives the norm before clipping.  A NaN anywhere makes the norm and every output NaN; an infinite norm makes the factor 0.
  */
 typedef struct hvs_tensor {
     const void *data;
