@@ -66,12 +66,24 @@ __global__ __launch_bounds__(GROUP_CHUNK) void group_count_kernel(const int32_t 
 // 16 waves take turns.  Inside a wave lanes of one bin find each other with one ballot per bit of the bin.
 #define GROUP_SELF 16
 #define GROUP_FEW_BINS 512
-template <bool FEW_BINS>
-__global__ __launch_bounds__(GROUP_CHUNK) void group_place_kernel(const int32_t *__restrict__ codes, int n, int S, int bits, int chunks,
-                                                                  const uint32_t *__restrict__ counts, uint32_t *__restrict__ order,
-                                                                  int32_t *__restrict__ scodes, uint32_t *__restrict__ seg_begin, PieceTable pieces) {
+struct GroupParams {
+    const int32_t *codes;
+    int n, S, bits, chunks;  // bits: of a bin's number
+    uint32_t *counts;        // [chunks][S + 2] of group_count_kernel
+    uint32_t *order;
+    int32_t *scodes;
+    uint32_t *seg_begin;
+    PieceTable pieces;
+};
+// next: LDS, [S + 2] next free place of every bin, then [S + 2] its rows before this block's
+template <bool FEW_BINS> __device__ __forceinline__ void group_place(const GroupParams &p, uint32_t *next) {
     constexpr int WAVES = GROUP_CHUNK / 64;
-    extern __shared__ uint32_t next[];  // [S + 2] next free place of every bin; [S + 2] its rows before this block's
+    const int32_t *__restrict__ codes = p.codes;
+    const uint32_t *__restrict__ counts = p.counts;
+    uint32_t *__restrict__ order = p.order, *__restrict__ seg_begin = p.seg_begin;
+    int32_t *__restrict__ scodes = p.scodes;
+    const PieceTable &pieces = p.pieces;
+    const int n = p.n, S = p.S, bits = p.bits, chunks = p.chunks;
     __shared__ uint32_t wave_sum[WAVES];
     __shared__ uint16_t by_wave[FEW_BINS ? WAVES : 1][FEW_BINS ? GROUP_FEW_BINS : 1];
     const int nb = S + 2, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, me = blockIdx.x;
@@ -189,6 +201,11 @@ __global__ __launch_bounds__(GROUP_CHUNK) void group_place_kernel(const int32_t 
             __syncthreads();
         }
     }
+}
+
+template <bool FEW_BINS> __global__ __launch_bounds__(GROUP_CHUNK) void group_place_kernel(GroupParams p) {
+    extern __shared__ uint32_t lds[];
+    group_place<FEW_BINS>(p, lds);
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -908,43 +925,53 @@ __global__ __launch_bounds__(256) void pack_rows_kernel(const E *__restrict__ sr
 }
 
 // dst[z][c][r] = src[z][r][c] for `count` matrices of R x C; dst rows have pitch ld (>= R), filled with zeros past R
+// tiles of 2^12, 2^13, 2^14 elements: 96 rows of fp32 weights 768 x 768 5.2, 6.1, 7.8 us; 8192 rows, bf16 1536 x 1536 14.9, 12.0, 12.6
+#define TILE_LOG 13
+#define TILE_LOG_NARROW 4
 struct TransposeJob {
     const void *src;
     void *dst;
-    int R, C, ld, tiles_c, tiles_r, log_c;  // tiles of 4096 elements, 2^log_c columns wide: narrow matrices get narrow tiles
+    int R, C, ld, tiles_c, tiles_r, log_c;  // tiles of 2^TILE_LOG elements, 2^log_c columns wide: narrow matrices get narrow tiles
     int64_t blocks;                         // tiles_c tiles_r count
 };
 struct TransposeJobs {
     TransposeJob job[3];
 };
-// all transposed weights of a backward pass in one launch: a block per tile, jobs one after the other
-template <typename E> __global__ __launch_bounds__(256) void transpose_kernel(TransposeJobs jobs) {
-    __shared__ E tile[256 * 17];  // rows of 2^log_c + 1 elements: 256 x 17, 64 x 65 or 16 x 257
-    int64_t at = blockIdx.x;
+// All transposed weights of a backward pass in one launch, a block per tile, jobs one after the other; the first group_blocks
+// blocks group the rows meanwhile, where they count them by themselves (a launch of its own took 4 us more at 96 rows).
+template <typename E> __global__ __launch_bounds__(GROUP_CHUNK) void layout_kernel(TransposeJobs jobs, GroupParams group, int group_blocks) {
+    extern __shared__ uint32_t lds[];
+    if ((int)blockIdx.x < group_blocks) {
+        group_place<true>(group, lds);
+        return;
+    }
+    E *tile = reinterpret_cast<E *>(lds);  // rows of 2^log_c + 1 elements
+    constexpr int PER = (1 << TILE_LOG) / GROUP_CHUNK;
+    int64_t at = (int64_t)blockIdx.x - group_blocks;
     int which = 0;
     while (which < 2 && at >= jobs.job[which].blocks) at -= jobs.job[which++].blocks;
     const TransposeJob &t = jobs.job[which];
     const int64_t z = at / (t.tiles_c * t.tiles_r);
     const int rest = (int)(at - z * (t.tiles_c * t.tiles_r));
-    const int log_c = t.log_c, log_r = 12 - log_c, pitch = (1 << log_c) + 1;
+    const int log_c = t.log_c, log_r = TILE_LOG - log_c, pitch = (1 << log_c) + 1;
     const E *s = reinterpret_cast<const E *>(t.src) + z * (int64_t)t.R * t.C;
     E *d = reinterpret_cast<E *>(t.dst) + z * (int64_t)t.C * t.ld;
     const int r0 = rest / t.tiles_c << log_r, c0 = rest % t.tiles_c << log_c;
-    E v[16];
+    E v[PER];
 #pragma unroll
-    for (int k = 0; k < 16; k++) {
-        const int i = threadIdx.x + 256 * k, r = r0 + (i >> log_c), c = c0 + (i & ((1 << log_c) - 1));
+    for (int k = 0; k < PER; k++) {
+        const int i = threadIdx.x + GROUP_CHUNK * k, r = r0 + (i >> log_c), c = c0 + (i & ((1 << log_c) - 1));
         v[k] = r < t.R && c < t.C ? s[(int64_t)r * t.C + c] : (E)0.0f;
     }
 #pragma unroll
-    for (int k = 0; k < 16; k++) {
-        const int i = threadIdx.x + 256 * k;
+    for (int k = 0; k < PER; k++) {
+        const int i = threadIdx.x + GROUP_CHUNK * k;
         tile[(i >> log_c) * pitch + (i & ((1 << log_c) - 1))] = v[k];
     }
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < 16; k++) {
-        const int i = threadIdx.x + 256 * k, c = i >> log_r, r = i & ((1 << log_r) - 1);
+    for (int k = 0; k < PER; k++) {
+        const int i = threadIdx.x + GROUP_CHUNK * k, c = i >> log_r, r = i & ((1 << log_r) - 1);
         if (c0 + c < t.C && r0 + r < t.ld) d[(int64_t)(c0 + c) * t.ld + r0 + r] = tile[r * pitch + c];
     }
 }
@@ -1163,20 +1190,24 @@ extern "C" int hvs_adapters_workspace(const hvs_adapters *ad, int64_t n, int64_t
     return 0;
 }
 
-static int launch_group(hipStream_t st, const int32_t *codes, int n, int S, const AdapterWs &ws) {
-    const int chunks = (n + GROUP_CHUNK - 1) / GROUP_CHUNK;
-    const size_t lds = (size_t)(S + 2) * 4;
+static GroupParams group_params(const int32_t *codes, int n, int S, const AdapterWs &ws) {
     int bits = 1;
     while ((1 << bits) < S + 2) bits++;
-    if (chunks > GROUP_SELF) {
+    return {codes, n, S, bits, (n + GROUP_CHUNK - 1) / GROUP_CHUNK, ws.counts, ws.order, ws.scodes, ws.seg_begin, ws.pieces};
+}
+static bool group_alone(const GroupParams &g) { return g.chunks <= GROUP_SELF && g.S + 2 <= GROUP_FEW_BINS; }  // by one launch, in little LDS
+
+static int launch_group(hipStream_t st, const GroupParams &g) {
+    const size_t lds = (size_t)(g.S + 2) * 4;
+    if (g.chunks > GROUP_SELF) {
         HVS_TRY((learn_allow_lds<group_count_kernel>((int)lds)));
-        group_count_kernel<<<chunks, GROUP_CHUNK, lds, st>>>(codes, n, S, ws.counts);
+        group_count_kernel<<<g.chunks, GROUP_CHUNK, lds, st>>>(g.codes, g.n, g.S, g.counts);
     }
-    if (S + 2 <= GROUP_FEW_BINS) {
-        group_place_kernel<true><<<chunks, GROUP_CHUNK, 2 * lds, st>>>(codes, n, S, bits, chunks, ws.counts, ws.order, ws.scodes, ws.seg_begin, ws.pieces);
+    if (g.S + 2 <= GROUP_FEW_BINS) {
+        group_place_kernel<true><<<g.chunks, GROUP_CHUNK, 2 * lds, st>>>(g);
     } else {
         HVS_TRY((learn_allow_lds<group_place_kernel<false>>((int)(2 * lds))));
-        group_place_kernel<false><<<chunks, GROUP_CHUNK, 2 * lds, st>>>(codes, n, S, bits, chunks, ws.counts, ws.order, ws.scodes, ws.seg_begin, ws.pieces);
+        group_place_kernel<false><<<g.chunks, GROUP_CHUNK, 2 * lds, st>>>(g);
     }
     HVS_HIP(hipGetLastError());
     return 0;
@@ -1259,8 +1290,8 @@ template <int DT> static int launch_pack(hipStream_t st, const void *src, int64_
 static TransposeJob transpose_job(const void *src, int64_t count, int R, int C, int ld, void *dst) {
     TransposeJob t = {};
     t.src = src, t.dst = dst, t.R = R, t.C = C, t.ld = ld;
-    t.log_c = C <= 32 ? 4 : (ld <= 32 ? 8 : 6);
-    const int tc = 1 << t.log_c, tr = 4096 >> t.log_c;
+    t.log_c = C <= 32 ? TILE_LOG_NARROW : (ld <= 32 ? TILE_LOG - TILE_LOG_NARROW : TILE_LOG / 2);
+    const int tc = 1 << t.log_c, tr = (1 << TILE_LOG) >> t.log_c;
     t.tiles_c = (C + tc - 1) / tc, t.tiles_r = (ld + tr - 1) / tr;  // the row tiles cover the pitch, so that the padding is written
     t.blocks = count * t.tiles_c * t.tiles_r;
     return t;
@@ -1316,7 +1347,7 @@ static int run_direction(hipStream_t st, const hvs_adapters *ad, const Direction
         p.hidden = s.hidden;
         return launch_few<DT>(st, p);
     }
-    if (!grouped) HVS_TRY(launch_group(st, codes, n, s.S, ws));
+    if (!grouped) HVS_TRY(launch_group(st, group_params(codes, n, s.S, ws)));
     s.codes = ws.scodes, s.order = ws.order;
     if (d.out) s.u_hi = ws.u_hi, s.u_lo = ws.u_lo, s.factor = ws.factor;
     HVS_TRY(launch_shrink<DT>(st, s, SHRINK_SHARES));
@@ -1446,12 +1477,17 @@ static int run_backward(hipStream_t st, const hvs_adapters *ad, const void *grad
         jobs.job[k++] = transpose_job(ad->a, ad->n_adapters, ad->rank, ad->d_in, rp, ws.a_t);
     }
     const int64_t blocks = jobs.job[0].blocks + jobs.job[1].blocks + jobs.job[2].blocks;
-    HVS_REQUIRE(blocks <= 0x7FFFFFFF, "hvs_adapters_backward: %d adapters of %d x %d x %d are too many for one launch", ad->n_adapters, ad->rank, ad->d_in, ad->d_out);
-    transpose_kernel<typename Elem<DT>::type><<<(unsigned)blocks, 256, 0, st>>>(jobs);
+    const GroupParams first = group_params(codes, (int)(n < nc ? n : nc), ad->n_adapters, ws);
+    const int beside = group_alone(first) ? first.chunks : 0;
+    const size_t tile_lds = ((1 << TILE_LOG) + (1 << (TILE_LOG - TILE_LOG_NARROW))) * sizeof(typename Elem<DT>::type), group_lds = (size_t)(ad->n_adapters + 2) * 8;
+    const size_t lds = beside && group_lds > tile_lds ? group_lds : tile_lds;
+    HVS_TRY((learn_allow_lds<layout_kernel<typename Elem<DT>::type>>((int)lds)));
+    HVS_REQUIRE(blocks <= 0x7FFFFFFF - GROUP_SELF, "hvs_adapters_backward: %d adapters of %d x %d x %d are too many for one launch", ad->n_adapters, ad->rank, ad->d_in, ad->d_out);
+    layout_kernel<typename Elem<DT>::type><<<(unsigned)(blocks + beside), GROUP_CHUNK, lds, st>>>(jobs, first, beside);
     HVS_HIP(hipGetLastError());
     for (int64_t r0 = 0; r0 < n; r0 += nc) {
         const int rows = (int)(n - r0 < nc ? n - r0 : nc);
-        HVS_TRY(launch_group(st, codes + r0, rows, ad->n_adapters, ws));
+        if (r0 > 0 || !beside) HVS_TRY(launch_group(st, group_params(codes + r0, rows, ad->n_adapters, ws)));
         Direction d = {};
         d.x = (const char *)grad + r0 * ld_grad * es, d.ld_x = ld_grad;
         d.a = ws.b_t, d.lda = dop, d.w = ws.w_t, d.ldw = dop, d.b = ws.a_t, d.ldb = rp, d.b_padded = true;
