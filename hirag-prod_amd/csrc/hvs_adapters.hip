@@ -1001,10 +1001,10 @@ struct OuterParams {
 // rows; one of several leaves its sums in `partial`, and outer_join_kernel adds them in order.  A block per adapter and
 // piece keeps the blocks alike whether there are few adapters or hundreds (96 rows, 256 adapters: cutting the rows alone, so
 // that a block met many adapters one after the other, took twice as long).
-template <int DT, int RT, bool ALIGNED> __global__ __launch_bounds__(256) void outer_kernel(OuterParams p) {
+template <int DT, int RT, bool ALIGNED> __global__ __launch_bounds__(256, RT == 1 ? 5 : 1) void outer_kernel(OuterParams p) {
     typedef typename Elem<DT>::type E;
     constexpr int EPC = Elem<DT>::EPC, CC = 16 * EPC, COPIES = 2;
-    __shared__ float red[COPIES][RT * 16][CC + 1];
+    __shared__ float red[COPIES][RT * 16][CC + 4];  // column m EPC + e of a row lies at 16 e + m: the 64 lanes of a sum hit 64 banks
     __shared__ uint32_t rows[OUTER_ROWS];
     const Piece piece = p.pieces.piece[blockIdx.x];
     if (blockIdx.x >= *p.pieces.count) return;
@@ -1063,7 +1063,7 @@ template <int DT, int RT, bool ALIGNED> __global__ __launch_bounds__(256) void o
             for (int e = 0; e < EPC; e++)
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
-                    float *cell = &red[copy][t * 16 + 4 * g + k][m * EPC + e];
+                    float *cell = &red[copy][t * 16 + 4 * g + k][16 * e + m];
                     *cell = add ? *cell + acc[t][e][k] : acc[t][e][k];
                 }
     };
@@ -1077,7 +1077,7 @@ template <int DT, int RT, bool ALIGNED> __global__ __launch_bounds__(256) void o
     for (int k = tid; k < RT * 16 * CC; k += 256) {
         const int j = o.transposed ? k % (RT * 16) : k / CC, col = o.transposed ? k / (RT * 16) : k % CC;
         if (j >= rn || col >= cn) continue;
-        const float v = red[0][j][col] + red[1][j][col];
+        const float v = red[0][j][col % EPC * 16 + col / EPC] + red[1][j][col % EPC * 16 + col / EPC];
         float *cell = out + (o.transposed ? (int64_t)(c0 + col) * p.r + j0 + j : (int64_t)(j0 + j) * o.d + c0 + col);
         *cell = !whole ? v : (lo < hi ? s * v : 0.0f) + (p.accumulate ? *cell : 0.0f);  // no rows: 0, whatever s is
     }
