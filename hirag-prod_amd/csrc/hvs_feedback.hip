@@ -85,6 +85,7 @@ __global__ __launch_bounds__(64 * WAVES) void preference_kernel(PreferenceParams
     constexpr int TEAMS = WAVES / TW, SPAN = CH * TW * 512;  // SPAN: dim rounded up to what a team covers
     extern __shared__ __attribute__((aligned(16))) float smem[];  // TW 1: [2][SPAN] the queries, then [TEAMS][SPAN]; else [dim]
     __shared__ float sums[WAVES][2];
+    __shared__ double sums_query[TW > 1 ? WAVES : 1][2];
     __shared__ float num[TEAMS];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int team = wave / TW, tl = (wave % TW) * 64 + lane;
@@ -126,12 +127,15 @@ __global__ __launch_bounds__(64 * WAVES) void preference_kernel(PreferenceParams
     };
     fetch(a, b);
 
-    // y^ and y^ - y0^ (without a reference: y^), which the sums over a pair are taken with
+    // y^ and y^ - y0^ (without a reference: y^), which the sums over a pair are taken with.  After a few steps of training y is close
+    // to y0: an error of 2^-24 in either norm, or in the smaller product, would be many steps of the difference.  So the norms are
+    // held in double precision, their inverses as two floats, and the product y0 / |y0| keeps what its rounding cuts off
+    // (difference 1e-2 of the queries, 16 pairs: margins off by 1e-7 instead of 5e-6 of their size).
     float y_own[TW > 1 ? CH * 8 : 1], d_own[TW > 1 ? CH * 8 : 1], g[CH * 8];
-    float inv_y, inv_f;
+    float inv_y;
     {
         Raw8<QDT> ry[CH], rf[CH];
-        float yy = 0.0f, ff = 0.0f;
+        double yy = 0.0, ff = 0.0;
 #pragma unroll
         for (int c = 0; c < CH; c++) {
             const int k = (c * TW * 64 + tl) * 8;
@@ -139,19 +143,32 @@ __global__ __launch_bounds__(64 * WAVES) void preference_kernel(PreferenceParams
             load8<QDT, ALIGNED>(p.y, q, p.ld_y, k, p.dim, ry[c]);
             raw8_to_float<QDT>(ry[c], v);
 #pragma unroll
-            for (int e = 0; e < 8; e++) yy = fmaf(v[e], v[e], yy);
+            for (int e = 0; e < 8; e++) yy = fma((double)v[e], (double)v[e], yy);
             if (p.ref) {
                 load8<QDT, ALIGNED>(p.ref, q, p.ld_ref, k, p.dim, rf[c]);
                 raw8_to_float<QDT>(rf[c], v);
 #pragma unroll
-                for (int e = 0; e < 8; e++) ff = fmaf(v[e], v[e], ff);
+                for (int e = 0; e < 8; e++) ff = fma((double)v[e], (double)v[e], ff);
             }
 #pragma unroll
             for (int e = 0; e < 8; e++) g[c * 8 + e] = 0.0f;
         }
-        team_sum(yy, ff);
-        inv_y = inverse_norm(yy);
-        inv_f = inverse_norm(ff);
+#pragma unroll
+        for (int o = 32; o >= 1; o >>= 1) {
+            yy += __shfl_xor(yy, o);
+            ff += __shfl_xor(ff, o);
+        }
+        if (TW > 1) {
+            if (lane == 0) sums_query[wave][0] = yy, sums_query[wave][1] = ff;
+            __syncthreads();
+            yy = ff = 0.0;
+#pragma unroll
+            for (int w = 0; w < TW; w++) yy += sums_query[team * TW + w][0], ff += sums_query[team * TW + w][1];
+        }
+        yy = yy < 1e-76 ? 0.0 : 1.0 / sqrt(yy);  // below 1e-38 the inverse is no fp32 number: such a norm counts as 0
+        ff = ff < 1e-76 ? 0.0 : 1.0 / sqrt(ff);
+        inv_y = (float)yy;
+        const float inv_f = (float)ff, rest_y = (float)(yy - (double)inv_y), rest_f = (float)(ff - (double)inv_f);
 #pragma unroll
         for (int c = 0; c < CH; c++) {
             const int k = (c * TW * 64 + tl) * 8;
@@ -160,7 +177,10 @@ __global__ __launch_bounds__(64 * WAVES) void preference_kernel(PreferenceParams
             if (p.ref) raw8_to_float<QDT>(rf[c], dv);
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                dv[e] = p.ref ? fmaf(yv[e], inv_y, -(dv[e] * inv_f)) : yv[e] * inv_y;
+                if (p.ref) {
+                    const float f = dv[e] * inv_f, cut = fmaf(dv[e], inv_f, -f);
+                    dv[e] = fmaf(yv[e], inv_y, -f) + (fmaf(yv[e], rest_y, -cut) - dv[e] * rest_f);
+                } else dv[e] = yv[e] * inv_y;
                 yv[e] *= inv_y;
                 if (TW > 1) y_own[c * 8 + e] = yv[e], d_own[c * 8 + e] = dv[e];
             }

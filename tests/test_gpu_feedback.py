@@ -537,3 +537,37 @@ def test_clip_graph_of_one_launch(env):
         graph.replay()
         torch.cuda.synchronize()
         check_clip(env, [g], 1.0, False, norm, [out])
+
+
+@pytest.mark.parametrize("qdt", ["f32", "f16"])
+@pytest.mark.parametrize("dim,counts", [(1536, [16]), (1536, [3] * 300), (768, [100, 2, 90]), (4000, [5] * 9)])
+def test_margins_close_to_the_reference(env, qdt, dim, counts):
+    """Queries that have hardly moved, near their chosen rows: the margin's error is a share of the move, not of the cosines."""
+    torch = env.torch
+    q, _, rows, c, r, off = make(env, qdt, "f16", len(counts), dim, 90, counts, seed=dim + len(counts))
+    first = c[off[:-1].clamp(max=len(c) - 1)]
+    base = (rows[first].float() + 0.3 * q.float()) * 3.7
+    ref = base.to(q.dtype)
+    q = (base * 1.3 + 1e-2 * torch.randn(base.shape, device=env.dev)).to(q.dtype)
+    _, margin, _ = env.hvs.preference_loss(q, rows, c, r, off, reference=ref, beta=10.0)
+    _, want, _, _ = lo.preference(np64(q), np64(rows), c.cpu().numpy(), r.cpu().numpy(), off.cpu().numpy(), np64(ref), 10.0, 0.0)
+    # margin = (y^ - y0^) . (c^ - r^): the first factor is right to a few roundings of its own size (and to 2^-45 of the unit
+    # vectors), the second to those of the unit rows
+    moved = np.linalg.norm(lo.unit(np64(q))[0] - lo.unit(np64(ref))[0], axis=1)
+    assert moved.max() < 0.02
+    cos_tol = lo.sum_error(1.0, dim) + 8 * 2.0**-24 + 2 * lo.sum_error(1.0, dim)
+    check(margin, want, np.repeat(moved, counts) * 4 * cos_tol + 2.0**-45 * dim**0.5, "margin")
+
+
+def test_norms_at_the_ends_of_the_range(env):
+    """Queries of norm 1e30 and 1e-30 are what their unit vectors are; below 1e-38 a norm counts as 0."""
+    torch = env.torch
+    q, ref, rows, c, r, off = make(env, "f32", "f16", 12, 64, 30, [4] * 12, seed=2)
+    want = env.hvs.preference_loss(q, rows, c, r, off, reference=ref, beta=10.0)
+    for size in (2.0**100, 2.0**-100):
+        got = env.hvs.preference_loss(q * size, rows, c, r, off, reference=ref * size, beta=10.0)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        assert bool((got[2].double() * size - want[2].double()).abs().max() <= 2.0**-126 * size + 2.0**-22 * want[2].abs().max())
+    none = env.hvs.preference_loss(q * 2.0**-140, rows, c, r, off, reference=ref, beta=10.0)
+    zero = env.hvs.preference_loss(q * 0.0, rows, c, r, off, reference=ref, beta=10.0)
+    assert all(torch.equal(a, b) and bool(a.isfinite().all()) for a, b in zip(none, zero)) and not none[2].any()
