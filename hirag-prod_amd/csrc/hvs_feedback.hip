@@ -85,7 +85,8 @@ __global__ __launch_bounds__(64 * WAVES) void preference_kernel(PreferenceParams
     constexpr int TEAMS = WAVES / TW, SPAN = CH * TW * 512;  // SPAN: dim rounded up to what a team covers
     extern __shared__ __attribute__((aligned(16))) float smem[];  // TW 1: [2][SPAN] the queries, then [TEAMS][SPAN]; else [dim]
     __shared__ float sums[WAVES][2];
-    __shared__ double sums_query[TW > 1 ? WAVES : 1][2];
+    __shared__ double sums_query[WAVES][2];
+    static_assert(TW == 1 ? CH <= WAVES : TW == WAVES, "a piece of the query for every wave, or one team");
     __shared__ float num[TEAMS];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int team = wave / TW, tl = (wave % TW) * 64 + lane;
@@ -133,46 +134,49 @@ __global__ __launch_bounds__(64 * WAVES) void preference_kernel(PreferenceParams
     // (difference 1e-2 of the queries, 16 pairs: margins off by 1e-7 instead of 5e-6 of their size).
     float y_own[TW > 1 ? CH * 8 : 1], d_own[TW > 1 ? CH * 8 : 1], g[CH * 8];
     float inv_y;
+#pragma unroll
+    for (int k = 0; k < CH * 8; k++) g[k] = 0.0f;
     {
-        Raw8<QDT> ry[CH], rf[CH];
+        // teams of one wave share the work: wave c takes piece c (there are at least as many waves)
+        constexpr int PIECES = TW > 1 ? CH : 1;
+        const bool has = TW > 1 || team < CH;
+        Raw8<QDT> ry[PIECES], rf[PIECES];
         double yy = 0.0, ff = 0.0;
 #pragma unroll
-        for (int c = 0; c < CH; c++) {
-            const int k = (c * TW * 64 + tl) * 8;
+        for (int c = 0; c < PIECES; c++) {
+            const int k = ((TW > 1 ? c : team) * TW * 64 + tl) * 8;
             float v[8];
+            if (!has) continue;
             load8<QDT, ALIGNED>(p.y, q, p.ld_y, k, p.dim, ry[c]);
+            if (p.ref) load8<QDT, ALIGNED>(p.ref, q, p.ld_ref, k, p.dim, rf[c]);
             raw8_to_float<QDT>(ry[c], v);
 #pragma unroll
             for (int e = 0; e < 8; e++) yy = fma((double)v[e], (double)v[e], yy);
-            if (p.ref) {
-                load8<QDT, ALIGNED>(p.ref, q, p.ld_ref, k, p.dim, rf[c]);
-                raw8_to_float<QDT>(rf[c], v);
+            if (!p.ref) continue;
+            raw8_to_float<QDT>(rf[c], v);
 #pragma unroll
-                for (int e = 0; e < 8; e++) ff = fma((double)v[e], (double)v[e], ff);
+            for (int e = 0; e < 8; e++) ff = fma((double)v[e], (double)v[e], ff);
+        }
+        if (has) {
+#pragma unroll
+            for (int o = 32; o >= 1; o >>= 1) {
+                yy += __shfl_xor(yy, o);
+                ff += __shfl_xor(ff, o);
             }
-#pragma unroll
-            for (int e = 0; e < 8; e++) g[c * 8 + e] = 0.0f;
-        }
-#pragma unroll
-        for (int o = 32; o >= 1; o >>= 1) {
-            yy += __shfl_xor(yy, o);
-            ff += __shfl_xor(ff, o);
-        }
-        if (TW > 1) {
             if (lane == 0) sums_query[wave][0] = yy, sums_query[wave][1] = ff;
-            __syncthreads();
-            yy = ff = 0.0;
-#pragma unroll
-            for (int w = 0; w < TW; w++) yy += sums_query[team * TW + w][0], ff += sums_query[team * TW + w][1];
         }
+        __syncthreads();
+        yy = ff = 0.0;
+#pragma unroll
+        for (int w = 0; w < (TW > 1 ? WAVES : CH); w++) yy += sums_query[w][0], ff += sums_query[w][1];
         yy = yy < 1e-76 ? 0.0 : 1.0 / sqrt(yy);  // below 1e-38 the inverse is no fp32 number: such a norm counts as 0
         ff = ff < 1e-76 ? 0.0 : 1.0 / sqrt(ff);
         inv_y = (float)yy;
         const float inv_f = (float)ff, rest_y = (float)(yy - (double)inv_y), rest_f = (float)(ff - (double)inv_f);
 #pragma unroll
-        for (int c = 0; c < CH; c++) {
-            const int k = (c * TW * 64 + tl) * 8;
+        for (int c = 0; c < PIECES; c++) {
             float yv[8], dv[8];
+            if (!has) continue;
             raw8_to_float<QDT>(ry[c], yv);
             if (p.ref) raw8_to_float<QDT>(rf[c], dv);
 #pragma unroll
@@ -184,7 +188,8 @@ __global__ __launch_bounds__(64 * WAVES) void preference_kernel(PreferenceParams
                 yv[e] *= inv_y;
                 if (TW > 1) y_own[c * 8 + e] = yv[e], d_own[c * 8 + e] = dv[e];
             }
-            if (TW == 1 && team == c % TEAMS) {  // every wave has all of both: one of them puts each piece down
+            if (TW == 1) {
+                const int k = (team * 64 + tl) * 8;
                 f32x4 *yl = reinterpret_cast<f32x4 *>(smem + k), *dl = reinterpret_cast<f32x4 *>(smem + SPAN + k);
                 yl[0] = f32x4{yv[0], yv[1], yv[2], yv[3]}, yl[1] = f32x4{yv[4], yv[5], yv[6], yv[7]};
                 dl[0] = f32x4{dv[0], dv[1], dv[2], dv[3]}, dl[1] = f32x4{dv[4], dv[5], dv[6], dv[7]};
