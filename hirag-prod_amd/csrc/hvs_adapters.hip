@@ -3,8 +3,8 @@
 //     y_i = W x_i + s_c B_c (A_c x_i),  c = code of row i            (forward)
 //     v_i = s_c B_c^T g_i,  dx_i = W^T g_i + A_c^T v_i,  dA_c = sum v_i x_i^T,  dB_c = s_c sum g_i u_i^T   (backward)
 //
-// Two routes.  Few rows (few_rows): every 16-column slice of W is read once by its own block, bound by the latency of
-// reading W; rows stay in arrival order.  Many rows: rows are ordered by code (a stable counting sort), so that a tile of
+// Two routes.  Few rows (few_rows): blocks of 16 x 16 to 32 x 32 outputs, rows in arrival order; bound by the latency of
+// reading W, from some hundred rows on by the L2 (about 6 TB/s into 32 x 32 blocks).  Many rows: rows are ordered by code (a stable counting sort), so that a tile of
 // rows meets few adapters; W x comes from the matrix-pipe loop the searches use, the low-rank term is added in its
 // accumulators, and y is rounded and written once.
 //
@@ -14,14 +14,18 @@
 // multiplied by that power and by s_c as it is added to W x.
 #include "hvs_learn.h"
 
-#define ONCE_ROWS 2  // rows up to which one launch does all
+// rows up to which one launch does all.  One launch / two, rows of as many tenants, 1536 x 1536, rank 16, us: fp32 1 row 8.3 / 12.3,
+// 2 rows 11.7 / 13.5, 4 rows 18.8 / 13.5; bf16 4.5 / 7.9, 6.1 / 7.9, 9.4 / 7.9
+#define ONCE_ROWS 2
 // rows up to which blocks of few outputs take the rows in arrival order; a whole call with 1536 x 1536 weights, this route
 // against the grouped tiles: fp32 1024 rows 99 / 112 us, 1536 rows 145 / 112; bf16 512 rows 24 / 36 us, 777 rows 34 / 34
 #define FEW_ROWS_F32 1024
 #define FEW_ROWS_16 768
 #define GROUP_CHUNK 1024  // rows per block of the grouping kernels
 #define MAX_CHUNK_ROWS 65536
-#define SHRINK_WIDE_ROWS 16384  // rows from which u = A x is taken 32 rows a wave instead of 16 a block
+// rows from which u = A x is taken 32 rows a wave instead of 16 a block.  A call with 64-column outputs, wide / narrow, us: 8192 rows of
+// 16 adapters 25.7 / 21.9, 16 384 29.0 / 28.6, 32 768 33.3 / 38.3, 65 536 42.3 / 58.5; 256 adapters 32.6 / 24.8, 40.4 / 41.0, 43.7 / 51.5, 53.8 / 72.5
+#define SHRINK_WIDE_ROWS 16384
 #define SHRINK_WAVES 8
 #define SHRINK_SHARES 4  // blocks that share the adapters among 16 rows in code order (1, 2, 4, 8: 11.2, 9.5, 8.9, 9.6 us, mean of three sizes)
 #define OUTER_ROWS 512       // rows whose numbers a block of the stack gradients holds at a time
@@ -65,7 +69,7 @@ __global__ __launch_bounds__(GROUP_CHUNK) void group_count_kernel(const int32_t 
 // FEW_BINS: the waves' counts per bin lie side by side in LDS and one barrier ranks the rows of the block; with more bins the
 // 16 waves take turns.  Inside a wave lanes of one bin find each other with one ballot per bit of the bin.
 #define GROUP_SELF 16
-#define GROUP_FEW_BINS 512
+#define GROUP_FEW_BINS 512  // (16 adapters with / without the waves' counts side by side: 2048 rows 16.5 / 17.3 us a call, 65 536 42.4 / 53.1)
 struct GroupParams {
     const int32_t *codes;
     int n, S, bits, chunks;  // bits: of a bin's number
@@ -225,8 +229,6 @@ struct ShrinkParams {
     const float *scale;
 };
 
-// One block per 16 rows (and per share blockIdx.y of the adapters among them): D[rank][row] on 16x16 matrix tiles, the
-// block's waves split K and add up through LDS.  Loads go straight to registers (a lane's 16 bytes are a fragment).
 // what the sums u of one row, spread over the lanes that hold them, become: the caller's fp32 copy, and the two 16-bit parts
 // (fp32 weights: u itself) with the factor of their product.  `largest` = max |u| of the row; 4 ranks j .. j + 3 per call
 template <int DT> __device__ __forceinline__ void shrink_store(const ShrinkParams &p, int64_t at, int j, const float *u, float largest, int32_t c) {
@@ -255,6 +257,9 @@ template <int DT> __device__ __forceinline__ void shrink_store(const ShrinkParam
     if (j == 0) p.factor[at] = known ? (DT == HVS_F32 ? p.scale[c] : ldexpf(p.scale[c], e2)) : 0.0f;
 }
 
+// One block per 16 rows (and per share blockIdx.y of the adapters among them): D[rank][row] on 16x16 matrix tiles, the
+// block's waves split K and add up through LDS.  4096 rows of 1536 bf16, 256 adapters: 10 us for 25 MB, bound by the latency of
+// two rounds of loads; the other round's loads ahead, or both at once, cost registers and were slower (11.4 us).
 template <int DT, int RT, bool ALIGNED>
 __global__ __launch_bounds__(64 * SHRINK_WAVES) void shrink_kernel(ShrinkParams p) {
     typedef typename Elem<DT>::type E;
@@ -1243,9 +1248,14 @@ template <int DT> static int launch_few(hipStream_t st, const ProjectParams &p) 
         if (al) project_few_kernel<DT, MT_, NT_, WAVES_, true><<<grid, 64 * WAVES_, 0, st>>>(p);                                  \
         else project_few_kernel<DT, MT_, NT_, WAVES_, false><<<grid, 64 * WAVES_, 0, st>>>(p);                                    \
     } while (0)
-    if (p.n <= 16) FEW(1, 1, 16);
-    else if (p.n <= 32) FEW(1, 2, 16);
-    else if (p.n <= 64) FEW(1, 4, 16);
+    // The smallest blocks while every CU has at most one (fp32, whose products take longer than their loads: two), then twice the rows,
+    // then 32 x 32, which read half as much.  A call with 1536 x 1536 weights, rank 16, blocks of 16 x 16 / 16 x 32 / 32 x 32, us: bf16
+    // 32 rows 8.9 / 9.9 / 11.3, 64 rows 12.2 / 9.9 / 11.5, 128 rows 15.1 / 13.9 / 11.9; fp32 32 rows 12.5 / 16.1 / 20.2, 64 rows 16.5 / 16.9 / 20.2,
+    // 128 rows 23.1 / 26.5 / 22.7, 512 rows 67 / 63 / 49
+    auto blocks = [&](int rows) { return (int64_t)((p.N + 15) / 16) * ((p.n + rows - 1) / rows); };
+    if (blocks(16) <= (DT == HVS_F32 ? 512 : 256)) FEW(1, 1, 16);
+    else if constexpr (DT == HVS_F32) FEW(2, 2, 8);
+    else if (blocks(32) <= 256) FEW(1, 2, 16);
     else FEW(2, 2, 8);
 #undef FEW
     HVS_HIP(hipGetLastError());
