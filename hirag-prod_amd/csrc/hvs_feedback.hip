@@ -345,7 +345,9 @@ template <int QDT> __global__ __launch_bounds__(64 * JOIN_WAVES) void preference
     reinterpret_cast<Q *>(p.grad)[q * p.ld_grad + k] = learn_from_float<Q>(inv_y * (v - sum * (inv_y * y)));
 }
 
-#define PREF_WAVE_DIM 2048  // columns up to which a wave takes a pair by itself
+// Columns up to which a wave takes a pair by itself; beyond, 4 waves take it together (past 8192 columns 8).  2000 queries x 8 pairs of fp16:
+// 2048 columns 40 us; 2560, 4096, 8192, 16 384 columns 65, 74, 165, 367 us (with 16 waves on a pair 199, 207, 250, 631)
+#define PREF_WAVE_DIM 2048
 
 // How the pairs are spread over the chip, by counts alone (the host does not see the offsets); 1536 columns, fp16 rows.
 struct PreferencePlan {
@@ -353,17 +355,20 @@ struct PreferencePlan {
     int per_block;  // pairs a block takes before another one joins in
     bool wide;      // 16 waves a block instead of 4
 };
-static PreferencePlan preference_plan(const hvs_preference *p) {
+static PreferencePlan preference_plan(const hvs_preference *p, int dim) {
     const int64_t nq = p->n_queries, pairs = p->n_pairs;
+    const bool one = dim > PREF_WAVE_DIM;  // the waves of a block take one pair together
     // queries enough for the chip: a block each
     if (nq < 1 || nq > 512) return {1, INT_MAX, false};
     // Few pairs each: a block each saves the join, which reads a vector per block (a block each / shared: 16 x 16 10.6 / 9.9 us,
     // 64 x 64 22.9 / 15.0; 100 x 16 10.5 / 13.0, 100 x 64 23.3 / 22.1, 400 x 32 27.5 / 36).  16 waves where there is a CU for each
     // block and more than one pair for a wave (4 waves / 16: 100 x 4 7.1 / 7.3, 250 x 8 9.1 / 8.7, 250 x 16 13.2 / 11.2, 400 x 16 17.4 / 22.8).
-    if (pairs <= (nq <= 64 ? 16 : 64) * nq) return {1, INT_MAX, nq <= 256 && pairs > 4 * nq};
-    // more: blocks of a pair for each of 4 waves, until they are 512; then more pairs each
+    // With a pair at a time (4096 columns, alone / shared): 1 x 4 12.7 / 9.5, 16 x 16 31 / 11; 100 x 4 13.3 / 20.7, 100 x 16 34 / 27; 400 x 8 28.5 / 61.
+    const int64_t alone = one ? (nq <= 64 ? 2 : nq <= 128 ? 8 : 64) : (nq <= 64 ? 16 : 64);
+    if (pairs <= alone * nq) return {1, INT_MAX, nq <= 256 && pairs > 4 * nq};
+    // more: blocks of a pair at a time, or one for each of 4 waves, until they are 512; then more pairs each
     // (4, 8, 16, 32 pairs a block: 1 x 64 10.9, 12.2, 15.8, 22.6 us; 64 x 64 16.9, 15.0, 16.5, 23.2)
-    const int64_t even = (pairs + 511) / 512, per = even < 4 ? 4 : (even + 3) / 4 * 4, most = 1024 / nq, shares = (pairs + per - 1) / per;
+    const int64_t even = (pairs + 511) / 512, per = one ? even : even < 4 ? 4 : (even + 3) / 4 * 4, most = 1024 / nq, shares = (pairs + per - 1) / per;
     return {(int)(shares < most ? shares : most), (int)(per < INT_MAX ? per : INT_MAX), false};
 }
 
@@ -381,7 +386,7 @@ static int check_preference(const char *who, const hvs_preference *p, int dim) {
 extern "C" int hvs_preference_workspace(const hvs_preference *p, int dim, uint64_t *out_bytes) {
     HVS_TRY(check_preference("hvs_preference_workspace", p, dim));
     HVS_REQUIRE(out_bytes != nullptr, "hvs_preference_workspace: NULL argument");
-    const int shares = preference_plan(p).shares;
+    const int shares = preference_plan(p, dim).shares;
     WorkspaceCut w(nullptr);
     if (shares > 1) {
         w.take<float>((uint64_t)p->n_queries * shares * dim * 4);
@@ -411,8 +416,9 @@ template <int QDT, int RDT> static int run_preference(hipStream_t st, const Pref
     const int qs = hvs_elem_size(QDT), rs = hvs_elem_size(RDT);
     const bool al = p.dim % 8 == 0 && learn_aligned(p.y, p.ld_y * qs, 0) && (!p.ref || learn_aligned(p.ref, p.ld_ref * qs, 0)) &&
                     learn_aligned(p.rows, p.ld_rows * rs, 0);
-    if (p.dim > 8192) HVS_TRY((launch_preference<QDT, RDT, 2, 16, 16>(st, p, nq, shares, al)));
-    else if (p.dim > PREF_WAVE_DIM) HVS_TRY((launch_preference<QDT, RDT, 1, 16, 16>(st, p, nq, shares, al)));
+    if (p.dim > 8192) HVS_TRY((launch_preference<QDT, RDT, 4, 8, 8>(st, p, nq, shares, al)));
+    else if (p.dim > 4096) HVS_TRY((launch_preference<QDT, RDT, 4, 4, 4>(st, p, nq, shares, al)));
+    else if (p.dim > PREF_WAVE_DIM) HVS_TRY((launch_preference<QDT, RDT, 2, 4, 4>(st, p, nq, shares, al)));
     else {
         const int ch = (p.dim + 511) / 512;
 #define PREF(CH_) (wide ? launch_preference<QDT, RDT, CH_, 1, 16>(st, p, nq, shares, al) : launch_preference<QDT, RDT, CH_, 1, 4>(st, p, nq, shares, al))
@@ -454,7 +460,7 @@ static int check_preference_buffers(const char *who, const hvs_preference *p, co
 }
 
 static int preference_core(hipStream_t st, const hvs_preference *p, const void *rows, int rows_dtype, int dim, int64_t ld_rows, int64_t n_rows, void *workspace) {
-    const PreferencePlan plan = preference_plan(p);
+    const PreferencePlan plan = preference_plan(p, dim);
     const int shares = plan.shares;
     PreferenceParams k = {};
     k.y = p->queries, k.ref = p->reference, k.ld_y = p->ld_queries, k.ld_ref = p->ld_reference;
@@ -533,7 +539,7 @@ extern "C" int hvs_index_preference_loss(hvs_index *idx, void *stream, const hvs
 // ---------------------------------------------------------------------------------------------------------------
 #define CLIP_BATCH 64      // tensors per launch: their table travels in the kernel's arguments
 #define CLIP_CHUNK 8192    // most elements a block takes at a time,
-#define CLIP_CHUNK_MIN 1024  // ... and fewest: small sets are spread over as many blocks as that gives
+#define CLIP_CHUNK_MIN 1024  // ... and fewest: small sets are spread over as many blocks as that gives (1024 / 8192 alone: 100 000 elements 6.0 / 8.0 us)
 // Up to so many elements in so few tensors one block does it all.  One launch / two, 2 tensors of 24 576 fp32 elements: 9.2 / 6.1 us
 // on the GPU (16 000 elements in all: 5.7 / 6.1), 12.0 / 15.4 us on the host, which is what an eager call waits for; 30 tensors
 // one after the other would take 33 us.

@@ -571,3 +571,13 @@ def test_norms_at_the_ends_of_the_range(env):
     none = env.hvs.preference_loss(q * 2.0**-140, rows, c, r, off, reference=ref, beta=10.0)
     zero = env.hvs.preference_loss(q * 0.0, rows, c, r, off, reference=ref, beta=10.0)
     assert all(torch.equal(a, b) and bool(a.isfinite().all()) for a, b in zip(none, zero)) and not none[2].any()
+
+
+@pytest.mark.parametrize("qdt,rdt", [("f32", "bf16"), ("f16", "f32")])
+@pytest.mark.parametrize("dim", [2056, 4096, 4104, 8200, 12001])
+@pytest.mark.parametrize("counts", [[9], [3] * 70, [40] + [1] * 69, [9] * 100, [2] * 300])
+def test_wide_rows(env, qdt, rdt, dim, counts):
+    """Rows that several waves take together, one block a query and shared."""
+    q, ref, rows, c, r, off = make(env, qdt, rdt, len(counts), dim, 30, counts, seed=dim + len(counts))
+    got = env.hvs.preference_loss(q, rows, c, r, off, reference=ref, beta=10.0)
+    check_preference(q, ref, rows, c, r, off, got, qdt, 10.0, 0.0)
