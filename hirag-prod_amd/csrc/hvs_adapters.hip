@@ -1001,15 +1001,16 @@ struct OuterParams {
     int r, S, accumulate;
 };
 
-// A block takes one piece of an adapter's rows and 16 chunks of columns; fp32 matrix products (16x16x4: lane = (rank or column
+// A block takes one piece of an adapter's rows, 16 ranks and 16 chunks of columns (more ranks a block read X less often and held fewer
+// blocks a CU: 4096 rows, rank 128, 64 ranks a block / 16: bf16 223 / 148 us a call, fp32 209 / 198); fp32 matrix products (16x16x4: lane = (rank or column
 // chunk, row), so q needs no rounding and X no transposition).  An adapter of one piece is written out, zeros where it has no
 // rows; one of several leaves its sums in `partial`, and outer_join_kernel adds them in order.  A block per adapter and
 // piece keeps the blocks alike whether there are few adapters or hundreds (96 rows, 256 adapters: cutting the rows alone, so
 // that a block met many adapters one after the other, took twice as long).
-template <int DT, int RT, bool ALIGNED> __global__ __launch_bounds__(256, RT == 1 ? 5 : 1) void outer_kernel(OuterParams p) {
+template <int DT, bool ALIGNED> __global__ __launch_bounds__(256, 5) void outer_kernel(OuterParams p) {
     typedef typename Elem<DT>::type E;
     constexpr int EPC = Elem<DT>::EPC, CC = 16 * EPC, COPIES = 2;
-    __shared__ float red[COPIES][RT * 16][CC + 4];  // column m EPC + e of a row lies at 16 e + m: the 64 lanes of a sum hit 64 banks
+    __shared__ float red[COPIES][16][CC + 4];  // column m EPC + e of a row lies at 16 e + m: the 64 lanes of a sum hit 64 banks
     __shared__ uint32_t rows[OUTER_ROWS];
     const Piece piece = p.pieces.piece[blockIdx.x];
     if (blockIdx.x >= *p.pieces.count) return;
@@ -1017,45 +1018,37 @@ template <int DT, int RT, bool ALIGNED> __global__ __launch_bounds__(256, RT == 
     const int m = lane & 15, g = lane >> 4;
     const bool second = (int)blockIdx.y >= p.problem[0].cols;
     const OuterProblem &o = p.problem[second ? 1 : 0];
-    const int c0 = ((int)blockIdx.y - (second ? p.problem[0].cols : 0)) * CC, j0 = blockIdx.z * (RT * 16);
+    const int c0 = ((int)blockIdx.y - (second ? p.problem[0].cols : 0)) * CC, j0 = blockIdx.z * 16;
     const int32_t c = piece.adapter;
     const int lo = (int)piece.begin, hi = (int)piece.end;
     const bool whole = piece.slot < 0;
     if (lo >= hi && p.accumulate) return;
     const float s = p.scale[c];
-    f32x4 acc[RT][EPC];
+    f32x4 acc[EPC];
 #pragma unroll
-    for (int t = 0; t < RT; t++)
-#pragma unroll
-        for (int e = 0; e < EPC; e++) acc[t][e] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int e = 0; e < EPC; e++) acc[e] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     for (int base = lo; base < hi; base += OUTER_ROWS) {
         const int end = base + OUTER_ROWS < hi ? base + OUTER_ROWS : hi;
         for (int i = base + tid; i < end; i += 256) rows[i - base] = p.order[i];
         __syncthreads();
-        constexpr int UNROLL = RT <= 2 ? 4 : 2;
+        constexpr int UNROLL = 4;
         for (int b = base + 4 * wave; b < end; b += 16 * UNROLL) {
             f32x4 fx[UNROLL];
-            float fq[UNROLL][RT];
+            float fq[UNROLL];
 #pragma unroll
             for (int u = 0; u < UNROLL; u++) {
                 const int at = b + 16 * u + g;
                 const bool ok = at < end;
                 const int64_t row = rows[ok ? at - base : 0];
                 fx[u] = load_chunk<DT, ALIGNED>(reinterpret_cast<const E *>(o.x) + row * o.ld_x, c0 + m * EPC, ok ? o.d : 0);
-#pragma unroll
-                for (int t = 0; t < RT; t++) {
-                    const int j = j0 + t * 16 + m;
-                    fq[u][t] = ok && j < p.r ? o.q[row * p.r + j] : 0.0f;
-                }
+                fq[u] = ok && j0 + m < p.r ? o.q[row * p.r + j0 + m] : 0.0f;
             }
 #pragma unroll
             for (int u = 0; u < UNROLL; u++) {
                 float v[EPC];
                 chunk_to_float<DT>(fx[u], v);
 #pragma unroll
-                for (int t = 0; t < RT; t++)
-#pragma unroll
-                    for (int e = 0; e < EPC; e++) acc[t][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(fq[u][t], v[e], acc[t][e], 0, 0, 0);
+                for (int e = 0; e < EPC; e++) acc[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(fq[u], v[e], acc[e], 0, 0, 0);
             }
         }
         __syncthreads();
@@ -1063,14 +1056,12 @@ template <int DT, int RT, bool ALIGNED> __global__ __launch_bounds__(256, RT == 
     // the four waves' sums, in a fixed order: the upper two put theirs down, the lower two add to them
     auto put = [&](int copy, bool add) {
 #pragma unroll
-        for (int t = 0; t < RT; t++)
+        for (int e = 0; e < EPC; e++)
 #pragma unroll
-            for (int e = 0; e < EPC; e++)
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    float *cell = &red[copy][t * 16 + 4 * g + k][16 * e + m];
-                    *cell = add ? *cell + acc[t][e][k] : acc[t][e][k];
-                }
+            for (int k = 0; k < 4; k++) {
+                float *cell = &red[copy][4 * g + k][16 * e + m];
+                *cell = add ? *cell + acc[e][k] : acc[e][k];
+            }
     };
     if (wave >= 2) put(wave - 2, false);
     __syncthreads();
@@ -1078,9 +1069,9 @@ template <int DT, int RT, bool ALIGNED> __global__ __launch_bounds__(256, RT == 
     __syncthreads();
     const int64_t size = (int64_t)p.r * o.d;
     float *out = whole ? o.out + (int64_t)c * size : o.partial + (int64_t)piece.slot * size;
-    const int rn = p.r - j0 < RT * 16 ? p.r - j0 : RT * 16, cn = o.d - c0 < CC ? o.d - c0 : CC;
-    for (int k = tid; k < RT * 16 * CC; k += 256) {
-        const int j = o.transposed ? k % (RT * 16) : k / CC, col = o.transposed ? k / (RT * 16) : k % CC;
+    const int rn = p.r - j0 < 16 ? p.r - j0 : 16, cn = o.d - c0 < CC ? o.d - c0 : CC;
+    for (int k = tid; k < 16 * CC; k += 256) {
+        const int j = o.transposed ? k % 16 : k / CC, col = o.transposed ? k / 16 : k % CC;
         if (j >= rn || col >= cn) continue;
         const float v = red[0][j][col % EPC * 16 + col / EPC] + red[1][j][col % EPC * 16 + col / EPC];
         float *cell = out + (o.transposed ? (int64_t)(c0 + col) * p.r + j0 + j : (int64_t)(j0 + j) * o.d + c0 + col);
@@ -1452,23 +1443,16 @@ template <int DT> static int launch_outer(hipStream_t st, const OuterParams &p, 
     // (the table says how many pieces there are; the launch has room for the most there can be)
     const int64_t most = p.S + (n + p.pieces.rows - 1) / p.pieces.rows;
     const int cols = p.problem[0].cols + p.problem[1].cols;
-#define OUTER(RT_)                                                                                                           \
-    do {                                                                                                                     \
-        const dim3 grid((unsigned)most, cols, (p.r + 16 * RT_ - 1) / (16 * RT_));                                            \
-        if (al) outer_kernel<DT, RT_, true><<<grid, 256, 0, st>>>(p);                                                        \
-        else outer_kernel<DT, RT_, false><<<grid, 256, 0, st>>>(p);                                                          \
-    } while (0)
-    if (p.r <= 16) OUTER(1);
-    else if (p.r <= 32) OUTER(2);
-    else OUTER(4);
-#undef OUTER
+    const dim3 grid((unsigned)most, cols, (p.r + 15) / 16);
+    if (al) outer_kernel<DT, true><<<grid, 256, 0, st>>>(p);
+    else outer_kernel<DT, false><<<grid, 256, 0, st>>>(p);
     HVS_HIP(hipGetLastError());
     if (n <= p.pieces.rows) return 0;
     const int wide = p.problem[0].d > p.problem[1].d ? p.problem[0].d : p.problem[1].d;
     const int64_t by = (int64_t)p.r * wide / 1024;
-    const dim3 grid(p.S, (unsigned)(by < 1 ? 1 : (by > 64 ? 64 : by)), 2);
-    if (vec) outer_join_kernel<4><<<grid, 256, 0, st>>>(p);
-    else outer_join_kernel<1><<<grid, 256, 0, st>>>(p);
+    const dim3 join_grid(p.S, (unsigned)(by < 1 ? 1 : (by > 64 ? 64 : by)), 2);
+    if (vec) outer_join_kernel<4><<<join_grid, 256, 0, st>>>(p);
+    else outer_join_kernel<1><<<join_grid, 256, 0, st>>>(p);
     HVS_HIP(hipGetLastError());
     return 0;
 }
