@@ -17,10 +17,13 @@
 // rows up to which one launch does all.  One launch / two, rows of as many tenants, 1536 x 1536, rank 16, us: fp32 1 row 8.3 / 12.3,
 // 2 rows 11.7 / 13.5, 4 rows 18.8 / 13.5; bf16 4.5 / 7.9, 6.1 / 7.9, 9.4 / 7.9
 #define ONCE_ROWS 2
-// rows up to which blocks of few outputs take the rows in arrival order; a whole call with 1536 x 1536 weights, this route
-// against the grouped tiles: fp32 1024 rows 99 / 112 us, 1536 rows 145 / 112; bf16 512 rows 24 / 36 us, 777 rows 34 / 34
-#define FEW_ROWS_F32 1024
-#define FEW_ROWS_16 768
+// Rows, and outputs (rows times columns), up to which blocks of few outputs take the rows in arrival order.  That costs by outputs
+// times K, the grouped tiles by K alone until they fill the chip.  A call of 32 adapters of rank 16, this route / the tiles, us:
+// fp32 1536 x 1536 1024 rows (1.6 million outputs) 94 / 108; 4096 x 4096 400 rows (1.6) 222 / 265, 600 rows (2.5) 316 / 268, 1024 rows 515 / 271
+// bf16 1536 x 1536 600 rows (0.9) 25 / 29, 768 rows (1.2) 29 / 30; 4096 x 4096 256 rows (1.05) 43 / 56, 400 rows (1.6) 72 / 56, 768 rows 135 / 60
+#define FEW_ROWS 1024
+#define FEW_OUTPUTS_F32 1900000
+#define FEW_OUTPUTS_16 1100000
 #define GROUP_CHUNK 1024  // rows per block of the grouping kernels
 #define MAX_CHUNK_ROWS 65536
 // rows from which u = A x is taken 32 rows a wave instead of 16 a block.  A call with 64-column outputs, wide / narrow, us: 8192 rows of
@@ -1115,7 +1118,7 @@ static int check_adapters(const char *who, const hvs_adapters *ad) {
     return 0;
 }
 static bool once(int64_t n, int rank) { return n <= ONCE_ROWS && rank <= 64; }
-static int few_rows(int dtype) { return dtype == HVS_F32 ? FEW_ROWS_F32 : FEW_ROWS_16; }
+static bool few_rows(int dtype, int64_t n, int N) { return n <= FEW_ROWS && n * N <= (dtype == HVS_F32 ? FEW_OUTPUTS_F32 : FEW_OUTPUTS_16); }
 static int round_up(int v, int to) { return (v + to - 1) / to * to; }
 static int elems_per_chunk(int dtype) { return dtype == HVS_F32 ? 4 : 8; }
 
@@ -1151,6 +1154,7 @@ static uint64_t cut_workspace(const hvs_adapters *ad, int64_t nc, int backward, 
     const int es = hvs_elem_size(ad->dtype), epc = elems_per_chunk(ad->dtype), rp = round_up(ad->rank, 16);
     const int64_t chunks = (nc + GROUP_CHUNK - 1) / GROUP_CHUNK;
     const int wide = ad->d_in > ad->d_out ? ad->d_in : ad->d_out;
+    const bool few = few_rows(ad->dtype, nc, backward ? ad->d_in : ad->d_out);
     ws->hidden = w.take<float>(nc * ad->rank * 4);
     ws->order = w.take<uint32_t>(nc * 4);
     ws->scodes = w.take<int32_t>(nc * 4);
@@ -1159,8 +1163,8 @@ static uint64_t cut_workspace(const hvs_adapters *ad, int64_t nc, int backward, 
     ws->factor = w.take<float>(nc * 4);
     ws->u_hi = w.take<char>(nc * rp * es);
     ws->u_lo = w.take<char>(ad->dtype == HVS_F32 ? 0 : nc * rp * es);
-    ws->packed_w = w.take<char>(nc > few_rows(ad->dtype) ? (uint64_t)wide * round_up(wide, epc) * es : 0);
-    ws->packed_x = w.take<char>(nc > few_rows(ad->dtype) ? (uint64_t)nc * round_up(wide, epc) * es : 0);
+    ws->packed_w = w.take<char>(!few ? (uint64_t)wide * round_up(wide, epc) * es : 0);
+    ws->packed_x = w.take<char>(!few ? (uint64_t)nc * round_up(wide, epc) * es : 0);
     if (backward) {
         ws->w_t = w.take<char>((uint64_t)ad->d_in * round_up(ad->d_out, epc) * es);
         ws->b_t = w.take<char>((uint64_t)ad->n_adapters * ad->rank * round_up(ad->d_out, epc) * es);
@@ -1312,7 +1316,7 @@ struct Direction {
 template <int DT>
 static int run_direction(hipStream_t st, const hvs_adapters *ad, const Direction &d, const int32_t *codes, int n, float *hidden, AdapterWs &ws, bool grouped) {
     const int es = hvs_elem_size(DT), epc = Elem<DT>::EPC;
-    const bool few = n <= few_rows(DT);
+    const bool few = few_rows(DT, n, d.N);
     Direction dd = d;
     if (!few && d.out) {
         // the tile loads take whole 16-byte chunks: rows that do not offer them are brought to that pitch first

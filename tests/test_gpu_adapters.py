@@ -549,3 +549,14 @@ def test_columns_of_one_tensor(env, n):
     if n > 1:
         with pytest.raises(env.hvs.HvsError, match="overlaps"):
             ad.apply(wide[:n, :24], codes, out=wide.view(-1)[24 : 24 + n * 20].view(n, 20))
+
+
+@pytest.mark.parametrize("dtype,n,d_in,d_out", [("bf16", 300, 90, 3333), ("bf16", 301, 3400, 100), ("f16", 130, 72, 8200), ("f32", 600, 100, 3300), ("f32", 500, 4001, 130),
+                                                ("f16", 1024, 64, 900), ("f32", 1024, 64, 1800), ("bf16", 65, 40, 16384)])
+def test_routes_by_outputs(env, dtype, n, d_in, d_out):
+    """Row counts that one direction takes in arrival order and the other grouped."""
+    torch = env.torch
+    ad, x, codes, gen = make(env, dtype, n, d_in, d_out, 6, 4)
+    _, hidden = check_apply(env, ad, x, codes, dtype)
+    g = torch.randn(n, d_out, generator=gen).to(env.dev, x.dtype)
+    check_backward(ad, g, x, codes, hidden, dtype, *ad.backward(g, x, codes, hidden))
