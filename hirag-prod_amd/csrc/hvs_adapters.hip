@@ -250,7 +250,8 @@ template <int DT> __device__ __forceinline__ void shrink_store(const ShrinkParam
     vec hi, lo;
 #pragma unroll
     for (int e = 0; e < 4; e++) {
-        const float v = known ? (DT == HVS_F32 ? u[e] : ldexpf(u[e], -e2)) : 0.0f;
+        // ranks past r: A's rows there are zeros, but zeros times an infinite element of x are NaN
+        const float v = known && j + e < p.r ? (DT == HVS_F32 ? u[e] : ldexpf(u[e], -e2)) : 0.0f;
         hi[e] = learn_from_float<E>(v);
         const float rest = v - learn_to_float((E)hi[e]);
         lo[e] = learn_from_float<E>(largest < __builtin_inff() ? rest : 0.0f);  // inf - inf: the first part says it all
@@ -647,7 +648,7 @@ __global__ __launch_bounds__(1024) void project_once_kernel(ProjectParams p, flo
                 float s = 0.0f;
 #pragma unroll
                 for (int k = 0; k < WAVES; k++) s += part_u[k][row][j];
-                u_all[row][j] = s;
+                u_all[row][j] = j < p.r ? s : 0.0f;  // ranks past r: 0 times an infinite element of x is NaN
                 if (hidden && blockIdx.x == 0 && j < p.r) hidden[(int64_t)row * p.r + j] = s;
             }
         }

@@ -560,3 +560,29 @@ def test_routes_by_outputs(env, dtype, n, d_in, d_out):
     _, hidden = check_apply(env, ad, x, codes, dtype)
     g = torch.randn(n, d_out, generator=gen).to(env.dev, x.dtype)
     check_backward(ad, g, x, codes, hidden, dtype, *ad.backward(g, x, codes, hidden))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n", [1, 2, 30, 1100, 17000])
+@pytest.mark.parametrize("rank", [3, 16, 20])
+def test_infinite_rows_at_any_rank(env, dtype, n, rank):
+    """A row with an infinite element: with positive weights every sum is +inf and none is NaN, whatever the rank is a multiple of;
+    the other rows are what they are without it.  The same for a row of the gradient."""
+    torch = env.torch
+    t = getattr(torch, DT[dtype])
+    gen = torch.Generator().manual_seed(n + rank)
+    pos = lambda *s: (0.1 + torch.rand(*s, generator=gen)).to(env.dev, t)
+    ad = env.hvs.QueryAdapters(pos(40, 64), pos(2, rank, 64), pos(2, 40, rank), torch.ones(2, device=env.dev))
+    x, g = pos(n, 64), pos(n, 40)
+    codes = torch.arange(n, device=env.dev, dtype=torch.int32) % 2
+    y, hidden = ad.apply(x, codes, return_hidden=True)
+    dx, _, _ = ad.backward(g, x, codes, hidden)
+    bad = n // 2
+    x2, g2 = x.clone(), g.clone()
+    x2[bad, 5], g2[bad, 7] = torch.inf, torch.inf
+    y2, hidden2 = ad.apply(x2, codes, return_hidden=True)
+    dx2, _, _ = ad.backward(g2, x, codes, hidden)
+    others = torch.arange(n, device=env.dev) != bad
+    for got, clean in ((y2, y), (hidden2, hidden), (dx2, dx)):
+        assert bool((got[bad] == torch.inf).all())
+        assert torch.equal(got[others], clean[others])
