@@ -260,3 +260,31 @@ def test_lists_off_their_elements_and_wide_pitches_are_refused():
     for name, off in (("offsets", 4), ("chosen", 4), ("rejected", 1), ("weights", 2), ("loss", 2), ("margin", 1)):
         p = HvsPreferenceStruct(**{**ok, name: ok[name] + off})
         refused(lib.hvs_preference_loss(0, None, ctypes.byref(p), R, 1, 16, 16, 50, W, 1 << 30), "aligned")
+
+
+def preference_case(dim, counts, seed, n_rows=50):
+    rng = np.random.default_rng(seed)
+    rows = rng.standard_normal((n_rows, dim)).astype(np.float16).astype(np.float64)
+    q = rng.standard_normal((len(counts), dim)).astype(np.float32).astype(np.float64)
+    ref = (q + 0.2 * rng.standard_normal(q.shape)).astype(np.float32).astype(np.float64)
+    off = np.concatenate([[0], np.cumsum(counts)])
+    c, r = rng.integers(0, n_rows, off[-1]), rng.integers(0, n_rows, off[-1])
+    return q, rows, c, r, off, ref, rng.random(off[-1])
+
+
+@pytest.mark.parametrize("dim", [2, 768, 8193, 16384])
+@pytest.mark.parametrize("counts", [[9], [16], [17], [500], [40, 0, 33], [3] * 70])
+def test_gradient_tolerance_refuses_wrong_gradients(dim, counts):
+    """The tolerance that the GPU tests hold gradients to is no gradient's size: for every query with a gradient, nothing, the
+    negative, half and 1.1 times of it are outside, and so is the gradient without one of the query's pairs."""
+    q, rows, c, r, off, ref, w = preference_case(dim, counts, dim + len(counts))
+    _, _, grad, _ = lo.preference(q, rows, c, r, off, ref, 10.0, 0.0, w)
+    _, _, tol = lo.preference_tolerance(q, rows, c, r, off, ref, 10.0, 0.0, w, "f32")
+    c2 = c.copy()
+    c2[off[:-1][np.array(counts) > 0]] = -1
+    without = lo.preference(q, rows, c2, r, off, ref, 10.0, 0.0, w)[2]
+    for k in range(len(counts)):
+        if grad[k].any():
+            for wrong in (0 * grad[k], -grad[k], 0.5 * grad[k], 1.1 * grad[k], without[k]):
+                # (the first pair may name one row twice, and have no gradient)
+                assert np.array_equal(wrong, grad[k]) or (np.abs(wrong - grad[k]) > tol[k]).any(), (dim, k)

@@ -581,3 +581,35 @@ def test_wide_rows(env, qdt, rdt, dim, counts):
     q, ref, rows, c, r, off = make(env, qdt, rdt, len(counts), dim, 30, counts, seed=dim + len(counts))
     got = env.hvs.preference_loss(q, rows, c, r, off, reference=ref, beta=10.0)
     check_preference(q, ref, rows, c, r, off, got, qdt, 10.0, 0.0)
+
+
+def check_by_terms(q, ref, rows, chosen, rejected, offsets, got, qdt, beta, smoothing, weights=None):
+    """Every element against a tolerance made of its own terms (tests/test_adapters_cpu.py shows what that refuses)."""
+    args = (np64(q), np64(rows), chosen.cpu().numpy(), rejected.cpu().numpy(), offsets.cpu().numpy(), None if ref is None else np64(ref), beta, smoothing,
+            None if weights is None else np64(weights))
+    loss, margin, grad, _ = lo.preference(*args)
+    loss_tol, margin_tol, grad_tol = lo.preference_tolerance(*args, qdt)
+    check(got[1], margin, margin_tol, "margin")
+    check(got[0], loss, loss_tol, "loss")
+    check(got[2], grad, grad_tol, "grad")
+
+
+@pytest.mark.parametrize("qdt,rdt", [("f32", "f16"), ("f32", "f32"), ("bf16", "bf16")])
+@pytest.mark.parametrize("dim", [2, 40, 768, 1536, 2049, 8192, 8193, 16384])
+@pytest.mark.parametrize("counts", [[1], [16], [17], [500], [0, 70, 1, 0], [40, 0, 33], [3] * 70])
+def test_values_by_their_terms(env, qdt, rdt, dim, counts):
+    """Several waves on a pair, shared queries and their join, one block a query."""
+    q, ref, rows, c, r, off = make(env, qdt, rdt, len(counts), dim, 50, counts, seed=dim + len(counts))
+    weights = env.torch.rand(len(c), device=env.dev)
+    got = env.hvs.preference_loss(q, rows, c, r, off, reference=ref, beta=10.0, weights=weights)
+    check_by_terms(q, ref, rows, c, r, off, got, qdt, 10.0, 0.0, weights)
+
+
+@pytest.mark.parametrize("nq,most,dim", [(1, 300, 1536), (100, 16, 768), (250, 12, 1536), (400, 5, 300), (700, 3, 1536)])
+def test_values_of_batches_by_their_terms(env, nq, most, dim):
+    counts = [(i * 7) % (most + 1) if nq > 1 else most for i in range(nq)]
+    for qdt, rdt, reference, smoothing in (("f32", "f16", True, 0.0), ("f16", "bf16", False, 0.1), ("bf16", "f32", True, 0.1)):
+        q, ref, rows, c, r, off = make(env, qdt, rdt, nq, dim, 90, counts, seed=nq)
+        ref = ref if reference else None
+        got = env.hvs.preference_loss(q, rows, c, r, off, reference=ref, beta=20.0, label_smoothing=smoothing)
+        check_by_terms(q, ref, rows, c, r, off, got, qdt, 20.0, smoothing)
