@@ -288,3 +288,59 @@ def test_gradient_tolerance_refuses_wrong_gradients(dim, counts):
             for wrong in (0 * grad[k], -grad[k], 0.5 * grad[k], 1.1 * grad[k], without[k]):
                 # (the first pair may name one row twice, and have no gradient)
                 assert np.array_equal(wrong, grad[k]) or (np.abs(wrong - grad[k]) > tol[k]).any(), (dim, k)
+
+
+f4 = np.float32
+
+
+def tree_dot(a, b):
+    """fp32 sum of products over the last axis, added up as the kernel does: 8 elements a lane, 64 lanes, then in pairs."""
+    t = a.astype(np.float64) * b.astype(np.float64)  # exact: one rounding at the addition
+    t = np.concatenate([t, np.zeros(t.shape[:-1] + ((-t.shape[-1]) % 512,))], -1).reshape(*t.shape[:-1], -1, 64, 8)
+    acc = np.zeros(t.shape[:-3] + (64,), f4)
+    for c in range(t.shape[-3]):
+        for e in range(8):
+            acc = (acc + t[..., c, :, e]).astype(f4)
+    while acc.shape[-1] > 1:
+        acc = acc[..., 0::2] + acc[..., 1::2]
+    return acc[..., 0]
+
+
+def fma(a, b, c):
+    return (a.astype(np.float64) * b.astype(np.float64) + c.astype(np.float64)).astype(f4)
+
+
+def margin_forms(q, ref, c, r):
+    """The margin in fp32: as the kernel takes it, as two differences of cosines, and from fp32 unit vectors."""
+    inv = lambda v: f4(1) / np.sqrt(tree_dot(v, v))[:, None]
+    inv64 = lambda v: 1 / np.sqrt((v.astype(np.float64) ** 2).sum(-1, keepdims=True))
+    iy, i0 = inv64(q), inv64(ref)
+    hy, h0 = iy.astype(f4), i0.astype(f4)
+    f = ref * h0
+    d = fma(q, hy, -f) + (fma(q, (iy - hy).astype(f4), -fma(ref, h0, -f)) - ref * (i0 - h0).astype(f4))
+    kernel = tree_dot(d, fma(c, inv(c), -(r * inv(r))))
+    cu, ru, yu, zu = (v * inv(v) for v in (c, r, q, ref))
+    return kernel, (tree_dot(yu, cu) - tree_dot(yu, ru)) - (tree_dot(zu, cu) - tree_dot(zu, ru)), tree_dot(yu - zu, cu - ru)
+
+
+def near_queries(rng, rows, c, off, move, t):
+    """A reference near every query's first chosen row, and a query of another length that has moved a little."""
+    base = (rows[c[off[:-1]]] + 0.3 * rng.standard_normal((len(off) - 1, rows.shape[1]))) * 3.7
+    return (base * 1.3 + move * rng.standard_normal(base.shape)).astype(t), base.astype(t)
+
+
+@pytest.mark.parametrize("move", [1e-2, 1e-3])
+@pytest.mark.parametrize("t", [np.float32, np.float16])
+@pytest.mark.parametrize("dim,counts", [(1536, [16]), (1536, [3] * 300), (768, [100, 2, 90]), (4000, [5] * 9), (9000, [4] * 5)])
+def test_margin_tolerance_refuses_plain_forms(move, t, dim, counts):
+    """What margins next to the reference are held to: the kernel's formula in fp32 stays far within, the plain fp32 forms do not."""
+    rng = np.random.default_rng(dim + len(counts))
+    rows = rng.standard_normal((90, dim)).astype(np.float16).astype(f4)
+    off = np.concatenate([[0], np.cumsum(counts)])
+    c, r = rng.integers(0, 90, off[-1]), rng.integers(0, 90, off[-1])
+    q, ref = (v.astype(f4) for v in near_queries(rng, rows, c, off, move, t))
+    own, apart = np.repeat(np.arange(len(counts)), counts), c != r
+    args = (q.astype(float), rows.astype(float), c, r, off, ref.astype(float), 10.0, 0.0, None)
+    want, tol = lo.preference(*args)[1], lo.preference_tolerance(*args, "f32")[1]
+    kernel, cosines, units = (np.abs(m - want)[apart] / tol[apart] for m in margin_forms(q[own], ref[own], rows[c], rows[r]))
+    assert kernel.max() < 0.25 and cosines.max() > 2 and units.max() > 2, (kernel.max(), cosines.max(), units.max())

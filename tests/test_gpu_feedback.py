@@ -613,3 +613,21 @@ def test_values_of_batches_by_their_terms(env, nq, most, dim):
         ref = ref if reference else None
         got = env.hvs.preference_loss(q, rows, c, r, off, reference=ref, beta=20.0, label_smoothing=smoothing)
         check_by_terms(q, ref, rows, c, r, off, got, qdt, 20.0, smoothing)
+
+
+@pytest.mark.parametrize("move", [1e-2, 1e-3])
+@pytest.mark.parametrize("qdt", ["f32", "f16"])
+@pytest.mark.parametrize("dim,counts", [(1536, [16]), (1536, [3] * 300), (768, [100, 2, 90]), (4000, [5] * 9), (9000, [4] * 5)])
+def test_small_moves_by_their_terms(env, move, qdt, dim, counts):
+    """Margins next to the reference, to a precision that plain fp32 forms miss (test_margin_tolerance_refuses_plain_forms)."""
+    from tests.test_adapters_cpu import near_queries
+
+    torch = env.torch
+    rng = np.random.default_rng(dim + len(counts))
+    rows = rng.standard_normal((90, dim)).astype(np.float16)
+    off = np.concatenate([[0], np.cumsum(counts)])
+    c, r = rng.integers(0, 90, off[-1]), rng.integers(0, 90, off[-1])
+    q, ref = near_queries(rng, rows.astype(np.float32), c, off, move, {"f32": np.float32, "f16": np.float16}[qdt])
+    q, ref, rows, c, r, off = (torch.from_numpy(np.ascontiguousarray(v)).to(env.dev) for v in (q, ref, rows, c, r, off))
+    got = env.hvs.preference_loss(q, rows, c, r, off, reference=ref, beta=10.0)
+    check_by_terms(q, ref, rows, c, r, off, got, qdt, 10.0, 0.0)
