@@ -63,6 +63,43 @@ template <int DT, int CH> __device__ __forceinline__ void keep_raw(Raw8<DT> (&a)
 __device__ __forceinline__ float softplus(float z) { return fmaxf(z, 0.0f) + log1pf(expf(-fabsf(z))); }
 __device__ __forceinline__ float inverse_norm(float sum_of_squares) { return sum_of_squares == 0.0f ? 0.0f : 1.0f / sqrtf(sum_of_squares); }
 
+// Rows of fp32 and bf16 may be longer than 2^64 or shorter than 2^-50: their squares leave fp32, or its normal numbers.  The squares
+// of such a row are added up again, of its elements times the power of two that brings the largest to [0.5, 1).
+__device__ __forceinline__ bool plain_square_sum(float v) { return v >= 0x1p-100f && v < __builtin_inff(); }
+// use(element) for the elements of a row's part, four bytes at a time: what this seldom path holds in registers the usual one pays for
+template <int DT, int CH, class USE> __device__ __forceinline__ void for_each_element(const Raw8<DT> (&r)[CH], float &state, USE use) {
+    static_assert(DT == HVS_F32 || DT == HVS_BF16, "no such rows of fp16");
+    constexpr int EPC = Elem<DT>::EPC;
+#pragma unroll
+    for (int i = 0; i < CH * 32 / EPC; i++) {
+        float word = r[i / (32 / EPC)].c[i / 4 % (8 / EPC)][i % 4];
+        asm volatile("" : "+v"(word), "+v"(state));  // one word after the other
+        if (DT == HVS_F32) use(word);
+        else {
+            use(__uint_as_float(__float_as_uint(word) << 16));
+            use(__uint_as_float(__float_as_uint(word) & 0xFFFF0000u));
+        }
+    }
+}
+template <int DT, int CH> __device__ __forceinline__ float row_largest(const Raw8<DT> (&r)[CH]) {
+    float largest = 0.0f;
+    for_each_element<DT, CH>(r, largest, [&](float v) { largest = fmaxf(largest, fabsf(v)); });
+    return largest;
+}
+template <int DT, int CH> __device__ __forceinline__ float row_square_sum(const Raw8<DT> (&r)[CH], int exponent) {
+    float sum = 0.0f;
+    for_each_element<DT, CH>(r, sum, [&](float v) {
+        v = ldexpf(v, -exponent);
+        sum = fmaf(v, v, sum);
+    });
+    return sum;
+}
+// 1 / norm from such a sum; a norm whose inverse is no fp32 number counts as 0
+__device__ __forceinline__ float inverse_norm(float sum_of_squares, int exponent) {
+    const float inv = ldexpf(inverse_norm(sum_of_squares), -exponent);
+    return inv == __builtin_inff() ? 0.0f : inv;
+}
+
 // how the pairs [b0, b1) of a query are shared out; the same on every side that asks
 __device__ __forceinline__ void pair_share(const PreferenceParams &p, int64_t q, int shares, int64_t &b0, int64_t &b1, int64_t &per, int &used) {
     b0 = p.offsets[q];
@@ -79,8 +116,9 @@ __device__ __forceinline__ void pair_share(const PreferenceParams &p, int64_t q,
 // the rows of the team's next pair are on their way meanwhile.  Teams of one wave read the query and the reference query
 // from LDS (registers then allow four waves per SIMD), larger teams hold their part.  The block's teams take the pairs of
 // its share in turn and are added up in team order.  Bound by reading the rows.
+// (513 - 1024 columns: registers for five waves a SIMD; with four, 4096 queries x 8 pairs of 1024 bf16 columns take 49.7 instead of 45.6 us)
 template <int QDT, int RDT, int CH, int TW, int WAVES, bool ALIGNED>
-__global__ __launch_bounds__(64 * WAVES) void preference_kernel(PreferenceParams p) {
+__global__ __launch_bounds__(64 * WAVES, TW == 1 && CH == 2 && WAVES == 4 ? 5 : 1) void preference_kernel(PreferenceParams p) {
     typedef typename Elem<QDT>::type Q;
     constexpr int TEAMS = WAVES / TW, SPAN = CH * TW * 512;  // SPAN: dim rounded up to what a team covers
     extern __shared__ __attribute__((aligned(16))) float smem[];  // TW 1: [2][SPAN] the queries, then [TEAMS][SPAN]; else [dim]
@@ -108,6 +146,17 @@ __global__ __launch_bounds__(64 * WAVES) void preference_kernel(PreferenceParams
             a = b = 0.0f;
 #pragma unroll
             for (int w = 0; w < TW; w++) a += sums[team * TW + w][0], b += sums[team * TW + w][1];
+        }
+    };
+    auto team_max = [&](float &a, float &b) {
+        learn_wave_max2(a, b);
+        if (TW > 1) {
+            __syncthreads();
+            if (lane == 0) sums[wave][0] = a, sums[wave][1] = b;
+            __syncthreads();
+            a = b = 0.0f;
+#pragma unroll
+            for (int w = 0; w < TW; w++) a = fmaxf(a, sums[team * TW + w][0]), b = fmaxf(b, sums[team * TW + w][1]);
         }
     };
     auto left_out = [&](int64_t a, int64_t b) { return a < 0 || b < 0 || a >= p.n_rows || b >= p.n_rows; };
@@ -226,9 +275,22 @@ __global__ __launch_bounds__(64 * WAVES) void preference_kernel(PreferenceParams
                 for (int e = 0; e < 8; e++) ia = fmaf(av[e], av[e], ia), ib = fmaf(bv[e], bv[e], ib);
             }
             team_sum(ia, ib);
+            int ea = 0, eb = 0;
+            if constexpr (RDT != HVS_F16) {  // (squares of fp16 stay well inside)
+                if (!(plain_square_sum(ia) && plain_square_sum(ib))) {
+                    float ma = row_largest<RDT, CH>(ra), mb = row_largest<RDT, CH>(rb);
+                    team_max(ma, mb);
+                    // exponents that bring the largest element to [0.5, 1); 0 where that is 0 or not finite.  The same in every lane
+                    ea = __builtin_amdgcn_readfirstlane(__builtin_amdgcn_frexp_expf(ma));
+                    eb = __builtin_amdgcn_readfirstlane(__builtin_amdgcn_frexp_expf(mb));
+                    ia = row_square_sum<RDT, CH>(ra, ea);
+                    ib = row_square_sum<RDT, CH>(rb, eb);
+                    team_sum(ia, ib);
+                }
+            }
             // a row against itself is no preference: exactly 0, whatever the roundings below
-            ia = a == b ? 0.0f : inverse_norm(ia);
-            ib = a == b ? 0.0f : inverse_norm(ib);
+            ia = a == b ? 0.0f : inverse_norm(ia, ea);
+            ib = a == b ? 0.0f : inverse_norm(ib, eb);
             keep_raw(ra, rb);
 #pragma unroll
             for (int c = 0; c < CH; c++) {

@@ -95,20 +95,28 @@ __device__ __forceinline__ float learn_wave_sum(float v) {
 template <int CTRL> __device__ __forceinline__ float learn_dpp(float v) {
     return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), CTRL, 0xF, 0xF, true));
 }
-// Two sums over the wave at once, in vector registers alone: the halves trade places, so that each works on one value; rows of
-// 16 lanes add up by rotation, then the two rows of a half.  a and b become the sums, the same in every lane.
-__device__ __forceinline__ void learn_wave_sum2(float &a, float &b) {
+// Two sums (or two largest values) over the wave at once, in vector registers alone: the halves trade places, so that each works on
+// one value; rows of 16 lanes are joined by rotation, then the two rows of a half.  a and b become the results, the same in every lane.
+struct LearnAdd {
+    __device__ __forceinline__ float operator()(float a, float b) const { return a + b; }
+};
+struct LearnMax {  // of a number and a NaN: the number
+    __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); }
+};
+template <class OP> __device__ __forceinline__ void learn_wave_join2(float &a, float &b, OP op) {
     auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
-    float u = __uint_as_float(r[0]) + __uint_as_float(r[1]);  // lanes 0-31: a, lanes 32-63: b
-    u += learn_dpp<0x128>(u);                                 // rotations by 8, 4, 2, 1
-    u += learn_dpp<0x124>(u);
-    u += learn_dpp<0x122>(u);
-    u += learn_dpp<0x121>(u);
+    float u = op(__uint_as_float(r[0]), __uint_as_float(r[1]));  // lanes 0-31: a, lanes 32-63: b
+    u = op(u, learn_dpp<0x128>(u));                              // rotations by 8, 4, 2, 1
+    u = op(u, learn_dpp<0x124>(u));
+    u = op(u, learn_dpp<0x122>(u));
+    u = op(u, learn_dpp<0x121>(u));
     r = __builtin_amdgcn_permlane16_swap(__float_as_uint(u), __float_as_uint(u), false, false);
-    const uint32_t s = __float_as_uint(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+    const uint32_t s = __float_as_uint(op(__uint_as_float(r[0]), __uint_as_float(r[1])));
     a = __uint_as_float(__builtin_amdgcn_readlane(s, 0));
     b = __uint_as_float(__builtin_amdgcn_readlane(s, 32));
 }
+__device__ __forceinline__ void learn_wave_sum2(float &a, float &b) { learn_wave_join2(a, b, LearnAdd()); }
+__device__ __forceinline__ void learn_wave_max2(float &a, float &b) { learn_wave_join2(a, b, LearnMax()); }
 
 // Makes `device` current for a call and the caller's device current again after it.
 struct DeviceGuard {
