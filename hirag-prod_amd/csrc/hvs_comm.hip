@@ -216,7 +216,7 @@ extern "C" int hvs_search_sharded(hvs_index *idx, hvs_comm *comm, const float *q
     HVS_REQUIRE(k >= 1 && k <= HVS_MAX_K, "hvs_search_sharded: k %d not in [1, %d]", k, HVS_MAX_K);
     HVS_REQUIRE(!comm->nccl || comm->device == idx->device, "hvs_search_sharded: the communicator was made for device %d, the index lives on %d",
                 comm->device, idx->device);
-    HVS_HIP(hipSetDevice(idx->device));
+    HVS_TRY(hvs_index_enter(idx));
     const int W = comm->world;
     const size_t o_ids = up256((size_t)nq * k * 4), o_cnt = o_ids + up256((size_t)nq * k * 8), o_status = o_cnt + up256((size_t)nq * 4),
                  rec = o_status + 256;
@@ -301,7 +301,7 @@ extern "C" int hvs_allreduce_centroids(hvs_index *idx, hvs_comm *comm, float *su
     HVS_REQUIRE(idx != nullptr && comm != nullptr, "hvs_allreduce_centroids: NULL index or communicator");
     HVS_REQUIRE(sums && counts && n_centroids >= 1, "hvs_allreduce_centroids: NULL or empty argument");
     if (comm->world == 1 && !comm->nccl) return 0;
-    HVS_HIP(hipSetDevice(idx->device));
+    HVS_TRY(hvs_index_enter(idx));
     const size_t n_sum = (size_t)n_centroids * idx->dim, sum_bytes = n_sum * 4, cnt_bytes = (size_t)n_centroids * 8;
     if (comm->nccl) {
         float *d_sums = sums;

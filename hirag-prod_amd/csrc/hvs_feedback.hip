@@ -574,23 +574,29 @@ extern "C" int hvs_index_preference_loss(hvs_index *idx, void *stream, const hvs
     DeviceGuard guard(idx->device);
     HVS_HIP(guard.status);
     hipStream_t st = (hipStream_t)stream;
-    hipStreamCaptureStatus capturing = hipStreamCaptureStatusNone;
-    if (st != nullptr) HVS_HIP(hipStreamIsCapturing(st, &capturing));
-    HVS_REQUIRE(capturing == hipStreamCaptureStatusNone, "%s: the stream is being captured; a graph would keep the address of rows the table may move", who);
+    for (hipStream_t own : {st, idx->stream}) {
+        hipStreamCaptureStatus capturing = hipStreamCaptureStatusNone;
+        if (own != nullptr) HVS_HIP(hipStreamIsCapturing(own, &capturing));
+        HVS_REQUIRE(capturing == hipStreamCaptureStatusNone, "%s: the %s is being captured; a graph would keep the address of rows the table may move", who,
+                    own == st ? "stream" : "table's stream");
+    }
     if (st == idx->stream) return preference_core(st, p, idx->rows, idx->dtype, idx->dim, idx->ld, idx->n, workspace);
-    hipEvent_t &ev = idx->ev_reader;
-    if (ev == nullptr) HVS_HIP(hipEventCreateWithFlags(&ev, hipEventDisableTiming | hipEventDisableSystemFence));
-    // the event is about to stand for this read: an earlier one on another stream is waited for by the table's stream now
-    if (idx->reader_pending && idx->reader_stream != st) HVS_HIP(hipStreamWaitEvent(idx->stream, ev, 0));
+    for (hipEvent_t *ev : {&idx->ev_table, &idx->ev_reader})
+        if (*ev == nullptr) HVS_HIP(hipEventCreateWithFlags(ev, hipEventDisableTiming | hipEventDisableSystemFence));
     // after the work the table's stream holds; mostly it holds none, and then there is nothing to wait for
     const hipError_t idle = hipStreamQuery(idx->stream);
     if (idle == hipErrorNotReady) {
         (void)hipGetLastError();  // an answer, not an error to be found by the next launch
-        HVS_HIP(hipEventRecord(ev, idx->stream));
-        HVS_HIP(hipStreamWaitEvent(st, ev, 0));
+        HVS_HIP(hipEventRecord(idx->ev_table, idx->stream));
+        HVS_HIP(hipStreamWaitEvent(st, idx->ev_table, 0));
     } else HVS_HIP(idle);
-    HVS_TRY(preference_core(st, p, idx->rows, idx->dtype, idx->dim, idx->ld, idx->n, workspace));
-    HVS_HIP(hipEventRecord(ev, st));
+    // ev_reader is about to stand for this read: the table's stream waits now for an earlier one on another stream
+    if (idx->reader_pending && idx->reader_stream != st) HVS_TRY(hvs_index_enter(idx));
+    const int failed = preference_core(st, p, idx->rows, idx->dtype, idx->dim, idx->ld, idx->n, workspace);
+    const hipError_t recorded = hipEventRecord(idx->ev_reader, st);
+    if (failed || recorded != hipSuccess) (void)hipStreamSynchronize(st);  // a read that no event stands for must not be left behind
+    HVS_TRY(failed);
+    HVS_HIP(recorded);
     idx->reader_stream = st;
     idx->reader_pending = true;
     return 0;

@@ -546,7 +546,7 @@ extern "C" int hvs_index_set_attributes(hvs_index *idx, int64_t first_pos, int64
     HVS_REQUIRE(first_pos >= 0 && n >= 0 && first_pos + n <= idx->n, "hvs_index_set_attributes: rows [%lld, %lld) outside [0, %lld)",
                 (long long)first_pos, (long long)(first_pos + n), (long long)idx->n);
     if (n == 0 || (!workspace && !knowledge_base && !uri && !is_private)) return 0;
-    HVS_HIP(hipSetDevice(idx->device));
+    HVS_TRY(hvs_index_enter(idx));
     HVS_TRY(hvs_attrs_ensure(idx));
     // staging (workspace 3): the four host arrays, 256-byte aligned
     auto up = [](size_t v) { return (v + 255) & ~(size_t)255; };
@@ -634,6 +634,7 @@ extern "C" int hvs_index_destroy(hvs_index *idx) {
     hipEventDestroy(idx->tm0);
     hipEventDestroy(idx->tm1);
     if (idx->ev_reader) hipEventDestroy(idx->ev_reader);
+    if (idx->ev_table) hipEventDestroy(idx->ev_table);
     if (idx->own_stream) hipStreamDestroy(idx->stream);
     delete idx;
     return 0;
@@ -652,21 +653,11 @@ static int grow(hvs_index *idx, P **ptr, size_t old_count, size_t new_count, boo
     return 0;
 }
 
-// Called before rows move, change or go: the table's stream waits for the reads of its rows that callers' streams still hold
-// (hvs_index_preference_loss).
-static int readers_wait(hvs_index *idx) {
-    if (!idx->reader_pending) return 0;
-    HVS_HIP(hipStreamWaitEvent(idx->stream, idx->ev_reader, 0));
-    idx->reader_pending = false;
-    return 0;
-}
-
 extern "C" int hvs_index_reserve(hvs_index *idx, int64_t capacity_rows) {
     HVS_REQUIRE(idx != nullptr, "hvs_index_reserve: idx is NULL");
     HVS_REQUIRE(capacity_rows < (int64_t)0xFFFFFFFFll, "hvs_index_reserve: at most 2^32-1 rows per index");
     if (capacity_rows <= idx->cap) return 0;
-    HVS_HIP(hipSetDevice(idx->device));
-    HVS_TRY(readers_wait(idx));
+    HVS_TRY(hvs_index_enter(idx));
     const size_t row_bytes = (size_t)idx->ld * idx->elem_size;
     {
         // Rows beyond n and HVS_ROWS_SLACK bytes after the last one are kept zero: the MFMA kernels fetch whole
@@ -706,9 +697,25 @@ extern "C" int hvs_index_info(hvs_index *idx, int *dim, int *dtype, int *device_
     return 0;
 }
 
+// Called first by every entry point that gives work to the table's stream: makes its GPU current, and that work waits for the reads
+// of rows that callers' streams still hold (hvs_index_preference_loss).  A stream under capture (hvs_search_noalloc) does not run now
+// and must not wait for an event from outside its graph: it is left alone, and the next call that does run waits.
+int hvs_index_enter(hvs_index *idx) {
+    HVS_HIP(hipSetDevice(idx->device));
+    if (!idx->reader_pending) return 0;
+    if (!idx->own_stream) {
+        hipStreamCaptureStatus capturing = hipStreamCaptureStatusNone;
+        HVS_HIP(hipStreamIsCapturing(idx->stream, &capturing));
+        if (capturing != hipStreamCaptureStatusNone) return 0;
+    }
+    HVS_HIP(hipStreamWaitEvent(idx->stream, idx->ev_reader, 0));
+    idx->reader_pending = false;
+    return 0;
+}
+
 extern "C" int hvs_sync(hvs_index *idx) {
     HVS_REQUIRE(idx != nullptr, "hvs_sync: idx is NULL");
-    HVS_HIP(hipSetDevice(idx->device));
+    HVS_TRY(hvs_index_enter(idx));
     HVS_HIP(hipStreamSynchronize(idx->stream));
     return 0;
 }
@@ -749,7 +756,7 @@ extern "C" int hvs_index_add(hvs_index *idx, const void *rows, int src_dtype, in
     if (n == 0) return 0;
     HVS_REQUIRE(rows != nullptr, "hvs_index_add: rows is NULL");
     HVS_REQUIRE(src_dtype == HVS_F32 || src_dtype == idx->dtype, "hvs_index_add: source dtype %d not accepted by index dtype %d", src_dtype, idx->dtype);
-    HVS_HIP(hipSetDevice(idx->device));
+    HVS_TRY(hvs_index_enter(idx));
     if (idx->n + n > idx->cap) {
         int64_t want = idx->cap * 2;
         if (want < idx->n + n) want = idx->n + n;
@@ -818,8 +825,7 @@ extern "C" int hvs_index_update(hvs_index *idx, const int64_t *positions, const 
     if (n <= 0) return 0;
     HVS_REQUIRE(positions && rows, "hvs_index_update: NULL argument");
     HVS_REQUIRE(src_dtype == HVS_F32 || src_dtype == idx->dtype, "hvs_index_update: source dtype %d not accepted", src_dtype);
-    HVS_HIP(hipSetDevice(idx->device));
-    HVS_TRY(readers_wait(idx));
+    HVS_TRY(hvs_index_enter(idx));
     const size_t src_row_bytes = (size_t)idx->dim * hvs_elem_size(src_dtype);
     if (on_device) {
         HVS_TRY(validate_device_positions(idx, positions, n, "hvs_index_update"));
@@ -844,7 +850,7 @@ extern "C" int hvs_index_set_deleted(hvs_index *idx, const int64_t *positions, i
     HVS_REQUIRE(positions != nullptr, "hvs_index_set_deleted: positions is NULL");
     for (int64_t i = 0; i < n; i++)
         HVS_REQUIRE(positions[i] >= 0 && positions[i] < idx->n, "hvs_index_set_deleted: position %lld out of range", (long long)positions[i]);
-    HVS_HIP(hipSetDevice(idx->device));
+    HVS_TRY(hvs_index_enter(idx));
     if (!idx->deleted) {
         const size_t words = (size_t)(idx->cap + 31) / 32;
         HVS_HIP(hipMalloc((void **)&idx->deleted, words * 4));
@@ -873,7 +879,7 @@ extern "C" int hvs_index_deleted_count(hvs_index *idx, int64_t *out_rows) {
 
 extern "C" int hvs_index_prepare(hvs_index *idx, int *out_ready) {
     HVS_REQUIRE(idx != nullptr, "hvs_index_prepare: idx is NULL");
-    HVS_HIP(hipSetDevice(idx->device));
+    HVS_TRY(hvs_index_enter(idx));
     bool ok = false;
     if (idx->dtype == HVS_F32 && idx->n > 0 && !getenv("HVS_NO_SPLIT")) {
         idx->split_failed = false;  // an explicit request tries again: memory may have been freed since the copy was refused
@@ -890,7 +896,7 @@ extern "C" int hvs_index_search_copy(hvs_index *idx, int allow, int64_t *out_byt
     if (allow >= 0) {
         idx->split_allowed = allow != 0;
         if (!idx->split_allowed && idx->split) {  // give the memory back now
-            HVS_HIP(hipSetDevice(idx->device));
+            HVS_TRY(hvs_index_enter(idx));
             HVS_HIP(hipStreamSynchronize(idx->stream));
             (void)hipFree(idx->split);
             (void)hipFree(idx->split_inv);
@@ -913,7 +919,7 @@ extern "C" int hvs_index_export(hvs_index *idx, int64_t first, int64_t n, void *
     HVS_REQUIRE(first >= 0 && n >= 0 && first + n <= idx->n, "hvs_index_export: rows [%lld, %lld) outside [0, %lld)",
                 (long long)first, (long long)(first + n), (long long)idx->n);
     if (n == 0) return 0;
-    HVS_HIP(hipSetDevice(idx->device));
+    HVS_TRY(hvs_index_enter(idx));
     hipStream_t s = idx->stream;
     if (rows) {
         const size_t row_bytes = (size_t)idx->dim * idx->elem_size, pitch = (size_t)idx->ld * idx->elem_size;
@@ -940,7 +946,6 @@ extern "C" int hvs_index_export(hvs_index *idx, int64_t first, int64_t n, void *
 // new arrays sized for them, the old ones released only when every copy has succeeded.  Tombstones are gone afterwards
 // (the caller lists live rows only).  renumber_ids: ids become the new positions.
 static int rebuild_rows(hvs_index *idx, const uint32_t *positions, int64_t n_live, int renumber_ids, const char *who) {
-    HVS_TRY(readers_wait(idx));
     const size_t pitch = (size_t)idx->ld * idx->elem_size;
     const int64_t cap = n_live > 1024 ? n_live : 1024;
     char *rows = nullptr;
@@ -1128,7 +1133,7 @@ static int build_part_table(hvs_index *idx, int64_t part_n) {
 
 extern "C" int hvs_index_partition(hvs_index *idx, int renumber_ids, int64_t *out_rows, int64_t *out_old_positions) {
     HVS_REQUIRE(idx != nullptr, "hvs_index_partition: idx is NULL");
-    HVS_HIP(hipSetDevice(idx->device));
+    HVS_TRY(hvs_index_enter(idx));
     const int64_t n = idx->n;
     if (n == 0) {
         idx->part_n = 0;
@@ -1197,7 +1202,7 @@ extern "C" int hvs_index_set_ids(hvs_index *idx, int64_t first_pos, int64_t n, c
                 (long long)first_pos, (long long)(first_pos + n), (long long)idx->n);
     if (n == 0) return 0;
     HVS_REQUIRE(ids != nullptr, "hvs_index_set_ids: ids is NULL");
-    HVS_HIP(hipSetDevice(idx->device));
+    HVS_TRY(hvs_index_enter(idx));
     HVS_HIP(hipMemcpyAsync(idx->ids + first_pos, ids, (size_t)n * 8, hipMemcpyHostToDevice, idx->stream));
     HVS_HIP(hipStreamSynchronize(idx->stream));
     return 0;
@@ -1205,7 +1210,7 @@ extern "C" int hvs_index_set_ids(hvs_index *idx, int64_t first_pos, int64_t n, c
 
 extern "C" int hvs_index_compact(hvs_index *idx, int renumber_ids, int64_t *out_rows) {
     HVS_REQUIRE(idx != nullptr, "hvs_index_compact: idx is NULL");
-    HVS_HIP(hipSetDevice(idx->device));
+    HVS_TRY(hvs_index_enter(idx));
     if (idx->n_deleted > 0 && idx->n > 0) {
         // compaction keeps the order of the survivors, so the ordered part of a partitioned table stays ordered: it
         // shrinks to its live rows and the range table is rebuilt below
@@ -1240,7 +1245,7 @@ extern "C" int hvs_index_fill_synthetic(hvs_index *idx, int64_t n, uint64_t seed
     HVS_REQUIRE(idx != nullptr, "hvs_index_fill_synthetic: idx is NULL");
     HVS_REQUIRE(n >= 0 && first_global_row >= 0, "hvs_index_fill_synthetic: negative argument");
     if (n == 0) return 0;
-    HVS_HIP(hipSetDevice(idx->device));
+    HVS_TRY(hvs_index_enter(idx));
     if (idx->n + n > idx->cap) HVS_TRY(hvs_index_reserve(idx, idx->n + n));
     const int64_t first = idx->n;
     // splitmix64(seed) on the host, same function as the device's
@@ -1281,7 +1286,7 @@ extern "C" int hvs_index_fill_clustered(hvs_index *idx, int64_t n, uint64_t seed
     HVS_REQUIRE(n >= 0 && first_global_row >= 0, "hvs_index_fill_clustered: negative argument");
     HVS_REQUIRE(n_clusters >= 1, "hvs_index_fill_clustered: n_clusters %lld < 1", (long long)n_clusters);
     if (n == 0) return 0;
-    HVS_HIP(hipSetDevice(idx->device));
+    HVS_TRY(hvs_index_enter(idx));
     if (idx->n + n > idx->cap) HVS_TRY(hvs_index_reserve(idx, idx->n + n));
     const int64_t first = idx->n;
     hvs_cluster_params cp;
@@ -1317,7 +1322,7 @@ extern "C" int hvs_gather(hvs_index *idx, const int64_t *positions, int64_t n, f
     HVS_REQUIRE(idx != nullptr, "hvs_gather: idx is NULL");
     if (n <= 0) return 0;
     HVS_REQUIRE(positions && out, "hvs_gather: NULL argument");
-    HVS_HIP(hipSetDevice(idx->device));
+    HVS_TRY(hvs_index_enter(idx));
     const int64_t *d_pos = positions;
     float *d_out = out;
     const size_t out_bytes = (size_t)n * idx->dim * 4;
@@ -1369,14 +1374,14 @@ extern "C" int hvs_profile_reset(hvs_index *idx) {
 
 extern "C" int hvs_timer_start(hvs_index *idx) {
     HVS_REQUIRE(idx != nullptr, "hvs_timer_start: idx is NULL");
-    HVS_HIP(hipSetDevice(idx->device));
+    HVS_TRY(hvs_index_enter(idx));
     HVS_HIP(hipEventRecord(idx->tm0, idx->stream));
     return 0;
 }
 
 extern "C" int hvs_timer_stop(hvs_index *idx, double *elapsed_ms) {
     HVS_REQUIRE(idx && elapsed_ms, "hvs_timer_stop: NULL argument");
-    HVS_HIP(hipSetDevice(idx->device));
+    HVS_TRY(hvs_index_enter(idx));
     HVS_HIP(hipEventRecord(idx->tm1, idx->stream));
     HVS_HIP(hipEventSynchronize(idx->tm1));
     float ms = 0.0f;

@@ -109,12 +109,13 @@ struct hvs_index {
     hipEvent_t ev0 = nullptr, ev1 = nullptr;  // profiling pair
     hipEvent_t tm0 = nullptr, tm1 = nullptr;  // user timer pair
     // reads of the rows on a caller's stream (hvs_index_preference_loss): the last one, and whether this index's stream has yet
-    // to wait for it before rows move, change or go
-    hipEvent_t ev_reader = nullptr;
+    // to wait for it (hvs_index_enter); ev_table: the work of this index's stream such a read comes after
+    hipEvent_t ev_reader = nullptr, ev_table = nullptr;
     hipStream_t reader_stream = nullptr;
     bool reader_pending = false;
 };
 
+int hvs_index_enter(hvs_index *idx);
 int hvs_ws_get(hvs_index *idx, int slot, size_t bytes, void **out);
 int hvs_pinned_get(hvs_index *idx, size_t bytes, void **out);  // pinned host memory, grown like a workspace
 

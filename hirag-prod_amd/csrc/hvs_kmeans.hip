@@ -459,7 +459,7 @@ extern "C" int hvs_kmeans_assign(hvs_index *idx, const float *centroids, int n_c
         if (out_sums) {
             const size_t sum_bytes = (size_t)n_centroids * idx->dim * 4, cnt_bytes = (size_t)n_centroids * 8;
             if (on_device) {
-                HVS_HIP(hipSetDevice(idx->device));
+                HVS_TRY(hvs_index_enter(idx));
                 HVS_HIP(hipMemsetAsync(out_sums, 0, sum_bytes, idx->stream));
                 HVS_HIP(hipMemsetAsync(out_counts, 0, cnt_bytes, idx->stream));
             } else {
@@ -469,7 +469,7 @@ extern "C" int hvs_kmeans_assign(hvs_index *idx, const float *centroids, int n_c
         }
         return 0;
     }
-    HVS_HIP(hipSetDevice(idx->device));
+    HVS_TRY(hvs_index_enter(idx));
     const int K = n_centroids, dim = idx->dim, ld = idx->ld;
     const int ldc = (ld + 31) / 32 * 32;
     hipStream_t st = idx->stream;

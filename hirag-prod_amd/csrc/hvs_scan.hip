@@ -1124,7 +1124,7 @@ extern "C" int hvs_search_filtered(hvs_index *idx, const float *queries, int nq,
     HVS_REQUIRE(idx != nullptr, "hvs_search_filtered: idx is NULL");
     const uint32_t *d_mask = nullptr;
     if (filter && nq > 0) {
-        HVS_HIP(hipSetDevice(idx->device));
+        HVS_TRY(hvs_index_enter(idx));
         HVS_TRY(hvs_filter_mask(idx, filter, &d_mask, row_begin, row_end));
     }
     return hvs_search_core(idx, queries, nq, fold, k, filter ? filter->group : -1, d_mask, true, max_distance, row_begin, row_end, out_dist,
@@ -1246,7 +1246,7 @@ int hvs_search_core(hvs_index *idx, const float *queries, int nq, int fold, int 
     if (row_end < 0 || row_end > idx->n) row_end = idx->n;
     if (row_begin < 0) row_begin = 0;
     if (row_begin > row_end) row_begin = row_end;
-    HVS_HIP(hipSetDevice(idx->device));
+    HVS_TRY(hvs_index_enter(idx));
     const float thr = hvs_ceil_to_float(max_distance);
     const int nq_total = nq * fold;
 
@@ -1380,7 +1380,7 @@ extern "C" int hvs_search_noalloc(hvs_index *idx, const float *queries, int nq, 
     HVS_REQUIRE(q_end <= HVS_NOALLOC_QUERY_BYTES,
                 "hvs_search_noalloc: %d query embeddings of %d columns take %zu bytes, the scratch array keeps %zu for them", nq_total,
                 idx->dim, q_end, HVS_NOALLOC_QUERY_BYTES);
-    HVS_HIP(hipSetDevice(idx->device));
+    HVS_TRY(hvs_index_enter(idx));
     HVS_TRY(hvs_noalloc_setup(idx->device));  // a table look-up after hvs_index_create has run on this device
     char *scratch = (char *)g_noalloc_ptr[idx->device];
 
@@ -1486,7 +1486,7 @@ extern "C" int hvs_distances(hvs_index *idx, const float *queries, int fold, int
     if (row_end < 0 || row_end > idx->n) row_end = idx->n;
     if (row_begin < 0) row_begin = 0;
     if (row_begin >= row_end) return 0;
-    HVS_HIP(hipSetDevice(idx->device));
+    HVS_TRY(hvs_index_enter(idx));
     const int64_t n_rows = row_end - row_begin;
     float *d_out = out;
     if (!on_device) {
@@ -1515,7 +1515,7 @@ extern "C" int hvs_range_search_filtered(hvs_index *idx, const float *queries, i
     HVS_REQUIRE(idx != nullptr, "hvs_range_search_filtered: idx is NULL");
     const uint32_t *d_mask = nullptr;
     if (filter) {
-        HVS_HIP(hipSetDevice(idx->device));
+        HVS_TRY(hvs_index_enter(idx));
         HVS_TRY(hvs_filter_mask(idx, filter, &d_mask, row_begin, row_end));
     }
     return hvs_range_search_core(idx, queries, fold, filter ? filter->group : -1, d_mask, true, max_distance, row_begin, row_end, capacity,
@@ -1545,7 +1545,7 @@ int hvs_range_search_core(hvs_index *idx, const float *queries, int fold, int32_
     } else if (row_begin < row_end)
         segs[n_segs++] = {row_begin, row_end, group_filter};
     if (n_segs > 0) {
-        HVS_HIP(hipSetDevice(idx->device));
+        HVS_TRY(hvs_index_enter(idx));
         int64_t widest = 0;
         for (int i = 0; i < n_segs; i++) widest = segs[i].e - segs[i].b > widest ? segs[i].e - segs[i].b : widest;
         // staging (workspace 3): [distance column][mask words, if they come from the host][outputs, if they go to the host]

@@ -540,8 +540,9 @@ int hvs_preference_workspace(const hvs_preference *p, int dim, uint64_t *out_byt
 int hvs_preference_loss(int device_id, void *stream, const hvs_preference *p, const void *rows, int rows_dtype, int dim,
                         int64_t ld_rows, int64_t n_rows, void *workspace, uint64_t workspace_bytes);
 /* over the rows of a table (positions as in hvs_gather; deleted rows count as rows).  Runs on `stream`, after the work the
- * table's own stream holds, and the table's later work runs after it.  A captured graph would keep the address of rows
- * that the table may move, so a stream under capture is refused. */
+ * table's own stream holds, and what later calls give to the table's stream (searches and hvs_sync among them) runs after
+ * it.  A captured graph would keep the address of rows that the table may move: refused while `stream` or the table's stream
+ * is being captured. */
 int hvs_index_preference_loss(hvs_index *idx, void *stream, const hvs_preference *p, void *workspace, uint64_t workspace_bytes);
 
 /*

@@ -655,3 +655,127 @@ def test_row_norms_at_the_ends_of_the_range(env, rdt, dim, counts):
     loss, margin, _ = env.hvs.preference_loss(q, sized, c, r, off, reference=ref, beta=10.0)
     touched = (c == 4) | (r == 4)
     assert torch.equal(loss.isnan(), touched) and torch.equal(margin.isnan(), touched)
+
+
+def table_calls():
+    """Calls of a table that return when their work on its stream is done."""
+    rng = np.random.default_rng(0)
+    q = rng.standard_normal((2, 64)).astype(np.float32)
+    rows = rng.standard_normal((5, 64)).astype(np.float32)
+    return dict(sync=lambda t: t.sync(), search=lambda t: t.search(q, k=3), range_search=lambda t: t.range_search(q, 0.5), distances=lambda t: t.distances(q),
+                filtered=lambda t: t.search(q, k=3, filter=dict(workspace=0)), gather=lambda t: t.gather([1, 2]), kmeans=lambda t: t.kmeans_assign(rows),
+                ids=lambda t: t.ids(), export=lambda t: t.export(), set_ids=lambda t: t.set_ids(0, [7, 8]), delete=lambda t: t.set_deleted([3]),
+                compact=lambda t: t.compact(), partition=lambda t: t.partition(), add=lambda t: (t.add(rows), t.sync()),
+                update=lambda t: (t.update([0], rows[:1]), t.sync()), timer=lambda t: (t.timer_start(), t.timer_stop()))
+
+
+@pytest.mark.parametrize("call", list(table_calls()))
+def test_table_work_runs_after_the_loss(env, call):
+    """What is given to a table after a loss over its rows runs after that loss, which waits on its stream behind other work."""
+    torch = env.torch
+    q, ref, rows, c, r, off = make(env, "f32", "f32", 20, 64, 3000, None, seed=1)
+    big = torch.randn(4096, 4096, device=env.dev)
+    out = torch.empty_like(big)
+    idx = env.hvs.HvsIndex(64, "f32", device=0)
+    idx.add(rows.cpu().numpy(), group_codes=np.arange(3000, dtype=np.int32) % 3)
+    idx.set_attributes(0, workspace=np.zeros(3000, dtype=np.int32))
+    table_calls()[call](idx)  # what the call sets up on its first time
+    if call == "compact":
+        idx.set_deleted([5])  # without a deleted row it has nothing to do
+    want = idx.preference_loss(q, c, r, off, reference=ref)
+    side = torch.cuda.Stream()
+    torch.mm(big, big, out=out)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for _ in range(24):  # tens of milliseconds
+            torch.mm(big, big, out=out)
+        got = idx.preference_loss(q, c, r, off, reference=ref)
+    assert not side.query(), "the stream was not busy: the test says nothing"
+    table_calls()[call](idx)
+    assert side.query(), f"{call} did not wait for the loss"
+    if call not in ("compact", "partition", "update", "delete"):
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    idx.close()
+
+
+def test_search_after_a_loss_sees_the_queries_it_was_given(env):
+    """Queries made on a stream, a loss on that stream, then a search of the same table by device pointers."""
+    import ctypes
+
+    from hirag_prod_amd import _lib
+
+    torch, lib = env.torch, env.hvs.load_library()
+    q, ref, rows, c, r, off = make(env, "f32", "f32", 4, 64, 3000, None, seed=2)
+    idx = env.hvs.HvsIndex(64, "f32", device=0)
+    idx.add(rows)
+    want = idx.search(q, k=5)
+    late, big = torch.zeros_like(q), torch.randn(4096, 4096, device=env.dev)
+    out = torch.empty_like(big)
+    outs = torch.empty(4, 5, device=env.dev), torch.empty(4, 5, dtype=torch.int64, device=env.dev), torch.empty(4, dtype=torch.int32, device=env.dev)
+    torch.mm(big, big, out=out)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        for _ in range(24):
+            torch.mm(big, big, out=out)
+        late.copy_(q)
+        idx.preference_loss(late, c, r, off, reference=ref)
+    assert not side.query()
+    ptr = lambda t: ctypes.c_void_p(t.data_ptr())
+    _lib.check(lib.hvs_search(idx._h, ptr(late), 4, 1, 5, -1, None, math.inf, 0, -1, *(ptr(t) for t in outs), 1, _lib.HVS_ALGO_AUTO))
+    _lib.check(lib.hvs_sync(idx._h))
+    assert all(torch.equal(a, b) for a, b in zip(outs, want))
+    idx.close()
+
+
+def test_search_captured_while_a_loss_reads_the_table(env):
+    """Recording a search neither waits nor fails while a loss is under way; the next call that runs waits for it."""
+    import ctypes
+
+    torch, lib = env.torch, env.hvs.load_library()
+    q, ref, rows, c, r, off = make(env, "f32", "f32", 4, 64, 3000, None, seed=2)
+    stream = torch.cuda.Stream()
+    idx = env.hvs.HvsIndex(64, "f32", device=0, stream=stream.cuda_stream)
+    idx.add(rows)
+    dist, ids, cnt = idx.search(q, k=5)
+    outs = torch.empty_like(dist), torch.empty_like(ids), torch.empty_like(cnt)
+    ptr = lambda t: ctypes.c_void_p(t.data_ptr())
+    call = lambda: lib.hvs_search_noalloc(idx._h, ptr(q), 4, 1, 5, -1, None, math.inf, 0, -1, *(ptr(t) for t in outs))
+    assert call() == 0
+    idx.sync()
+    big = torch.randn(4096, 4096, device=env.dev)
+    out = torch.empty_like(big)
+    torch.mm(big, big, out=out)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    refused = []
+    with torch.cuda.stream(side):
+        for _ in range(24):
+            torch.mm(big, big, out=out)
+        got = idx.preference_loss(q, c, r, off, reference=ref)
+        assert not side.query()
+    # by hand: torch.cuda.graph waits for the whole GPU first
+    with torch.cuda.stream(stream):
+        graph.capture_begin(capture_error_mode="thread_local")
+        rc = call()
+        with torch.cuda.stream(side):
+            try:
+                idx.preference_loss(q, c, r, off, reference=ref)
+            except env.hvs.HvsError as e:
+                refused.append(str(e))
+        graph.capture_end()
+    assert rc == 0 and refused and "table's stream is being captured" in refused[0]
+    assert not side.query()
+    idx.sync()
+    assert side.query()
+    for _ in range(3):
+        for t in outs:
+            t.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, (dist, ids, cnt)))
+    assert all(torch.equal(a, b) for a, b in zip(got, env.hvs.preference_loss(q, rows, c, r, off, reference=ref)))
+    del graph
+    idx.close()
