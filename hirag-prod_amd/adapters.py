@@ -179,9 +179,9 @@ class QueryAdapters:
         return cls(torch.eye(dim, dtype=t, device=dev), a, torch.zeros(n_adapters, dim, rank, dtype=t, device=dev),
                    torch.full((n_adapters,), float(scale), dtype=torch.float32, device=dev))
 
-    def _struct(self) -> HvsAdaptersStruct:
-        return HvsAdaptersStruct(self.projection.data_ptr(), self.a.data_ptr(), self.b.data_ptr(), self.scale.data_ptr(), self._code, self.d_in,
-                                 self.d_out, self.rank, self.n_adapters)
+    def _struct(self, scale=None) -> HvsAdaptersStruct:
+        return HvsAdaptersStruct(self.projection.data_ptr(), self.a.data_ptr(), self.b.data_ptr(), (self.scale if scale is None else scale).data_ptr(),
+                                 self._code, self.d_in, self.d_out, self.rank, self.n_adapters)
 
     def _workspace(self, n: int, max_ld: int, backward: int):
         size = _adapters_workspace(self._code, self.d_in, self.d_out, self.rank, self.n_adapters, n, max_ld, backward)
@@ -221,6 +221,10 @@ class QueryAdapters:
         -> ``(grad_x, grad_a, grad_b)``: grad_x [n, d_in] in the adapters' dtype (None without ``input_grad``), grad_a and
         grad_b float32 in the shapes of ``a`` and ``b``, zero for adapters no row uses.  The projection is frozen.  The same
         call gives the same bits."""
+        return self._backward(grad, x, codes, hidden, input_grad, None)
+
+    def _backward(self, grad, x, codes, hidden, input_grad, scale):
+        """``backward`` with another ``scale`` in place of the adapters' (None: theirs)."""
         x, ld_x = _rows("x", x, self.d_in, self.dtype, self.device)
         n = x.shape[0]
         grad, ld_grad = _rows("grad", grad, self.d_out, self.dtype, self.device, n)
@@ -231,8 +235,8 @@ class QueryAdapters:
         grad_a = torch.empty(self.a.shape, dtype=torch.float32, device=self.device)
         grad_b = torch.empty(self.b.shape, dtype=torch.float32, device=self.device)
         ws, ws_ptr, size = self._workspace(n, max(ld_x, ld_grad), 1)
-        check(self._lib.hvs_adapters_backward(self.device.index, _stream(self.device), ctypes.byref(self._struct()), grad.data_ptr(), ld_grad, x.data_ptr(),
-                                              ld_x, codes.data_ptr(), hidden.data_ptr(), n, grad_x.data_ptr() if input_grad and n else None, self.d_in,
+        check(self._lib.hvs_adapters_backward(self.device.index, _stream(self.device), ctypes.byref(self._struct(scale)), grad.data_ptr(), ld_grad,
+                                              x.data_ptr(), ld_x, codes.data_ptr(), hidden.data_ptr(), n, grad_x.data_ptr() if input_grad and n else None, self.d_in,
                                               grad_a.data_ptr(), grad_b.data_ptr(), ws_ptr, size))
         return grad_x, grad_a, grad_b
 
@@ -240,15 +244,28 @@ class QueryAdapters:
                            weights=None, max_norm: float = math.inf) -> FeedbackGradients:
         """The gradients of one training step on rated answers: adapt the queries ``x``, take the preference loss of their
         pairs of rows of ``table`` (an ``HvsIndex``, or a tensor of rows) against the unadapted projection ``W x`` as the
-        reference policy, go back to the adapters and clip.  Apply them with any optimizer, in place."""
+        reference policy, go back to the adapters and clip.  Apply them with any optimizer, in place.
+
+        For float16 adapters the loss's gradient is taken in float32 and goes back multiplied by a power of two that puts its
+        largest element below 2^14, which ``scale`` takes out again: the mean over many pairs has elements far below what
+        float16 holds."""
         y, hidden = self.apply(x, codes, return_hidden=True)
         reference = self.apply(x, torch.full((len(y),), -1, dtype=torch.int32, device=self.device))
+        half = self.dtype is torch.float16
+        if half:
+            y, reference = y.float(), reference.float()
         args = dict(reference=reference, beta=beta, label_smoothing=label_smoothing, weights=weights)
         if isinstance(table, torch.Tensor):
             loss, margin, grad = preference_loss(y, table, chosen, rejected, offsets, **args)
         else:
             loss, margin, grad = table.preference_loss(y, chosen, rejected, offsets, **args)
-        _, grad_a, grad_b = self.backward(grad, x, codes, hidden, input_grad=False)
+        scale = None
+        if half:
+            # (of the finite ones: a query with a code past the last adapter has none, and adds nothing; max_norm inf scales nothing)
+            largest = clip_grad_norm([grad.nan_to_num(0.0, 0.0, 0.0)], math.inf, norm_type=math.inf).clamp_(min=2.0**-100)
+            power = largest / torch.frexp(largest).mantissa  # exact: the power of two above it
+            grad, scale = (grad * (2.0**14 / power)).to(torch.float16), self.scale * (power / 2.0**14)
+        _, grad_a, grad_b = self._backward(grad, x, codes, hidden, False, scale)
         norm = clip_grad_norm([grad_a, grad_b], max_norm)
         return FeedbackGradients(loss, margin, grad_a, grad_b, norm)
 
@@ -294,7 +311,8 @@ def preference_loss(queries, rows, chosen, rejected, offsets, reference=None, be
     ``loss = -(1 - s) log sigmoid(beta margin) - s log sigmoid(-beta margin)`` with ``s = label_smoothing`` in [0, 0.5].
 
     -> ``(loss [pairs], margin [pairs], grad [nq, dim])``: grad, in the queries' dtype, is the gradient of
-    ``sum(weights * loss)``; without ``weights`` of the mean.  A pair with a negative position is left out (loss and margin
+    ``sum(weights * loss)``; without ``weights`` of the mean (whose elements fall below what float16 holds as pairs grow: take
+    float32 queries, or larger weights).  A pair with a negative position is left out (loss and margin
     0); one with a position past the last row is NaN and makes its query's gradient NaN."""
     _need_tensor("queries", queries)
     _need_tensor("rows", rows, queries.device)

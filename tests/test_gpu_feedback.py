@@ -779,3 +779,92 @@ def test_search_captured_while_a_loss_reads_the_table(env):
     assert all(torch.equal(a, b) for a, b in zip(got, env.hvs.preference_loss(q, rows, c, r, off, reference=ref)))
     del graph
     idx.close()
+
+
+def step_case(env, dtype, n=4096, pairs_each=16, dim=96, rank=4, tenants=5, seed=0):
+    torch = env.torch
+    t = getattr(torch, DT[dtype])
+    gen = torch.Generator().manual_seed(seed)
+    rnd = lambda *s: torch.randn(*s, generator=gen)
+    ad = env.hvs.QueryAdapters((torch.eye(dim) + 0.05 * rnd(dim, dim)).to(env.dev, t), (rnd(tenants, rank, dim) / dim**0.5).to(env.dev, t),
+                               (0.3 * rnd(tenants, dim, rank)).to(env.dev, t), (0.5 + torch.rand(tenants, generator=gen)).to(env.dev))
+    x = rnd(n, dim).to(env.dev, t)
+    codes = torch.randint(-1, tenants, (n,), generator=gen).to(env.dev, torch.int32)
+    rows = rnd(500, dim).to(env.dev)
+    off = torch.arange(0, n * pairs_each + 1, pairs_each, device=env.dev)
+    c, r = (torch.randint(0, 500, (n * pairs_each,), generator=gen).to(env.dev) for _ in range(2))
+    return ad, x, codes, rows, c, r, off
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("satisfied", [False, True])
+@pytest.mark.parametrize("length", [1.0, 40.0])
+def test_step_of_many_pairs(env, dtype, satisfied, length):
+    """The stack gradients of a whole step over 65 536 pairs, mean loss: against float64 from the adapted queries on.  Satisfied pairs
+    (a large margin by weights of the loss's slope) and long queries make the query gradients smaller still."""
+    torch = env.torch
+    ad, x, codes, rows, c, r, off = step_case(env, dtype)
+    x = x * length
+    y, hidden = ad.apply(x, codes, return_hidden=True)
+    ref = ad.apply(x, torch.full_like(codes, -1))
+    weights = torch.full((len(c),), 1e-3 / len(c), device=env.dev) if satisfied else None
+    got = ad.feedback_gradients(rows, x, codes, c, r, off, beta=20.0, weights=weights)
+    args = (np64(y), np64(rows), c.cpu().numpy(), r.cpu().numpy(), off.cpu().numpy(), np64(ref), 20.0, 0.0, None if weights is None else np64(weights))
+    _, _, g, _ = lo.preference(*args)
+    _, _, g_tol = lo.preference_tolerance(*args, "f32")
+    if dtype != "f32":  # one rounding to the type; fp16: below 2^-14 of a largest element of 2^13 or more, steps of 2^-24
+        g_tol += lo.HALF_STEP[dtype] * np.abs(g) + (2.0**-38 * np.abs(g).max() if dtype == "f16" else 0.0)
+    cn, x64, u64 = codes.cpu().numpy(), np64(x), np64(hidden)
+    a64, b64, s64 = np64(ad.a), np64(ad.b), np64(ad.scale)
+    for k in range(ad.n_adapters):
+        at = cn == k
+        gk, tk, xk, uk = g[at], g_tol[at], x64[at], u64[at]
+        rms = lambda p, q: np.sqrt((p * p).T @ (q * q))
+        v, v_tol = gk @ b64[k], tk @ np.abs(b64[k]) + lo.sum_error(np.sqrt((gk * gk) @ (b64[k] ** 2)), g.shape[1])
+        for what, mine, want, tol in (("grad_a", got.grad_a[k], v.T @ xk, v_tol.T @ np.abs(xk) + lo.sum_error(rms(v, xk), at.sum())),
+                                      ("grad_b", got.grad_b[k], gk.T @ uk, tk.T @ np.abs(uk) + lo.sum_error(rms(gk, uk), at.sum()))):
+            check(mine, s64[k] * want, s64[k] * tol + 4 * 2.0**-24 * np.abs(s64[k] * want), f"{what} {k}")
+
+
+def test_half_precision_step_without_a_gradient(env):
+    """Every pair left out, and a pair past the last row: zeros, and NaN, as in the other types."""
+    torch = env.torch
+    ad, x, codes, rows, c, r, off = step_case(env, "f16", n=64, pairs_each=3)
+    got = ad.feedback_gradients(rows, x, codes, torch.full_like(c, -1), r, off)
+    assert not got.grad_a.any() and not got.grad_b.any() and float(got.norm) == 0.0
+    bad = c.clone()
+    bad[int(off[int((codes >= 0).nonzero()[0])])] = len(rows)
+    got = ad.feedback_gradients(rows, x, codes, bad, r, off)
+    assert bool(got.norm.isnan()) and bool(got.loss.isnan().sum() == 1)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_step_with_a_code_past_the_last_adapter(env, dtype):
+    """Its query's pairs are NaN and add nothing to the gradients of the others."""
+    torch = env.torch
+    ad, x, codes, rows, c, r, off = step_case(env, dtype, n=64, pairs_each=3)
+    left = c.clone()
+    left[21:24] = -1  # the pairs of query 7
+    want = ad.feedback_gradients(rows, x, codes, left, r, off)
+    codes[7] = 5
+    got = ad.feedback_gradients(rows, x, codes, c, r, off)
+    assert torch.equal(got.loss.isnan().nonzero()[:, 0].cpu(), torch.tensor([21, 22, 23]))
+    assert all(torch.equal(a, b) and bool(a.isfinite().all()) for a, b in zip(got[2:], want[2:]))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_step_graph(env, dtype):
+    """A whole step captured and replayed, with other work between the replays."""
+    torch = env.torch
+    ad, x, codes, rows, c, r, off = step_case(env, dtype, n=300, pairs_each=5)
+    call = lambda: ad.feedback_gradients(rows, x, codes, c, r, off, max_norm=1e-3)
+    call()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = call()
+    for turn in range(4):
+        x.copy_(torch.randn(x.shape, generator=torch.Generator().manual_seed(turn)).to(env.dev, x.dtype))
+        want = call()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want)), turn
