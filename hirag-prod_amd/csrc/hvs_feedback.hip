@@ -23,7 +23,7 @@ struct PreferenceParams {
     float *loss, *margin;
     void *grad;
     int64_t ld_grad;
-    int64_t n_pairs;
+    int64_t n_pairs, n_queries, first_query;  // first_query: of this launch
     const void *rows;
     int64_t ld_rows, n_rows;
     int dim;
@@ -128,7 +128,7 @@ __global__ __launch_bounds__(64 * WAVES, TW == 1 && CH == 2 && WAVES == 4 ? 5 : 
     __shared__ float num[TEAMS];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int team = wave / TW, tl = (wave % TW) * 64 + lane;
-    const int64_t q = blockIdx.x;
+    const int64_t q = p.first_query + blockIdx.x;
     const int z = blockIdx.y, shares = gridDim.y;
     int64_t b0, b1, per;
     int used;
@@ -367,7 +367,7 @@ __global__ __launch_bounds__(64 * WAVES, TW == 1 && CH == 2 && WAVES == 4 ? 5 : 
     if (z == 0) {
         if (q == 0)
             for (int64_t k = tid; k < b0; k += 64 * WAVES) p.loss[k] = p.margin[k] = 0.0f;
-        if (q == (int64_t)gridDim.x - 1)
+        if (q == p.n_queries - 1)
             for (int64_t k = b1 + tid; k < p.n_pairs; k += 64 * WAVES) p.loss[k] = p.margin[k] = 0.0f;
     }
     if (used > 1 && tid == 0) {
@@ -459,18 +459,20 @@ extern "C" int hvs_preference_workspace(const hvs_preference *p, int dim, uint64
     return 0;
 }
 
+// Queries of one launch: a grid dimension ends below 2^32 threads, 2^23 blocks of 512.
+#define PREF_LAUNCH_QUERIES (1ll << 22)
 template <int QDT, int RDT, int CH, int TW, int WAVES>
-static int launch_preference(hipStream_t st, const PreferenceParams &p, int64_t nq, int shares, bool aligned) {
-    const dim3 grid((unsigned)nq, shares);
+static int launch_preference(hipStream_t st, PreferenceParams p, int64_t nq, int shares, bool aligned) {
     const size_t lds = (TW == 1 ? (size_t)(2 + WAVES) * CH * 512 : (size_t)p.dim) * 4;
-    if (aligned) {
-        HVS_TRY((learn_allow_lds<preference_kernel<QDT, RDT, CH, TW, WAVES, true>>((int)lds)));
-        preference_kernel<QDT, RDT, CH, TW, WAVES, true><<<grid, 64 * WAVES, lds, st>>>(p);
-    } else {
-        HVS_TRY((learn_allow_lds<preference_kernel<QDT, RDT, CH, TW, WAVES, false>>((int)lds)));
-        preference_kernel<QDT, RDT, CH, TW, WAVES, false><<<grid, 64 * WAVES, lds, st>>>(p);
+    if (aligned) HVS_TRY((learn_allow_lds<preference_kernel<QDT, RDT, CH, TW, WAVES, true>>((int)lds)));
+    else HVS_TRY((learn_allow_lds<preference_kernel<QDT, RDT, CH, TW, WAVES, false>>((int)lds)));
+    for (p.first_query = 0; p.first_query < nq; p.first_query += PREF_LAUNCH_QUERIES) {
+        const int64_t left = nq - p.first_query;
+        const dim3 grid((unsigned)(left < PREF_LAUNCH_QUERIES ? left : PREF_LAUNCH_QUERIES), shares);
+        if (aligned) preference_kernel<QDT, RDT, CH, TW, WAVES, true><<<grid, 64 * WAVES, lds, st>>>(p);
+        else preference_kernel<QDT, RDT, CH, TW, WAVES, false><<<grid, 64 * WAVES, lds, st>>>(p);
+        HVS_HIP(hipGetLastError());
     }
-    HVS_HIP(hipGetLastError());
     return 0;
 }
 
@@ -527,7 +529,7 @@ static int preference_core(hipStream_t st, const hvs_preference *p, const void *
     PreferenceParams k = {};
     k.y = p->queries, k.ref = p->reference, k.ld_y = p->ld_queries, k.ld_ref = p->ld_reference;
     k.offsets = p->offsets, k.chosen = p->chosen, k.rejected = p->rejected, k.weights = p->weights;
-    k.loss = p->loss, k.margin = p->margin, k.grad = p->grad, k.ld_grad = p->ld_grad, k.n_pairs = p->n_pairs;
+    k.loss = p->loss, k.margin = p->margin, k.grad = p->grad, k.ld_grad = p->ld_grad, k.n_pairs = p->n_pairs, k.n_queries = p->n_queries;
     k.rows = rows, k.ld_rows = ld_rows, k.n_rows = n_rows, k.dim = dim;
     k.beta = p->beta, k.smoothing = p->label_smoothing, k.default_weight = p->n_pairs > 0 ? (float)(1.0 / (double)p->n_pairs) : 0.0f;
     k.per_block = plan.per_block;

@@ -868,3 +868,26 @@ def test_step_graph(env, dtype):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(outs, want)), turn
+
+
+@pytest.mark.parametrize("dim", [1, 2])
+def test_more_queries_than_a_launch_takes(env, dim):
+    """2^24 + 7 queries, most of them without pairs, and pairs of no query behind the last one."""
+    torch = env.torch
+    nq = 2**24 + 7
+    at = torch.tensor([0, 1, 2**22 - 1, 2**22, 2**22 + 1, 2**23, 2**24 - 1, 2**24, nq - 1], device=env.dev)
+    counts = torch.zeros(nq, dtype=torch.int64, device=env.dev)
+    counts[at] = torch.tensor([3, 0, 2, 5, 1, 4, 2, 1, 3], device=env.dev)
+    off = torch.zeros(nq + 1, dtype=torch.int64, device=env.dev)
+    off[1:] = counts.cumsum(0)
+    _, _, rows, c, r, few_off = make(env, "f32", "f32", len(at), dim, 40, counts[at].cpu(), seed=dim)
+    q = torch.randn(nq, dim, device=env.dev)
+    ref = q + 0.1
+    w = torch.rand(len(c), device=env.dev)
+    more = torch.full((5,), 2, device=env.dev)
+    loss, margin, grad = env.hvs.preference_loss(q, rows, torch.cat([c, more]), torch.cat([r, more + 1]), off, reference=ref, beta=5.0,
+                                                 weights=torch.cat([w, torch.ones(5, device=env.dev)]))
+    check_by_terms(q[at], ref[at], rows, c, r, few_off, (loss[:-5], margin[:-5], grad[at]), "f32", 5.0, 0.0, w)
+    assert not loss[-5:].any() and not margin[-5:].any()
+    grad[at] = 0
+    assert not grad.any()
