@@ -948,7 +948,9 @@ struct TransposeJobs {
 };
 // All transposed weights of a backward pass in one launch, a block per tile, jobs one after the other; the first group_blocks
 // blocks group the rows meanwhile, where they count them by themselves (a launch of its own took 4 us more at 96 rows).
-template <typename E> __global__ __launch_bounds__(GROUP_CHUNK) void layout_kernel(TransposeJobs jobs, GroupParams group, int group_blocks) {
+// first: the launch's first tile (a grid dimension ends below 2^32 threads: LAYOUT_TILES tiles a launch, 2^31 elements).
+#define LAYOUT_TILES (1ll << 18)
+template <typename E> __global__ __launch_bounds__(GROUP_CHUNK) void layout_kernel(TransposeJobs jobs, int64_t first, GroupParams group, int group_blocks) {
     extern __shared__ uint32_t lds[];
     if ((int)blockIdx.x < group_blocks) {
         group_place<true>(group, lds);
@@ -956,7 +958,7 @@ template <typename E> __global__ __launch_bounds__(GROUP_CHUNK) void layout_kern
     }
     E *tile = reinterpret_cast<E *>(lds);  // rows of 2^log_c + 1 elements
     constexpr int PER = (1 << TILE_LOG) / GROUP_CHUNK;
-    int64_t at = (int64_t)blockIdx.x - group_blocks;
+    int64_t at = first + blockIdx.x - group_blocks;
     int which = 0;
     while (which < 2 && at >= jobs.job[which].blocks) at -= jobs.job[which++].blocks;
     const TransposeJob &t = jobs.job[which];
@@ -1481,9 +1483,12 @@ static int run_backward(hipStream_t st, const hvs_adapters *ad, const void *grad
     const size_t tile_lds = ((1 << TILE_LOG) + (1 << (TILE_LOG - TILE_LOG_NARROW))) * sizeof(typename Elem<DT>::type), group_lds = (size_t)(ad->n_adapters + 2) * 8;
     const size_t lds = beside && group_lds > tile_lds ? group_lds : tile_lds;
     HVS_TRY((learn_allow_lds<layout_kernel<typename Elem<DT>::type>>((int)lds)));
-    HVS_REQUIRE(blocks <= 0x7FFFFFFF - GROUP_SELF, "hvs_adapters_backward: %d adapters of %d x %d x %d are too many for one launch", ad->n_adapters, ad->rank, ad->d_in, ad->d_out);
-    layout_kernel<typename Elem<DT>::type><<<(unsigned)(blocks + beside), GROUP_CHUNK, lds, st>>>(jobs, first, beside);
-    HVS_HIP(hipGetLastError());
+    for (int64_t at = 0; at < blocks; at += LAYOUT_TILES) {
+        const int64_t tiles = blocks - at < LAYOUT_TILES ? blocks - at : LAYOUT_TILES;
+        const int grouping = at == 0 ? beside : 0;
+        layout_kernel<typename Elem<DT>::type><<<(unsigned)(tiles + grouping), GROUP_CHUNK, lds, st>>>(jobs, at, first, grouping);
+        HVS_HIP(hipGetLastError());
+    }
     for (int64_t r0 = 0; r0 < n; r0 += nc) {
         const int rows = (int)(n - r0 < nc ? n - r0 : nc);
         if (r0 > 0 || !beside) HVS_TRY(launch_group(st, group_params(codes + r0, rows, ad->n_adapters, ws)));

@@ -586,3 +586,29 @@ def test_infinite_rows_at_any_rank(env, dtype, n, rank):
     for got, clean in ((y2, y), (hidden2, hidden), (dx2, dx)):
         assert bool((got[bad] == torch.inf).all())
         assert torch.equal(got[others], clean[others])
+
+
+@pytest.mark.parametrize("d_in,d_out,rank", [(16384, 64, 33), (64, 16384, 65)])
+def test_transposed_weights_past_one_launch(env, d_in, d_out, rank):
+    """Stacks whose transposed copies take more tiles than a launch has (2^18): 256 for each of 1030 adapters."""
+    torch = env.torch
+    n, s = 40, 1030
+    gen = torch.Generator(device=env.dev).manual_seed(1)
+    rnd = lambda *shape: torch.randn(*shape, generator=gen, device=env.dev, dtype=torch.float32)
+    used = torch.tensor([0, 1, 500, 1022, 1023, 1024, 1028, 1029], device=env.dev)
+    w = (rnd(d_out, d_in) / d_in**0.5).bfloat16()
+    a, b = torch.zeros(s, rank, d_in, dtype=torch.bfloat16, device=env.dev), torch.zeros(s, d_out, rank, dtype=torch.bfloat16, device=env.dev)
+    a[used], b[used] = (rnd(len(used), rank, d_in) / d_in**0.5).bfloat16(), (rnd(len(used), d_out, rank) / rank**0.5).bfloat16()
+    scale = 0.5 + torch.rand(s, generator=gen, device=env.dev)
+    place = torch.arange(n, device=env.dev) % len(used)
+    codes, x, g = used[place].to(torch.int32), rnd(n, d_in).bfloat16(), rnd(n, d_out).bfloat16()
+    ad = env.hvs.QueryAdapters(w, a, b, scale)
+    _, hidden = ad.apply(x, codes, return_hidden=True)
+    dx, da, db = ad.backward(g, x, codes, hidden)
+    # the same rows over the used adapters alone, which fit one launch
+    small = env.hvs.QueryAdapters(w, a[used].contiguous(), b[used].contiguous(), scale[used].contiguous())
+    want = small.backward(g, x, place.to(torch.int32), hidden)
+    assert torch.equal(dx, want[0]) and torch.equal(da[used], want[1]) and torch.equal(db[used], want[2])
+    check_backward(small, g, x, place.to(torch.int32), hidden, "bf16", *want)
+    da[used], db[used] = 0, 0
+    assert not da.any() and not db.any()
