@@ -136,7 +136,8 @@ class QueryAdapters:
 
     ``projection`` [d_out, d_in], ``a`` [adapters, rank, d_in], ``b`` [adapters, d_out, rank]: contiguous tensors of one
     dtype (float32, float16 or bfloat16) on one GPU; ``scale`` [adapters] float32.  The object keeps the tensors it is
-    given: a training loop that changes them in place changes the adapters.  For float16 and bfloat16, sums are held in fp32
+    given: a training loop that changes them in place changes the adapters, and another tensor like the old one may take its
+    place.  For float16 and bfloat16, sums are held in fp32
     and every output is rounded once; ``A[c] x`` is kept in fp32 on its way into ``B[c]``.
     """
 
@@ -162,9 +163,11 @@ class QueryAdapters:
                               ("rank", self.rank, _lib.HVS_MAX_ADAPTER_RANK), ("adapters", self.n_adapters, _lib.HVS_MAX_ADAPTERS)):
             if not 1 <= v <= most:
                 raise ValueError(f"{what} must be in [1, {most}], got {v}")
-        self.projection, self.a, self.b, self.scale = projection, a, b, scale
         self.device, self.dtype = device, projection.dtype
         self._lib = load_library()
+        self._like = dict(projection=projection.shape, a=a.shape, b=b.shape, scale=scale.shape)
+        self.projection, self.a, self.b, self.scale = projection, a, b, scale
+        self._hold()
 
     @classmethod
     def create(cls, dim: int, n_adapters: int, rank: int = 16, dtype: str = "f32", device: int = 0, scale: float = 1.0, seed: int = 0) -> "QueryAdapters":
@@ -179,9 +182,35 @@ class QueryAdapters:
         return cls(torch.eye(dim, dtype=t, device=dev), a, torch.zeros(n_adapters, dim, rank, dtype=t, device=dev),
                    torch.full((n_adapters,), float(scale), dtype=torch.float32, device=dev))
 
+    def __setattr__(self, name, value):
+        """Another weight takes the place of the old one if it is like it."""
+        if name in self.__dict__.get("_like", ()):
+            self._check_weight(name, value)
+        super().__setattr__(name, value)
+
+    def _check_weight(self, name: str, t) -> None:
+        dtype = torch.float32 if name == "scale" else self.dtype
+        _need_tensor(name, t, self.device)
+        if t.shape != self._like[name] or t.dtype != dtype or not t.is_contiguous():
+            raise ValueError(f"{name} must stay a contiguous {tuple(self._like[name])} tensor of {dtype}, got {tuple(t.shape)} of {t.dtype}; "
+                             "make another QueryAdapters for other weights")
+
+    def _hold(self) -> None:
+        """Checks the weights and holds on to their memory, so that what the kernels read is there whatever becomes of the tensors."""
+        weights = self.projection, self.a, self.b, self.scale
+        for name, t in zip(self._like, weights):
+            self._check_weight(name, t)
+        where = tuple(t.data_ptr() for t in weights)
+        self._held = where, HvsAdaptersStruct(*where, self._code, self.d_in, self.d_out, self.rank, self.n_adapters), [t.detach() for t in weights]
+
     def _struct(self, scale=None) -> HvsAdaptersStruct:
-        return HvsAdaptersStruct(self.projection.data_ptr(), self.a.data_ptr(), self.b.data_ptr(), (self.scale if scale is None else scale).data_ptr(),
-                                 self._code, self.d_in, self.d_out, self.rank, self.n_adapters)
+        """The weights as the library takes them."""
+        if (self.projection.data_ptr(), self.a.data_ptr(), self.b.data_ptr(), self.scale.data_ptr()) != self._held[0]:
+            self._hold()  # other memory: a weight was replaced (``ad.a = ...``, ``ad.a.data = ...``)
+        where, struct, _ = self._held
+        if scale is None:
+            return struct
+        return HvsAdaptersStruct(*where[:3], scale.data_ptr(), self._code, self.d_in, self.d_out, self.rank, self.n_adapters)
 
     def _workspace(self, n: int, max_ld: int, backward: int):
         size = _adapters_workspace(self._code, self.d_in, self.d_out, self.rank, self.n_adapters, n, max_ld, backward)

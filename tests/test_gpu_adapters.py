@@ -612,3 +612,34 @@ def test_transposed_weights_past_one_launch(env, d_in, d_out, rank):
     check_backward(small, g, x, place.to(torch.int32), hidden, "bf16", *want)
     da[used], db[used] = 0, 0
     assert not da.any() and not db.any()
+
+
+@pytest.mark.parametrize("name", ["projection", "a", "b", "scale"])
+def test_weights_put_in_anothers_place(env, name):
+    """A tensor like the old one takes its place; one that the kernels would read wrongly, or past its end, is refused."""
+    torch = env.torch
+    ad, x, codes, gen = make(env, "f32", 30, 24, 24, 24, 24)
+    _, hidden = ad.apply(x, codes, return_hidden=True)
+    g = torch.randn(30, 24, generator=gen).to(env.dev)
+    old = getattr(ad, name)
+    setattr(ad, name, old * 2)
+    check_apply(env, ad, x, codes, "f32")
+    old2 = getattr(ad, name)
+    old2.data = old2.data * 0.5
+    assert torch.equal(ad.apply(x, codes), env.hvs.QueryAdapters(*[old if k == name else getattr(ad, k) for k in ("projection", "a", "b", "scale")]).apply(x, codes))
+    bad = [old.half(), old.bfloat16(), old[:-1], old.cpu(), torch.cat([old, old]), old.double(), None]
+    if old.dim() > 1:
+        bad += [old.transpose(-1, -2), old.reshape(-1)]
+    want = ad.apply(x, codes)
+    for t in bad:
+        with pytest.raises(ValueError):
+            setattr(ad, name, t)
+        assert torch.equal(ad.apply(x, codes), want)
+    for t in (old.half(), old[:-1].clone(), old.expand(2, *old.shape).reshape(-1)):
+        old2.data = t
+        with pytest.raises(ValueError, match="must stay"):
+            ad.apply(x, codes)
+        with pytest.raises(ValueError, match="must stay"):
+            ad.backward(g, x, codes, hidden)
+    old2.data = old.clone()
+    assert torch.equal(ad.apply(x, codes), want)
