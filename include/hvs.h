@@ -550,7 +550,9 @@ int hvs_index_preference_loss(hvs_index *idx, void *stream, const hvs_preference
  * absolute value with infinity_norm; out = data * min(1, max_norm / (norm + 1e-6)), rounded once.  The sum of squares is
  * held in double precision.  out may be data itself (in place) or separate memory of the same type; tensors may differ in
  * type; what is written shares no memory with any other tensor of the call.  tensors is a HOST array, read before the call
- * returns; norm (device float) receives the norm before clipping.  A NaN anywhere makes the norm and every output NaN; an infinite norm makes the factor 0.
+ * returns; norm (device float) receives the norm before clipping.  A NaN anywhere makes the norm and every output NaN; an
+ * infinite norm makes the factor 0 (infinite elements NaN).  max_norm infinite: the factor is 1, also for an infinite norm,
+ * and outputs are the data unless the norm is NaN.
  */
 typedef struct hvs_tensor {
     const void *data;

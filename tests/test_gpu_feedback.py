@@ -891,3 +891,18 @@ def test_more_queries_than_a_launch_takes(env, dim):
     assert not loss[-5:].any() and not margin[-5:].any()
     grad[at] = 0
     assert not grad.any()
+
+
+@pytest.mark.parametrize("n", [100, 70000])
+def test_clip_without_a_limit_and_an_infinite_norm(env, n):
+    """max_norm inf: the data as they are, also next to infinities."""
+    torch = env.torch
+    for infinity in (2.0, math.inf):
+        g = torch.randn(n, device=env.dev)
+        g[3], g[4] = torch.inf, -torch.inf
+        out = [torch.zeros_like(g)]
+        norm = env.hvs.clip_grad_norm([g], math.inf, norm_type=infinity, out=out)
+        assert float(norm) == math.inf and torch.equal(out[0], g)
+        same = g.clone()
+        env.hvs.clip_grad_norm([same], math.inf, norm_type=infinity)
+        assert torch.equal(same, g)
