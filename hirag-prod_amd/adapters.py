@@ -223,7 +223,7 @@ class QueryAdapters:
         A torch tensor of the adapters' dtype gives a torch tensor (``out``, when given); with ``return_hidden`` also the
         float32 [n, rank] values ``A[c] x`` that ``backward`` takes.  A numpy array (float32, from an embedding service)
         gives a float32 numpy array.  A code past the last adapter makes its row NaN.  ``out`` must not overlap ``x``
-        (columns of one wide tensor do not)."""
+        (columns of one wide tensor do not) or the weights."""
         if not isinstance(x, torch.Tensor):
             if out is not None or return_hidden:
                 raise ValueError("out and return_hidden need device tensors")

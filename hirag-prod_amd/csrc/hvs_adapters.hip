@@ -1408,6 +1408,17 @@ static int check_weights(const char *who, const hvs_adapters *ad) {
     return 0;
 }
 
+// what is written (rows of `width` elements) is no part of the weights that are read meanwhile
+static int check_apart_from_weights(const char *who, const char *what, const hvs_adapters *ad, const void *p, int64_t rows, int64_t ld, int width) {
+    const int64_t es = hvs_elem_size(ad->dtype), ranks = (int64_t)ad->n_adapters * ad->rank;
+    const struct {
+        const void *p;
+        int64_t bytes;
+    } weights[] = {{ad->projection, (int64_t)ad->d_out * ad->d_in * es}, {ad->a, ranks * ad->d_in * es}, {ad->b, ranks * ad->d_out * es}, {ad->scale, (int64_t)ad->n_adapters * 4}};
+    for (const auto &w : weights) HVS_REQUIRE(!learn_overlap(p, rows, ld * es, width * es, w.p, 1, 0, w.bytes), "%s: %s overlaps the weights", who, what);
+    return 0;
+}
+
 extern "C" int hvs_adapters_apply(int device_id, void *stream, const hvs_adapters *ad, const void *x, int64_t ld_x, const int32_t *codes, int64_t n,
                                   void *out, int64_t ld_out, float *hidden, void *workspace, uint64_t workspace_bytes) {
     const char *who = "hvs_adapters_apply";
@@ -1422,6 +1433,7 @@ extern "C" int hvs_adapters_apply(int device_id, void *stream, const hvs_adapter
     HVS_REQUIRE(((uintptr_t)codes | (uintptr_t)hidden) % 4 == 0, "%s: codes or hidden is not aligned to its elements", who);
     HVS_REQUIRE(!learn_overlap(x, n, ld_x * es, (int64_t)ad->d_in * es, out, n, ld_out * es, (int64_t)ad->d_out * es), "%s: out overlaps x", who);
     const int64_t max_ld = ld_x > ld_out ? ld_x : ld_out;
+    HVS_TRY(check_apart_from_weights(who, "out", ad, out, n, ld_out, ad->d_out));
     HVS_TRY(check_workspace(who, ad, n, max_ld, 0, workspace, workspace_bytes));
     DeviceGuard guard(device_id);
     HVS_HIP(guard.status);
@@ -1539,6 +1551,7 @@ extern "C" int hvs_adapters_backward(int device_id, void *stream, const hvs_adap
         HVS_REQUIRE(!learn_overlap(grad, n, ld_grad * es, (int64_t)ad->d_out * es, grad_x, n, ld_gx * es, (int64_t)ad->d_in * es) &&
                         !learn_overlap(x, n, ld_x * es, (int64_t)ad->d_in * es, grad_x, n, ld_gx * es, (int64_t)ad->d_in * es),
                     "%s: grad_x overlaps an input", who);
+        HVS_TRY(check_apart_from_weights(who, "grad_x", ad, grad_x, n, ld_gx, ad->d_in));
         max_ld = max_ld > ld_gx ? max_ld : ld_gx;
     }
     HVS_TRY(check_workspace(who, ad, n, max_ld, 1, workspace, workspace_bytes));

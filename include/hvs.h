@@ -485,6 +485,7 @@ int hvs_adapters_workspace(const hvs_adapters *ad, int64_t n, int64_t max_ld, in
  * [n, d_out] (row pitch ld_out), of the weights' dtype, rounded once from fp32 sums.  A code < 0 means no adapter (W x
  * alone); a code >= n_adapters makes the row NaN.  hidden: float [n, rank] or NULL, receives A[c] x (0 without adapter),
  * which hvs_adapters_backward takes.  out must not overlap x (columns of one wide tensor, at one pitch, do not overlap).
+ * What is written shares no memory with the weights.
  */
 int hvs_adapters_apply(int device_id, void *stream, const hvs_adapters *ad, const void *x, int64_t ld_x,
                        const int32_t *codes, int64_t n, void *out, int64_t ld_out, float *hidden,

@@ -344,3 +344,19 @@ def test_margin_tolerance_refuses_plain_forms(move, t, dim, counts):
     want, tol = lo.preference(*args)[1], lo.preference_tolerance(*args, "f32")[1]
     kernel, cosines, units = (np.abs(m - want)[apart] / tol[apart] for m in margin_forms(q[own], ref[own], rows[c], rows[r]))
     assert kernel.max() < 0.25 and cosines.max() > 2 and units.max() > 2, (kernel.max(), cosines.max(), units.max())
+
+
+@pytest.mark.parametrize("weight", ["projection", "a", "b", "scale"])
+def test_what_is_written_is_no_weight(weight):
+    import hirag_prod_amd as hvs
+
+    lib = hvs.load_library()
+    size = dict(projection=32 * 24 * 4, a=3 * 4 * 32 * 4, b=3 * 24 * 4 * 4, scale=12)[weight]
+    ad = adapters(**{weight: R})
+    apply = lambda out: lib.hvs_adapters_apply(0, None, ctypes.byref(ad), 2 * R, 32, P, 5, out, 24, None, None, 0)
+    back = lambda gx: lib.hvs_adapters_backward(0, None, ctypes.byref(ad), 2 * R, 24, 3 * R, 32, P, P, 5, gx, 32, Q, Q, None, 0)
+    for call, row in ((apply, 24 * 4), (back, 32 * 4)):
+        for at in (R, R + size - 4, R - 5 * row + 4):
+            refused(call(at), "overlaps the weights")
+        for at in (R + size, R - 5 * row):  # next to it; only the workspace is missing
+            refused(call(at), "workspace")
