@@ -79,7 +79,8 @@ def _numbers(name: str, values, n: Optional[int], dtype, device):
             and (n is None or values.shape[0] == n)):
         return values
     if not isinstance(values, torch.Tensor):
-        values = torch.as_tensor(np.ascontiguousarray(values), device=device)
+        values = np.ascontiguousarray(values)
+        values = torch.as_tensor(values if values.size else values.astype(np.int64), device=device)  # (an empty list has no type)
     _need_tensor(name, values, device)
     if values.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"{name} must be whole numbers (int32 or int64), got {values.dtype}")

@@ -906,3 +906,25 @@ def test_clip_without_a_limit_and_an_infinite_norm(env, n):
         same = g.clone()
         env.hvs.clip_grad_norm([same], math.inf, norm_type=infinity)
         assert torch.equal(same, g)
+
+
+def test_lists_and_arrays(env):
+    """Codes, positions and offsets as Python lists and numpy arrays, empty ones among them; a step without queries."""
+    torch, hvs = env.torch, env.hvs
+    q, ref, rows, c, r, off = make(env, "f32", "f32", 4, 16, 10, [1, 2, 0, 1])
+    want = hvs.preference_loss(q, rows, c, r, off, reference=ref)
+    for kind in (lambda t: t.tolist(), lambda t: t.cpu().numpy(), lambda t: t.int().cpu().numpy()):
+        got = hvs.preference_loss(q, rows, kind(c), kind(r), kind(off), reference=ref)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    loss, margin, grad = hvs.preference_loss(q, rows, [], [], [0] * 5)
+    assert len(loss) == 0 and len(margin) == 0 and grad.shape == (4, 16) and not grad.any()
+    for dtype in DT:
+        ad, x, _, table, _, _, _ = step_case(env, dtype, n=3, pairs_each=1)
+        assert ad.apply(x[:0], []).shape == (0, 96)
+        step = ad.feedback_gradients(table, x[:0], [], [], [], [0])
+        assert len(step.loss) == 0 and not step.grad_a.any() and not step.grad_b.any() and float(step.norm) == 0.0
+        step = ad.feedback_gradients(table, x, [0, -1, 2], [], [], [0, 0, 0, 0])
+        assert len(step.loss) == 0 and not step.grad_a.any() and not step.grad_b.any()
+    for bad in ([0.5], np.array([1.0]), ["1"]):
+        with pytest.raises((ValueError, TypeError)):
+            hvs.preference_loss(q, rows, bad, bad, [0, 1, 1, 1, 1])
