@@ -139,7 +139,9 @@ class QueryAdapters:
     dtype (float32, float16 or bfloat16) on one GPU; ``scale`` [adapters] float32.  The object keeps the tensors it is
     given: a training loop that changes them in place changes the adapters, and another tensor like the old one may take its
     place.  For float16 and bfloat16, sums are held in fp32
-    and every output is rounded once; ``A[c] x`` is kept in fp32 on its way into ``B[c]``.
+    and every output is rounded once; ``A[c] x`` is kept in fp32 on its way into ``B[c]``.  An infinite element of a row stays
+    with that row, a weight that is not finite with its tenant's rows (an infinite ``B`` of a 16-bit type may give NaN where
+    the formula gives an infinity: it meets ``A[c] x`` in two parts).
     """
 
     def __init__(self, projection, a, b, scale):
@@ -223,7 +225,7 @@ class QueryAdapters:
 
         A torch tensor of the adapters' dtype gives a torch tensor (``out``, when given); with ``return_hidden`` also the
         float32 [n, rank] values ``A[c] x`` that ``backward`` takes.  A numpy array (float32, from an embedding service)
-        gives a float32 numpy array.  A code past the last adapter makes its row NaN.  ``out`` must not overlap ``x``
+        gives a float32 numpy array, rounded to the adapters' dtype on its way in.  A code past the last adapter makes its row NaN.  ``out`` must not overlap ``x``
         (columns of one wide tensor do not) or the weights."""
         if not isinstance(x, torch.Tensor):
             if out is not None or return_hidden:
@@ -335,7 +337,8 @@ def preference_loss(queries, rows, chosen, rejected, offsets, reference=None, be
     """Preference loss of pairs of rows and its gradient for the queries, in one pass over the rows.
 
     ``queries`` [nq, dim]; ``rows`` [n, dim]; pairs ``offsets[i] .. offsets[i + 1]`` (``offsets`` [nq + 1], ascending)
-    belong to query i, and pairs outside all of them are left out; ``chosen`` / ``rejected`` are row positions.  With a policy that picks rows by softmax(beta cos(query, row)),
+    belong to query i, and pairs outside all of them are left out; ``chosen`` / ``rejected`` are row positions.  With a
+    policy that picks rows by softmax(beta cos(query, row)),
     ``margin = (cos(q, chosen) - cos(q, rejected)) - (cos(q0, chosen) - cos(q0, rejected))`` for the reference policy's
     queries q0 (``reference`` [nq, dim]; None: without that term) is the paired log ratio over beta, and
     ``loss = -(1 - s) log sigmoid(beta margin) - s log sigmoid(-beta margin)`` with ``s = label_smoothing`` in [0, 0.5].

@@ -808,7 +808,8 @@ class HipVectorStore(BaseVDB):
         search.  ``codes``: (workspace id, knowledge base id) -> adapter number; pairs that are not named go through the
         shared projection alone.  The stored rows stay as they are, so this may change at any time; a query uses the
         adapters that are set when its embedding arrives.  Queries run on torch's default stream: weights that a training loop
-        changes in place should be changed there too, or be swapped for another object.  Not part of ``save``: the weights
+        changes in place should be changed there too, or be swapped for another object.  Adapters of float16 or bfloat16
+        round every embedding to that type on its way, also of pairs that are not named.  Not part of ``save``: the weights
         are the caller's."""
         codes = {(str(w), str(k)): int(c) for (w, k), c in (codes or {}).items()}
         if adapters is not None:

@@ -511,8 +511,9 @@ int hvs_adapters_backward(int device_id, void *stream, const hvs_adapters *ad, c
  *     loss   = -(1 - label_smoothing) log sigmoid(beta margin) - label_smoothing log sigmoid(-beta margin)
  * q0 = the reference policy's query (the embedding before adaptation); reference NULL: its term is 0.  Pairs
  * offsets[i] .. offsets[i + 1] - 1 belong to query i (int64 [n_queries + 1], ascending within 0 .. n_pairs; a query may
- * have none, and pairs before offsets[0] and from offsets[n_queries] on are left out).  chosen / rejected: int64 row positions.  A pair with a negative position is left out (loss and margin 0, no
- * gradient); one with a position past the last row gets a NaN loss and margin and makes its query's gradient NaN.
+ * have none, and pairs before offsets[0] and from offsets[n_queries] on are left out).  chosen / rejected: int64 row
+ * positions.  A pair with a negative position is left out (loss and margin 0, no gradient); one with a position past the
+ * last row gets a NaN loss and margin and makes its query's gradient NaN.
  * grad [n_queries, dim], the queries' dtype: gradient of sum_p weights[p] loss[p]; weights NULL = 1 / n_pairs each (the
  * mean).  A query of norm 0 gets gradient 0.  A norm below 2^-126, whose inverse is no float, counts as 0; norms up to 2^100 keep
  * full precision.  Sums run in a fixed order.

@@ -928,3 +928,64 @@ def test_lists_and_arrays(env):
     for bad in ([0.5], np.array([1.0]), ["1"]):
         with pytest.raises((ValueError, TypeError)):
             hvs.preference_loss(q, rows, bad, bad, [0, 1, 1, 1, 1])
+
+
+def test_training_on_what_a_store_found(env):
+    """From a store's hits and keys to a step and back: rows by key, whatever order its table is in, positions among those."""
+    import asyncio
+
+    import hirag_prod_amd.store as st
+    from tests import store_cases
+
+    torch = env.torch
+    dim, tenants = store_cases.DIM, [("ws1", "kb1"), ("ws1", "kb2"), ("ws2", "kb1")]
+    ad = env.hvs.QueryAdapters.create(dim, n_adapters=3, rank=4, dtype="f32", seed=3)
+    s = st.HipVectorStore.create(store_cases.make_embedding_func(), vector_type="vector")
+
+    async def scenario():
+        for i in range(30):  # interleaved, so that a partition moves every row
+            for w, k in tenants:
+                p = store_cases.chunk_props(i, w, k)
+                await s.upsert_texts([p["text"]], [p], "Chunks")
+        await s.partition("Chunks")
+        s.set_query_adapters(ad, {t: c for c, t in enumerate(tenants)})
+        x, codes, pairs, offsets = [], [], [], [0]
+        found, place = [], {}
+        for c, (w, k) in enumerate(tenants):
+            for i in range(4):
+                hits = [h["documentKey"] for h in await s.query(f"question {i}", w, k, "Chunks", topk=6, topn=6, distance_threshold=3.0)]
+                x.append(store_cases.embed_text(f"question {i}"))
+                codes.append(c)
+                pairs += [(hits[3], h) for h in hits if h != hits[3]]  # the fourth hit was the useful one
+                offsets.append(len(pairs))
+            keys = sorted({h for pair in pairs[offsets[4 * c] :] for h in pair})
+            for r in await s.query_by_keys(keys, w, k, "Chunks", columns_to_select=["documentKey", "vector"]):
+                place[r["documentKey"]] = len(found)
+                found.append(r["vector"])
+        rows = torch.tensor(found, device=env.dev)
+        x = torch.tensor(np.array(x), dtype=torch.float32, device=env.dev)
+        chosen, rejected = ([place[p[side]] for p in pairs] for side in (0, 1))
+        for key, at in place.items():
+            _, w, k, i = key.split("-")
+            assert np.array_equal(np64(rows[at]), store_cases.embed_text(f"text {w} {k} {i}").astype(np.float32).astype(np.float64))
+        step = ad.feedback_gradients(rows, x, codes, chosen, rejected, offsets, beta=5.0)
+        cn, off = np.array(codes), np.array(offsets)
+        y, _, u, _ = lo.adapters_apply(np64(x), cn, *(np64(t) for t in (ad.projection, ad.a, ad.b, ad.scale)))
+        grad = lo.preference(y, np64(rows), np.array(chosen), np.array(rejected), off, np64(x), 5.0, 0.0)[2]
+        _, _, want, _ = lo.adapters_backward(grad, np64(x), cn, u, *(np64(t) for t in (ad.projection, ad.a, ad.b, ad.scale)))
+        assert not step.grad_a.any()  # B is zero at the start
+        # fp32 sums over 4 queries of 5 pairs; sizes of the terms are at most the norms along the way
+        assert np.abs(np64(step.grad_b) - want).max() <= 1e-5 * np.linalg.norm(grad, axis=1).sum() * np.abs(u).max()
+        with torch.no_grad():
+            ad.b -= 2.0 * step.grad_b
+        for (w, k), c in zip(tenants, range(3)):
+            q = store_cases.embed_text("question 1").astype(np.float32).astype(np.float64)
+            moved = q + np64(ad.b[c]) @ (np64(ad.a[c]) @ q)
+            texts = np.stack([store_cases.embed_text(f"text {w} {k} {j}") for j in range(30)])
+            dist = 1 - (texts @ moved) / np.linalg.norm(texts, axis=1) / np.linalg.norm(moved)
+            order = np.argsort(dist, kind="stable")[:6]
+            hits = await s.query("question 1", w, k, "Chunks", topk=6, topn=6, distance_threshold=3.0)
+            store_cases.same_hits([h["documentKey"] for h in hits], [f"chunk-{w}-{k}-{j}" for j in order], dist[order], [h["distance"] for h in hits])
+
+    asyncio.run(scenario())
+    s.close()
