@@ -119,8 +119,8 @@ def preference_tolerance(queries, rows, chosen, rejected, offsets, reference, be
     * an element of e: 2 roundings of the unit rows' elements; independent of each other, as are those of d (4 of its size) and, below
       both, 2^-45 of the unit queries (their norms are held in double precision)
     * a sum: ``sum_error`` of the root of its squared terms
-    * the slope: 12 roundings (smoothing, weight, exponential, its quotient, the products), one of h in its exponential, and its
-      derivative times the margin's error
+    * the slope: 12 roundings (smoothing, weight, exponential, its quotient, the products), one of h in its exponential, its
+      derivative times the margin's error, and beta 2^-127: past h = 88.7 the exponential is infinite in fp32, and sigma(-h) < 2^-127 is 0
     * the sum over the pairs: every addition rounds by 2^-24 of what is added up, at most the sum of sizes; two additions a pair, and
       20 more in joining teams and blocks and in the last line
     """
@@ -160,7 +160,7 @@ def preference_tolerance(queries, rows, chosen, rejected, offsets, reference, be
         if y_len[q, 0] == 0:
             continue
         g = weights[at] * np.abs(slope)
-        dg = weights[at] * (beta * beta * up * down * (dm + step * np.abs(m)) + step * np.abs(h) * size + 12 * step * size)
+        dg = weights[at] * (beta * beta * up * down * (dm + step * np.abs(m)) + step * np.abs(h) * size + 12 * step * size + beta * 2.0**-127)
         pull = e - s[:, None] * y
         grows = (2 * len(at) + 20) * step
         error = (dg[:, None] * np.abs(pull)).sum(0)
