@@ -295,8 +295,9 @@ class QueryAdapters:
         if half:
             # (of the finite ones: a query with a code past the last adapter has none, and adds nothing; max_norm inf scales nothing)
             largest = clip_grad_norm([grad.nan_to_num(0.0, 0.0, 0.0)], math.inf, norm_type=math.inf).clamp_(min=2.0**-100)
-            power = largest / torch.frexp(largest).mantissa  # exact: the power of two above it
-            grad, scale = (grad * (2.0**14 / power)).to(torch.float16), self.scale * (power / 2.0**14)
+            unit = (largest / torch.frexp(largest).mantissa).mul_(2.0**-14)  # exact: the power of two above it, over 2^14
+            grad = torch.div(grad, unit, out=torch.empty(grad.shape, dtype=torch.float16, device=self.device))
+            scale = self.scale * unit
         _, grad_a, grad_b = self._backward(grad, x, codes, hidden, False, scale)
         norm = clip_grad_norm([grad_a, grad_b], max_norm)
         return FeedbackGradients(loss, margin, grad_a, grad_b, norm)
