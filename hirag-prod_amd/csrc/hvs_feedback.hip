@@ -63,41 +63,46 @@ template <int DT, int CH> __device__ __forceinline__ void keep_raw(Raw8<DT> (&a)
 __device__ __forceinline__ float softplus(float z) { return fmaxf(z, 0.0f) + log1pf(expf(-fabsf(z))); }
 __device__ __forceinline__ float inverse_norm(float sum_of_squares) { return sum_of_squares == 0.0f ? 0.0f : 1.0f / sqrtf(sum_of_squares); }
 
-// Rows of fp32 and bf16 may be longer than 2^64 or shorter than 2^-50: their squares leave fp32, or its normal numbers.  The squares
-// of such a row are added up again, of its elements times the power of two that brings the largest to [0.5, 1).
+// Rows of fp32 and bf16 may be longer than 2^64 or shorter than 2^-50: their squares leave fp32, or its normal numbers.  Only the
+// direction of a row counts, so the elements of such a row are multiplied by the power of two that brings the largest to
+// [0.5, 1): exact, but for those that are then below 2^-126 and do not matter beside it.
 __device__ __forceinline__ bool plain_square_sum(float v) { return v >= 0x1p-100f && v < __builtin_inff(); }
-// use(element) for the elements of a row's part, four bytes at a time: what this seldom path holds in registers the usual one pays for
-template <int DT, int CH, class USE> __device__ __forceinline__ void for_each_element(const Raw8<DT> (&r)[CH], float &state, USE use) {
+// use(element) -> what becomes of it, for the elements of a row's part, four bytes at a time: what this seldom path holds in
+// registers the usual one pays for
+template <int DT, int CH, class USE> __device__ __forceinline__ void for_each_element(Raw8<DT> (&r)[CH], float &state, USE use) {
     static_assert(DT == HVS_F32 || DT == HVS_BF16, "no such rows of fp16");
     constexpr int EPC = Elem<DT>::EPC;
 #pragma unroll
     for (int i = 0; i < CH * 32 / EPC; i++) {
-        float word = r[i / (32 / EPC)].c[i / 4 % (8 / EPC)][i % 4];
+        f32x4 &four = r[i / (32 / EPC)].c[i / 4 % (8 / EPC)];
+        float word = four[i % 4];
         asm volatile("" : "+v"(word), "+v"(state));  // one word after the other
-        if (DT == HVS_F32) use(word);
+        if (DT == HVS_F32) four[i % 4] = use(word);
         else {
-            use(__uint_as_float(__float_as_uint(word) << 16));
-            use(__uint_as_float(__float_as_uint(word) & 0xFFFF0000u));
+            const uint32_t low = __float_as_uint(use(__uint_as_float(__float_as_uint(word) << 16)));
+            const uint32_t high = __float_as_uint(use(__uint_as_float(__float_as_uint(word) & 0xFFFF0000u)));
+            four[i % 4] = __uint_as_float((high & 0xFFFF0000u) | (low >> 16));
         }
     }
 }
-template <int DT, int CH> __device__ __forceinline__ float row_largest(const Raw8<DT> (&r)[CH]) {
+template <int DT, int CH> __device__ __forceinline__ float row_largest(Raw8<DT> (&r)[CH]) {
     float largest = 0.0f;
-    for_each_element<DT, CH>(r, largest, [&](float v) { largest = fmaxf(largest, fabsf(v)); });
+    for_each_element<DT, CH>(r, largest, [&](float v) {
+        largest = fmaxf(largest, fabsf(v));
+        return v;
+    });
     return largest;
 }
-template <int DT, int CH> __device__ __forceinline__ float row_square_sum(const Raw8<DT> (&r)[CH], int exponent) {
+// scales the row (not if there is nothing but zeros, or an infinite element) and returns its sum of squares
+template <int DT, int CH> __device__ __forceinline__ float row_scale(Raw8<DT> (&r)[CH], float largest) {
+    const int exponent = __builtin_amdgcn_readfirstlane(-__builtin_amdgcn_frexp_expf(largest));  // the same in every lane
     float sum = 0.0f;
     for_each_element<DT, CH>(r, sum, [&](float v) {
-        v = ldexpf(v, -exponent);
+        v = ldexpf(v, exponent);
         sum = fmaf(v, v, sum);
+        return v;
     });
     return sum;
-}
-// 1 / norm from such a sum; a norm whose inverse is no fp32 number counts as 0
-__device__ __forceinline__ float inverse_norm(float sum_of_squares, int exponent) {
-    const float inv = ldexpf(inverse_norm(sum_of_squares), -exponent);
-    return inv == __builtin_inff() ? 0.0f : inv;
 }
 
 // how the pairs [b0, b1) of a query are shared out; the same on every side that asks
@@ -275,22 +280,18 @@ __global__ __launch_bounds__(64 * WAVES, TW == 1 && CH == 2 && WAVES == 4 ? 5 : 
                 for (int e = 0; e < 8; e++) ia = fmaf(av[e], av[e], ia), ib = fmaf(bv[e], bv[e], ib);
             }
             team_sum(ia, ib);
-            int ea = 0, eb = 0;
             if constexpr (RDT != HVS_F16) {  // (squares of fp16 stay well inside)
                 if (!(plain_square_sum(ia) && plain_square_sum(ib))) {
                     float ma = row_largest<RDT, CH>(ra), mb = row_largest<RDT, CH>(rb);
                     team_max(ma, mb);
-                    // exponents that bring the largest element to [0.5, 1); 0 where that is 0 or not finite.  The same in every lane
-                    ea = __builtin_amdgcn_readfirstlane(__builtin_amdgcn_frexp_expf(ma));
-                    eb = __builtin_amdgcn_readfirstlane(__builtin_amdgcn_frexp_expf(mb));
-                    ia = row_square_sum<RDT, CH>(ra, ea);
-                    ib = row_square_sum<RDT, CH>(rb, eb);
+                    ia = row_scale<RDT, CH>(ra, ma);
+                    ib = row_scale<RDT, CH>(rb, mb);
                     team_sum(ia, ib);
                 }
             }
             // a row against itself is no preference: exactly 0, whatever the roundings below
-            ia = a == b ? 0.0f : inverse_norm(ia, ea);
-            ib = a == b ? 0.0f : inverse_norm(ib, eb);
+            ia = a == b ? 0.0f : inverse_norm(ia);
+            ib = a == b ? 0.0f : inverse_norm(ib);
             keep_raw(ra, rb);
 #pragma unroll
             for (int c = 0; c < CH; c++) {

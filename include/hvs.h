@@ -515,8 +515,8 @@ int hvs_adapters_backward(int device_id, void *stream, const hvs_adapters *ad, c
  * positions.  A pair with a negative position is left out (loss and margin 0, no gradient); one with a position past the
  * last row gets a NaN loss and margin and makes its query's gradient NaN.
  * grad [n_queries, dim], the queries' dtype: gradient of sum_p weights[p] loss[p]; weights NULL = 1 / n_pairs each (the
- * mean).  A query of norm 0 gets gradient 0.  A norm below 2^-126, whose inverse is no float, counts as 0; norms up to 2^100 keep
- * full precision.  Sums run in a fixed order.
+ * mean).  A query of norm 0 gets gradient 0, and so does one of a norm below 1e-38, whose inverse is no float; queries of norms up
+ * to 2^126 and rows of any norm keep full precision.  Sums run in a fixed order.
  */
 typedef struct hvs_preference {
     const void *queries;    /* [n_queries, dim] */

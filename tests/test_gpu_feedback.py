@@ -636,21 +636,17 @@ def test_small_moves_by_their_terms(env, move, qdt, dim, counts):
 @pytest.mark.parametrize("rdt", ["f32", "bf16"])
 @pytest.mark.parametrize("dim,counts", [(64, [4] * 12), (1100, [3] * 20), (1536, [40]), (2049, [9, 1]), (3000, [4] * 130), (9000, [5, 2])])
 def test_row_norms_at_the_ends_of_the_range(env, rdt, dim, counts):
-    """Rows of fp32's range have squares past it or below it: still only their direction counts, beside ordinary rows and each other;
-    rows too short for an inverse in fp32 count as zero rows, and an infinite element makes a pair NaN."""
+    """Rows of fp32's range have squares past it or below it: still only their direction counts, beside ordinary rows and each other,
+    down to subnormal elements; an infinite element makes a pair NaN."""
     torch = env.torch
     q, ref, rows, c, r, off = make(env, "f32", rdt, len(counts), dim, 30, counts, seed=dim)
-    exponent = torch.tensor([0, 100, -100, 64, -64, -52, 90, -110, 70, 0], device=env.dev).repeat(3)
-    sized = (rows.float() * torch.exp2(exponent.float())[:, None]).to(rows.dtype)
-    assert bool(sized.isfinite().all())
-    got = env.hvs.preference_loss(q, sized, c, r, off, reference=ref, beta=10.0)
-    check_by_terms(q, ref, sized, c, r, off, got, "f32", 10.0, 0.0)
-    short = rows.clone()
-    short[::3] = (short[::3].float() * 2.0**-140).to(rows.dtype)
-    zero = rows.clone()
-    zero[::3] = 0
-    got, want = (env.hvs.preference_loss(q, t, c, r, off, reference=ref, beta=10.0) for t in (short, zero))
-    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    weights = torch.exp2(torch.arange(len(c), device=env.dev) % 61 - 30.0)
+    exponent = torch.tensor([0, 100, -100, 64, -64, -52, 120, -110, 70, -131], device=env.dev).repeat(3)
+    sized = (rows.double() * torch.exp2(exponent.double())[:, None]).to(rows.dtype)
+    assert bool(sized.isfinite().all()) and bool((sized != 0).any(1).all())
+    for w in (None, weights):
+        got = env.hvs.preference_loss(q, sized, c, r, off, reference=ref, beta=10.0, weights=w)
+        check_by_terms(q, ref, sized, c, r, off, got, "f32", 10.0, 0.0, w)
     sized[4, 5] = torch.inf
     loss, margin, _ = env.hvs.preference_loss(q, sized, c, r, off, reference=ref, beta=10.0)
     touched = (c == 4) | (r == 4)
